@@ -127,9 +127,10 @@ uint64_t tk_launch_count(const tk_ctx *ctx);
  * tk_profile_read synchronizes the device and returns the summed event time
  * (ms) and number of recorded launches of one kernel family.  TK_PROF_COMM:
  * the reduce-scatter's owner reduce (with its wait for the peers' tiles) and
- * the peer collectives' kernels. */
+ * the peer collectives' kernels.  TK_PROF_SERVE: the key/value cache, the
+ * attention over it and the verification of drafted tokens. */
 enum { TK_PROF_GEMM = 0, TK_PROF_DEQUANT = 1, TK_PROF_SPLIT = 2, TK_PROF_GEMV = 3, TK_PROF_LMHEAD = 4,
-       TK_PROF_COMM = 5 };
+       TK_PROF_COMM = 5, TK_PROF_SERVE = 6 };
 tk_status tk_profile(tk_ctx *ctx, int enable);
 tk_status tk_profile_read(tk_ctx *ctx, int kind, double *total_ms, uint64_t *launches);
 
@@ -227,6 +228,96 @@ enum { TK_GEMV_MAXSEG = 4 };
 tk_status tk_gemv_multi(tk_ctx *ctx, int qtype, int nseg, const void *const *W, const int *rows,
                         float *const *y, const int *ldy, size_t row_bytes, int K, const float *x,
                         int ldx, int M, void *stream);
+
+/* ---- 4-bit key/value cache and attention over it -------------------------- */
+/* The serving step between the q/k/v projections and o_proj: new keys and
+ * values are rounded to 4 bits into a paged cache (tk_kv_append), and
+ * attention reads the cache in that form (tk_kv_attend).  The reference keeps
+ * an fp32 cache and runs attn_cache over it (tier/tier.cpp:2240-2259).
+ *
+ * One layer's cache.  Per token and key/value head: head_dim values (64 or
+ * 128) in groups of 32, each group a scale d (fp16, at most 8 significant
+ * bits) and whole numbers n in -8..7; the value n * d is exact in fp16.
+ *   k_q, v_q  [n_pages, n_kv_heads, page_tokens, head_dim / 2] bytes: a
+ *             32-bit word holds 8 consecutive values, value e in bits
+ *             4 * ((e >> 1) + 4 * (e & 1)) .. + 3, two's complement
+ *   k_s, v_s  [n_pages, n_kv_heads, page_tokens, head_dim / 32] fp16 scales
+ * Token t of a sequence is row t % page_tokens of its page t / page_tokens.
+ * page_tokens: 16, 32, 64, 128 or 256.  All four are device pointers,
+ * 16-byte aligned.  Rows never written may hold anything. */
+typedef struct tk_kvcache {
+    int n_pages, page_tokens, n_kv_heads, head_dim;
+    void *k_q, *k_s, *v_q, *v_s;
+} tk_kvcache;
+/* A batch of sequences with their new tokens packed one after the other:
+ * sequence b owns rows q_start[b] .. q_start[b+1]-1 of the packed arrays, the
+ * LAST q_start[b+1]-q_start[b] of its kv_len[b] cached tokens (kv_len counts
+ * them), in the pages pages[b * max_pages + i].  q_start, kv_len and pages are
+ * device pointers (a captured graph may be replayed with other contents);
+ * n_tokens = rows of the packed arrays, max_new >= any sequence's new tokens.
+ * A sequence may have no new tokens; a row whose position is negative (more
+ * new tokens than kv_len) has no place in the cache: it is not appended, reads
+ * back as zeros and attends to nothing.  Contents that do not fit (q_start
+ * that decreases or passes n_tokens, more than max_new new tokens, kv_len
+ * beyond max_pages pages, a page outside the cache) make tk_sync_status report
+ * TK_ERR_DEVICE; the affected sequence's results are then unspecified, but
+ * nothing outside the caller's arrays is read or written. */
+typedef struct tk_seqs {
+    int n_seqs, n_tokens, max_new, max_pages;
+    const int32_t *q_start, *kv_len, *pages;
+} tk_seqs;
+/* Cached rows of the batch's new tokens = k, v [n_tokens, n_kv_heads *
+ * head_dim] (fp32, fp16 or bf16; row strides ldk, ldv in elements, rows
+ * 16-byte aligned) rounded to 4 bits.  Per group of 32: m = the value of
+ * largest magnitude (the first of several), d = m / -8 rounded to 8
+ * significant bits, |d| <= 8160, in fp16; n = floor(x * (1 / d) + 8.5) clamped
+ * to 0..15, minus 8 (fp32 arithmetic).  NaN and infinities are stored as 0
+ * and make tk_sync_status report TK_ERR_DEVICE.  No two rows of one call may
+ * name the same cached token. */
+tk_status tk_kv_append(tk_ctx *ctx, const tk_kvcache *cache, const tk_seqs *seqs, const void *k, const void *v,
+                       int x_dtype, int ldk, int ldv, void *stream);
+/* k, v [n_tokens, n_kv_heads * head_dim] (out_dtype) = the values that the
+ * cache holds for the batch's new tokens (for a whole context: seqs whose new
+ * tokens are all its tokens).  fp32 and fp16 hold them exactly. */
+tk_status tk_kv_read(tk_ctx *ctx, const tk_kvcache *cache, const tk_seqs *seqs, void *k, void *v, int out_dtype,
+                     int ldk, int ldv, void *stream);
+/* out[i, h] = sum_j softmax_j(scale * q[i, h] . k_j) v_j over the cached
+ * tokens j that row i sees: j <= its position, and j > position - window when
+ * window > 0.  q, out [n_tokens, n_heads * head_dim] in x_dtype; head h reads
+ * key/value head h / (n_heads / n_kv_heads).  A row that sees nothing is zero.
+ * fp32 rows are computed to fp32 accuracy (q and the probabilities as two fp16
+ * parts), fp16 and bf16 rows with one fp16 part of the probabilities; all sums
+ * are fp32.  Cached rows that no row sees do not matter, whatever they hold.
+ * Replaces attn_cache (tier/tier.cpp:2240-2259). */
+tk_status tk_kv_attend(tk_ctx *ctx, const tk_kvcache *cache, const tk_seqs *seqs, const void *q, int x_dtype,
+                       int ldq, int n_heads, float scale, int window, void *out, int ldo, void *stream);
+
+/* ---- verification of drafted tokens --------------------------------------- */
+/* Sequence b has rows row_start[b] .. row_start[b+1]-1 (device int32, at least
+ * one row): row i holds the target model's logits after token tokens[i], and
+ * tokens[i + 1], while it is a row of the same sequence, is the drafted token
+ * that row i judges.  With p = softmax(target / temperature) and
+ * q = softmax(draft / temperature) (draft's rows as target's; the last row of a
+ * sequence is not used; draft == NULL: q = 1 for the drafted token), drafted
+ * tokens are accepted in turn while u_accept[i] * q(x) < p(x).  At the first
+ * refusal the sequence's next token is drawn from max(p - q, 0), or from p at
+ * its last row: the lowest token whose running sum of weights passes
+ * u_sample[b] times their total.  Weights are whole multiples of 2^-38, so the
+ * draw depends on no order of summation.  temperature == 0: accepted while the
+ * drafted token is the row's largest logit (the lowest of several), which is
+ * also the next token.
+ * Out: n_accept[b] = drafted tokens accepted; next[b]; logp[i] (nullable) = log
+ * p of the token that row i settled (accepted or drawn; at temperature 0 for
+ * temperature 1), 0 for rows after the refusal.
+ * Logits of -inf have probability 0.  Random numbers are in [0, 1).  A row that
+ * is needed and holds NaN, +inf or only -inf ends its sequence with next = -1,
+ * as does a row_start that does not fit, and tk_sync_status reports
+ * TK_ERR_DEVICE.  A drafted token outside the vocabulary is refused.
+ * No counterpart in the reference, which decodes one token at a time. */
+tk_status tk_draft_verify(tk_ctx *ctx, int n_seqs, const int32_t *row_start, int n_rows, int vocab,
+                          const float *target, long ldt, const float *draft, long ldd, const int32_t *tokens,
+                          const float *u_accept, const float *u_sample, float temperature, int32_t *n_accept,
+                          int32_t *next, float *logp, void *stream);
 
 /* ---- linear layers (tensor cores) --------------------------------------- */
 /* Y[M, N] = X[M, K] . W^T (+ Y if beta == 1).  X dtype per x_dtype with row

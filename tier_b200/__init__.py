@@ -49,7 +49,7 @@ IPC_HANDLE_BYTES = 64   # TK_IPC_HANDLE_BYTES
 WFROZEN = 0x200  # OR into tk_gemv's qtype: W is never written by earlier kernels (early weight fetch)
 WREUSE = 0x400   # OR into linear products: reuse the previous call's fp16 expansion of the same (unchanged) W
 # kernel families for profiling
-PROF_GEMM, PROF_DEQUANT, PROF_SPLIT, PROF_GEMV, PROF_LMHEAD, PROF_COMM = range(6)
+PROF_GEMM, PROF_DEQUANT, PROF_SPLIT, PROF_GEMV, PROF_LMHEAD, PROF_COMM, PROF_SERVE = range(7)
 
 
 class TierkError(RuntimeError):
@@ -67,6 +67,20 @@ class Weight(ctypes.Structure):
 class IqGrids(ctypes.Structure):
     """tk_iq_grids: host pointers to the six lattice tables (int8)."""
     _fields_ = [(n, ctypes.c_void_p) for n in ("iq2xxs", "iq2xs", "iq2s", "iq3xxs", "iq3s", "iq1s")]
+
+
+class KvCache(ctypes.Structure):
+    """tk_kvcache: one layer's 4-bit key/value cache on the device."""
+    _fields_ = [("n_pages", ctypes.c_int), ("page_tokens", ctypes.c_int), ("n_kv_heads", ctypes.c_int),
+                ("head_dim", ctypes.c_int), ("k_q", ctypes.c_void_p), ("k_s", ctypes.c_void_p),
+                ("v_q", ctypes.c_void_p), ("v_s", ctypes.c_void_p)]
+
+
+class Seqs(ctypes.Structure):
+    """tk_seqs: a batch of sequences with packed new tokens."""
+    _fields_ = [("n_seqs", ctypes.c_int), ("n_tokens", ctypes.c_int), ("max_new", ctypes.c_int),
+                ("max_pages", ctypes.c_int), ("q_start", ctypes.c_void_p), ("kv_len", ctypes.c_void_p),
+                ("pages", ctypes.c_void_p)]
 
 
 # (name, rows, cols) of each table, in tk_iq_grids order
@@ -92,6 +106,7 @@ _P = ctypes.c_void_p
 _I = ctypes.c_int
 _SZ = ctypes.c_size_t
 _F = ctypes.c_float
+_L = ctypes.c_long
 
 # (name, restype, argtypes) -- mirrors include/tierk.h
 SIGNATURES = [
@@ -110,6 +125,10 @@ SIGNATURES = [
     ("tk_dequant", _I, [_P, _I, _P, _SZ, _I, _I, _I, _I, _P, _P]),
     ("tk_gemv", _I, [_P, _I, _P, _SZ, _I, _I, _P, _I, _I, _P, _I, _P]),
     ("tk_gemv_multi", _I, [_P, _I, _I, _P, _P, _P, _P, _SZ, _I, _P, _I, _I, _P]),
+    ("tk_kv_append", _I, [_P, ctypes.POINTER(KvCache), ctypes.POINTER(Seqs), _P, _P, _I, _I, _I, _P]),
+    ("tk_kv_read", _I, [_P, ctypes.POINTER(KvCache), ctypes.POINTER(Seqs), _P, _P, _I, _I, _I, _P]),
+    ("tk_kv_attend", _I, [_P, ctypes.POINTER(KvCache), ctypes.POINTER(Seqs), _P, _I, _I, _I, _F, _I, _P, _I, _P]),
+    ("tk_draft_verify", _I, [_P, _I, _P, _I, _I, _P, _L, _P, _L, _P, _P, _P, _F, _P, _P, _P, _P]),
     ("tk_linear_fwd", _I, [_P, ctypes.POINTER(Weight), _P, _I, _I, _I, _P, _I, _F, _I, _P]),
     ("tk_linear_dx", _I, [_P, ctypes.POINTER(Weight), _P, _I, _I, _I, _P, _I, _F, _I, _P]),
     ("tk_linear_fwd_noalloc", _I, [_P, ctypes.POINTER(Weight), _P, _I, _I, _I, _P, _I, _F, _I, _P]),
@@ -312,6 +331,39 @@ class Context:
                                     _stream(stream)))
         return out
 
+    # ---- 4-bit key/value cache, attention over it, drafted tokens ----
+    def kv_append(self, cache: KvCache, seqs: Seqs, k, v, x_dtype=DT_F32, ldk=None, ldv=None, stream=None):
+        """Round the batch's new keys and values to 4 bits into the cache (tk_kv_append)."""
+        _check(self.lib.tk_kv_append(self.h, ctypes.byref(cache), ctypes.byref(seqs), _ptr(k), _ptr(v), x_dtype,
+                                     ldk or k.stride(0), ldv or v.stride(0), _stream(stream)))
+
+    def kv_read(self, cache: KvCache, seqs: Seqs, k, v, out_dtype=DT_F32, ldk=None, ldv=None, stream=None):
+        """k, v = the values that the cache holds for the batch's new tokens (tk_kv_read)."""
+        _check(self.lib.tk_kv_read(self.h, ctypes.byref(cache), ctypes.byref(seqs), _ptr(k), _ptr(v), out_dtype,
+                                   ldk or k.stride(0), ldv or v.stride(0), _stream(stream)))
+        return k, v
+
+    def kv_attend(self, cache: KvCache, seqs: Seqs, q, n_heads, out, x_dtype=DT_F32, scale=None, window=0, ldq=None,
+                  ldo=None, stream=None):
+        """out = attention of the batch's new tokens over the cache (tk_kv_attend);
+        scale defaults to 1 / sqrt(head_dim)."""
+        scale = cache.head_dim ** -0.5 if scale is None else scale
+        _check(self.lib.tk_kv_attend(self.h, ctypes.byref(cache), ctypes.byref(seqs), _ptr(q), x_dtype,
+                                     ldq or q.stride(0), n_heads, scale, window, _ptr(out), ldo or out.stride(0),
+                                     _stream(stream)))
+        return out
+
+    def draft_verify(self, target, tokens, row_start, u_accept, u_sample, n_accept, next_token, logp=None, draft=None,
+                     temperature=1.0, stream=None):
+        """Accept drafted tokens against the target's logits and draw each
+        sequence's next token (tk_draft_verify)."""
+        _check(self.lib.tk_draft_verify(self.h, n_accept.numel(), _ptr(row_start), target.shape[0], target.shape[1],
+                                        _ptr(target), target.stride(0), _ptr(draft),
+                                        draft.stride(0) if draft is not None else 0, _ptr(tokens), _ptr(u_accept),
+                                        _ptr(u_sample), temperature, _ptr(n_accept), _ptr(next_token), _ptr(logp),
+                                        _stream(stream)))
+        return n_accept, next_token
+
     # ---- reduce-scatter over peer memory (multi-GPU) ----
     def comm_init(self, rank: int, world: int, recv_bytes: int) -> bytes:
         """Allocate this rank's receive buffer; returns its IPC handle (64 bytes)."""
@@ -421,7 +473,44 @@ def make_weight(qtype: int, rows: int, cols: int, data, scale_log2: int = 0) -> 
     return w
 
 
+def make_kvcache(k_q, k_s, v_q, v_s) -> KvCache:
+    """Describe a cache's four device tensors (layout: tk_kvcache in tierk.h):
+    k_q, v_q uint8 [pages, kv_heads, page_tokens, head_dim / 2], k_s, v_s
+    float16 [pages, kv_heads, page_tokens, head_dim / 32]."""
+    n, h, p, half = k_q.shape
+    for t, shape, size in ((k_q, (n, h, p, half), 1), (v_q, (n, h, p, half), 1), (k_s, (n, h, p, half // 16), 2),
+                           (v_s, (n, h, p, half // 16), 2)):
+        if tuple(t.shape) != shape or t.element_size() != size or not t.is_contiguous():
+            raise ValueError(f"cache tensor {tuple(t.shape)}: expected contiguous {shape} of {size}-byte elements")
+    c = KvCache(n, p, h, 2 * half, k_q.data_ptr(), k_s.data_ptr(), v_q.data_ptr(), v_s.data_ptr())
+    c._owner = (k_q, k_s, v_q, v_s)   # the descriptor keeps its device memory alive
+    return c
+
+
+def alloc_kvcache(n_pages: int, page_tokens: int, n_kv_heads: int, head_dim: int, device="cuda") -> KvCache:
+    """A zeroed cache of n_pages pages."""
+    import torch
+    shape = (n_pages, n_kv_heads, page_tokens)
+    q = [torch.zeros(*shape, head_dim // 2, dtype=torch.uint8, device=device) for _ in "kv"]
+    s = [torch.zeros(*shape, head_dim // 32, dtype=torch.float16, device=device) for _ in "kv"]
+    return make_kvcache(q[0], s[0], q[1], s[1])
+
+
+def make_seqs(q_start, kv_len, pages, n_tokens: int, max_new: int) -> Seqs:
+    """Describe a batch (tk_seqs in tierk.h): int32 device tensors q_start
+    [n_seqs + 1], kv_len [n_seqs], pages [n_seqs, max_pages]."""
+    B = kv_len.numel()
+    for t in (q_start, kv_len, pages):
+        if t.element_size() != 4 or t.is_floating_point() or not t.is_contiguous():
+            raise ValueError("q_start, kv_len and pages must be contiguous int32 tensors")
+    if q_start.numel() != B + 1 or pages.dim() != 2 or pages.shape[0] != B:
+        raise ValueError("q_start must have n_seqs + 1 entries and pages n_seqs rows")
+    s = Seqs(B, n_tokens, max_new, pages.shape[1], q_start.data_ptr(), kv_len.data_ptr(), pages.data_ptr())
+    s._owner = (q_start, kv_len, pages)
+    return s
+
+
 from .host import LinearPath, LMHead  # noqa: E402  (host-side mirror of the reference's operators)
 
-__all__ = ["Context", "Weight", "make_weight", "load", "row_bytes", "lmhead_chunk", "IqGrids", "IQ_GRID_SHAPES",
+__all__ = ["Context", "Weight", "make_weight", "KvCache", "Seqs", "make_kvcache", "alloc_kvcache", "make_seqs", "load", "row_bytes", "lmhead_chunk", "IqGrids", "IQ_GRID_SHAPES",
            "iq_grids_from_gguf", "LinearPath", "LMHead", "TierkError"]

@@ -630,6 +630,86 @@ tk_status tk_gemv_multi(tk_ctx* ctx, int qtype, int nseg, const void* const* W, 
     return TK_OK;
 }
 
+// ---- 4-bit key/value cache, attention over it, drafted tokens --------------
+// Checks shared by the cache's entry points; `ld` row strides of the packed
+// arrays of `width` elements of `dtype`.
+static tk_status kv_check(tk_ctx* ctx, const tk_kvcache* c, const tk_seqs* s, const void* a, const void* b, int dtype,
+                          long width_a, long width_b, int lda, int ldb, const char* fn) {
+    if (!ctx) return fail(TK_ERR_INVALID, std::string(fn) + ": null context");
+    if (!c || !s) return fail(TK_ERR_INVALID, std::string(fn) + ": null cache or batch");
+    if (c->head_dim != 64 && c->head_dim != 128)
+        return fail(TK_ERR_UNSUPPORTED, std::string(fn) + ": head_dim must be 64 or 128");
+    if (c->page_tokens < 16 || c->page_tokens > 256 || (c->page_tokens & (c->page_tokens - 1)))
+        return fail(TK_ERR_INVALID, std::string(fn) + ": page_tokens must be 16, 32, 64, 128 or 256");
+    if (c->n_pages <= 0 || c->n_kv_heads <= 0 || c->n_kv_heads > 65535)
+        return fail(TK_ERR_INVALID, std::string(fn) + ": empty cache");
+    if (!c->k_q || !c->k_s || !c->v_q || !c->v_s) return fail(TK_ERR_INVALID, std::string(fn) + ": null cache tensor");
+    if (!aligned16(c->k_q) || !aligned16(c->k_s) || !aligned16(c->v_q) || !aligned16(c->v_s))
+        return fail(TK_ERR_INVALID, std::string(fn) + ": cache tensors must be 16-byte aligned");
+    if (s->n_seqs < 0 || s->n_tokens < 0 || s->max_new < 0 || s->max_pages < 0)
+        return fail(TK_ERR_INVALID, std::string(fn) + ": negative batch size");
+    if (s->n_seqs == 0 || s->n_tokens == 0 || s->max_new == 0) return TK_OK;
+    if (s->max_pages == 0 || (long)s->max_pages * c->page_tokens > INT32_MAX)
+        return fail(TK_ERR_INVALID, std::string(fn) + ": max_pages out of range");
+    if (!s->q_start || !s->kv_len || !s->pages) return fail(TK_ERR_INVALID, std::string(fn) + ": null batch array");
+    if (!a || !b) return fail(TK_ERR_INVALID, std::string(fn) + ": null rows");
+    if (dtype != TK_DT_F32 && dtype != TK_DT_F16 && dtype != TK_DT_BF16)
+        return fail(TK_ERR_INVALID, std::string(fn) + ": element type");
+    const int unit = dtype == TK_DT_F32 ? 4 : 8;
+    if (lda < width_a || ldb < width_b) return fail(TK_ERR_INVALID, std::string(fn) + ": row stride too small");
+    if (!aligned16(a) || !aligned16(b) || lda % unit || ldb % unit)
+        return fail(TK_ERR_INVALID, std::string(fn) + ": rows must be 16-byte aligned");
+    return TK_OK;
+}
+static bool kv_empty(const tk_seqs* s) { return s->n_seqs == 0 || s->n_tokens == 0 || s->max_new == 0; }
+
+tk_status tk_kv_append(tk_ctx* ctx, const tk_kvcache* cache, const tk_seqs* seqs, const void* k, const void* v,
+                       int x_dtype, int ldk, int ldv, void* stream) {
+    const long w = cache ? (long)cache->n_kv_heads * cache->head_dim : 0;
+    const tk_status st = kv_check(ctx, cache, seqs, k, v, x_dtype, w, w, ldk, ldv, "tk_kv_append");
+    if (st != TK_OK || kv_empty(seqs)) return st;
+    return launch_kv_append(ctx, *cache, *seqs, k, v, x_dtype, ldk, ldv, static_cast<cudaStream_t>(stream));
+}
+
+tk_status tk_kv_read(tk_ctx* ctx, const tk_kvcache* cache, const tk_seqs* seqs, void* k, void* v, int out_dtype,
+                     int ldk, int ldv, void* stream) {
+    const long w = cache ? (long)cache->n_kv_heads * cache->head_dim : 0;
+    const tk_status st = kv_check(ctx, cache, seqs, k, v, out_dtype, w, w, ldk, ldv, "tk_kv_read");
+    if (st != TK_OK || kv_empty(seqs)) return st;
+    return launch_kv_read(ctx, *cache, *seqs, k, v, out_dtype, ldk, ldv, static_cast<cudaStream_t>(stream));
+}
+
+tk_status tk_kv_attend(tk_ctx* ctx, const tk_kvcache* cache, const tk_seqs* seqs, const void* q, int x_dtype, int ldq,
+                       int n_heads, float scale, int window, void* out, int ldo, void* stream) {
+    const long w = cache ? (long)n_heads * cache->head_dim : 0;
+    const tk_status st = kv_check(ctx, cache, seqs, q, out, x_dtype, w, w, ldq, ldo, "tk_kv_attend");
+    if (st != TK_OK) return st;
+    if (n_heads <= 0 || n_heads % cache->n_kv_heads)
+        return fail(TK_ERR_INVALID, "tk_kv_attend: n_heads must be a multiple of the cache's n_kv_heads");
+    if (!std::isfinite(scale)) return fail(TK_ERR_INVALID, "tk_kv_attend: scale must be finite");
+    if (window < 0) return fail(TK_ERR_INVALID, "tk_kv_attend: negative window");
+    if (kv_empty(seqs)) return TK_OK;
+    return launch_kv_attend(ctx, *cache, *seqs, q, x_dtype, ldq, n_heads, scale, window, out, ldo,
+                            static_cast<cudaStream_t>(stream));
+}
+
+tk_status tk_draft_verify(tk_ctx* ctx, int n_seqs, const int32_t* row_start, int n_rows, int vocab,
+                          const float* target, long ldt, const float* draft, long ldd, const int32_t* tokens,
+                          const float* u_accept, const float* u_sample, float temperature, int32_t* n_accept,
+                          int32_t* next, float* logp, void* stream) {
+    if (!ctx) return fail(TK_ERR_INVALID, "tk_draft_verify: null context");
+    if (n_seqs < 0 || n_rows < 0) return fail(TK_ERR_INVALID, "tk_draft_verify: bad row count");
+    if (n_seqs == 0) return TK_OK;
+    if (vocab <= 0 || n_rows == 0) return fail(TK_ERR_INVALID, "tk_draft_verify: no rows or empty vocabulary");
+    if (!row_start || !target || !tokens || !n_accept || !next) return fail(TK_ERR_INVALID, "tk_draft_verify: null pointer");
+    if (!(temperature >= 0.0f) || !std::isfinite(temperature) || (temperature > 0.0f && temperature < 1e-4f))
+        return fail(TK_ERR_INVALID, "tk_draft_verify: temperature must be 0 or at least 1e-4");
+    if (temperature > 0.0f && (!u_accept || !u_sample)) return fail(TK_ERR_INVALID, "tk_draft_verify: null random numbers");
+    if (ldt < vocab || (draft && ldd < vocab)) return fail(TK_ERR_INVALID, "tk_draft_verify: row stride too small");
+    return launch_draft_verify(ctx, n_seqs, row_start, n_rows, vocab, target, ldt, draft, ldd, tokens, u_accept, u_sample,
+                               temperature, n_accept, next, logp, static_cast<cudaStream_t>(stream));
+}
+
 tk_status tk_linear_fwd(tk_ctx* ctx, const tk_weight* W, const void* X, int x_dtype, int M, int ldx, float* Y, int ldy,
                         float beta, int products, void* stream) {
     return linear(ctx, W, X, x_dtype, M, ldx, Y, ldy, beta, products, static_cast<cudaStream_t>(stream), false);

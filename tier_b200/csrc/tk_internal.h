@@ -73,7 +73,8 @@ inline cudaError_t smem_attr_once(K* kern, int bytes, int device, std::atomic<ui
 }
 
 // Kernel families for tk_profile_read (TK_PROF_* in tierk.h).
-enum ProfKind { PK_GEMM = 0, PK_DEQUANT = 1, PK_SPLIT = 2, PK_GEMV = 3, PK_LMHEAD = 4, PK_COMM = 5, PK_COUNT = 6 };
+enum ProfKind { PK_GEMM = 0, PK_DEQUANT = 1, PK_SPLIT = 2, PK_GEMV = 3, PK_LMHEAD = 4, PK_COMM = 5, PK_SERVE = 6,
+                PK_COUNT = 7 };
 int prof_begin(tk_ctx* ctx, cudaStream_t s);
 void prof_end(tk_ctx* ctx, cudaStream_t s, int slot, int kind);
 struct ProfScope {
@@ -169,6 +170,19 @@ struct RsDesc {
     int* counter = nullptr;
     int world = 0, rpo = 0, epoch = 0;
 };
+
+// ---- tk_kvcache.cu, tk_kvattn.cu: the 4-bit key/value cache and attention over it (arguments checked) ----
+tk_status launch_kv_append(tk_ctx* ctx, const tk_kvcache& c, const tk_seqs& s, const void* k, const void* v, int dtype,
+                           long ldk, long ldv, cudaStream_t st);
+tk_status launch_kv_read(tk_ctx* ctx, const tk_kvcache& c, const tk_seqs& s, void* k, void* v, int dtype, long ldk,
+                         long ldv, cudaStream_t st);
+tk_status launch_kv_attend(tk_ctx* ctx, const tk_kvcache& c, const tk_seqs& s, const void* q, int dtype, long ldq,
+                           int n_heads, float scale, int window, void* out, long ldo, cudaStream_t st);
+// ---- tk_verify.cu ----
+tk_status launch_draft_verify(tk_ctx* ctx, int n_seqs, const int32_t* row_start, int n_rows, int vocab,
+                              const float* target, long ldt, const float* draft, long ldd, const int32_t* tokens,
+                              const float* u_accept, const float* u_sample, float temperature, int32_t* n_accept,
+                              int32_t* next, float* logp, cudaStream_t s);
 
 // ---- tk_quant.cu: quantizers byte-exact with the reference's CPU ones ----
 tk_status launch_quantize(tk_ctx* ctx, int qtype, const float* x, long ldx, int rows, int cols, uint8_t* out,
