@@ -254,7 +254,8 @@ typedef struct tk_kvcache {
  * LAST q_start[b+1]-q_start[b] of its kv_len[b] cached tokens (kv_len counts
  * them), in the pages pages[b * max_pages + i].  q_start, kv_len and pages are
  * device pointers (a captured graph may be replayed with other contents);
- * n_tokens = rows of the packed arrays, max_new >= any sequence's new tokens.
+ * n_tokens = rows of the packed arrays, max_new >= any sequence's new tokens,
+ * max_pages * page_tokens <= 2^30.
  * A sequence may have no new tokens; a row whose position is negative (more
  * new tokens than kv_len) has no place in the cache: it is not appended, reads
  * back as zeros and attends to nothing.  Contents that do not fit (q_start

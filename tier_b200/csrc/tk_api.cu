@@ -458,6 +458,7 @@ void tk_destroy(tk_ctx* ctx) {
     if (ctx->flags) cudaFree(ctx->flags);
     if (ctx->iq_tab) cudaFree(ctx->iq_tab);
     if (ctx->sched) cudaFree(ctx->sched);
+    if (ctx->kv_count) cudaFree(ctx->kv_count);
     comm_destroy(ctx);
     for (cudaEvent_t e : ctx->prof.ev) cudaEventDestroy(e);
     delete ctx;
@@ -649,7 +650,7 @@ static tk_status kv_check(tk_ctx* ctx, const tk_kvcache* c, const tk_seqs* s, co
     if (s->n_seqs < 0 || s->n_tokens < 0 || s->max_new < 0 || s->max_pages < 0)
         return fail(TK_ERR_INVALID, std::string(fn) + ": negative batch size");
     if (s->n_seqs == 0 || s->n_tokens == 0 || s->max_new == 0) return TK_OK;
-    if (s->max_pages == 0 || (long)s->max_pages * c->page_tokens > INT32_MAX)
+    if (s->max_pages == 0 || (long)s->max_pages * c->page_tokens > (1L << 30))
         return fail(TK_ERR_INVALID, std::string(fn) + ": max_pages out of range");
     if (!s->q_start || !s->kv_len || !s->pages) return fail(TK_ERR_INVALID, std::string(fn) + ": null batch array");
     if (!a || !b) return fail(TK_ERR_INVALID, std::string(fn) + ": null rows");

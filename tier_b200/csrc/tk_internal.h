@@ -44,6 +44,9 @@ struct tk_ctx {
     int* sched = nullptr;
     size_t sched_cap = 0;            // ints
     std::vector<long> sched_key;
+    // tk_kv_attend: finished parts per (sequence, key/value head), zero between calls
+    int* kv_count = nullptr;
+    size_t kv_count_len = 0;
 };
 
 namespace tk {

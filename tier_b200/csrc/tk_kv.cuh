@@ -84,4 +84,33 @@ __device__ __forceinline__ int kv_nibble(uint32_t w, int e) {
     return (int)(((w >> (4 * f)) & 15u) ^ 8u) - 8;
 }
 
+// ---- 4-bit numbers to fp16 -------------------------------------------------
+// x: four 4-bit fields of each 16-bit half.  An fp16 with exponent bits 0x6400
+// counts in ones from 1024, so OR-ing a field n + 8 into its low bits gives
+// 1024 + (n + 8), or 1024 + 16 (n + 8) for the second field; the XOR in the
+// same LOP3 turns two's complement n into n + 8.  Both are brought back to n
+// exactly (|n| <= 8), then scaled: n * d is exact for d of 8 significant bits.
+__device__ __forceinline__ uint32_t lop_and_xor(uint32_t x, uint32_t mask, uint32_t flip) {
+    uint32_t r;
+    asm("lop3.b32 %0, %1, %2, %3, 0x6a;" : "=r"(r) : "r"(x), "r"(mask), "r"(flip));   // (x & mask) ^ flip
+    return r;
+}
+__device__ __forceinline__ __half2 as_half2(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
+__device__ __forceinline__ uint32_t as_u32(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
+__device__ __forceinline__ void kv_fields(uint32_t x, __half2 d, uint32_t (&out)[4]) {
+    const __half2 one = as_half2(0xe408e408u);                       // -1032
+    const __half2 sixteenth = as_half2(0x2c002c00u), off = as_half2(0xd480d480u);   // 1/16, -72
+    const uint32_t y = x >> 8;
+    out[0] = as_u32(__hmul2(__hadd2(as_half2(lop_and_xor(x, 0x000f000fu, 0x64086408u)), one), d));
+    out[1] = as_u32(__hmul2(__hfma2(as_half2(lop_and_xor(x, 0x00f000f0u, 0x64806480u)), sixteenth, off), d));
+    out[2] = as_u32(__hmul2(__hadd2(as_half2(lop_and_xor(y, 0x000f000fu, 0x64086408u)), one), d));
+    out[3] = as_u32(__hmul2(__hfma2(as_half2(lop_and_xor(y, 0x00f000f0u, 0x64806480u)), sixteenth, off), d));
+}
+
+__device__ __forceinline__ float fast_exp2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
 }  // namespace tk
