@@ -110,9 +110,9 @@ __device__ __forceinline__ void kv_store_out(const KvaArgs& a, const Item& it, i
 
 // The last of a head's parts to finish joins them, in the order of the keys
 // (the result does not depend on which block that is): parts are [16 rows, D]
-// of O, then (m, l) of each row.  The counter is left at zero for the next call.
+// of O, then (m, l) of each row; smem holds a factor per part and row.  The counter is left at zero for the next call.
 template <int D, int DT, class Item>
-__device__ __forceinline__ void kv_join_last(const KvaArgs& a, const Item& it, int live, int* sh_last) {
+__device__ __forceinline__ void kv_join_last(const KvaArgs& a, const Item& it, int live, uint8_t* smem, int* sh_last) {
     __threadfence();
     __syncthreads();
     if (threadIdx.x == 0) {
@@ -124,44 +124,80 @@ __device__ __forceinline__ void kv_join_last(const KvaArgs& a, const Item& it, i
     __syncthreads();
     if (!*sh_last) return;
     __threadfence();
-    const float* base = a.part + (size_t)it.first * (16 * (D + 2));
+    constexpr int P = 16 * (D + 2);                                // floats of a part
+    auto part_of = [&](int c) { return a.part + (size_t)(2 * (it.c0 + c) + (c == 0 ? it.odd : 0)) * P; };
+    float* fac = reinterpret_cast<float*>(smem);                   // [chunks][live] m, then factor; the same of l; [live] sums
+    float* ls = fac + it.chunks * live;
+    float* sum = ls + it.chunks * live;
+    for (int i = threadIdx.x; i < it.chunks * live; i += blockDim.x) {
+        const int c = i / live, r = i - c * live;
+        const float2 ml = __ldcg(reinterpret_cast<const float2*>(part_of(c) + 16 * D + 2 * r));
+        fac[i] = ml.x;
+        ls[i] = ml.y;
+    }
+    __syncthreads();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    for (int r = warp; r < live; r += blockDim.x >> 5) {
+        float m = -INFINITY, l = 0.0f;
+        for (int c = lane; c < it.chunks; c += 32) m = fmaxf(m, fac[c * live + r]);
+        for (int i = 16; i; i >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, i));
+        const float ref = m == -INFINITY ? 0.0f : m;
+        for (int c = lane; c < it.chunks; c += 32) {
+            const float f = fast_exp2(fac[c * live + r] - ref);
+            fac[c * live + r] = f;
+            l += ls[c * live + r] * f;
+        }
+        for (int i = 16; i; i >>= 1) l += __shfl_xor_sync(~0u, l, i);
+        if (lane == 0) sum[r] = l;
+    }
+    __syncthreads();
     for (int i = threadIdx.x; i < live * (D / 4); i += blockDim.x) {
         const int r = i / (D / 4), e = (i - r * (D / 4)) * 4;
-        float m = -INFINITY, l = 0.0f;
-        for (int c = 0; c < it.chunks; ++c) m = fmaxf(m, __ldcg(base + (size_t)c * (16 * (D + 2)) + 16 * D + 2 * r));
-        const float ref = m == -INFINITY ? 0.0f : m;
-        float4 o = make_float4(0, 0, 0, 0);
-        for (int c = 0; c < it.chunks; ++c) {
-            const float* part = base + (size_t)c * (16 * (D + 2));
-            const float f = fast_exp2(__ldcg(part + 16 * D + 2 * r) - ref);
-            const float4 v = __ldcg(reinterpret_cast<const float4*>(part + r * D + e));
-            l += __ldcg(part + 16 * D + 2 * r + 1) * f;
+        const float* first = part_of(0) + r * D + e;
+        const float* rest = a.part + (size_t)2 * it.c0 * P + r * D + e;
+        float4 o = __ldcg(reinterpret_cast<const float4*>(first));
+        const float f0 = fac[r];
+        o.x *= f0; o.y *= f0; o.z *= f0; o.w *= f0;
+#pragma unroll 16
+        for (int c = 1; c < it.chunks; ++c) {
+            const float f = fac[c * live + r];
+            const float4 v = __ldcg(reinterpret_cast<const float4*>(rest + (size_t)c * (2 * P)));
             o.x += v.x * f; o.y += v.y * f; o.z += v.z * f; o.w += v.w * f;
         }
-        kv_store_out<DT, D>(a, it, r, e, o, l);
+        kv_store_out<DT, D>(a, it, r, e, o, sum[r]);
     }
 }
 
 // ---------------------------------------------------------------------------
-// Few rows per key/value head (new tokens x heads of the group <= 16, or <= 8
-// for fp32): the cache is streamed once, divided among thread blocks.
+// Few rows per key/value head (new tokens x heads of the group <= 16): the
+// cache is streamed once, divided among thread blocks.
 //
-// One warp takes units of 32 keys.  S = Q K^T and O += P V are m16n8k16 fp16
-// products: the 16 matrix rows are the query rows (fp32: 8 rows as hi and lo
-// fp16 parts, so that q and p keep 22 bits; their products meet in one lane).
-// The order of the reduction index is free, so lane (g, t) = (lane / 4,
-// lane % 4) uses what it can load in one piece: for K the t-th quarter of a
-// key's row (16 bytes at head_dim 128), for V the g-th eighth of rows t and
-// t + 4 of each 8 keys.  A key's scale multiplies its fp16 numbers exactly.
+// One warp takes units of 32 keys.  S^T = K Q^T and O^T += V^T P^T are
+// m16n8k16 fp16 products with the keys, or the values of a head, as the 16
+// matrix rows and the query rows as the 8 columns (NT sets of 8): what the
+// cache holds is read and turned to fp16 once, and 8 query rows cost 32
+// registers of O.  fp32 rows enter as hi and lo fp16 parts (two products), so
+// that q and p keep 22 bits.  The order of a reduction index is free, so lane
+// (g, t) = (lane / 4, lane % 4) uses what it can load in one piece: of K the
+// t-th quarter of a key's row (16 bytes at head_dim 128), of V the g-th eighth
+// of two rows of each 8 keys.  A key's scale multiplies its fp16
+// numbers exactly.  P^T's fragments are S^T's turned by movmatrix.
 //
-// The softmax keeps a reference exponent per row that moves only when a unit
-// exceeds it by 2^8 (p stays below 2^8, fp16's rounding is relative, and the
-// rescaling of O is rare); l is summed per lane in fp32 and joined at the end.
+// The softmax keeps a reference per row that moves only when a unit exceeds
+// it by 2^8: p stays below 2^8 (fp16 rounds relatively), the rescaling of O is
+// rare, and otherwise no lane needs another's maximum.  l is summed per lane
+// in fp32 and joined at the end.
 //
-// Rows are copied by cp.async.bulk into each warp's own ring (no barrier
-// between warps), as far ahead as the ring is deep.
+// Rows are copied by 16-byte cp.async into each warp's own ring (no barrier
+// between warps), as far ahead as the ring is deep: nine instructions a unit,
+// where bulk copies of the four pieces cost about a hundred in addresses and
+// barrier handling.  The keys' order within 8 (kd_key) and an exchange of
+// half rows of V keep the fragment loads free of bank conflicts.
 // ---------------------------------------------------------------------------
-constexpr int KD_WARPS = 4, KD_STAGES = 4, KD_UNIT = 32;
+#ifndef KD_CTAS
+#define KD_CTAS 3
+#endif
+constexpr int KD_WARPS = 4, KD_STAGES = KD_CTAS == 3 ? 3 : 2, KD_UNIT = 32;
 
 template <int D>
 struct KdGeo {
@@ -172,14 +208,25 @@ struct KdGeo {
     static constexpr int SMEM = RING > JOIN ? RING : JOIN;
 };
 
-// What one block works on: part `chunk` of `chunks` of one sequence and
-// key/value head.  Every block finds its own from the device's lengths: units
-// of all sequences and heads are divided so that about `slots` blocks' worth
-// of equal parts results, no part below `least` units.
+// How the units of all sequences and key/value heads are divided among the
+// blocks, all of which are resident at once; each block works it out from the
+// lengths on the device.  With `per` the equal share of a block:
+//   whole parts: every head is cut into ceil(units / p) even parts, one a
+//     block, for the smallest p of per, 1.04, 1.09 and 1.15 per that leaves no
+//     more parts than blocks.  A short batch (p = `least`) is always cut the
+//     same way, whatever else it holds.
+//   runs: otherwise (many heads of very different length) the units, one head
+//     after the other, are cut into equal runs; a run may end one head and
+//     begin others.
+// A head that lies in several blocks is joined by the last to finish its part.
+struct KdPlan {
+    long total, per;                       // units, or parts with `whole`; per block with runs; units of a part else
+    bool whole;
+};
 struct KdItem {
-    int b, head, chunk, chunks, u0, u1;    // units [u0, u1) of the sequence
-    int kv, n_new, row0, lo;               // keys [lo, kv) are seen by some row
-    long first;                            // item number of the head's chunk 0
+    int b, head, kv, n_new, row0, lo;      // keys [lo, kv) are seen by some row
+    int u0, u1;                            // units [u0, u1) of the sequence are this block's
+    int chunks, slot, c0, odd;             // parts of the head; place of this one; part 0's place is 2 c0 + odd, c's 2 (c0 + c)
 };
 __device__ __forceinline__ int kd_units(const SeqInfo& q, int window, int& lo) {
     lo = 0;
@@ -187,19 +234,43 @@ __device__ __forceinline__ int kd_units(const SeqInfo& q, int window, int& lo) {
     const int first = q.kv - q.n_new - window + 1;
     if (window > 0 && first > 0) lo = first;
     const int n = (q.kv + KD_UNIT - 1) / KD_UNIT - lo / KD_UNIT;
-    return n > 0 ? n : 1;                  // no key at all: one part that writes zeros
+    return n > 0 ? n : 1;                  // no key at all: one unit without keys, whose result is zero
 }
-__device__ __forceinline__ bool kd_find(const KvaArgs& a, long item, int slots, int least, KdItem& it) {
+__device__ __forceinline__ KdPlan kd_plan(const KvaArgs& a, int least) {
     const int lane = threadIdx.x & 31;
+    int lo, n = 0;
     long total = 0;
     for (int b0 = 0; b0 < a.s.n_seqs; b0 += 32) {
-        int lo, n = 0;
+        n = 0;
         if (b0 + lane < a.s.n_seqs) n = kd_units(seq_info(a.s, a.c.page_shift, b0 + lane, a.status), a.window, lo);
         total += __reduce_add_sync(~0u, n);
     }
-    total *= a.c.heads;
-    long per = (total + slots - 1) / slots;
-    if (per < least) per = least;
+    KdPlan p{total * a.c.heads, 0, false};
+    p.per = max((p.total + gridDim.x - 1) / gridDim.x, (long)least);
+    const uint32_t per = (uint32_t)min(p.per, 1L << 30);
+    const uint32_t tried[4] = {per, per + (per + 24) / 25, per + (per + 10) / 11, per + (per + 5) / 6};
+    long parts[4] = {};
+    for (int b0 = 0; b0 < a.s.n_seqs; b0 += 32) {
+        if (a.s.n_seqs > 32) {
+            n = 0;
+            if (b0 + lane < a.s.n_seqs) n = kd_units(seq_info(a.s, a.c.page_shift, b0 + lane, nullptr), a.window, lo);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) parts[k] += __reduce_add_sync(~0u, (n + tried[k] - 1) / tried[k]);
+    }
+#pragma unroll
+    for (int k = 3; k >= 0; --k)
+        if (parts[k] * a.c.heads <= (long)gridDim.x) {
+            p.per = tried[k];
+            p.whole = true;
+            total = parts[k] * a.c.heads;
+        }
+    if (p.whole) p.total = total;
+    return p;
+}
+// The sequence and head of unit (with whole parts: part) x, and what of it lies before `end`.
+__device__ __forceinline__ void kd_find(const KvaArgs& a, const KdPlan& plan, long x, long end, KdItem& it) {
+    const int lane = threadIdx.x & 31;
     long before = 0;
     for (int b0 = 0; b0 < a.s.n_seqs; b0 += 32) {
         SeqInfo q{0, 0, 0};
@@ -208,45 +279,77 @@ __device__ __forceinline__ bool kd_find(const KvaArgs& a, long item, int slots, 
             q = seq_info(a.s, a.c.page_shift, b0 + lane, nullptr);
             n = kd_units(q, a.window, lo);
         }
-        const int chunks = (int)((n + per - 1) / per);
-        const long mine = (long)chunks * a.c.heads;
-        long sum = mine;                   // items up to and with this lane's sequence
+        const int each = plan.whole ? (int)((n + (uint32_t)plan.per - 1) / (uint32_t)plan.per) : n;
+        const long mine = (long)each * a.c.heads;
+        long sum = mine;                   // units or parts up to and with this lane's sequence
         for (int i = 1; i < 32; i <<= 1) {
             const long o = __shfl_up_sync(~0u, sum, i);
             if (lane >= i) sum += o;
         }
-        const unsigned hit = __ballot_sync(~0u, item < before + sum);
+        const unsigned hit = __ballot_sync(~0u, x < before + sum);
         if (hit) {
             const int src = __ffs(hit) - 1;
             it.b = b0 + src;
-            it.chunks = __shfl_sync(~0u, chunks, src);
             it.kv = __shfl_sync(~0u, q.kv, src);
             it.n_new = __shfl_sync(~0u, q.n_new, src);
             it.row0 = __shfl_sync(~0u, q.row0, src);
             it.lo = __shfl_sync(~0u, lo, src);
             n = __shfl_sync(~0u, n, src);
-            const long at = item - before - __shfl_sync(~0u, sum - mine, src);
-            it.head = (int)(at / it.chunks);
-            it.chunk = (int)(at - (long)it.head * it.chunks);
-            it.first = item - it.chunk;
-            const int u = it.lo / KD_UNIT;
-            it.u0 = u + (int)((long)n * it.chunk / it.chunks);
-            it.u1 = u + (int)((long)n * (it.chunk + 1) / it.chunks);
-            return true;
+            const int count = __shfl_sync(~0u, each, src);
+            const long at = x - before - __shfl_sync(~0u, sum - mine, src);
+            it.head = (int)(at / count);
+            const int off = (int)(at - (long)it.head * count), u = it.lo / KD_UNIT;
+            if (plan.whole) {
+                it.u0 = u + (int)((long)n * off / count);
+                it.u1 = u + (int)((long)n * (off + 1) / count);
+                it.chunks = count;
+                it.c0 = blockIdx.x - off;
+                it.odd = 0;
+                it.slot = 2 * blockIdx.x;
+            } else {
+                // a block has one part of a head begun before it at most, and one of a head that goes on behind it
+                const long h0 = x - off, h1 = h0 + n;
+                it.u0 = u + off;
+                it.u1 = u + (int)(min(h1, end) - h0);
+                it.c0 = (int)(h0 / plan.per);
+                it.chunks = (int)((h1 - 1) / plan.per) - it.c0 + 1;
+                it.odd = 1;
+                it.slot = 2 * blockIdx.x + (off == 0);
+            }
+            return;
         }
         before += __shfl_sync(~0u, sum, 31);
     }
-    return false;
+}
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+// Key of matrix index i within its 8: 0 5 2 7 1 4 3 6.  Neighbours (one fp16
+// pair of P^T, two rows of K) differ in parity, so that 64-byte rows fall on
+// different banks; the even and the odd four are distinct modulo 4.
+__device__ __forceinline__ int kd_key(int i) {
+    const int b = ((i & 2) | ((i >> 2) & 1));
+    return (i & 1) ? 4 + (b ^ 1) : b;
 }
 
 __device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
     uint32_t r;
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+// 8 x 8 fp16 matrix, row lane / 4, columns 2 (lane % 4), + 1: transposed.
+__device__ __forceinline__ uint32_t turn8x8(uint32_t x) {
+    uint32_t r;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
     return r;
 }
 template <int DT>
@@ -278,272 +381,330 @@ __device__ __forceinline__ float q_unit(float max, float& back) {
     return __uint_as_float((uint32_t)(254 - (e - 13)) << 23);
 }
 
-template <int D, int DT>
-__global__ void __launch_bounds__(KD_WARPS * 32, 3) kv_decode_kernel(const KvaArgs a, int slots, int least) {
+template <int D, int DT, int NT>
+__global__ void __launch_bounds__(KD_WARPS * 32, KD_CTAS) kv_decode_kernel(const KvaArgs a, int least) {
     using G = KdGeo<D>;
     constexpr bool SPLIT = DT == TK_DT_F32;
-    constexpr int ROWS = SPLIT ? 8 : 16, NR = SPLIT ? 1 : 2;       // query rows of the block, of a lane
+    constexpr int ROWS = 8 * NT, PARTS = SPLIT ? 2 : 1;            // query rows, fp16 parts of q and p
     constexpr int KW = D / 32, VW = D / 64;                        // 32-bit words of a lane's piece of a key / value row
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ uint64_t bar[KD_WARPS][KD_STAGES];
+    constexpr bool QREG = NT == 1;                                 // q's fragments stay in registers
+    __shared__ uint4 qsm[NT][PARTS][QREG ? 1 : KW][32];            // or, as the fragments of a word's two steps, here
     __shared__ int sh_last;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    KdItem it;
-    if (!kd_find(a, blockIdx.x, slots, least, it)) return;
+    const int kg = kd_key(g), k0 = kd_key(2 * t), k1 = kd_key(2 * t + 1);
+    const KdPlan plan = kd_plan(a, least);
+    long x = plan.whole ? blockIdx.x : blockIdx.x * plan.per;
+    const long end = min(x + (plan.whole ? 1 : plan.per), plan.total);
     uint8_t* ring = smem + warp * (KD_STAGES * G::STAGE);
-    if (lane == 0) {
-        for (int s = 0; s < KD_STAGES; ++s) mbar_init(&bar[warp][s], 1);
-        fence_mbar_init();
-    }
-    __syncwarp();
+
+  for (; x < end; ) {
+    KdItem it;
+    kd_find(a, plan, x, end, it);
+    x += plan.whole ? 1 : it.u1 - it.u0;
+    // ---- the warp's units: u0 + warp, + 4, ... ----
+    const int mine = it.u1 - it.u0 > warp && it.kv > 0 ? (it.u1 - it.u0 - warp + KD_WARPS - 1) / KD_WARPS : 0;
+    const int page_mask = (1 << a.c.page_shift) - 1;
+    const long head_rows = (long)it.head << a.c.page_shift, page_rows = (long)a.c.heads << a.c.page_shift;
+    const bool small = a.c.page_shift < 5;                         // 16-token pages: two a unit
+    constexpr int HALF = G::QB / 1024;                             // copies of 512 bytes in 16 rows
+    const uint8_t* kp = a.c.kq + lane * 16;
+    const uint8_t* vp = a.c.vq + lane * 16;
+    constexpr int SL = G::SB / 16;                                 // lanes that copy one plane's scales
+    const uint8_t* sp = reinterpret_cast<const uint8_t*>(lane < SL ? a.c.ks : a.c.vs) + (lane % SL) * 16;
+    const uint32_t to0 = smem_u32(ring) + lane * 16, tov = to0 ^ (D == 128 ? (lane & 8) << 2 : 0);
+    int pid = 0, pid2 = 0;
+    auto issue = [&](int i, int stage) {
+        if (i < mine) {
+            const int pos = (it.u0 + warp + i * KD_WARPS) * KD_UNIT;
+            if ((i & 31) == 0) {                                   // page ids of the next 32 units, one a lane
+                const int p = pos + lane * (KD_WARPS * KD_UNIT);
+                if (i + lane < mine) {
+                    pid = page_of(a.s, a.c, it.b, p, a.status);
+                    if (small && p + 16 < it.kv) pid2 = page_of(a.s, a.c, it.b, p + 16, a.status);
+                }
+            }
+            long row = __shfl_sync(~0u, pid, i & 31) * page_rows + head_rows + (pos & page_mask), row2 = row + 16;
+            const int last = it.kv - pos > 16 ? 32 : 16;           // whole 16-row pieces: inside the page
+            if (small) row2 = __shfl_sync(~0u, pid2, i & 31) * page_rows + head_rows;
+            const uint32_t st = stage * G::STAGE;
+#pragma unroll
+            for (int c = 0; c < HALF; ++c) {
+                cp_async16(to0 + st + c * 512, kp + row * (D / 2) + c * 512);
+                cp_async16(tov + st + G::QB + c * 512, vp + row * (D / 2) + c * 512);
+            }
+            if (last == 32)
+#pragma unroll
+                for (int c = 0; c < HALF; ++c) {
+                    cp_async16(to0 + st + (HALF + c) * 512, kp + row2 * (D / 2) + c * 512);
+                    cp_async16(tov + st + G::QB + (HALF + c) * 512, vp + row2 * (D / 2) + c * 512);
+                }
+            const bool second = (lane % SL) * 16 >= 16 * (D / 16);
+            if (lane < 2 * SL && (!second || last == 32))
+                cp_async16(to0 + st + 2 * G::QB, sp + (second && small ? row2 - 16 : row) * (D / 16));
+        }
+        cp_async_commit();
+    };
+    for (int i = 0; i < KD_STAGES - 1; ++i) issue(i, i);
 
     // ---- rows: row r of the block is token r / group, head r % group ----
     const int rows = it.n_new * a.group, pos0 = it.kv - it.n_new;
-    uint32_t qf[2 * KW][4];
-    float sc[NR];
-    int limit[NR], from[NR];                                       // keys [from, limit) are seen
-    {
-        float x[NR][KW][8];
+    // lane (g, t) loads the t-th quarter of row g and keeps the statistics of rows 2 t and 2 t + 1
+    uint4 qr[PARTS][KW];
+    float sc[NT][2];
+    int limit[NT][2], from[NT][2];                                 // keys [from, limit) are seen
 #pragma unroll
-        for (int i = 0; i < NR; ++i) {
-            const int r = g + 8 * i;
-            float mx = 0.0f;
-            limit[i] = from[i] = 0;
-            if (r < rows) {
-                const int tok = r / a.group;
-                limit[i] = pos0 + tok + 1;
-                from[i] = a.window > 0 ? limit[i] - a.window : 0;
-                const size_t at = (size_t)(it.row0 + tok) * a.ldq + (size_t)(it.head * a.group + r % a.group) * D + t * (D / 4);
+    for (int n = 0; n < NT; ++n) {
+        const int r = g + 8 * n;
+        float x[KW][8], mx = 0.0f;
+        int lim = INT32_MAX;
+        if (r < rows) {
+            const int tok = r / a.group;
+            lim = max(pos0 + tok + 1, 0);
+            const size_t at = (size_t)(it.row0 + tok) * a.ldq + (size_t)(it.head * a.group + r % a.group) * D + t * (D / 4);
 #pragma unroll
-                for (int w = 0; w < KW; ++w) {
-                    load_pairs8<DT>(a.q, at + w * 8, x[i][w]);
+            for (int w = 0; w < KW; ++w) {
+                load_pairs8<DT>(a.q, at + w * 8, x[w]);
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(x[i][w][e]));
-                }
-            } else {
-#pragma unroll
-                for (int w = 0; w < KW; ++w)
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) x[i][w][e] = 0.0f;
+                for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(x[w][e]));
             }
-            mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 1));
-            mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 2));
-            float back;
-            const float up = copysignf(q_unit(mx, back), a.scale2);
-            sc[i] = back * fabsf(a.scale2);
+        } else {
 #pragma unroll
             for (int w = 0; w < KW; ++w)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) x[i][w][e] *= up;
+                for (int e = 0; e < 8; ++e) x[w][e] = 0.0f;
+        }
+        mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 2));
+        float back;
+        const float up = copysignf(q_unit(mx, back), a.scale2);
+        back *= fabsf(a.scale2);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            sc[n][c] = __shfl_sync(~0u, back, 4 * (2 * t + c));
+            limit[n][c] = __shfl_sync(~0u, lim, 4 * (2 * t + c));
+            from[n][c] = a.window > 0 && limit[n][c] != INT32_MAX ? max(limit[n][c] - a.window, 0) : 0;
         }
 #pragma unroll
-        for (int w = 0; w < KW; ++w)
+        for (int w = 0; w < KW; ++w) {
+            if (!QREG && warp != w % KD_WARPS) continue;           // each warp lays out its share
+            uint32_t hi[4], lo[4];
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
+            for (int p = 0; p < 4; ++p) {
+                const float u = x[w][2 * p] * up, v = x[w][2 * p + 1] * up;
+                hi[p] = pack_half2(u, v);
+                const __half2 hh = as_half2(hi[p]);
+                lo[p] = pack_half2(u - __low2float(hh), v - __high2float(hh));
+            }
+            uint4& to = QREG ? qr[0][w] : qsm[n][0][QREG ? 0 : w][lane];
+            to = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+            if constexpr (SPLIT) {
+                uint4& to2 = QREG ? qr[PARTS - 1][w] : qsm[n][PARTS - 1][QREG ? 0 : w][lane];
+                to2 = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+            }
+        }
+    }
+    if constexpr (!QREG) __syncthreads();
+
+    float o[NT][D / 16][4], nm[NT][2], l[NT][2];                   // nm: minus the reference, +inf before the first
 #pragma unroll
-                for (int p = 0; p < 2; ++p) {
-                    const int e = 4 * h + 2 * p;
-                    const uint32_t hi = pack_half2(x[0][w][e], x[0][w][e + 1]);
-                    qf[2 * w + h][2 * p] = hi;
-                    if constexpr (SPLIT) {
-                        const __half2 hh = as_half2(hi);
-                        qf[2 * w + h][2 * p + 1] = pack_half2(x[0][w][e] - __low2float(hh), x[0][w][e + 1] - __high2float(hh));
-                    } else {
-                        qf[2 * w + h][2 * p + 1] = pack_half2(x[1][w][e], x[1][w][e + 1]);
-                    }
-                }
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.0f;
+        nm[n][0] = nm[n][1] = INFINITY;
+        l[n][0] = l[n][1] = 0.0f;
     }
 
-    float o[D / 8][4], m[NR], l[NR];
-#pragma unroll
-    for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
-#pragma unroll
-    for (int i = 0; i < NR; ++i) { m[i] = -INFINITY; l[i] = 0.0f; }
-
-    // ---- the warp's units: u0 + warp, + 4, ... ----
-    const int mine = it.u1 - it.u0 > warp && it.kv > 0 ? (it.u1 - it.u0 - warp + KD_WARPS - 1) / KD_WARPS : 0;
-    const size_t page_rows = (size_t)1 << a.c.page_shift;
-    const int ppu = a.c.page_shift < 5 ? 2 : 1;                    // pages per unit (16-token pages: two)
-    const int run = KD_UNIT / ppu;
-    int pid[2] = {0, 0};
-    auto issue = [&](int i) {                                      // whole warp; lane 0 copies
-        if (i >= mine) return;
-        const int u = it.u0 + warp + i * KD_WARPS, stage = i % KD_STAGES;
-        if ((i & 31) == 0) {                                       // page ids of the next 32 units, one a lane
-            const int pos = (it.u0 + warp + (i + lane) * KD_WARPS) * KD_UNIT;
-#pragma unroll
-            for (int p = 0; p < 2; ++p)
-                if (p < ppu && pos + p * run < it.kv) pid[p] = page_of(a.s, a.c, it.b, pos + p * run, a.status);
-        }
-        const int id0 = __shfl_sync(~0u, pid[0], i & 31), id1 = __shfl_sync(~0u, pid[1], i & 31);
-        if (lane == 0) {
-            const int pos = u * KD_UNIT, n = ppu == 2 && pos + run < it.kv ? 2 : 1;
-            uint8_t* dst = ring + stage * G::STAGE;
-            mbar_arrive_expect_tx(&bar[warp][stage], (uint32_t)(n * run * (D + D / 8)));
-            for (int p = 0; p < n; ++p) {
-                const size_t row = ((size_t)(p ? id1 : id0) * a.c.heads + it.head) * page_rows + ((pos + p * run) & (page_rows - 1));
-                const int at = p * run;
-                bulk_load(dst + at * (D / 2), a.c.kq + row * (D / 2), run * (D / 2), &bar[warp][stage]);
-                bulk_load(dst + G::QB + at * (D / 2), a.c.vq + row * (D / 2), run * (D / 2), &bar[warp][stage]);
-                bulk_load(dst + 2 * G::QB + at * (D / 16), a.c.ks + row * (D / 32), run * (D / 16), &bar[warp][stage]);
-                bulk_load(dst + 2 * G::QB + G::SB + at * (D / 16), a.c.vs + row * (D / 32), run * (D / 16), &bar[warp][stage]);
-            }
-        }
-    };
-    for (int i = 0; i < KD_STAGES - 1; ++i) issue(i);
-
+    int stage = 0;
     for (int i = 0; i < mine; ++i) {
-        issue(i + KD_STAGES - 1);
-        const int stage = i % KD_STAGES, key0 = (it.u0 + warp + i * KD_WARPS) * KD_UNIT;
-        if (!__all_sync(~0u, mbar_wait(&bar[warp][stage], (i / KD_STAGES) & 1, a.status))) {
-            for (int k = i + 1; k < min(i + KD_STAGES, mine); ++k)  // reported; the copies in flight end first
-                mbar_wait(&bar[warp][k % KD_STAGES], (k / KD_STAGES) & 1, a.status);
-            break;
-        }
+        issue(i + KD_STAGES - 1, stage == 0 ? KD_STAGES - 1 : stage - 1);
+        cp_async_wait<KD_STAGES - 1>();
+        __syncwarp();
+        const int key0 = (it.u0 + warp + i * KD_WARPS) * KD_UNIT;
         const uint8_t* kq = ring + stage * G::STAGE;
         const uint8_t* vq = kq + G::QB;
-        const __half* ks = reinterpret_cast<const __half*>(kq + 2 * G::QB);
-        const __half* vs = reinterpret_cast<const __half*>(kq + 2 * G::QB + G::SB);
-
-        // S: matrix column n of tile j is key 8 j + (n >> 1) + 4 (n & 1), so
-        // that lane t's two columns are keys t and t + 4 of the 8
-        float s[4][4];
+        __half* ks = reinterpret_cast<__half*>(ring + stage * G::STAGE + 2 * G::QB);
+        __half* vs = ks + G::SB / 2;
+        const bool edge = key0 + 32 > pos0 + 1 || key0 < it.lo + it.n_new;
+        if (edge) {     // a row that nothing sees may hold any scale
+            const int key = key0 + lane;
+            if (key >= it.kv || key < it.lo)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.0f;
-            const int key = 8 * j + (g >> 1) + 4 * (g & 1);
-            uint32_t w[KW];
-            if constexpr (KW == 4) {
-                const uint4 u = *reinterpret_cast<const uint4*>(kq + key * (D / 2) + t * 16);
-                w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
-            } else {
-                const uint2 u = *reinterpret_cast<const uint2*>(kq + key * (D / 2) + t * 8);
-                w[0] = u.x; w[1] = u.y;
+                for (int e = 0; e < D / 32; ++e) ks[lane * (D / 32) + e] = vs[lane * (D / 32) + e] = __ushort_as_half(0);
+            __syncwarp();
+        }
+
+        // S^T: matrix row r of an 8-row half is key kd_key(r) of its 8
+        float s[NT][2][4];
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) {
+            uint32_t w[2][KW];
+            __half2 d[2];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int key = 16 * kt + 8 * j + kg;
+                if constexpr (KW == 4) {
+                    const uint4 u = *reinterpret_cast<const uint4*>(kq + key * (D / 2) + t * 16);
+                    w[j][0] = u.x; w[j][1] = u.y; w[j][2] = u.z; w[j][3] = u.w;
+                } else {
+                    const uint2 u = *reinterpret_cast<const uint2*>(kq + key * (D / 2) + t * 8);
+                    w[j][0] = u.x; w[j][1] = u.y;
+                }
+                d[j] = __half2half2(ks[key * (D / 32) + (t * D / 128)]);
             }
-            const __half2 d = __half2half2(ks[key * (D / 32) + (t * D / 128)]);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) s[n][kt][0] = s[n][kt][1] = s[n][kt][2] = s[n][kt][3] = 0.0f;
 #pragma unroll
             for (int i2 = 0; i2 < KW; ++i2) {
-                uint32_t b[4];
-                kv_fields(w[i2], d, b);
-                mma_16816(s[j], qf[2 * i2], b[0], b[1]);
-                mma_16816(s[j], qf[2 * i2 + 1], b[2], b[3]);
+                uint32_t fa[4], fb[4];
+                kv_fields(w[0][i2], d[0], fa);
+                kv_fields(w[1][i2], d[1], fb);
+                const uint32_t a0[4] = {fa[0], fb[0], fa[1], fb[1]}, a1[4] = {fa[2], fb[2], fa[3], fb[3]};
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int p = PARTS - 1; p >= 0; --p) {         // low parts first
+                        const uint4 q = QREG ? qr[p][i2] : qsm[n][p][QREG ? 0 : i2][lane];
+                        mma_16816(s[n][kt], a0, q.x, q.y);
+                        mma_16816(s[n][kt], a1, q.z, q.w);
+                    }
             }
         }
-        const bool edge = key0 + KD_UNIT > pos0 + 1 || key0 < it.lo + it.n_new;
-        float p[NR][8];
-        float top[NR];
+        // exponents: value j of a row is key 8 j + kd_key(g)
+        const int at = key0 + kg;
+        float v[NT][2][4];
+        auto exponents = [&]() {
 #pragma unroll
-        for (int r = 0; r < NR; ++r) {
-            top[r] = -INFINITY;
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                float v = SPLIT ? s[j >> 1][j & 1] + s[j >> 1][2 + (j & 1)] : s[j >> 1][2 * r + (j & 1)];
-                v *= sc[r];
-                if (edge) {
-                    const int key = key0 + 8 * (j >> 1) + t + 4 * (j & 1);
-                    if (key >= limit[r] || key < from[r]) v = -INFINITY;
+                for (int c = 0; c < 2; ++c)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) v[n][c][j] = fmaf(s[n][j >> 1][2 * (j & 1) + c], sc[n][c], nm[n][c]);
+            if (edge) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        const unsigned width = limit[n][c] - from[n][c];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            if ((unsigned)(at + 8 * j - from[n][c]) >= width) v[n][c][j] = -INFINITY;
+                    }
+            }
+        };
+        exponents();
+        float top = -INFINITY;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) top = fmaxf(top, v[n][c][j]);
+        if (__any_sync(~0u, top > 8.0f)) {                         // a row's reference moves
+            float old[NT][2];
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) { old[n][c] = nm[n][c]; nm[n][c] = 0.0f; }
+            exponents();
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    float mx = fmaxf(fmaxf(v[n][c][0], v[n][c][1]), fmaxf(v[n][c][2], v[n][c][3]));
+#pragma unroll
+                    for (int i2 = 4; i2 < 32; i2 <<= 1) mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, i2));
+                    const float now = fminf(old[n][c], -mx), f = now == INFINITY ? 1.0f : fast_exp2(now - old[n][c]);
+                    nm[n][c] = now;
+                    l[n][c] *= f;
+#pragma unroll
+                    for (int i2 = 0; i2 < D / 16; ++i2) {
+                        o[n][i2][c] *= f;
+                        o[n][i2][2 + c] *= f;
+                    }
                 }
-                p[r][j] = v;
-                top[r] = fmaxf(top[r], v);
-            }
-            top[r] = fmaxf(top[r], __shfl_xor_sync(~0u, top[r], 1));
-            top[r] = fmaxf(top[r], __shfl_xor_sync(~0u, top[r], 2));
+            exponents();
+#pragma unroll
+            for (int n = 0; n < NT; ++n)                           // a row that has seen nothing yet: no weight
+#pragma unroll
+                for (int c = 0; c < 2; ++c)
+                    if (nm[n][c] == INFINITY)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) v[n][c][j] = v[n][c][j] != v[n][c][j] ? v[n][c][j] : -INFINITY;
         }
-        bool move = top[0] > m[0] + 8.0f;
-        if constexpr (NR == 2) move |= top[1] > m[1] + 8.0f;
-        if (__any_sync(~0u, move)) {
-            float f[NR];
+        uint32_t pb[NT][PARTS][4];                                 // P^T fragments of the four 8-key groups
 #pragma unroll
-            for (int r = 0; r < NR; ++r) {
-                const float mn = fmaxf(m[r], top[r]);
-                f[r] = mn == -INFINITY ? 1.0f : fast_exp2(m[r] - mn);
-                m[r] = mn;
-                l[r] *= f[r];
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float p0 = fast_exp2(v[n][0][j]), p1 = fast_exp2(v[n][1][j]);
+                l[n][0] += p0;
+                l[n][1] += p1;
+                const uint32_t hi = pack_half2(p0, p1);
+                pb[n][0][j] = turn8x8(hi);
+                if constexpr (SPLIT) {
+                    const __half2 hh = as_half2(hi);
+                    pb[n][PARTS - 1][j] = turn8x8(pack_half2(p0 - __low2float(hh), p1 - __high2float(hh)));
+                }
             }
-#pragma unroll
-            for (int i2 = 0; i2 < D / 8; ++i2) {
-                o[i2][0] *= f[0]; o[i2][1] *= f[0];
-                o[i2][2] *= f[NR - 1]; o[i2][3] *= f[NR - 1];
-            }
-        }
-        uint32_t pa[2][4];
-#pragma unroll
-        for (int r = 0; r < NR; ++r) {
-            const float ref = m[r] == -INFINITY ? 0.0f : m[r];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                p[r][j] = fast_exp2(p[r][j] - ref);
-                l[r] += p[r][j];
-            }
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const uint32_t hi = pack_half2(p[0][2 * j], p[0][2 * j + 1]);
-            pa[j >> 1][2 * (j & 1)] = hi;
-            if constexpr (SPLIT) {
-                const __half2 hh = as_half2(hi);
-                pa[j >> 1][2 * (j & 1) + 1] = pack_half2(p[0][2 * j] - __low2float(hh), p[0][2 * j + 1] - __high2float(hh));
-            } else {
-                pa[j >> 1][2 * (j & 1) + 1] = pack_half2(p[1][2 * j], p[1][2 * j + 1]);
-            }
-        }
-        // O: matrix column n of tile e' is value (D / 8) n + e' of the head
+        // O^T: matrix rows g and g + 8 of tile i are values (D / 8) g + 2 i and + 1 of the head
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            uint32_t w[4][VW];                                     // keys 16 h + t, + 4, + 8, + 12
+            uint32_t w[4][VW];                                     // the two keys of lane t, of both 8-key groups
             __half d[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const int key = 16 * h + 4 * j + t;
+                const int key = 16 * h + 8 * (j >> 1) + (j & 1 ? k1 : k0);
                 if constexpr (VW == 2) {
-                    const uint2 u = *reinterpret_cast<const uint2*>(vq + key * (D / 2) + g * 8);
+                    const uint2 u = *reinterpret_cast<const uint2*>(vq + key * (D / 2) + ((g * 8) ^ ((k0 & 2) << 4)));
                     w[j][0] = u.x; w[j][1] = u.y;
                 } else {
                     w[j][0] = *reinterpret_cast<const uint32_t*>(vq + key * (D / 2) + g * 4);
                 }
                 d[j] = vs[key * (D / 32) + (g * D / 256)];
-                // a row that nothing sees may hold any scale
-                if (edge && (key0 + key >= it.kv || key0 + key < it.lo)) d[j] = __ushort_as_half(0);
             }
             const __half2 d0 = __halves2half2(d[0], d[1]), d1 = __halves2half2(d[2], d[3]);
 #pragma unroll
-            for (int i2 = 0; i2 < VW; ++i2)
+            for (int i2 = 0; i2 < VW; ++i2) {
+                uint32_t f0[4], f1[4], f2[4], f3[4];               // fields 0..3: values 0 2 4 6; 4..7: 1 3 5 7
+                kv_fields(__byte_perm(w[0][i2], w[1][i2], 0x5410u), d0, f0);
+                kv_fields(__byte_perm(w[0][i2], w[1][i2], 0x7632u), d0, f1);
+                kv_fields(__byte_perm(w[2][i2], w[3][i2], 0x5410u), d1, f2);
+                kv_fields(__byte_perm(w[2][i2], w[3][i2], 0x7632u), d1, f3);
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {             // fields 0..3: values 0 2 4 6; 4..7: 1 3 5 7
-                    uint32_t b0[4], b1[4];
-                    const uint32_t sel = half ? 0x7632u : 0x5410u;
-                    kv_fields(__byte_perm(w[0][i2], w[1][i2], sel), d0, b0);
-                    kv_fields(__byte_perm(w[2][i2], w[3][i2], sel), d1, b1);
+                for (int f = 0; f < 4; ++f) {
+                    const uint32_t av[4] = {f0[f], f1[f], f2[f], f3[f]};
 #pragma unroll
-                    for (int f = 0; f < 4; ++f) mma_16816(o[8 * i2 + 2 * f + half], pa[h], b0[f], b1[f]);
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int p = PARTS - 1; p >= 0; --p)
+                            mma_16816(o[n][4 * i2 + f], av, pb[n][p][2 * h], pb[n][p][2 * h + 1]);
                 }
+            }
         }
         __syncwarp();                                              // the stage may be overwritten
+        if (++stage == KD_STAGES) stage = 0;
     }
 
     // ---- join the warps: lane sums, then O in the ring's memory ----
-#pragma unroll
-    for (int r = 0; r < NR; ++r) {
-        l[r] += __shfl_xor_sync(~0u, l[r], 1);
-        l[r] += __shfl_xor_sync(~0u, l[r], 2);
-    }
     __syncthreads();                                               // every warp is done with its ring
     constexpr int OLD = D + 4;
     float* osh = reinterpret_cast<float*>(smem);
-    float* msh = osh + KD_WARPS * 16 * OLD;
+    float* msh = osh + KD_WARPS * ROWS * OLD;
 #pragma unroll
-    for (int r = 0; r < NR; ++r) {
-        float* to = osh + (warp * 16 + g + 8 * r) * OLD;
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int e = 0; e < D / 8; ++e)
+        for (int c = 0; c < 2; ++c) {
+            for (int i = 4; i < 32; i <<= 1) l[n][c] += __shfl_xor_sync(~0u, l[n][c], i);
+            const int r = warp * ROWS + 8 * n + 2 * t + c;
 #pragma unroll
-            for (int c = 0; c < 2; ++c)
-                to[(2 * t + c) * (D / 8) + e] = SPLIT ? o[e][c] + o[e][2 + c] : o[e][2 * r + c];
-        if (t == 0) {
-            msh[(warp * 16 + g + 8 * r) * 2] = m[r];
-            msh[(warp * 16 + g + 8 * r) * 2 + 1] = l[r];
+            for (int i = 0; i < D / 16; ++i)
+                *reinterpret_cast<float2*>(osh + r * OLD + (D / 8) * g + 2 * i) = make_float2(o[n][i][c], o[n][i][2 + c]);
+            if (g == 0) {
+                msh[r * 2] = -nm[n][c];
+                msh[r * 2 + 1] = l[n][c];
+            }
         }
-    }
     __syncthreads();
     const bool whole = it.chunks == 1;
     const int live = min(rows, ROWS);
@@ -551,20 +712,20 @@ __global__ void __launch_bounds__(KD_WARPS * 32, 3) kv_decode_kernel(const KvaAr
         const int r = i / (D / 4), e = (i - r * (D / 4)) * 4;
         float mm = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < KD_WARPS; ++w) mm = fmaxf(mm, msh[(w * 16 + r) * 2]);
+        for (int w = 0; w < KD_WARPS; ++w) mm = fmaxf(mm, msh[(w * ROWS + r) * 2]);
         const float ref = mm == -INFINITY ? 0.0f : mm;
         float ll = 0.0f;
         float4 acc = make_float4(0, 0, 0, 0);
 #pragma unroll
         for (int w = 0; w < KD_WARPS; ++w) {
-            const float f = fast_exp2(msh[(w * 16 + r) * 2] - ref);
-            const float4 v = *reinterpret_cast<const float4*>(osh + (w * 16 + r) * OLD + e);
-            ll += msh[(w * 16 + r) * 2 + 1] * f;
+            const float f = fast_exp2(msh[(w * ROWS + r) * 2] - ref);
+            const float4 v = *reinterpret_cast<const float4*>(osh + (w * ROWS + r) * OLD + e);
+            ll += msh[(w * ROWS + r) * 2 + 1] * f;
             acc.x += v.x * f; acc.y += v.y * f; acc.z += v.z * f; acc.w += v.w * f;
         }
         if (whole) kv_store_out<DT, D>(a, it, r, e, acc, ll);
         else {
-            float* part = a.part + (size_t)blockIdx.x * (16 * (D + 2));
+            float* part = a.part + (size_t)it.slot * (16 * (D + 2));
             *reinterpret_cast<float4*>(part + r * D + e) = acc;
             if (e == 0) {
                 part[16 * D + 2 * r] = mm;
@@ -572,8 +733,9 @@ __global__ void __launch_bounds__(KD_WARPS * 32, 3) kv_decode_kernel(const KvaAr
             }
         }
     }
-    if (whole) return;
-    kv_join_last<D, DT>(a, it, live, &sh_last);
+    if (!whole) kv_join_last<D, DT>(a, it, live, smem, &sh_last);
+    __syncthreads();
+  }
 }
 
 template <int D>
@@ -600,32 +762,34 @@ static tk_status count_ensure(tk_ctx* ctx, size_t n) {
     return TK_OK;
 }
 
-template <int D, int DT>
-static tk_status go_decode_t(tk_ctx* ctx, const KvaArgs& a, unsigned grid, int slots, int least, cudaStream_t st) {
+template <int D, int DT, int NT>
+static tk_status go_decode_t(tk_ctx* ctx, const KvaArgs& a, unsigned grid, int least, cudaStream_t st) {
     static std::atomic<uint64_t> attr_done{0};
-    auto kern = kv_decode_kernel<D, DT>;
+    auto kern = kv_decode_kernel<D, DT, NT>;
     cudaError_t e = smem_attr_once(kern, KdGeo<D>::SMEM, ctx->device, attr_done);
     if (e != cudaSuccess) return cuda_fail(e, "kv decode smem attribute");
     ProfScope ps(ctx, st, PK_SERVE);
-    kern<<<grid, KD_WARPS * 32, KdGeo<D>::SMEM, st>>>(a, slots, least);
+    kern<<<grid, KD_WARPS * 32, KdGeo<D>::SMEM, st>>>(a, least);
     ctx->launches++;
     return cuda_fail(cudaGetLastError(), "kv decode launch");
 }
 
 template <int D>
 static tk_status go_decode(tk_ctx* ctx, KvaArgs& a, int dtype, cudaStream_t st) {
-    const long pairs = (long)a.s.n_seqs * a.c.heads;
-    const int slots = 3 * ctx->num_sms, least = KD_WARPS;
-    const long grid = slots + pairs;      // no division has more parts: sum of ceil(units / per) < total / per + pairs
-    if (grid > INT32_MAX) return fail(TK_ERR_INVALID, "tk_kv_attend: too many sequences");
-    tk_status r = ws_ensure(ctx, (size_t)grid * (16 * (D + 2)) * sizeof(float), st);
-    if (r == TK_OK) r = count_ensure(ctx, (size_t)pairs);
+    const size_t pairs = (size_t)a.s.n_seqs * a.c.heads;
+    const unsigned grid = KD_CTAS * ctx->num_sms;   // what is resident at once
+    const int least = KD_WARPS;               // a unit for every warp
+    tk_status r = ws_ensure(ctx, (size_t)grid * 2 * (16 * (D + 2)) * sizeof(float), st);
+    if (r == TK_OK) r = count_ensure(ctx, pairs);
     if (r != TK_OK) return r;
     a.part = static_cast<float*>(ctx->ws);
     a.count = ctx->kv_count;
-    if (dtype == TK_DT_F32) return go_decode_t<D, TK_DT_F32>(ctx, a, (unsigned)grid, slots, least, st);
-    if (dtype == TK_DT_F16) return go_decode_t<D, TK_DT_F16>(ctx, a, (unsigned)grid, slots, least, st);
-    return go_decode_t<D, TK_DT_BF16>(ctx, a, (unsigned)grid, slots, least, st);
+    const bool two = (long)a.s.max_new * a.group > 8;
+    if (dtype == TK_DT_F32)
+        return two ? go_decode_t<D, TK_DT_F32, 2>(ctx, a, grid, least, st) : go_decode_t<D, TK_DT_F32, 1>(ctx, a, grid, least, st);
+    if (dtype == TK_DT_F16)
+        return two ? go_decode_t<D, TK_DT_F16, 2>(ctx, a, grid, least, st) : go_decode_t<D, TK_DT_F16, 1>(ctx, a, grid, least, st);
+    return two ? go_decode_t<D, TK_DT_BF16, 2>(ctx, a, grid, least, st) : go_decode_t<D, TK_DT_BF16, 1>(ctx, a, grid, least, st);
 }
 
 tk_status launch_kv_attend(tk_ctx* ctx, const tk_kvcache& c, const tk_seqs& s, const void* q, int dtype, long ldq,
@@ -642,7 +806,7 @@ tk_status launch_kv_attend(tk_ctx* ctx, const tk_kvcache& c, const tk_seqs& s, c
     a.status = ctx->status;
     const long grid = ((long)s.n_tokens * n_heads + 3) / 4;
     if (grid > INT32_MAX) return fail(TK_ERR_INVALID, "tk_kv_attend: too many rows");
-    if ((long)s.max_new * a.group <= (dtype == TK_DT_F32 ? 8 : 16))
+    if ((long)s.max_new * a.group <= 16)
         return c.head_dim == 64 ? go_decode<64>(ctx, a, dtype, st) : go_decode<128>(ctx, a, dtype, st);
     ProfScope ps(ctx, st, PK_SERVE);
     if (c.head_dim == 64) go_rows<64>(a, dtype, (unsigned)grid, st);
