@@ -153,16 +153,17 @@ __device__ __forceinline__ void kv_join_last(const KvaArgs& a, const Item& it, i
     __syncthreads();
     for (int i = threadIdx.x; i < live * (D / 4); i += blockDim.x) {
         const int r = i / (D / 4), e = (i - r * (D / 4)) * 4;
-        const float* first = part_of(0) + r * D + e;
-        const float* rest = a.part + (size_t)2 * it.c0 * P + r * D + e;
-        float4 o = __ldcg(reinterpret_cast<const float4*>(first));
-        const float f0 = fac[r];
-        o.x *= f0; o.y *= f0; o.z *= f0; o.w *= f0;
-#pragma unroll 16
-        for (int c = 1; c < it.chunks; ++c) {
-            const float f = fac[c * live + r];
-            const float4 v = __ldcg(reinterpret_cast<const float4*>(rest + (size_t)c * (2 * P)));
-            o.x += v.x * f; o.y += v.y * f; o.z += v.z * f; o.w += v.w * f;
+        float4 o = make_float4(0, 0, 0, 0);
+        for (int c0 = 0; c0 < it.chunks; c0 += 16) {               // 16 loads in flight, whatever is left of them
+            float4 v[16];
+#pragma unroll
+            for (int c = 0; c < 16; ++c)
+                v[c] = __ldcg(reinterpret_cast<const float4*>(part_of(min(c0 + c, it.chunks - 1)) + r * D + e));
+#pragma unroll
+            for (int c = 0; c < 16; ++c) {
+                const float f = c0 + c < it.chunks ? fac[(c0 + c) * live + r] : 0.0f;
+                o.x += v[c].x * f; o.y += v[c].y * f; o.z += v[c].z * f; o.w += v[c].w * f;
+            }
         }
         kv_store_out<DT, D>(a, it, r, e, o, sum[r]);
     }
@@ -219,73 +220,74 @@ struct KdGeo {
 //     after the other, are cut into equal runs; a run may end one head and
 //     begin others.
 // A head that lies in several blocks is joined by the last to finish its part.
+struct KdSeq {
+    int kv, n_new, row0, lo, units;        // keys [lo, kv) are seen by some row
+};
 struct KdPlan {
-    long total, per;                       // units, or parts with `whole`; per block with runs; units of a part else
+    uint32_t total, per;                   // units, or parts with `whole`; per block with runs; units of a part else
     bool whole;
+    KdSeq mine;                            // lane's sequence, if there are at most 32
 };
 struct KdItem {
-    int b, head, kv, n_new, row0, lo;      // keys [lo, kv) are seen by some row
+    int b, head, kv, n_new, row0, lo;
     int u0, u1;                            // units [u0, u1) of the sequence are this block's
     int chunks, slot, c0, odd;             // parts of the head; place of this one; part 0's place is 2 c0 + odd, c's 2 (c0 + c)
 };
-__device__ __forceinline__ int kd_units(const SeqInfo& q, int window, int& lo) {
-    lo = 0;
-    if (q.n_new == 0) return 0;
-    const int first = q.kv - q.n_new - window + 1;
-    if (window > 0 && first > 0) lo = first;
-    const int n = (q.kv + KD_UNIT - 1) / KD_UNIT - lo / KD_UNIT;
-    return n > 0 ? n : 1;                  // no key at all: one unit without keys, whose result is zero
+__device__ __forceinline__ KdSeq kd_seq(const KvaArgs& a, int b, int* status) {
+    KdSeq s{0, 0, 0, 0, 0};
+    if (b >= a.s.n_seqs) return s;
+    const SeqInfo q = seq_info(a.s, a.c.page_shift, b, status);
+    if (q.n_new == 0) return s;
+    s.kv = q.kv; s.n_new = q.n_new; s.row0 = q.row0;
+    const int first = q.kv - q.n_new - a.window + 1;
+    if (a.window > 0 && first > 0) s.lo = first;
+    // no key at all: one unit without keys, whose result is zero
+    s.units = max((q.kv + KD_UNIT - 1) / KD_UNIT - s.lo / KD_UNIT, 1);
+    return s;
 }
-__device__ __forceinline__ KdPlan kd_plan(const KvaArgs& a, int least) {
+// (the host bounds all units by 2^31)
+__device__ __forceinline__ KdPlan kd_plan(const KvaArgs& a, uint32_t least) {
     const int lane = threadIdx.x & 31;
-    int lo, n = 0;
-    long total = 0;
+    KdPlan p;
+    uint32_t total = 0;
     for (int b0 = 0; b0 < a.s.n_seqs; b0 += 32) {
-        n = 0;
-        if (b0 + lane < a.s.n_seqs) n = kd_units(seq_info(a.s, a.c.page_shift, b0 + lane, a.status), a.window, lo);
-        total += __reduce_add_sync(~0u, n);
+        p.mine = kd_seq(a, b0 + lane, a.status);
+        total += __reduce_add_sync(~0u, p.mine.units);
     }
-    KdPlan p{total * a.c.heads, 0, false};
-    p.per = max((p.total + gridDim.x - 1) / gridDim.x, (long)least);
-    const uint32_t per = (uint32_t)min(p.per, 1L << 30);
-    const uint32_t tried[4] = {per, per + (per + 24) / 25, per + (per + 10) / 11, per + (per + 5) / 6};
-    long parts[4] = {};
-    for (int b0 = 0; b0 < a.s.n_seqs; b0 += 32) {
-        if (a.s.n_seqs > 32) {
-            n = 0;
-            if (b0 + lane < a.s.n_seqs) n = kd_units(seq_info(a.s, a.c.page_shift, b0 + lane, nullptr), a.window, lo);
+    p.total = total * a.c.heads;
+    p.whole = false;
+    p.per = max((p.total + gridDim.x - 1) / gridDim.x, least);
+    const uint32_t room = gridDim.x / a.c.heads;                   // parts that a head may have, over all sequences
+    uint32_t tried[4] = {p.per, p.per + (p.per + 24) / 25, p.per + (p.per + 10) / 11, p.per + (p.per + 5) / 6};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        uint32_t parts = 0;
+        for (int b0 = 0; b0 < a.s.n_seqs; b0 += 32) {
+            const int n = a.s.n_seqs > 32 ? kd_seq(a, b0 + lane, nullptr).units : p.mine.units;
+            parts += __reduce_add_sync(~0u, (n + tried[k] - 1) / tried[k]);
         }
-#pragma unroll
-        for (int k = 0; k < 4; ++k) parts[k] += __reduce_add_sync(~0u, (n + tried[k] - 1) / tried[k]);
-    }
-#pragma unroll
-    for (int k = 3; k >= 0; --k)
-        if (parts[k] * a.c.heads <= (long)gridDim.x) {
+        if (parts <= room) {
             p.per = tried[k];
             p.whole = true;
-            total = parts[k] * a.c.heads;
+            p.total = parts * a.c.heads;
+            break;
         }
-    if (p.whole) p.total = total;
+    }
     return p;
 }
 // The sequence and head of unit (with whole parts: part) x, and what of it lies before `end`.
-__device__ __forceinline__ void kd_find(const KvaArgs& a, const KdPlan& plan, long x, long end, KdItem& it) {
+__device__ __forceinline__ void kd_find(const KvaArgs& a, const KdPlan& plan, uint32_t x, uint32_t end, KdItem& it) {
     const int lane = threadIdx.x & 31;
-    long before = 0;
+    uint32_t before = 0;
     for (int b0 = 0; b0 < a.s.n_seqs; b0 += 32) {
-        SeqInfo q{0, 0, 0};
-        int lo = 0, n = 0;
-        if (b0 + lane < a.s.n_seqs) {
-            q = seq_info(a.s, a.c.page_shift, b0 + lane, nullptr);
-            n = kd_units(q, a.window, lo);
-        }
-        const int each = plan.whole ? (int)((n + (uint32_t)plan.per - 1) / (uint32_t)plan.per) : n;
-        const long mine = (long)each * a.c.heads;
-        long sum = mine;                   // units or parts up to and with this lane's sequence
-        for (int i = 1; i < 32; i <<= 1) {
-            const long o = __shfl_up_sync(~0u, sum, i);
-            if (lane >= i) sum += o;
-        }
+        const KdSeq q = a.s.n_seqs > 32 ? kd_seq(a, b0 + lane, nullptr) : plan.mine;
+        const uint32_t each = plan.whole ? (q.units + plan.per - 1) / plan.per : q.units, mine = each * a.c.heads;
+        uint32_t sum = mine;               // units or parts up to and with this lane's sequence
+        if (a.s.n_seqs > 1)
+            for (int i = 1; i < 32; i <<= 1) {
+                const uint32_t o = __shfl_up_sync(~0u, sum, i);
+                if (lane >= i) sum += o;
+            }
         const unsigned hit = __ballot_sync(~0u, x < before + sum);
         if (hit) {
             const int src = __ffs(hit) - 1;
@@ -293,26 +295,28 @@ __device__ __forceinline__ void kd_find(const KvaArgs& a, const KdPlan& plan, lo
             it.kv = __shfl_sync(~0u, q.kv, src);
             it.n_new = __shfl_sync(~0u, q.n_new, src);
             it.row0 = __shfl_sync(~0u, q.row0, src);
-            it.lo = __shfl_sync(~0u, lo, src);
-            n = __shfl_sync(~0u, n, src);
-            const int count = __shfl_sync(~0u, each, src);
-            const long at = x - before - __shfl_sync(~0u, sum - mine, src);
-            it.head = (int)(at / count);
-            const int off = (int)(at - (long)it.head * count), u = it.lo / KD_UNIT;
+            it.lo = __shfl_sync(~0u, q.lo, src);
+            const uint32_t n = __shfl_sync(~0u, q.units, src), count = __shfl_sync(~0u, each, src);
+            const uint32_t at = x - before - __shfl_sync(~0u, sum - mine, src);
+            it.head = at / count;
+            const uint32_t off = at - it.head * count;
+            const int u = it.lo / KD_UNIT;
             if (plan.whole) {
-                it.u0 = u + (int)((long)n * off / count);
-                it.u1 = u + (int)((long)n * (off + 1) / count);
+                // ceil(n / count) or one less units a part
+                const uint32_t big = (n + count - 1) / count, cut = n - (big - 1) * count;
+                it.u0 = u + off * big - (off > cut ? off - cut : 0);
+                it.u1 = it.u0 + big - (off >= cut);
                 it.chunks = count;
                 it.c0 = blockIdx.x - off;
                 it.odd = 0;
                 it.slot = 2 * blockIdx.x;
             } else {
                 // a block has one part of a head begun before it at most, and one of a head that goes on behind it
-                const long h0 = x - off, h1 = h0 + n;
+                const uint32_t h0 = x - off, h1 = h0 + n;
                 it.u0 = u + off;
-                it.u1 = u + (int)(min(h1, end) - h0);
-                it.c0 = (int)(h0 / plan.per);
-                it.chunks = (int)((h1 - 1) / plan.per) - it.c0 + 1;
+                it.u1 = u + (min(h1, end) - h0);
+                it.c0 = h0 / plan.per;
+                it.chunks = (h1 - 1) / plan.per - it.c0 + 1;
                 it.odd = 1;
                 it.slot = 2 * blockIdx.x + (off == 0);
             }
@@ -382,7 +386,7 @@ __device__ __forceinline__ float q_unit(float max, float& back) {
 }
 
 template <int D, int DT, int NT>
-__global__ void __launch_bounds__(KD_WARPS * 32, KD_CTAS) kv_decode_kernel(const KvaArgs a, int least) {
+__global__ void __launch_bounds__(KD_WARPS * 32, KD_CTAS) kv_decode_kernel(const KvaArgs a, uint32_t least) {
     using G = KdGeo<D>;
     constexpr bool SPLIT = DT == TK_DT_F32;
     constexpr int ROWS = 8 * NT, PARTS = SPLIT ? 2 : 1;            // query rows, fp16 parts of q and p
@@ -394,14 +398,36 @@ __global__ void __launch_bounds__(KD_WARPS * 32, KD_CTAS) kv_decode_kernel(const
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int kg = kd_key(g), k0 = kd_key(2 * t), k1 = kd_key(2 * t + 1);
     const KdPlan plan = kd_plan(a, least);
-    long x = plan.whole ? blockIdx.x : blockIdx.x * plan.per;
-    const long end = min(x + (plan.whole ? 1 : plan.per), plan.total);
+    uint32_t x = plan.whole ? blockIdx.x : blockIdx.x * plan.per;
+    const uint32_t end = min(x + (plan.whole ? 1 : plan.per), plan.total);
     uint8_t* ring = smem + warp * (KD_STAGES * G::STAGE);
 
   for (; x < end; ) {
     KdItem it;
     kd_find(a, plan, x, end, it);
     x += plan.whole ? 1 : it.u1 - it.u0;
+    // ---- rows: row r of the block is token r / group, head r % group; lane (g, t) loads the t-th quarter of row
+    // g (before the copies below queue up in front of it) and keeps the statistics of rows 2 t and 2 t + 1 ----
+    const int rows = it.n_new * a.group, pos0 = it.kv - it.n_new;
+    float x0[NT][KW][8];
+    int lim[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        const int r = g + 8 * n;
+        lim[n] = INT32_MAX;
+#pragma unroll
+        for (int w = 0; w < KW; ++w)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x0[n][w][e] = 0.0f;
+        if (r < rows) {
+            const int tok = r / a.group;
+            lim[n] = max(pos0 + tok + 1, 0);
+            const size_t at = (size_t)(it.row0 + tok) * a.ldq + (size_t)(it.head * a.group + r % a.group) * D + t * (D / 4);
+#pragma unroll
+            for (int w = 0; w < KW; ++w) load_pairs8<DT>(a.q, at + w * 8, x0[n][w]);
+        }
+    }
+
     // ---- the warp's units: u0 + warp, + 4, ... ----
     const int mine = it.u1 - it.u0 > warp && it.kv > 0 ? (it.u1 - it.u0 - warp + KD_WARPS - 1) / KD_WARPS : 0;
     const int page_mask = (1 << a.c.page_shift) - 1;
@@ -447,33 +473,16 @@ __global__ void __launch_bounds__(KD_WARPS * 32, KD_CTAS) kv_decode_kernel(const
     };
     for (int i = 0; i < KD_STAGES - 1; ++i) issue(i, i);
 
-    // ---- rows: row r of the block is token r / group, head r % group ----
-    const int rows = it.n_new * a.group, pos0 = it.kv - it.n_new;
-    // lane (g, t) loads the t-th quarter of row g and keeps the statistics of rows 2 t and 2 t + 1
     uint4 qr[PARTS][KW];
     float sc[NT][2];
     int limit[NT][2], from[NT][2];                                 // keys [from, limit) are seen
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-        const int r = g + 8 * n;
-        float x[KW][8], mx = 0.0f;
-        int lim = INT32_MAX;
-        if (r < rows) {
-            const int tok = r / a.group;
-            lim = max(pos0 + tok + 1, 0);
-            const size_t at = (size_t)(it.row0 + tok) * a.ldq + (size_t)(it.head * a.group + r % a.group) * D + t * (D / 4);
+        float mx = 0.0f;
 #pragma unroll
-            for (int w = 0; w < KW; ++w) {
-                load_pairs8<DT>(a.q, at + w * 8, x[w]);
+        for (int w = 0; w < KW; ++w)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(x[w][e]));
-            }
-        } else {
-#pragma unroll
-            for (int w = 0; w < KW; ++w)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) x[w][e] = 0.0f;
-        }
+            for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(x0[n][w][e]));
         mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 1));
         mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 2));
         float back;
@@ -482,7 +491,7 @@ __global__ void __launch_bounds__(KD_WARPS * 32, KD_CTAS) kv_decode_kernel(const
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
             sc[n][c] = __shfl_sync(~0u, back, 4 * (2 * t + c));
-            limit[n][c] = __shfl_sync(~0u, lim, 4 * (2 * t + c));
+            limit[n][c] = __shfl_sync(~0u, lim[n], 4 * (2 * t + c));
             from[n][c] = a.window > 0 && limit[n][c] != INT32_MAX ? max(limit[n][c] - a.window, 0) : 0;
         }
 #pragma unroll
@@ -491,7 +500,7 @@ __global__ void __launch_bounds__(KD_WARPS * 32, KD_CTAS) kv_decode_kernel(const
             uint32_t hi[4], lo[4];
 #pragma unroll
             for (int p = 0; p < 4; ++p) {
-                const float u = x[w][2 * p] * up, v = x[w][2 * p + 1] * up;
+                const float u = x0[n][w][2 * p] * up, v = x0[n][w][2 * p + 1] * up;
                 hi[p] = pack_half2(u, v);
                 const __half2 hh = as_half2(hi[p]);
                 lo[p] = pack_half2(u - __low2float(hh), v - __high2float(hh));
@@ -779,6 +788,8 @@ static tk_status go_decode(tk_ctx* ctx, KvaArgs& a, int dtype, cudaStream_t st) 
     const size_t pairs = (size_t)a.s.n_seqs * a.c.heads;
     const unsigned grid = KD_CTAS * ctx->num_sms;   // what is resident at once
     const int least = KD_WARPS;               // a unit for every warp
+    if (pairs * ((size_t)a.s.max_pages << a.c.page_shift) / KD_UNIT + pairs > (1ull << 31))
+        return fail(TK_ERR_UNSUPPORTED, "tk_kv_attend: sequences x heads x table length beyond 2^36 tokens");
     tk_status r = ws_ensure(ctx, (size_t)grid * 2 * (16 * (D + 2)) * sizeof(float), st);
     if (r == TK_OK) r = count_ensure(ctx, pairs);
     if (r != TK_OK) return r;
