@@ -9,20 +9,20 @@
 // weight / S come out the same for any division.
 //
 // Two launches.  dv_rows reads every logit once (the bound: memory) and leaves
-// each part's exponent, sum and largest logit.  dv_pick, a cluster of eight
-// blocks per sequence, finds the first refused row from these and draws the
-// next token from that one row: whole weights (multiples of 2^-38) summed per
-// 128 tokens, the blocks' totals exchanged in shared memory, then the one
-// piece that holds the draw searched again.
+// each part's exponent, sum and largest logit.  dv_pick, a cluster of blocks
+// per sequence, finds the first refused row from these and draws the next
+// token from that one row: whole weights (multiples of 2^-38) summed per 128
+// tokens, the blocks' totals exchanged in shared memory, then the one piece
+// that holds the draw searched again.
 #include <climits>
 #include "tk_device.cuh"
 #include "tk_internal.h"
 
 namespace tk {
 
-constexpr int DV_THREADS = 256, DV_QUADS = 16;     // dv_rows: quads (4 logits) a thread holds in registers
-constexpr int DP_THREADS = 512, DP_CLUSTER = 8, DP_WARPS = DP_THREADS / 32;
-constexpr int DP_GROUPS = 64;                      // dv_pick: sums kept per warp
+constexpr int DV_THREADS = 256, DV_QUADS = 16;     // dv_rows: quads (4 logits) a thread holds in registers at most
+constexpr int DP_THREADS = 256, DP_CLUSTER = 16, DP_WARPS = DP_THREADS / 32;   // dv_pick: blocks of a cluster at most
+constexpr int DP_GROUPS = 128, DP_AHEAD = 8;       // sums kept per warp; of these, groups whose logits are loaded at once
 
 // A part of a row, or a whole one: largest whole exponent, the weights' sum
 // relative to it, the largest logit and its first place; bad: NaN, +inf or
@@ -46,12 +46,18 @@ struct DvArgs {
     float* logp;
     DvStat* stat;             // [2][n_rows][parts]: target's rows, then draft's
     int parts, part_quads;    // parts of a row, quads of a part
+    int cluster;              // blocks of a sequence in dv_pick
     int* status;
 };
 
-__device__ __forceinline__ float dv_exp2(float x) {
+__device__ __forceinline__ float dv_exp2(float x) {        // x in [0, 1)
     float r;
-    asm("ex2.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float dv_max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
     return r;
 }
 // 2^d for a whole d in [-126, 0]: d + 1.5 * 2^23 has d in its low bits.
@@ -62,6 +68,23 @@ __device__ __forceinline__ float dv_scale(float w, float d) {
 __device__ __forceinline__ float dv_weight(float x, float c, float top) {
     const float y = __fmul_rn(x, c), i = floorf(y), d = i - top;
     return d >= -100.0f ? dv_scale(dv_exp2(y - i), d) : 0.0f;      // also y = -inf
+}
+// weight / S rounded once.  With r = 1 / S rounded to nearest, q = w r and the
+// exact remainder w - q S give the correctly rounded quotient q + (w - q S) r
+// for every S whose significand is not all ones (Markstein 1990); for that
+// one, and for what is drawn only once, the division itself.
+struct DvInv {
+    float s, r;
+    bool divide;
+};
+__device__ __forceinline__ DvInv dv_inv(const DvStat& st) {
+    const float s = (float)st.sum;
+    return DvInv{s, __frcp_rn(s), (__float_as_uint(s) & 0x7fffffu) == 0x7fffffu};
+}
+__device__ __forceinline__ float dv_quotient(float w, const DvInv& i) {
+    if (i.divide) return __fdiv_rn(w, i.s);
+    const float q = __fmul_rn(w, i.r);
+    return __fmaf_rn(__fmaf_rn(-q, i.s, w), i.r, q);
 }
 __device__ __forceinline__ float dv_prob(float x, float c, const DvStat& s) {
     return __fdiv_rn(dv_weight(x, c, s.top), (float)s.sum);
@@ -109,12 +132,12 @@ __device__ __forceinline__ float4 dv_quad(const float* x, int off, long q, int v
 }
 __device__ __forceinline__ int dv_off(const float* x) { return (int)((reinterpret_cast<uintptr_t>(x) >> 2) & 3); }
 
-// A block takes one part of one row into registers (16 loads of 16 bytes a
+// A block takes one part of one row into registers (QUADS loads of 16 bytes a
 // thread in flight), finds its largest logit, then sums the weights: each
 // thread in fp32 with the rounding errors kept beside (exact to 2^-46), the
 // block in 64 bits.
-template <bool GREEDY>
-__global__ void __launch_bounds__(DV_THREADS, 2) dv_rows_kernel(const DvArgs a) {
+template <bool GREEDY, int QUADS>
+__global__ void __launch_bounds__(DV_THREADS, QUADS > 8 ? 2 : 4) dv_rows_kernel(const DvArgs a) {
     __shared__ float smax[DV_THREADS / 32];
     __shared__ DvStat sst[DV_THREADS / 32];
     pdl_trigger();
@@ -124,29 +147,33 @@ __global__ void __launch_bounds__(DV_THREADS, 2) dv_rows_kernel(const DvArgs a) 
     const int off = dv_off(x);
     const long quads = ((long)off + a.vocab + 3) / 4, q0 = (long)part * a.part_quads;
     const int n = (int)max(0L, min((long)a.part_quads, quads - q0));
-    float4 v[DV_QUADS];
+    float4 v[QUADS];
 #pragma unroll
-    for (int k = 0; k < DV_QUADS; ++k) {
-        const int q = k * DV_THREADS + tid;
-        v[k] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-        if (q < n) v[k] = dv_quad(x, off, q0 + q, a.vocab);
+    for (int k = 0; k < QUADS; ++k) v[k] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+    if (4 * q0 >= off && 4 * (q0 + n) - off <= a.vocab) {          // no quad reaches over the row's ends
+        const float4* from = reinterpret_cast<const float4*>(x + (4 * q0 - off)) + tid;
+#pragma unroll
+        for (int k = 0; k < QUADS; ++k)
+            if (k * DV_THREADS + tid < n) v[k] = __ldg(from + k * DV_THREADS);
+    } else {
+#pragma unroll
+        for (int k = 0; k < QUADS; ++k)
+            if (k * DV_THREADS + tid < n) v[k] = dv_quad(x, off, q0 + k * DV_THREADS + tid, a.vocab);
     }
-    float mx = -INFINITY;
+    float mx = -INFINITY, nan = -INFINITY;
     int arg = INT_MAX;
-    bool bad = false;
 #pragma unroll
-    for (int k = 0; k < DV_QUADS; ++k) {
+    for (int k = 0; k < QUADS; ++k) {
         const float e[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            bad |= !(e[i] <= 3.402823466e38f);
-            if constexpr (GREEDY) {
-                if (e[i] > mx) { mx = e[i]; arg = (int)(4 * (q0 + k * DV_THREADS + tid) - off) + i; }
-            } else {
-                mx = fmaxf(mx, e[i]);
-            }
+            nan = dv_max_nan(nan, e[i]);
+            if (GREEDY && e[i] > mx) { mx = e[i]; arg = 4 * (k * DV_THREADS) + i; }
         }
     }
+    if (GREEDY && arg != INT_MAX) arg += (int)(4 * (q0 + tid) - off);
+    const bool bad = !(nan <= 3.402823466e38f);
+    if (!GREEDY) mx = bad ? 0.0f : nan;
     float big = mx;
     for (int i = 16; i; i >>= 1) big = fmaxf(big, __shfl_xor_sync(~0u, big, i));
     if ((tid & 31) == 0) smax[tid >> 5] = big;
@@ -158,7 +185,7 @@ __global__ void __launch_bounds__(DV_THREADS, 2) dv_rows_kernel(const DvArgs a) 
         // s2 >= any weight from the start, so that t - s2 and its difference to the weight are exact
         float s2 = 2.0f, err = 0.0f;
 #pragma unroll
-        for (int k = 0; k < DV_QUADS; ++k) {
+        for (int k = 0; k < QUADS; ++k) {
             if (k * DV_THREADS >= n) break;
             const float e[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
 #pragma unroll
@@ -200,11 +227,11 @@ __device__ __forceinline__ DvStat dv_row(const DvArgs& a, size_t row) {
     return s;
 }
 
-__global__ void __cluster_dims__(DP_CLUSTER, 1, 1) __launch_bounds__(DP_THREADS) dv_pick_kernel(const DvArgs a) {
+__global__ void __launch_bounds__(DP_THREADS, 2) dv_pick_kernel(const DvArgs a) {
     __shared__ DvStat st_t[DP_WARPS], st_d[DP_WARPS];
     __shared__ int verdict[DP_WARPS];              // 0: accepted, 1: the row draws, 2: no distribution
     __shared__ unsigned long long wsum[DP_GROUPS][DP_WARPS], ctot[2];
-    const int b = blockIdx.x / DP_CLUSTER, rank = (int)cluster_ctarank(), tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int cluster = a.cluster, b = blockIdx.x / cluster, rank = (int)cluster_ctarank(), tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int V = a.vocab;
     pdl_wait();
     const int r0 = a.row_start[b], r1 = a.row_start[b + 1];
@@ -278,49 +305,65 @@ __global__ void __cluster_dims__(DP_CLUSTER, 1, 1) __launch_bounds__(DP_THREADS)
     const int off = dv_off(t);
     const bool same = !d || dv_off(d) == off;
     const long quads = ((long)off + V + 3) / 4;
-    const int share = (int)((quads + DP_CLUSTER - 1) / DP_CLUSTER);
+    const int share = (int)((quads + cluster - 1) / cluster);
     const int runs = (share + DP_GROUPS * DP_THREADS - 1) / (DP_GROUPS * DP_THREADS);
     const int groups = (share + runs * DP_THREADS - 1) / (runs * DP_THREADS);
     const long q0 = (long)rank * groups * runs * DP_THREADS;
-    auto weights = [&](long q, bool rest, unsigned long long (&w)[4]) {
-        const float4 tv = dv_quad(t, off, q, V);
-        const float e[4] = {tv.x, tv.y, tv.z, tv.w};
-        float de[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-        const long j = 4 * q - off;
+    const DvInv it = dv_inv(st), id = dv_inv(sd);
+    auto load = [&](long q, bool rest, float4& tv, float4& dv) {
+        tv = dv_quad(t, off, q, V);
+        dv = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
         if (d && rest) {
-            if (same) {
-                const float4 dv = dv_quad(d, off, q, V);
-                de[0] = dv.x; de[1] = dv.y; de[2] = dv.z; de[3] = dv.w;
-            } else {
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (j + i >= 0 && j + i < V) de[i] = d[j + i];
+            if (same) dv = dv_quad(d, off, q, V);
+            else {
+                const long j = 4 * q - off;
+                if (j >= 0 && j < V) dv.x = d[j];
+                if (j + 1 >= 0 && j + 1 < V) dv.y = d[j + 1];
+                if (j + 2 >= 0 && j + 2 < V) dv.z = d[j + 2];
+                if (j + 3 >= 0 && j + 3 < V) dv.w = d[j + 3];
             }
         }
+    };
+    // floor(w 2^38) = hi 2^19 + lo: adding 2^23 downwards leaves a whole number in the low bits
+    auto weights = [&](long q, bool rest, const float4& tv, const float4& dv, uint32_t (&hi)[4], uint32_t (&lo)[4]) {
+        const float e[4] = {tv.x, tv.y, tv.z, tv.w}, f[4] = {dv.x, dv.y, dv.z, dv.w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            float p = dv_prob(e[i], a.c, st);
+            float p = dv_quotient(dv_weight(e[i], a.c, st.top), it);
             if (rest) {
-                if (d) p = fmaxf(p - dv_prob(de[i], a.c, sd), 0.0f);
-                else if (j + i == x) p = 0.0f;
+                if (d) p = fmaxf(p - dv_quotient(dv_weight(f[i], a.c, sd.top), id), 0.0f);
+                else if (4 * q - off + i == x) p = 0.0f;
             }
-            w[i] = (unsigned long long)(p * 274877906944.0f);
+            const float u = p * 524288.0f, h = __fadd_rd(u, 8388608.0f);
+            hi[i] = __float_as_uint(h) & 0xfffffu;
+            lo[i] = __float_as_uint(__fmaf_rd(u - (h - 8388608.0f), 524288.0f, 8388608.0f)) & 0xfffffu;
         }
     };
     for (int pass = 0; pass < 2; ++pass) {         // what is left of p over q; p itself if that is nothing
         const bool rest = pass == 0 && !last;
         unsigned long long own = 0;
-        for (int gr = 0; gr < groups; ++gr) {
-            unsigned long long s = 0;
+        // (more than one run a group: vocabularies beyond 2^19 tokens and a block, whose groups are loaded one by one)
+        for (int g0 = 0; g0 < groups; g0 += DP_AHEAD) {
+            float4 tv[DP_AHEAD], dv[DP_AHEAD];
             for (int k = 0; k < runs; ++k) {
-                const long q = q0 + ((long)(gr * DP_WARPS + warp) * runs + k) * 32 + lane;
-                if (q >= quads) break;
-                unsigned long long w[4];
-                weights(q, rest, w);
-                s += w[0] + w[1] + w[2] + w[3];
+#pragma unroll
+                for (int j = 0; j < DP_AHEAD; ++j) {
+                    const long q = q0 + ((long)((g0 + j) * DP_WARPS + warp) * runs + k) * 32 + lane;
+                    tv[j] = dv[j] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+                    if (g0 + j < groups && q < quads) load(q, rest, tv[j], dv[j]);
+                }
+#pragma unroll
+                for (int j = 0; j < DP_AHEAD; ++j) {
+                    if (g0 + j >= groups) break;
+                    const long q = q0 + ((long)((g0 + j) * DP_WARPS + warp) * runs + k) * 32 + lane;
+                    uint32_t hi[4], lo[4];
+                    weights(q, rest, tv[j], dv[j], hi, lo);
+                    const uint32_t h = __reduce_add_sync(~0u, hi[0] + hi[1] + hi[2] + hi[3]);
+                    const uint32_t l = __reduce_add_sync(~0u, lo[0] + lo[1] + lo[2] + lo[3]);
+                    const unsigned long long s = ((unsigned long long)h << 19) + l;
+                    if (lane == 0) wsum[g0 + j][warp] = k ? wsum[g0 + j][warp] + s : s;
+                }
             }
-            for (int i = 16; i; i >>= 1) s += __shfl_xor_sync(~0u, s, i);
-            if (lane == 0) wsum[gr][warp] = s;
         }
         __syncthreads();
         if (warp == 0) {
@@ -330,7 +373,7 @@ __global__ void __cluster_dims__(DP_CLUSTER, 1, 1) __launch_bounds__(DP_THREADS)
         }
         cluster_sync();
         unsigned long long total = 0, before = 0;
-        for (int c = 0; c < DP_CLUSTER; ++c) {
+        for (int c = 0; c < cluster; ++c) {
             unsigned long long v;
             asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(mapa_shared(smem_u32(&ctot[pass]), c)) : "memory");
             if (c < rank) before += v;
@@ -359,7 +402,14 @@ __global__ void __cluster_dims__(DP_CLUSTER, 1, 1) __launch_bounds__(DP_THREADS)
             for (int k = 0; k < runs; ++k) {
                 const long q = q0 + ((long)at * runs + k) * 32 + lane;
                 unsigned long long w[4] = {0, 0, 0, 0};
-                if (q < quads) weights(q, rest, w);
+                if (q < quads) {
+                    float4 tv, dv;
+                    uint32_t hi[4], lo[4];
+                    load(q, rest, tv, dv);
+                    weights(q, rest, tv, dv, hi, lo);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) w[i] = ((unsigned long long)hi[i] << 19) + lo[i];
+                }
                 s = sum = w[0] + w[1] + w[2] + w[3];
                 for (int i = 1; i < 32; i <<= 1) {
                     const unsigned long long o = __shfl_up_sync(~0u, sum, i);
@@ -401,31 +451,45 @@ tk_status launch_draft_verify(tk_ctx* ctx, int n_seqs, const int32_t* row_start,
     a.c = (float)(1.4426950408889634 / (a.greedy ? 1.0 : (double)temperature));
     a.n_accept = n_accept; a.next = next; a.logp = logp;
     a.status = ctx->status;
-    // parts of at most what a block's registers hold; smaller ones (down to two
+    // parts of at most what a block's registers hold; smaller ones (down to four
     // quads a thread) while that gives every SM four blocks
     const long quads = ((long)vocab + 6) / 4, rows = (long)n_rows * (a.draft ? 2 : 1);
     long part = (quads * rows + 4L * ctx->num_sms - 1) / (4L * ctx->num_sms);
-    if (part < 2 * DV_THREADS) part = 2 * DV_THREADS;
+    if (part < 4 * DV_THREADS) part = 4 * DV_THREADS;
     if (part > DV_QUADS * DV_THREADS) part = DV_QUADS * DV_THREADS;
-    const long parts = (quads + part - 1) / part, grid = parts * rows, pick = (long)n_seqs * DP_CLUSTER;
+    // blocks of a sequence's draw: as many as are resident at once (two an SM), 16 at most
+    a.cluster = DP_CLUSTER;
+    while (a.cluster > 1 && (long)n_seqs * a.cluster > 2L * ctx->num_sms) a.cluster >>= 1;
+    const long parts = (quads + part - 1) / part, grid = parts * rows, pick = (long)n_seqs * a.cluster;
     if (grid > INT_MAX || pick > INT_MAX) return fail(TK_ERR_INVALID, "tk_draft_verify: too many rows");
     a.parts = (int)parts;
     a.part_quads = (int)((quads + parts - 1) / parts);
     tk_status st = ws_ensure(ctx, (size_t)grid * sizeof(DvStat), s);
     if (st != TK_OK) return st;
     a.stat = static_cast<DvStat*>(ctx->ws);
+    static std::atomic<uint64_t> attr_done{0};     // clusters of 16 are more than every GPU must offer: per device
+    if (!(attr_done.load(std::memory_order_relaxed) >> (ctx->device & 63) & 1)) {
+        const cudaError_t e = cudaFuncSetAttribute(dv_pick_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        if (e != cudaSuccess) return cuda_fail(e, "draft verify cluster attribute");
+        attr_done.fetch_or(1ull << (ctx->device & 63));
+    }
     ProfScope ps(ctx, s, PK_SERVE);
-    if (a.greedy) dv_rows_kernel<true><<<(unsigned)grid, DV_THREADS, 0, s>>>(a);
-    else dv_rows_kernel<false><<<(unsigned)grid, DV_THREADS, 0, s>>>(a);
+    const bool small = a.part_quads <= 4 * DV_THREADS;
+    auto kern = a.greedy ? (small ? dv_rows_kernel<true, 4> : dv_rows_kernel<true, DV_QUADS>)
+                         : (small ? dv_rows_kernel<false, 4> : dv_rows_kernel<false, DV_QUADS>);
+    kern<<<(unsigned)grid, DV_THREADS, 0, s>>>(a);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)pick);
     cfg.blockDim = dim3(DP_THREADS);
     cfg.stream = s;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = a.cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = 2;
     const cudaError_t e = cudaLaunchKernelEx(&cfg, dv_pick_kernel, a);
     ctx->launches += 2;
     if (e != cudaSuccess) return cuda_fail(e, "draft verify launch");
