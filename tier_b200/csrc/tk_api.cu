@@ -702,6 +702,7 @@ tk_status tk_draft_verify(tk_ctx* ctx, int n_seqs, const int32_t* row_start, int
     if (n_seqs < 0 || n_rows < 0) return fail(TK_ERR_INVALID, "tk_draft_verify: bad row count");
     if (n_seqs == 0) return TK_OK;
     if (vocab <= 0 || n_rows == 0) return fail(TK_ERR_INVALID, "tk_draft_verify: no rows or empty vocabulary");
+    if (vocab > (1 << 23)) return fail(TK_ERR_UNSUPPORTED, "tk_draft_verify: vocabulary beyond 2^23");
     if (!row_start || !target || !tokens || !n_accept || !next) return fail(TK_ERR_INVALID, "tk_draft_verify: null pointer");
     if (!(temperature >= 0.0f) || !std::isfinite(temperature) || (temperature > 0.0f && temperature < 1e-4f))
         return fail(TK_ERR_INVALID, "tk_draft_verify: temperature must be 0 or at least 1e-4");

@@ -20,9 +20,9 @@
 
 namespace tk {
 
-constexpr int DV_THREADS = 256, DV_QUADS = 16;     // dv_rows: quads (4 logits) a thread holds in registers at most
-constexpr int DP_THREADS = 256, DP_CLUSTER = 16, DP_WARPS = DP_THREADS / 32;   // dv_pick: blocks of a cluster at most
-constexpr int DP_GROUPS = 128, DP_AHEAD = 8;       // sums kept per warp; of these, groups whose logits are loaded at once
+constexpr int DV_THREADS = 256, DV_QUADS = 8;          // dv_rows: quads (4 logits) a thread holds in registers at most
+constexpr int DP_THREADS = 512, DP_CLUSTER = 16, DP_WARPS = DP_THREADS / 32;   // dv_pick: blocks of a cluster at most
+constexpr int DP_SUMS = 64, DP_AHEAD = 6;          // sums kept per warp; steps whose logits are on their way
 
 // A part of a row, or a whole one: largest whole exponent, the weights' sum
 // relative to it, the largest logit and its first place; bad: NaN, +inf or
@@ -69,22 +69,75 @@ __device__ __forceinline__ float dv_weight(float x, float c, float top) {
     const float y = __fmul_rn(x, c), i = floorf(y), d = i - top;
     return d >= -100.0f ? dv_scale(dv_exp2(y - i), d) : 0.0f;      // also y = -inf
 }
+// Two weights at once, for |top| < 2^22 and y no further than 110 below it
+// (clamped: what is further down weighs less than 2^-109 of the row).  Adding
+// 1.5 * 2^23 - top downwards leaves i - top in the low bits of the sum, which
+// shifted up are added to the exponent of 2^(y - i): the bits of dv_weight
+// without its conversions and comparisons.  Packed fp32 instructions take
+// both at once.
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 dv_pack(float a, float b) {
+    f32x2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void dv_unpack(f32x2 v, float& a, float& b) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ f32x2 dv_add2(f32x2 a, f32x2 b) {
+    f32x2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ f32x2 dv_mul2(f32x2 a, f32x2 b) {
+    f32x2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ f32x2 dv_fma2(f32x2 a, f32x2 b, f32x2 c) {
+    f32x2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ f32x2 dv_sub2(f32x2 a, f32x2 b) { return dv_fma2(b, dv_pack(-1.0f, -1.0f), a); }
+constexpr float DV_NEAR = 4194304.0f;              // |top| below this: dv_weight2
+struct DvFast {
+    f32x2 c, bias, nbias;
+    float low;
+};
+__device__ __forceinline__ DvFast dv_fast(float c, float top) {
+    const float m = 12582912.0f - top;
+    return DvFast{dv_pack(c, c), dv_pack(m, m), dv_pack(-m, -m), top - 110.0f};
+}
+__device__ __forceinline__ f32x2 dv_weight2(float x0, float x1, const DvFast& k) {
+    f32x2 y, t;
+    float y0, y1, f0, f1, t0, t1;
+    dv_unpack(dv_mul2(dv_pack(x0, x1), k.c), y0, y1);
+    y = dv_pack(fmaxf(y0, k.low), fmaxf(y1, k.low));
+    asm("add.rm.f32x2 %0, %1, %2;" : "=l"(t) : "l"(y), "l"(k.bias));
+    dv_unpack(dv_sub2(y, dv_add2(t, k.nbias)), f0, f1);
+    dv_unpack(t, t0, t1);
+    return dv_pack(__uint_as_float((__float_as_uint(t0) << 23) + __float_as_uint(dv_exp2(f0))),
+                   __uint_as_float((__float_as_uint(t1) << 23) + __float_as_uint(dv_exp2(f1))));
+}
+
 // weight / S rounded once.  With r = 1 / S rounded to nearest, q = w r and the
 // exact remainder w - q S give the correctly rounded quotient q + (w - q S) r
 // for every S whose significand is not all ones (Markstein 1990); for that
-// one, and for what is drawn only once, the division itself.
-struct DvInv {
-    float s, r;
-    bool divide;
+// one, and for what is needed only once, the division itself.
+struct DvProb {
+    DvFast fast;
+    f32x2 ns, r;              // -S, 1 / S
+    bool quick;               // both of the above hold
 };
-__device__ __forceinline__ DvInv dv_inv(const DvStat& st) {
-    const float s = (float)st.sum;
-    return DvInv{s, __frcp_rn(s), (__float_as_uint(s) & 0x7fffffu) == 0x7fffffu};
+__device__ __forceinline__ DvProb dv_prepare(const DvStat& st, float c) {
+    const float s = (float)st.sum, r = __frcp_rn(s);
+    return DvProb{dv_fast(c, st.top), dv_pack(-s, -s), dv_pack(r, r),
+                  fabsf(st.top) < DV_NEAR && (__float_as_uint(s) & 0x7fffffu) != 0x7fffffu};
 }
-__device__ __forceinline__ float dv_quotient(float w, const DvInv& i) {
-    if (i.divide) return __fdiv_rn(w, i.s);
-    const float q = __fmul_rn(w, i.r);
-    return __fmaf_rn(__fmaf_rn(-q, i.s, w), i.r, q);
+__device__ __forceinline__ f32x2 dv_prob2(float x0, float x1, const DvProb& k) {
+    const f32x2 w = dv_weight2(x0, x1, k.fast), q = dv_mul2(w, k.r);
+    return dv_fma2(dv_fma2(q, k.ns, w), k.r, q);
 }
 __device__ __forceinline__ float dv_prob(float x, float c, const DvStat& s) {
     return __fdiv_rn(dv_weight(x, c, s.top), (float)s.sum);
@@ -137,9 +190,10 @@ __device__ __forceinline__ int dv_off(const float* x) { return (int)((reinterpre
 // thread in fp32 with the rounding errors kept beside (exact to 2^-46), the
 // block in 64 bits.
 template <bool GREEDY, int QUADS>
-__global__ void __launch_bounds__(DV_THREADS, QUADS > 8 ? 2 : 4) dv_rows_kernel(const DvArgs a) {
+__global__ void __launch_bounds__(DV_THREADS, 4) dv_rows_kernel(const DvArgs a) {
     __shared__ float smax[DV_THREADS / 32];
-    __shared__ DvStat sst[DV_THREADS / 32];
+    __shared__ double ssum[DV_THREADS / 32];
+    __shared__ int sarg[DV_THREADS / 32];
     pdl_trigger();
     const int part = blockIdx.x % a.parts, row = blockIdx.x / a.parts, tid = threadIdx.x;
     const bool isd = row >= a.n_rows;
@@ -171,52 +225,69 @@ __global__ void __launch_bounds__(DV_THREADS, QUADS > 8 ? 2 : 4) dv_rows_kernel(
             if (GREEDY && e[i] > mx) { mx = e[i]; arg = 4 * (k * DV_THREADS) + i; }
         }
     }
-    if (GREEDY && arg != INT_MAX) arg += (int)(4 * (q0 + tid) - off);
     const bool bad = !(nan <= 3.402823466e38f);
-    if (!GREEDY) mx = bad ? 0.0f : nan;
-    float big = mx;
+    float big = bad ? 0.0f : nan;
     for (int i = 16; i; i >>= 1) big = fmaxf(big, __shfl_xor_sync(~0u, big, i));
     if ((tid & 31) == 0) smax[tid >> 5] = big;
-    __syncthreads();
+    const int any_bad = __syncthreads_or(bad);
 #pragma unroll
     for (int w = 0; w < DV_THREADS / 32; ++w) big = fmaxf(big, smax[w]);
-    DvStat s{0.0, floorf(__fmul_rn(big, a.c)), mx, arg, bad};
-    if (s.top > -3.402823466e38f) {
-        // s2 >= any weight from the start, so that t - s2 and its difference to the weight are exact
-        float s2 = 2.0f, err = 0.0f;
+    const float top = floorf(__fmul_rn(big, a.c));
+    double sum = 0.0;
+    if (fabsf(top) < DV_NEAR) {
+        // sums start above any weight, so that t - s2 and its difference to the weight are exact
+        const DvFast fast = dv_fast(a.c, top);
+        f32x2 s2 = dv_pack(2.0f, 2.0f), err = dv_pack(0.0f, 0.0f);
 #pragma unroll
         for (int k = 0; k < QUADS; ++k) {
             if (k * DV_THREADS >= n) break;
-            const float e[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float w = dv_weight(e[i], a.c, s.top), t = __fadd_rn(s2, w);
-                err = __fadd_rn(err, __fsub_rn(w, __fsub_rn(t, s2)));
+            for (int h = 0; h < 2; ++h) {
+                const f32x2 w = h ? dv_weight2(v[k].z, v[k].w, fast) : dv_weight2(v[k].x, v[k].y, fast), t = dv_add2(s2, w);
+                err = dv_add2(err, dv_sub2(w, dv_sub2(t, s2)));
                 s2 = t;
             }
         }
-        s.sum = ((double)s2 - 2.0) + (double)err;
+        float p0, p1, e0, e1;
+        dv_unpack(s2, p0, p1);
+        dv_unpack(err, e0, e1);
+        sum = (((double)p0 - 2.0) + ((double)p1 - 2.0)) + ((double)e0 + (double)e1);
+    } else if (top > -3.402823466e38f) {           // logits of such size: one by one
+#pragma unroll 1
+        for (int q = tid; q < n; q += DV_THREADS) {
+            const float4 u = dv_quad(x, off, q0 + q, a.vocab);
+            sum += ((double)dv_weight(u.x, a.c, top) + (double)dv_weight(u.y, a.c, top)) +
+                   ((double)dv_weight(u.z, a.c, top) + (double)dv_weight(u.w, a.c, top));
+        }
     }
-    for (int i = 16; i; i >>= 1) {
-        const DvStat o = dv_shfl(s, i);
-        s.sum += o.sum;
-        s.arg = s.max > o.max ? s.arg : o.max > s.max ? o.arg : min(s.arg, o.arg);
-        s.max = fmaxf(s.max, o.max);
-        s.bad |= o.bad;
+    if (GREEDY) {                                  // the first place of the block's largest
+        arg = arg != INT_MAX && mx == big ? arg + (int)(4 * (q0 + tid) - off) : INT_MAX;
+        arg = __reduce_min_sync(~0u, arg);
     }
-    if ((tid & 31) == 0) sst[tid >> 5] = s;
+    for (int i = 16; i; i >>= 1) sum += __shfl_xor_sync(~0u, sum, i);
+    if ((tid & 31) == 0) {
+        ssum[tid >> 5] = sum;
+        sarg[tid >> 5] = arg;
+    }
     __syncthreads();
     if (tid == 0) {
-        for (int w = 1; w < DV_THREADS / 32; ++w) {
-            const DvStat o = sst[w];
-            s.sum += o.sum;
-            s.arg = s.max > o.max ? s.arg : o.max > s.max ? o.arg : min(s.arg, o.arg);
-            s.max = fmaxf(s.max, o.max);
-            s.bad |= o.bad;
+        DvStat s{0.0, top, big, INT_MAX, any_bad};
+#pragma unroll
+        for (int w = 0; w < DV_THREADS / 32; ++w) {
+            s.sum += ssum[w];
+            s.arg = min(s.arg, sarg[w]);
         }
         a.stat[(size_t)row * a.parts + part] = s;
     }
 }
+
+__device__ __forceinline__ unsigned long long ld_cluster_u64(uint32_t addr) {
+    unsigned long long v;
+    asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
 // One row's parts joined by a warp (all lanes return it).
 __device__ __forceinline__ DvStat dv_row(const DvArgs& a, size_t row) {
@@ -230,7 +301,8 @@ __device__ __forceinline__ DvStat dv_row(const DvArgs& a, size_t row) {
 __global__ void __launch_bounds__(DP_THREADS, 2) dv_pick_kernel(const DvArgs a) {
     __shared__ DvStat st_t[DP_WARPS], st_d[DP_WARPS];
     __shared__ int verdict[DP_WARPS];              // 0: accepted, 1: the row draws, 2: no distribution
-    __shared__ unsigned long long wsum[DP_GROUPS][DP_WARPS], ctot[2];
+    __shared__ unsigned long long wsum[DP_WARPS][DP_SUMS], wtot[DP_WARPS], ctot[2];
+    extern __shared__ float4 ring[];               // [DP_AHEAD][target, draft][DP_THREADS]: each thread's own
     const int cluster = a.cluster, b = blockIdx.x / cluster, rank = (int)cluster_ctarank(), tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int V = a.vocab;
     pdl_wait();
@@ -249,18 +321,19 @@ __global__ void __launch_bounds__(DP_THREADS, 2) dv_pick_kernel(const DvArgs a) 
         const int mine = r + warp;
         if (mine < r1) {
             const bool last = mine == r1 - 1;
-            const DvStat t = dv_row(a, mine), d = a.draft && !last ? dv_row(a, (size_t)a.n_rows + mine) : t;
             const int x = last ? -1 : a.tokens[mine + 1];
+            const bool known = x >= 0 && x < V;
+            float lt = 0.0f, ld = 0.0f, u = 0.0f;
+            if (known && !a.greedy) {
+                lt = a.target[(size_t)mine * a.ldt + x];
+                if (a.draft) ld = a.draft[(size_t)mine * a.ldd + x];
+                u = a.u_accept[mine];
+            }
+            const DvStat t = dv_row(a, mine), d = a.draft && !last ? dv_row(a, (size_t)a.n_rows + mine) : t;
             int v = 1;
             if (t.bad || d.bad) v = 2;
-            else if (x >= 0 && x < V) {
-                const float lt = a.target[(size_t)mine * a.ldt + x];
-                if (a.greedy) v = x != t.arg;
-                else {
-                    const float q = a.draft ? dv_prob(a.draft[(size_t)mine * a.ldd + x], a.c, d) : 1.0f;
-                    v = !(__fmul_rn(a.u_accept[mine], q) < dv_prob(lt, a.c, t));
-                }
-            }
+            else if (known && a.greedy) v = x != t.arg;
+            else if (known) v = !(__fmul_rn(u, a.draft ? dv_prob(ld, a.c, d) : 1.0f) < dv_prob(lt, a.c, t));
             if (lane == 0) {
                 st_t[warp] = t;
                 st_d[warp] = d;
@@ -298,117 +371,142 @@ __global__ void __launch_bounds__(DP_THREADS, 2) dv_pick_kernel(const DvArgs a) 
             for (int i = r + 1 + tid; i < r1; i += DP_THREADS) a.logp[i] = 0.0f;
     }
     if (what == 2 || a.greedy) return;             // the whole cluster
-    // ---- draw from row r: the block's share is `runs` runs of 128 tokens a warp and group ----
+    // ---- draw from row r: a warp takes `mine` runs of 128 tokens one after the other, and keeps a sum of every
+    // `each` of them ----
     const float* d = a.draft && !last ? a.draft + (size_t)r * a.ldd : nullptr;
     const int x = last ? -1 : a.tokens[r + 1];
-    // both rows are read in quads of the target's alignment
+    // both rows are read in quads of the target's alignment (a draft row of another alignment value by value)
     const int off = dv_off(t);
     const bool same = !d || dv_off(d) == off;
     const long quads = ((long)off + V + 3) / 4;
-    const int share = (int)((quads + cluster - 1) / cluster);
-    const int runs = (share + DP_GROUPS * DP_THREADS - 1) / (DP_GROUPS * DP_THREADS);
-    const int groups = (share + runs * DP_THREADS - 1) / (runs * DP_THREADS);
-    const long q0 = (long)rank * groups * runs * DP_THREADS;
-    const DvInv it = dv_inv(st), id = dv_inv(sd);
-    auto load = [&](long q, bool rest, float4& tv, float4& dv) {
-        tv = dv_quad(t, off, q, V);
-        dv = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-        if (d && rest) {
-            if (same) dv = dv_quad(d, off, q, V);
-            else {
-                const long j = 4 * q - off;
-                if (j >= 0 && j < V) dv.x = d[j];
-                if (j + 1 >= 0 && j + 1 < V) dv.y = d[j + 1];
-                if (j + 2 >= 0 && j + 2 < V) dv.z = d[j + 2];
-                if (j + 3 >= 0 && j + 3 < V) dv.w = d[j + 3];
-            }
+    const int mine = (int)(((quads + 31) / 32 + cluster * DP_WARPS - 1) / (cluster * DP_WARPS));
+    const int each = max(4, (mine + DP_SUMS - 1) / DP_SUMS), sums = (mine + each - 1) / each;
+    const long q0 = (long)(rank * DP_WARPS + warp) * mine * 32 + lane;
+    const DvProb pt = dv_prepare(st, a.c), pd = dv_prepare(sd, a.c);
+    const bool quick = pt.quick && pd.quick;
+    // quad q of a row into a place of the ring: in the background where it lies inside the row
+    auto fetch = [&](const float* x, bool aligned, long q, float4* to) {
+        const long j = 4 * q - off;
+        if (aligned && j >= 0 && j + 4 <= V) {
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(to)), "l"(x + j) : "memory");
+        } else {
+            float e[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) e[i] = j + i >= 0 && j + i < V ? x[j + i] : -INFINITY;
+            *to = make_float4(e[0], e[1], e[2], e[3]);
         }
     };
-    // floor(w 2^38) = hi 2^19 + lo: adding 2^23 downwards leaves a whole number in the low bits
+    // floor(p 2^38) = hi 2^19 + lo: adding 2^23 downwards leaves a whole number in the low bits (above DP_BIAS)
+    constexpr uint32_t DP_BIAS = 0x4b000000u;
+    const f32x2 k19 = dv_pack(524288.0f, 524288.0f), k23 = dv_pack(8388608.0f, 8388608.0f), n23 = dv_pack(-8388608.0f, -8388608.0f);
     auto weights = [&](long q, bool rest, const float4& tv, const float4& dv, uint32_t (&hi)[4], uint32_t (&lo)[4]) {
-        const float e[4] = {tv.x, tv.y, tv.z, tv.w}, f[4] = {dv.x, dv.y, dv.z, dv.w};
+        const float e[4] = {tv.x, tv.y, tv.z, tv.w}, o[4] = {dv.x, dv.y, dv.z, dv.w};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            float p = dv_quotient(dv_weight(e[i], a.c, st.top), it);
-            if (rest) {
-                if (d) p = fmaxf(p - dv_quotient(dv_weight(f[i], a.c, sd.top), id), 0.0f);
-                else if (4 * q - off + i == x) p = 0.0f;
+        for (int i = 0; i < 4; i += 2) {
+            float p0, p1;
+            if (quick) {
+                f32x2 p = dv_prob2(e[i], e[i + 1], pt);
+                if (rest && d) p = dv_sub2(p, dv_prob2(o[i], o[i + 1], pd));
+                dv_unpack(p, p0, p1);
+            } else {
+                p0 = dv_prob(e[i], a.c, st);
+                p1 = dv_prob(e[i + 1], a.c, st);
+                if (rest && d) {
+                    p0 -= dv_prob(o[i], a.c, sd);
+                    p1 -= dv_prob(o[i + 1], a.c, sd);
+                }
             }
-            const float u = p * 524288.0f, h = __fadd_rd(u, 8388608.0f);
-            hi[i] = __float_as_uint(h) & 0xfffffu;
-            lo[i] = __float_as_uint(__fmaf_rd(u - (h - 8388608.0f), 524288.0f, 8388608.0f)) & 0xfffffu;
+            if (rest && !d) {
+                if (4 * q - off + i == x) p0 = 0.0f;
+                if (4 * q - off + i + 1 == x) p1 = 0.0f;
+            }
+            const f32x2 u = dv_mul2(dv_pack(fmaxf(p0, 0.0f), fmaxf(p1, 0.0f)), k19);
+            f32x2 h, l;
+            asm("add.rm.f32x2 %0, %1, %2;" : "=l"(h) : "l"(u), "l"(k23));
+            l = dv_sub2(u, dv_add2(h, n23));
+            asm("fma.rm.f32x2 %0, %1, %2, %3;" : "=l"(l) : "l"(l), "l"(k19), "l"(k23));
+            float v0, v1;
+            dv_unpack(h, v0, v1);
+            hi[i] = __float_as_uint(v0) - DP_BIAS;
+            hi[i + 1] = __float_as_uint(v1) - DP_BIAS;
+            dv_unpack(l, v0, v1);
+            lo[i] = __float_as_uint(v0) - DP_BIAS;
+            lo[i + 1] = __float_as_uint(v1) - DP_BIAS;
         }
     };
     for (int pass = 0; pass < 2; ++pass) {         // what is left of p over q; p itself if that is nothing
         const bool rest = pass == 0 && !last;
+        auto issue = [&](int i, int slot) {
+            const long q = q0 + 32L * i;
+            if (i < mine && q < quads) {
+                float4* at = ring + slot * 2 * DP_THREADS + tid;
+                fetch(t, true, q, at);
+                if (d && rest) fetch(d, same, q, at + DP_THREADS);
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+        for (int i = 0; i < DP_AHEAD - 1; ++i) issue(i, i);
+        uint32_t h = 0, l = 0;
+        int k = 0, e = 0;
         unsigned long long own = 0;
-        // (more than one run a group: vocabularies beyond 2^19 tokens and a block, whose groups are loaded one by one)
-        for (int g0 = 0; g0 < groups; g0 += DP_AHEAD) {
-            float4 tv[DP_AHEAD], dv[DP_AHEAD];
-            for (int k = 0; k < runs; ++k) {
-#pragma unroll
-                for (int j = 0; j < DP_AHEAD; ++j) {
-                    const long q = q0 + ((long)((g0 + j) * DP_WARPS + warp) * runs + k) * 32 + lane;
-                    tv[j] = dv[j] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-                    if (g0 + j < groups && q < quads) load(q, rest, tv[j], dv[j]);
-                }
-#pragma unroll
-                for (int j = 0; j < DP_AHEAD; ++j) {
-                    if (g0 + j >= groups) break;
-                    const long q = q0 + ((long)((g0 + j) * DP_WARPS + warp) * runs + k) * 32 + lane;
-                    uint32_t hi[4], lo[4];
-                    weights(q, rest, tv[j], dv[j], hi, lo);
-                    const uint32_t h = __reduce_add_sync(~0u, hi[0] + hi[1] + hi[2] + hi[3]);
-                    const uint32_t l = __reduce_add_sync(~0u, lo[0] + lo[1] + lo[2] + lo[3]);
-                    const unsigned long long s = ((unsigned long long)h << 19) + l;
-                    if (lane == 0) wsum[g0 + j][warp] = k ? wsum[g0 + j][warp] + s : s;
-                }
+#pragma unroll 1
+        for (int i = 0; i < mine; ++i) {
+            issue(i + DP_AHEAD - 1, (i + DP_AHEAD - 1) % DP_AHEAD);
+            asm volatile("cp.async.wait_group %0;" ::"n"(DP_AHEAD - 1) : "memory");
+            const long q = q0 + 32L * i;
+            if (q < quads) {
+                const float4* from = ring + i % DP_AHEAD * 2 * DP_THREADS + tid;
+                uint32_t hi[4], lo[4];
+                weights(q, rest, from[0], from[DP_THREADS], hi, lo);
+                h += hi[0] + hi[1] + hi[2] + hi[3];
+                l += lo[0] + lo[1] + lo[2] + lo[3];
+            }
+            if (++k == each || i == mine - 1) {
+                const unsigned long long s = ((unsigned long long)__reduce_add_sync(~0u, h) << 19) + __reduce_add_sync(~0u, l);
+                if (lane == 0) wsum[warp][e] = s;
+                own += s;
+                h = l = k = 0;
+                ++e;
             }
         }
+        if (lane == 0) wtot[warp] = own;
         __syncthreads();
-        if (warp == 0) {
-            for (int i = lane; i < groups * DP_WARPS; i += 32) own += wsum[i / DP_WARPS][i % DP_WARPS];
-            for (int i = 16; i; i >>= 1) own += __shfl_xor_sync(~0u, own, i);
-            if (lane == 0) ctot[pass] = own;
+        if (tid == 0) {
+            own = 0;
+            for (int w = 0; w < DP_WARPS; ++w) own += wtot[w];
+            ctot[pass] = own;
         }
         cluster_sync();
-        unsigned long long total = 0, before = 0;
-        for (int c = 0; c < cluster; ++c) {
-            unsigned long long v;
-            asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(mapa_shared(smem_u32(&ctot[pass]), c)) : "memory");
-            if (c < rank) before += v;
-            total += v;
+        unsigned long long total = lane < cluster ? ld_cluster_u64(mapa_shared(smem_u32(&ctot[pass]), lane)) : 0, before = 0;
+        for (int i = 1; i < 32; i <<= 1) {
+            const unsigned long long o = __shfl_up_sync(~0u, total, i);
+            if (lane >= i) total += o;
         }
+        if (rank > 0) before = __shfl_sync(~0u, total, rank - 1);
+        total = __shfl_sync(~0u, total, 31);
         if (total == 0 && pass == 0) continue;     // the whole cluster alike
         // [0, 1) in steps of 2^-24
         const unsigned long long u = (unsigned long long)(fminf(fmaxf(a.u_sample[b], 0.0f), 0.99999994f) * 16777216.0f);
         const unsigned long long goal = (total * u) >> 24;
-        const unsigned long long here = ctot[pass];
-        if (warp == 0 && goal >= before && goal < before + here) {
-            // the group and warp that hold it: a lane an even run of sums, then within the run
-            unsigned long long left = goal - before;
-            const int cnt = groups * DP_WARPS, per = (cnt + 31) / 32, i0 = min(cnt, lane * per), i1 = min(cnt, i0 + per);
-            unsigned long long s = 0, sum;
-            for (int i = i0; i < i1; ++i) s += wsum[i / DP_WARPS][i % DP_WARPS];
-            sum = s;
-            for (int i = 1; i < 32; i <<= 1) {
-                const unsigned long long o = __shfl_up_sync(~0u, sum, i);
-                if (lane >= i) sum += o;
-            }
-            const int src = __ffs(__ballot_sync(~0u, left < sum)) - 1;
-            left -= __shfl_sync(~0u, sum - s, src);
-            int at = min(cnt, src * per);
-            while (left >= wsum[at / DP_WARPS][at % DP_WARPS]) { left -= wsum[at / DP_WARPS][at % DP_WARPS]; ++at; }
-            for (int k = 0; k < runs; ++k) {
-                const long q = q0 + ((long)at * runs + k) * 32 + lane;
-                unsigned long long w[4] = {0, 0, 0, 0};
+        cluster_arrive();                          // (the totals have been read)
+        // the warp that holds it, the sum, the run, the token
+        if (goal >= before && goal < before + ctot[pass]) {
+            unsigned long long upto = before;
+            for (int w = 0; w < warp; ++w) upto += wtot[w];
+            if (goal < upto || goal >= upto + wtot[warp]) break;   // another warp's
+            unsigned long long left = goal - upto;
+            int e = 0;
+            while (e < sums - 1 && left >= wsum[warp][e]) left -= wsum[warp][e++];
+            for (int i = e * each; i < min(mine, (e + 1) * each); ++i) {
+                const long q = q0 + 32L * i;
+                unsigned long long w[4] = {0, 0, 0, 0}, s, sum;
                 if (q < quads) {
-                    float4 tv, dv;
                     uint32_t hi[4], lo[4];
-                    load(q, rest, tv, dv);
-                    weights(q, rest, tv, dv, hi, lo);
+                    fetch(t, false, q, ring + tid);
+                    if (d && rest) fetch(d, false, q, ring + DP_THREADS + tid);
+                    weights(q, rest, ring[tid], ring[DP_THREADS + tid], hi, lo);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) w[i] = ((unsigned long long)hi[i] << 19) + lo[i];
+                    for (int k2 = 0; k2 < 4; ++k2) w[k2] = ((unsigned long long)hi[k2] << 19) + lo[k2];
                 }
                 s = sum = w[0] + w[1] + w[2] + w[3];
                 for (int i = 1; i < 32; i <<= 1) {
@@ -422,9 +520,9 @@ __global__ void __launch_bounds__(DP_THREADS, 2) dv_pick_kernel(const DvArgs a) 
                 }
                 if (lane == __ffs(hit) - 1) {
                     left -= sum - s;
-                    int e = 0;
-                    while (e < 3 && left >= w[e]) left -= w[e++];
-                    const int tok = (int)(4 * q - off) + e;
+                    int k2 = 0;
+                    while (k2 < 3 && left >= w[k2]) left -= w[k2++];
+                    const int tok = (int)(4 * q - off) + k2;
                     a.next[b] = tok;
                     if (a.logp) a.logp[r] = dv_logp(t[tok], a.c, st);
                 }
@@ -433,7 +531,19 @@ __global__ void __launch_bounds__(DP_THREADS, 2) dv_pick_kernel(const DvArgs a) 
         }
         break;
     }
-    cluster_sync();                                // the totals are read by the others
+    cluster_wait();                                // no block ends while another reads its total
+}
+
+constexpr int DP_SMEM = DP_AHEAD * 2 * DP_THREADS * (int)sizeof(float4);
+
+// Blocks of a sequence's draw: 16 at most, and 4/3 an SM over all sequences.
+// Two an SM would hide more latency, but clusters stay within a GPC: 24
+// sequences by 10 blocks (240 of 296 places) ran in two waves (whole call 79.7
+// us), by 8 in one (72.0), by 6 with half the warps an SM (79.6).
+static int pick_cluster(const tk_ctx* ctx, int n_seqs, bool greedy) {
+    if (greedy) return 1;                          // a greedy row draws nothing
+    const int c = ctx->num_sms * 4 / 3 / n_seqs;
+    return c < 1 ? 1 : c > DP_CLUSTER ? DP_CLUSTER : c;
 }
 
 tk_status launch_draft_verify(tk_ctx* ctx, int n_seqs, const int32_t* row_start, int n_rows, int vocab,
@@ -457,9 +567,15 @@ tk_status launch_draft_verify(tk_ctx* ctx, int n_seqs, const int32_t* row_start,
     long part = (quads * rows + 4L * ctx->num_sms - 1) / (4L * ctx->num_sms);
     if (part < 4 * DV_THREADS) part = 4 * DV_THREADS;
     if (part > DV_QUADS * DV_THREADS) part = DV_QUADS * DV_THREADS;
-    // blocks of a sequence's draw: as many as are resident at once (two an SM), 16 at most
-    a.cluster = DP_CLUSTER;
-    while (a.cluster > 1 && (long)n_seqs * a.cluster > 2L * ctx->num_sms) a.cluster >>= 1;
+    a.cluster = pick_cluster(ctx, n_seqs, a.greedy);
+    static std::atomic<uint64_t> attr_smem{0}, attr_size{0};
+    cudaError_t e = smem_attr_once(dv_pick_kernel, DP_SMEM, ctx->device, attr_smem);
+    const uint64_t bit = 1ull << (ctx->device & 63);
+    if (e == cudaSuccess && !(attr_size.load(std::memory_order_relaxed) & bit)) {   // more than 8 blocks: on request
+        e = cudaFuncSetAttribute(dv_pick_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        if (e == cudaSuccess) attr_size.fetch_or(bit);
+    }
+    if (e != cudaSuccess) return cuda_fail(e, "draft verify attributes");
     const long parts = (quads + part - 1) / part, grid = parts * rows, pick = (long)n_seqs * a.cluster;
     if (grid > INT_MAX || pick > INT_MAX) return fail(TK_ERR_INVALID, "tk_draft_verify: too many rows");
     a.parts = (int)parts;
@@ -467,12 +583,6 @@ tk_status launch_draft_verify(tk_ctx* ctx, int n_seqs, const int32_t* row_start,
     tk_status st = ws_ensure(ctx, (size_t)grid * sizeof(DvStat), s);
     if (st != TK_OK) return st;
     a.stat = static_cast<DvStat*>(ctx->ws);
-    static std::atomic<uint64_t> attr_done{0};     // clusters of 16 are more than every GPU must offer: per device
-    if (!(attr_done.load(std::memory_order_relaxed) >> (ctx->device & 63) & 1)) {
-        const cudaError_t e = cudaFuncSetAttribute(dv_pick_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-        if (e != cudaSuccess) return cuda_fail(e, "draft verify cluster attribute");
-        attr_done.fetch_or(1ull << (ctx->device & 63));
-    }
     ProfScope ps(ctx, s, PK_SERVE);
     const bool small = a.part_quads <= 4 * DV_THREADS;
     auto kern = a.greedy ? (small ? dv_rows_kernel<true, 4> : dv_rows_kernel<true, DV_QUADS>)
@@ -481,6 +591,7 @@ tk_status launch_draft_verify(tk_ctx* ctx, int n_seqs, const int32_t* row_start,
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)pick);
     cfg.blockDim = dim3(DP_THREADS);
+    cfg.dynamicSmemBytes = DP_SMEM;
     cfg.stream = s;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -490,7 +601,7 @@ tk_status launch_draft_verify(tk_ctx* ctx, int n_seqs, const int32_t* row_start,
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, dv_pick_kernel, a);
+    e = cudaLaunchKernelEx(&cfg, dv_pick_kernel, a);
     ctx->launches += 2;
     if (e != cudaSuccess) return cuda_fail(e, "draft verify launch");
     return cuda_fail(cudaGetLastError(), "draft verify launch");
