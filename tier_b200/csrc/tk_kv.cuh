@@ -113,4 +113,82 @@ __device__ __forceinline__ float fast_exp2(float x) {
     return r;
 }
 
+
+// ---- attention ---------------------------------------------------------------
+struct KvaArgs {
+    KvView c;
+    SeqView s;
+    const void* q;
+    void* out;
+    long ldq, ldo;
+    int n_heads, group, window;
+    float scale2;         // scale * log2(e)
+    float* part;          // parts of divided rows (workspace)
+    int* count;           // finished parts of each sequence and key/value head, zero between calls
+    int* status;
+};
+
+__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+template <int DT>
+__device__ __forceinline__ void load_pairs8(const void* p, size_t at, float (&x)[8]) {
+    if constexpr (DT == TK_DT_F32) {
+        const float4* f = reinterpret_cast<const float4*>(static_cast<const float*>(p) + at);
+        const float4 u = f[0], v = f[1];
+        x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w; x[4] = v.x; x[5] = v.y; x[6] = v.z; x[7] = v.w;
+    } else {
+        const uint4 u = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + at);
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (DT == TK_DT_BF16) {
+                x[2 * i] = __uint_as_float(w[i] << 16);
+                x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+            } else {
+                x[2 * i] = h2f_bits((uint16_t)(w[i] & 0xffffu));
+                x[2 * i + 1] = h2f_bits((uint16_t)(w[i] >> 16));
+            }
+        }
+    }
+}
+// 2^e with max * 2^e in [2^13, 2^14); 1 for zero and for what is not finite.
+__device__ __forceinline__ float q_unit(float max, float& back) {
+    const int e = (int)(__float_as_uint(max) >> 23);
+    if (e < 14 || e >= 255) { back = 1.0f; return 1.0f; }
+    back = __uint_as_float((uint32_t)(e - 13) << 23);             // 2^(e - 127 - 13)
+    return __uint_as_float((uint32_t)(254 - (e - 13)) << 23);
+}
+
+// Values e .. e + 3 of an output row (packed row, head): O / l, zero where nothing was seen.
+struct KvaRow {
+    int row, head;
+};
+template <int DT, int D>
+__device__ __forceinline__ void kv_store_out(const KvaArgs& a, KvaRow r, int e, float4 o, float l) {
+    const float inv = l == 0.0f ? 0.0f : __fdividef(1.0f, l);
+    const size_t at = (size_t)r.row * a.ldo + (size_t)r.head * D + e;
+    if (l == 0.0f) o = make_float4(0, 0, 0, 0);
+    if constexpr (DT == TK_DT_F32) {
+        *reinterpret_cast<float4*>(static_cast<float*>(a.out) + at) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+    } else {
+        uint2 w;
+        if constexpr (DT == TK_DT_F16) {
+            w.x = (uint32_t)f2h_bits(o.x * inv) | ((uint32_t)f2h_bits(o.y * inv) << 16);
+            w.y = (uint32_t)f2h_bits(o.z * inv) | ((uint32_t)f2h_bits(o.w * inv) << 16);
+        } else {
+            w.x = (uint32_t)f2bf_bits(o.x * inv) | ((uint32_t)f2bf_bits(o.y * inv) << 16);
+            w.y = (uint32_t)f2bf_bits(o.z * inv) | ((uint32_t)f2bf_bits(o.w * inv) << 16);
+        }
+        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + at) = w;
+    }
+}
+
+// tk_kvattn_tc.cu
+tk_status launch_kv_prompt(tk_ctx* ctx, KvaArgs& a, int dtype, cudaStream_t st);
+// Zeroed counters for joins (tk_kvattn.cu).
+tk_status kv_count_ensure(tk_ctx* ctx, size_t n);
+
 }  // namespace tk

@@ -1,112 +1,8 @@
-// tk_kvattn.cu -- tk_kv_attend: attention of new tokens over the 4-bit cache.
+// tk_kvattn.cu -- tk_kv_attend: attention of new tokens over the 4-bit cache;
+// the streaming kernel for few rows (many: tk_kvattn_tc.cu).
 #include "tk_kv.cuh"
 
 namespace tk {
-
-struct KvaArgs {
-    KvView c;
-    SeqView s;
-    const void* q;
-    void* out;
-    long ldq, ldo;
-    int n_heads, group, window;
-    float scale2;         // scale * log2(e)
-    float* part;          // parts of divided rows (workspace)
-    int* count;           // finished parts of each sequence and key/value head, zero between calls
-    int* status;
-};
-
-template <int DT>
-__device__ __forceinline__ float ld_elem(const void* p, size_t i) {
-    if constexpr (DT == TK_DT_F32) return static_cast<const float*>(p)[i];
-    else if constexpr (DT == TK_DT_F16) return h2f_bits(static_cast<const uint16_t*>(p)[i]);
-    else return __uint_as_float((uint32_t) static_cast<const uint16_t*>(p)[i] << 16);
-}
-template <int DT>
-__device__ __forceinline__ void st_elem(void* p, size_t i, float x) {
-    if constexpr (DT == TK_DT_F32) static_cast<float*>(p)[i] = x;
-    else if constexpr (DT == TK_DT_F16) static_cast<uint16_t*>(p)[i] = f2h_bits(x);
-    else static_cast<uint16_t*>(p)[i] = f2bf_bits(x);
-}
-
-// One warp per (row, head): 32 keys at a time, a key per lane for the scores,
-// then head_dim / 32 outputs per lane over the 32 probabilities, with the
-// running maximum and sum of the softmax.
-template <int D, int DT>
-__global__ void __launch_bounds__(128) kv_attend_rows_kernel(const KvaArgs a) {
-    constexpr int E = D / 32;
-    __shared__ float qs[4][D];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const long item = (long)blockIdx.x * 4 + warp;
-    if (item >= (long)a.s.n_tokens * a.n_heads) return;
-    const int r = (int)(item / a.n_heads), h = (int)(item % a.n_heads), kh = h / a.group;
-    const int b = seq_of_row(a.s.q_start, a.s.n_seqs, r);
-    const SeqInfo sq = seq_info(a.s, a.c.page_shift, b, a.status);
-    if (r < sq.row0 || r - sq.row0 >= sq.n_new) return;
-    const int pos = sq.kv - sq.n_new + (r - sq.row0);
-    const int first = a.window > 0 && pos - a.window + 1 > 0 ? pos - a.window + 1 : 0;
-    for (int i = lane; i < D; i += 32) qs[warp][i] = ld_elem<DT>(a.q, (size_t)r * a.ldq + (size_t)h * D + i);
-    __syncwarp();
-    float o[E] = {}, m = -INFINITY, l = 0.0f;
-    for (int k0 = first; k0 <= pos; k0 += 32) {
-        const int key = k0 + lane;
-        float s = -INFINITY;
-        size_t row = 0;
-        if (key <= pos) {
-            row = kv_row(a.c, page_of(a.s, a.c, b, key, a.status), kh, key);
-            const uint32_t* w = reinterpret_cast<const uint32_t*>(a.c.kq) + row * (D / 8);
-            s = 0.0f;
-            for (int g = 0; g < D / 32; ++g) {
-                float t = 0.0f;
-                for (int j = 0; j < 4; ++j)
-                    for (int e = 0; e < 8; ++e) t += qs[warp][g * 32 + j * 8 + e] * (float)kv_nibble(w[g * 4 + j], e);
-                s += t * __half2float(a.c.ks[row * (D / 32) + g]);
-            }
-            s *= a.scale2;
-        }
-        float mx = s;
-        for (int i = 16; i; i >>= 1) mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, i));
-        const float mn = fmaxf(m, mx), fix = exp2f(m - mn);
-        m = mn;
-        const float p = key <= pos ? exp2f(s - m) : 0.0f;
-        float sum = p;
-        for (int i = 16; i; i >>= 1) sum += __shfl_xor_sync(~0u, sum, i);
-        l = l * fix + sum;
-        for (int e = 0; e < E; ++e) o[e] *= fix;
-        const int n = min(32, pos - k0 + 1);
-        for (int j = 0; j < n; ++j) {
-            const float pj = __shfl_sync(~0u, p, j);
-            const size_t rj = __shfl_sync(~0u, (unsigned long long)row, j);
-            const int e0 = lane * E;
-            const uint32_t w = reinterpret_cast<const uint32_t*>(a.c.vq)[rj * (D / 8) + (e0 >> 3)];
-            const float pd = pj * __half2float(a.c.vs[rj * (D / 32) + (e0 >> 5)]);
-            for (int e = 0; e < E; ++e) o[e] += pd * (float)kv_nibble(w, (e0 & 7) + e);
-        }
-    }
-    for (int e = 0; e < E; ++e)
-        st_elem<DT>(a.out, (size_t)r * a.ldo + (size_t)h * D + lane * E + e, l == 0.0f ? 0.0f : o[e] / l);
-}
-
-// Output of row r (of the block), values e .. e + 3: O / l, zero where nothing was seen.
-template <int DT, int D, class Item>
-__device__ __forceinline__ void kv_store_out(const KvaArgs& a, const Item& it, int r, int e, float4 o, float l) {
-    const float inv = l == 0.0f ? 0.0f : __fdividef(1.0f, l);
-    const size_t at = (size_t)(it.row0 + r / a.group) * a.ldo + (size_t)(it.head * a.group + r % a.group) * D + e;
-    if (l == 0.0f) o = make_float4(0, 0, 0, 0);
-    if constexpr (DT == TK_DT_F32) {
-        *reinterpret_cast<float4*>(static_cast<float*>(a.out) + at) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
-    } else {
-        uint2 w;
-        if constexpr (DT == TK_DT_F16) {
-            w.x = (uint32_t)f2h_bits(o.x * inv) | ((uint32_t)f2h_bits(o.y * inv) << 16);
-            w.y = (uint32_t)f2h_bits(o.z * inv) | ((uint32_t)f2h_bits(o.w * inv) << 16);
-        } else {
-            w.x = (uint32_t)f2bf_bits(o.x * inv) | ((uint32_t)f2bf_bits(o.y * inv) << 16);
-            w.y = (uint32_t)f2bf_bits(o.z * inv) | ((uint32_t)f2bf_bits(o.w * inv) << 16);
-        }
-        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + at) = w;
-    }
-}
 
 // The last of a head's parts to finish joins them, in the order of the keys
 // (the result does not depend on which block that is): parts are [16 rows, D]
@@ -165,7 +61,7 @@ __device__ __forceinline__ void kv_join_last(const KvaArgs& a, const Item& it, i
                 o.x += v[c].x * f; o.y += v[c].y * f; o.z += v[c].z * f; o.w += v[c].w * f;
             }
         }
-        kv_store_out<DT, D>(a, it, r, e, o, sum[r]);
+        kv_store_out<DT, D>(a, KvaRow{it.row0 + r / a.group, it.head * a.group + r % a.group}, e, o, sum[r]);
     }
 }
 
@@ -345,46 +241,12 @@ __device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4],
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
-    uint32_t r;
-    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-    return r;
-}
 // 8 x 8 fp16 matrix, row lane / 4, columns 2 (lane % 4), + 1: transposed.
 __device__ __forceinline__ uint32_t turn8x8(uint32_t x) {
     uint32_t r;
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
     return r;
 }
-template <int DT>
-__device__ __forceinline__ void load_pairs8(const void* p, size_t at, float (&x)[8]) {
-    if constexpr (DT == TK_DT_F32) {
-        const float4* f = reinterpret_cast<const float4*>(static_cast<const float*>(p) + at);
-        const float4 u = f[0], v = f[1];
-        x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w; x[4] = v.x; x[5] = v.y; x[6] = v.z; x[7] = v.w;
-    } else {
-        const uint4 u = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + at);
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if constexpr (DT == TK_DT_BF16) {
-                x[2 * i] = __uint_as_float(w[i] << 16);
-                x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-            } else {
-                x[2 * i] = h2f_bits((uint16_t)(w[i] & 0xffffu));
-                x[2 * i + 1] = h2f_bits((uint16_t)(w[i] >> 16));
-            }
-        }
-    }
-}
-// 2^e with max * 2^e in [2^13, 2^14); 1 for zero and for what is not finite.
-__device__ __forceinline__ float q_unit(float max, float& back) {
-    const int e = (int)(__float_as_uint(max) >> 23);
-    if (e < 14 || e >= 255) { back = 1.0f; return 1.0f; }
-    back = __uint_as_float((uint32_t)(e - 13) << 23);             // 2^(e - 127 - 13)
-    return __uint_as_float((uint32_t)(254 - (e - 13)) << 23);
-}
-
 template <int D, int DT, int NT>
 __global__ void __launch_bounds__(KD_WARPS * 32, KD_CTAS) kv_decode_kernel(const KvaArgs a, uint32_t least) {
     using G = KdGeo<D>;
@@ -732,7 +594,7 @@ __global__ void __launch_bounds__(KD_WARPS * 32, KD_CTAS) kv_decode_kernel(const
             ll += msh[(w * ROWS + r) * 2 + 1] * f;
             acc.x += v.x * f; acc.y += v.y * f; acc.z += v.z * f; acc.w += v.w * f;
         }
-        if (whole) kv_store_out<DT, D>(a, it, r, e, acc, ll);
+        if (whole) kv_store_out<DT, D>(a, KvaRow{it.row0 + r / a.group, it.head * a.group + r % a.group}, e, acc, ll);
         else {
             float* part = a.part + (size_t)it.slot * (16 * (D + 2));
             *reinterpret_cast<float4*>(part + r * D + e) = acc;
@@ -747,15 +609,8 @@ __global__ void __launch_bounds__(KD_WARPS * 32, KD_CTAS) kv_decode_kernel(const
   }
 }
 
-template <int D>
-static void go_rows(const KvaArgs& a, int dtype, unsigned grid, cudaStream_t st) {
-    if (dtype == TK_DT_F32) kv_attend_rows_kernel<D, TK_DT_F32><<<grid, 128, 0, st>>>(a);
-    else if (dtype == TK_DT_F16) kv_attend_rows_kernel<D, TK_DT_F16><<<grid, 128, 0, st>>>(a);
-    else kv_attend_rows_kernel<D, TK_DT_BF16><<<grid, 128, 0, st>>>(a);
-}
-
 // Zeroed counters for the join, grown on demand (synchronizes the device then).
-static tk_status count_ensure(tk_ctx* ctx, size_t n) {
+tk_status kv_count_ensure(tk_ctx* ctx, size_t n) {
     if (n <= ctx->kv_count_len) return TK_OK;
     cudaError_t e = cudaDeviceSynchronize();
     if (e != cudaSuccess) return cuda_fail(e, "tk_kv_attend: counter growth");
@@ -791,7 +646,7 @@ static tk_status go_decode(tk_ctx* ctx, KvaArgs& a, int dtype, cudaStream_t st) 
     if (pairs * ((size_t)a.s.max_pages << a.c.page_shift) / KD_UNIT + pairs > (1ull << 31))
         return fail(TK_ERR_UNSUPPORTED, "tk_kv_attend: sequences x heads x table length beyond 2^36 tokens");
     tk_status r = ws_ensure(ctx, (size_t)grid * 2 * (16 * (D + 2)) * sizeof(float), st);
-    if (r == TK_OK) r = count_ensure(ctx, pairs);
+    if (r == TK_OK) r = kv_count_ensure(ctx, pairs);
     if (r != TK_OK) return r;
     a.part = static_cast<float*>(ctx->ws);
     a.count = ctx->kv_count;
@@ -815,15 +670,10 @@ tk_status launch_kv_attend(tk_ctx* ctx, const tk_kvcache& c, const tk_seqs& s, c
     a.window = window;
     a.scale2 = (float)((double)scale * 1.4426950408889634);
     a.status = ctx->status;
-    const long grid = ((long)s.n_tokens * n_heads + 3) / 4;
-    if (grid > INT32_MAX) return fail(TK_ERR_INVALID, "tk_kv_attend: too many rows");
+    // few rows per key/value head are memory's work, many the tensor cores'
     if ((long)s.max_new * a.group <= 16)
         return c.head_dim == 64 ? go_decode<64>(ctx, a, dtype, st) : go_decode<128>(ctx, a, dtype, st);
-    ProfScope ps(ctx, st, PK_SERVE);
-    if (c.head_dim == 64) go_rows<64>(a, dtype, (unsigned)grid, st);
-    else go_rows<128>(a, dtype, (unsigned)grid, st);
-    ctx->launches++;
-    return cuda_fail(cudaGetLastError(), "kv attend launch");
+    return launch_kv_prompt(ctx, a, dtype, st);
 }
 
 }  // namespace tk

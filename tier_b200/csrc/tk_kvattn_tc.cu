@@ -1,0 +1,600 @@
+// tk_kvattn_tc.cu -- tk_kv_attend for many rows per key/value head (prompts,
+// chunks of them, long drafts): attention over the 4-bit cache on tcgen05.
+//
+// A block works on one key/value head of one sequence and up to two sets
+// ("streams") of 128 query rows (row = token * group + head of the group), one
+// tile of 128 keys after the other:
+//   S = Q K^T      both from shared memory, 128 x 128 in TMEM
+//   P = 2^(S - m)  one thread a row, written over S as fp16
+//   O += P V       P from TMEM, V from shared memory, 128 x head_dim in TMEM
+// fp32 rows enter as hi and lo fp16 parts, P too (two products each, one
+// stream's rows): 22 bits of each.  The tensor core works on one stream while
+// the other's softmax runs.  With at most 128 rows both streams take the same
+// rows and every other tile of keys, and are joined at the end.
+//
+// The keys and values of a tile are turned from 4 bits to fp16 once per block,
+// by four warps, a key a thread, one tile ahead in registers, straight into
+// the 128-byte-swizzled operand layout (the same bytes serve K, whose
+// reduction index is the head's values, and V, where it is the keys).
+//
+// As in the streaming kernel the softmax's reference moves only when a row
+// passes it by 2^8, so that O in TMEM is rarely rescaled.
+//
+// Warps (416 threads, one block an SM): 0-3 and 4-7 the streams' softmax, 8-11
+// the converters, 12 issues the products.  A row set that would leave SMs idle
+// is cut along the keys, and its parts joined by the last block to finish.
+#include "tk_kv.cuh"
+
+namespace tk {
+namespace kt {
+
+constexpr int ROWS = 128, KEYS = 128, THREADS = 13 * 32;
+
+template <int D, bool SPLIT>
+struct Geo {
+    static constexpr int TILE = 128 * D * 2;                       // bytes of 128 rows in fp16
+    static constexpr int PANEL = 128 * 128;                        // 64 columns of them
+    static constexpr int GROUP = SPLIT ? ROWS : 2 * ROWS;          // query rows of a block
+    static constexpr int SMEM = 6 * TILE + 1024;                   // q: 2 sets (or parts), K and V: 2 stages each
+    static constexpr uint32_t S = 0, O = 256;                      // TMEM columns: S of stream w at 128 w, O at 256 + D w
+    static constexpr int PART = GROUP * (D + 2);                   // floats of a part: O, then (m, l) of each row
+};
+
+struct Item {
+    int b, head, group, part, parts, id;   // id: of the row set (its counter)
+    int kv, n_new, row0, rows;             // rows: of this block, from row group * GROUP of the sequence
+    int lo, hi, t0, t1;                    // this part's tiles, and the keys [lo, hi) of them that some row may see
+};
+
+// What a sequence asks for: its row sets per head, and the tiles of the longest.
+struct Need {
+    SeqInfo q;
+    int groups, tiles;
+};
+template <int GROUP>
+__device__ __forceinline__ Need need(const KvaArgs& a, int b, int* status) {
+    Need n{SeqInfo{0, 0, 0}, 0, 0};
+    if (b >= a.s.n_seqs) return n;
+    n.q = seq_info(a.s, a.c.page_shift, b, status);
+    n.groups = (int)(((long)n.q.n_new * a.group + GROUP - 1) / GROUP);
+    n.tiles = (n.q.kv + KEYS - 1) / KEYS;
+    return n;
+}
+
+// Item `x`: sequences in order, within one the last rows (most keys) first,
+// heads innermost.  Row sets are cut into parts only while that leaves no more
+// blocks than SMs.
+template <int GROUP>
+__device__ __forceinline__ bool find(const KvaArgs& a, int x, int sms, Item& it) {
+    const int lane = threadIdx.x & 31;
+    int sets = 0;
+    long work = 0;                                                 // tiles of all row sets
+    for (int b0 = 0; b0 < a.s.n_seqs; b0 += 32) {
+        const Need n = need<GROUP>(a, b0 + lane, a.status);
+        sets += __reduce_add_sync(~0u, n.groups);
+        long w = (long)n.groups * n.tiles;
+        for (int i = 16; i; i >>= 1) w += __shfl_xor_sync(~0u, w, i);
+        work += w;
+    }
+    int per = INT32_MAX;                                           // tiles of a part
+    if (2 * sets * a.c.heads <= sms) {
+        // at most sms / 2 parts are begun and not full, so that twice the even
+        // share (six steps of an eighth) always fits
+        per = max(1, (int)((work * a.c.heads + sms - 1) / sms));
+        for (int step = 0; step < 6; ++step, per += (per + 7) / 8) {
+            int parts = 0;
+            for (int b0 = 0; b0 < a.s.n_seqs; b0 += 32) {
+                const Need n = need<GROUP>(a, b0 + lane, nullptr);
+                parts += __reduce_add_sync(~0u, n.groups * ((max(n.tiles, 1) + per - 1) / per));
+            }
+            if (parts * a.c.heads <= sms) break;
+        }
+        if (per < 2) per = 2;
+    }
+    int before = 0, id = 0;
+    for (int b0 = 0; b0 < a.s.n_seqs; b0 += 32) {
+        const Need n = need<GROUP>(a, b0 + lane, nullptr);
+        const int parts = per == INT32_MAX ? 1 : (max(n.tiles, 1) + per - 1) / per;
+        const int mine = n.groups * a.c.heads * parts;
+        int sum = mine, ids = n.groups * a.c.heads;
+        for (int i = 1; i < 32; i <<= 1) {
+            const int o = __shfl_up_sync(~0u, sum, i), p = __shfl_up_sync(~0u, ids, i);
+            if (lane >= i) { sum += o; ids += p; }
+        }
+        const unsigned hit = __ballot_sync(~0u, x < before + sum);
+        if (hit) {
+            const int src = __ffs(hit) - 1;
+            it.b = b0 + src;
+            it.kv = __shfl_sync(~0u, n.q.kv, src);
+            it.n_new = __shfl_sync(~0u, n.q.n_new, src);
+            it.row0 = __shfl_sync(~0u, n.q.row0, src);
+            it.parts = __shfl_sync(~0u, parts, src);
+            const int groups = __shfl_sync(~0u, n.groups, src);
+            const int at = x - before - __shfl_sync(~0u, sum - mine, src);
+            it.part = at % it.parts;
+            const int set = at / it.parts;
+            it.head = set % a.c.heads;
+            it.group = groups - 1 - set / a.c.heads;
+            it.id = id + __shfl_sync(~0u, ids - n.groups * a.c.heads, src) + set;
+            it.rows = (int)min((long)GROUP, (long)it.n_new * a.group - (long)it.group * GROUP);
+            const int pos0 = it.kv - it.n_new;
+            const int first = pos0 + (int)((long)it.group * GROUP / a.group);
+            const int last = pos0 + (int)(((long)it.group * GROUP + it.rows - 1) / a.group);
+            it.hi = max(last + 1, 0);
+            it.lo = a.window > 0 ? max(first + 1 - a.window, 0) : 0;
+            const int t = it.lo / KEYS, n2 = it.hi > it.lo ? (it.hi + KEYS - 1) / KEYS - t : 0;
+            it.t0 = t + (int)((long)n2 * it.part / it.parts);
+            it.t1 = t + (int)((long)n2 * (it.part + 1) / it.parts);
+            it.hi = min(it.hi, it.t1 * KEYS);                      // (a stream's last tile may lie behind the part)
+            return true;
+        }
+        before += __shfl_sync(~0u, sum, 31);
+        id += __shfl_sync(~0u, ids, 31);
+    }
+    return false;
+}
+
+__device__ __forceinline__ void tc_st_32x32b_x16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+__device__ __forceinline__ void tc_st_32x32b_x32(uint32_t taddr, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+        "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+__device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// D[tmem] (+)= A[tmem] * B[smem desc], kind::f16.
+__device__ __forceinline__ void tc_mma_f16_ta(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc,
+                                              uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+template <int D, int DT>
+__global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvaArgs a, int sms) {
+    constexpr bool SPLIT = DT == TK_DT_F32;
+    constexpr int PARTS = SPLIT ? 2 : 1;                           // fp16 parts of q and of P
+    using G = Geo<D, SPLIT>;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], q_full, s_full[2], p_full[2], o_full[2];
+    __shared__ uint32_t tmem_slot;
+    __shared__ float ml[2][ROWS][2];
+    __shared__ int sh_last;
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t *sq = smem, *sk = smem + 2 * G::TILE, *sv = smem + 4 * G::TILE;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    Item it;
+    if (!find<G::GROUP>(a, blockIdx.x, sms, it)) return;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&k_full[i], 128);
+            mbar_init(&v_full[i], 128);
+            mbar_init(&k_empty[i], 1);
+            mbar_init(&v_empty[i], 1);
+            mbar_init(&s_full[i], 1);
+            mbar_init(&p_full[i], 128);
+            mbar_init(&o_full[i], 1);
+        }
+        mbar_init(&q_full, 256);
+        fence_mbar_init();
+    }
+    if (warp == 12) {
+        tmem_alloc(&tmem_slot, 512);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot;
+
+    // both streams on the same rows, every other tile each
+    const bool same = SPLIT || it.rows <= ROWS;
+    const int tiles = it.t1 - it.t0;
+    const int steps = same ? (tiles + 1) / 2 : tiles;              // tiles of a stream
+    const int made = same ? 2 * steps : steps;                     // tiles made (the last may have no keys)
+    const int pos0 = it.kv - it.n_new;
+    // lane address of a softmax warp's rows
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    float l = 0.0f, nm = INFINITY;                                 // minus the reference; +inf before the first
+
+    if (warp < 8) {
+        // ---------------- softmax: thread = row ----------------
+        const int w = warp >> 2, r = (warp & 3) * 32 + lane, row = same ? r : w * ROWS + r;
+        const long grow = (long)it.group * G::GROUP + row;         // row of the sequence
+        const bool live = row < it.rows;
+        const int tok = live ? (int)(grow / a.group) : 0;
+        const int end = live ? max(pos0 + tok + 1, 0) : 0, from = a.window > 0 ? max(end - a.window, 0) : 0;
+        const int limit = min(end, it.hi);                         // keys [from, limit) are this part's and seen
+        float sc = 0.0f;
+        if (steps) {
+            // q to fp16 in shared memory: set w (of a split: both parts, by the first stream)
+            const size_t at = (size_t)(it.row0 + tok) * a.ldq + (size_t)(it.head * a.group + (live ? grow % a.group : 0)) * D;
+            float mx = 0.0f;
+            if (live)
+                for (int c = 0; c < D / 8; ++c) {
+                    float x[8];
+                    load_pairs8<DT>(a.q, at + c * 8, x);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(x[e]));
+                }
+            float back;
+            const float up = copysignf(q_unit(mx, back), a.scale2);
+            sc = back * fabsf(a.scale2);
+            if (w == 0 || !same)
+                for (int c = 0; c < D / 8; ++c) {
+                    float x[8] = {};
+                    if (live) load_pairs8<DT>(a.q, at + c * 8, x);
+                    uint32_t hi[4], lo[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float u = x[2 * e] * up, v = x[2 * e + 1] * up;
+                        hi[e] = pack_half2(u, v);
+                        lo[e] = pack_half2(u - __low2float(as_half2(hi[e])), v - __high2float(as_half2(hi[e])));
+                    }
+                    uint8_t* to = sq + w * G::TILE + (c >> 3) * G::PANEL + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+                    *reinterpret_cast<uint4*>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                    if constexpr (SPLIT) *reinterpret_cast<uint4*>(to + G::TILE) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                }
+            fence_async_shared();
+            mbar_arrive(&q_full);
+        }
+        const uint32_t ts = tmem + lanes + G::S + w * 128, to = tmem + lanes + G::O + w * D;
+        const bool any_live = __any_sync(~0u, live);
+        for (int j = 0; j < steps; ++j) {
+            const int key0 = (it.t0 + (same ? 2 * j + w : j)) * KEYS;
+            if (!__all_sync(~0u, mbar_wait(&s_full[w], j & 1, a.status))) break;
+            tc_fence_after();
+            if (any_live) {
+                const bool edge = __any_sync(~0u, live && (key0 + KEYS > limit || key0 < from));
+                const unsigned width = max(limit - from, 0);
+                const int rel = key0 - from;
+                float mx = -INFINITY;
+#pragma unroll 1
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t x[32];
+                    tc_ld_32x32b_x32(ts + c * 32, x);
+                    tc_wait_ld();
+                    if (edge) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i)
+                            if ((unsigned)(rel + c * 32 + i) < width) mx = fmaxf(mx, __uint_as_float(x[i]));
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) mx = fmaxf(mx, __uint_as_float(x[i]));
+                    }
+                }
+                mx *= sc;                                          // (-inf * 0 = NaN: no key and no scale)
+                const bool move = mx + nm > 8.0f;
+                if (__any_sync(~0u, move)) {
+                    const float now = move ? -mx : nm;
+                    const float f = now == INFINITY ? 1.0f : fast_exp2(now - nm);
+                    nm = now;
+                    l *= f;
+                    if (j > 0) {
+#pragma unroll 1
+                        for (int c = 0; c < D; c += 32) {
+                            uint32_t x[32];
+                            tc_ld_32x32b_x32(to + c, x);
+                            tc_wait_ld();
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) * f);
+                            tc_st_32x32b_x32(to + c, x);
+                        }
+                        tc_wait_st();
+                    }
+                }
+                const float ref = nm == INFINITY ? 0.0f : nm;
+                uint32_t low[PARTS == 2 ? 64 : 1];                 // P's lo parts wait until S has been read
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t x[32], hi[16];
+                    tc_ld_32x32b_x32(ts + c * 32, x);
+                    tc_wait_ld();
+#pragma unroll
+                    for (int i = 0; i < 32; i += 2) {
+                        float v0 = fmaf(__uint_as_float(x[i]), sc, ref), v1 = fmaf(__uint_as_float(x[i + 1]), sc, ref);
+                        if (edge) {
+                            if ((unsigned)(rel + c * 32 + i) >= width) v0 = -INFINITY;
+                            if ((unsigned)(rel + c * 32 + i + 1) >= width) v1 = -INFINITY;
+                        }
+                        const float p0 = fast_exp2(v0), p1 = fast_exp2(v1);
+                        l += p0 + p1;
+                        hi[i / 2] = pack_half2(p0, p1);
+                        if constexpr (SPLIT)
+                            low[c * 16 + i / 2] = pack_half2(p0 - __low2float(as_half2(hi[i / 2])),
+                                                             p1 - __high2float(as_half2(hi[i / 2])));
+                    }
+                    tc_st_32x32b_x16(ts + c * 16, hi);
+                }
+                if constexpr (SPLIT) {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t x[16];
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) x[i] = low[c * 16 + i];
+                        tc_st_32x32b_x16(ts + 64 + c * 16, x);
+                    }
+                }
+                tc_wait_st();
+            }
+            tc_fence_before();
+            mbar_arrive(&p_full[w]);
+        }
+        if (steps) {
+            mbar_wait(&o_full[w], 0, a.status);
+            tc_fence_after();
+        }
+        ml[w][r][0] = -nm;
+        ml[w][r][1] = l;
+    } else if (warp < 12) {
+        // ---------------- converters: thread = key of the tile ----------------
+        const int t = threadIdx.x - 256;
+        uint4 kr[D / 32], vr[D / 32];
+        uint32_t ks[D / 64], vs[D / 64];
+        auto fetch = [&](int i) {
+            const int pos = (it.t0 + i) * KEYS + t;
+            const bool in = i < made && pos >= it.lo && pos < it.hi;   // hi <= kv
+            const size_t row = in ? kv_row(a.c, page_of(a.s, a.c, it.b, pos, a.status), it.head, pos) : 0;
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c) {
+                kr[c] = vr[c] = make_uint4(0, 0, 0, 0);
+                if (in) {
+                    kr[c] = __ldg(reinterpret_cast<const uint4*>(a.c.kq + row * (D / 2)) + c);
+                    vr[c] = __ldg(reinterpret_cast<const uint4*>(a.c.vq + row * (D / 2)) + c);
+                }
+            }
+#pragma unroll
+            for (int c = 0; c < D / 64; ++c) {
+                ks[c] = vs[c] = 0;
+                if (in) {
+                    ks[c] = __ldg(reinterpret_cast<const uint32_t*>(a.c.ks + row * (D / 32)) + c);
+                    vs[c] = __ldg(reinterpret_cast<const uint32_t*>(a.c.vs + row * (D / 32)) + c);
+                }
+            }
+        };
+        auto store = [&](const uint4 (&x)[D / 32], const uint32_t (&s)[D / 64], uint8_t* to) {
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c) {
+                const __half2 sc2 = as_half2(s[c >> 1]);
+                const __half2 d = c & 1 ? __high2half2(sc2) : __low2half2(sc2);
+                const uint32_t w4[4] = {x[c].x, x[c].y, x[c].z, x[c].w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    uint32_t f[4];
+                    kv_fields(w4[i], d, f);
+                    const int chunk = 4 * c + i;
+                    *reinterpret_cast<uint4*>(to + (chunk >> 3) * G::PANEL + t * 128 + (((chunk & 7) ^ (t & 7)) << 4)) =
+                        make_uint4(f[0], f[1], f[2], f[3]);
+                }
+            }
+        };
+        if (made) fetch(0);
+        for (int i = 0; i < made; ++i) {
+            const int st = i & 1;
+            const uint32_t parity = ((i >> 1) & 1) ^ 1;
+            if (!__all_sync(~0u, mbar_wait(&k_empty[st], parity, a.status))) break;
+            store(kr, ks, sk + st * G::TILE);
+            fence_async_shared();
+            mbar_arrive(&k_full[st]);
+            if (!__all_sync(~0u, mbar_wait(&v_empty[st], parity, a.status))) break;
+            store(vr, vs, sv + st * G::TILE);
+            fence_async_shared();
+            mbar_arrive(&v_full[st]);
+            fetch(i + 1);
+        }
+    } else if (lane == 0 && steps) {
+        // ---------------- products ----------------
+        constexpr uint32_t id_s = idesc_f16(128, KEYS, 0, 0, 0), id_o = idesc_f16(128, D, 0, 0, 1);
+        const uint32_t q0 = smem_u32(sq), k0 = smem_u32(sk), v0 = smem_u32(sv);
+        bool ok = mbar_wait(&q_full, 0, a.status);
+        auto product_s = [&](int w, int i) {                       // stream w, tile i of the ring
+            const uint32_t kb = k0 + (i & 1) * G::TILE;
+#pragma unroll
+            for (int p = PARTS - 1; p >= 0; --p) {
+                const uint32_t qb = q0 + (SPLIT ? p : same ? 0 : w) * G::TILE;
+#pragma unroll
+                for (int kk = 0; kk < D / 16; ++kk) {
+                    const uint32_t off = (kk >> 2) * G::PANEL + (kk & 3) * 32;
+                    tc_mma_f16(tmem + G::S + w * 128, sdesc_sw128(qb + off, 16, 1024), sdesc_sw128(kb + off, 16, 1024), id_s,
+                               p != PARTS - 1 || kk > 0);
+                }
+            }
+            tc_commit(&s_full[w]);
+            if (same || w == 1) tc_commit(&k_empty[i & 1]);
+        };
+        for (int w = 0; w < 2 && ok; ++w) {
+            const int i = same ? w : 0;
+            ok = mbar_wait(&k_full[i & 1], (i >> 1) & 1, a.status);
+            tc_fence_after();
+            if (ok) product_s(w, i);
+        }
+        for (int j = 0; j < steps && ok; ++j)
+            for (int w = 0; w < 2 && ok; ++w) {
+                const int i = same ? 2 * j + w : j;
+                ok = mbar_wait(&v_full[i & 1], (i >> 1) & 1, a.status) && mbar_wait(&p_full[w], j & 1, a.status);
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t vb = v0 + (i & 1) * G::TILE;
+#pragma unroll
+                for (int p = PARTS - 1; p >= 0; --p)
+#pragma unroll
+                    for (int kk = 0; kk < KEYS / 16; ++kk)
+                        tc_mma_f16_ta(tmem + G::O + w * D, tmem + G::S + w * 128 + p * 64 + kk * 8,
+                                      sdesc_sw128(vb + kk * 2048, G::PANEL, 1024), id_o, j > 0 || p != PARTS - 1 || kk > 0);
+                if (same || w == 1) tc_commit(&v_empty[i & 1]);
+                if (j + 1 < steps) {
+                    const int n = same ? i + 2 : j + 1;
+                    ok = mbar_wait(&k_full[n & 1], (n >> 1) & 1, a.status);
+                    tc_fence_after();
+                    if (ok) product_s(w, n);
+                } else {
+                    tc_commit(&o_full[w]);
+                }
+            }
+        if (!ok) {      // reported; what was issued ends first
+            tc_commit(&o_full[0]);
+            tc_commit(&o_full[1]);
+            mbar_wait(&o_full[0], 0, a.status);
+            mbar_wait(&o_full[1], 0, a.status);
+        }
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();                                               // every product is done, ml is written
+    tc_fence_after();
+
+    // ---- output ----
+    const int w = warp >> 2, r = (warp & 3) * 32 + lane;
+    float* osh = reinterpret_cast<float*>(smem);                   // [128][D + 4]: the second stream's O of the same rows
+    if (same && warp >= 4 && warp < 8 && steps)
+#pragma unroll 1
+        for (int c = 0; c < D; c += 32) {
+            uint32_t x[32];
+            tc_ld_32x32b_x32(tmem + lanes + G::O + D + c, x);
+            tc_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; i += 4)
+                *reinterpret_cast<uint4*>(osh + r * (D + 4) + c + i) = make_uint4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+        }
+    if (same) __syncthreads();
+    if (warp < (same ? 4 : 8)) {
+        const int row = same ? r : w * ROWS + r;
+        float m = ml[w][r][0], sum = ml[w][r][1], f0 = 1.0f, f1 = 0.0f;
+        if (same) {
+            const float m1 = ml[1][r][0], big = fmaxf(m, m1), ref = big == -INFINITY ? 0.0f : big;
+            f0 = fast_exp2(m - ref);
+            f1 = fast_exp2(m1 - ref);
+            sum = sum * f0 + ml[1][r][1] * f1;
+            m = big;
+        }
+        const long grow = (long)it.group * G::GROUP + row;
+        const bool live = row < it.rows;
+        const KvaRow to{it.row0 + (int)(grow / a.group), it.head * a.group + (int)(grow % a.group)};
+        float* part = it.parts > 1 ? a.part + (size_t)blockIdx.x * G::PART : nullptr;
+        if (part && live) {
+            part[G::GROUP * D + 2 * row] = m;
+            part[G::GROUP * D + 2 * row + 1] = sum;
+        }
+#pragma unroll 1
+        for (int c = 0; c < D; c += 32) {
+            uint32_t x[32];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) x[i] = 0;
+            if (steps) {                                           // (uniform)
+                tc_ld_32x32b_x32(tmem + lanes + G::O + w * D + c, x);
+                tc_wait_ld();
+            }
+            if (!live) continue;
+#pragma unroll
+            for (int i = 0; i < 32; i += 4) {
+                float4 o = make_float4(__uint_as_float(x[i]) * f0, __uint_as_float(x[i + 1]) * f0,
+                                       __uint_as_float(x[i + 2]) * f0, __uint_as_float(x[i + 3]) * f0);
+                if (same && steps) {
+                    const float4 u = *reinterpret_cast<const float4*>(osh + r * (D + 4) + c + i);
+                    o.x += u.x * f1; o.y += u.y * f1; o.z += u.z * f1; o.w += u.w * f1;
+                }
+                if (part) *reinterpret_cast<float4*>(part + row * D + c + i) = o;
+                else kv_store_out<DT, D>(a, to, c + i, o, sum);
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 12) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+    if (it.parts == 1) return;
+    // ---- the last part of the rows to finish joins them, in the order of the keys ----
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        const int done = atomicAdd(a.count + it.id, 1) + 1;
+        sh_last = done == it.parts;
+        if (sh_last) a.count[it.id] = 0;
+    }
+    __syncthreads();
+    if (!sh_last) return;
+    __threadfence();
+    const float* base = a.part + (size_t)(blockIdx.x - it.part) * G::PART;
+    for (int i = threadIdx.x; i < it.rows * (D / 4); i += THREADS) {
+        const int row = i / (D / 4), e = (i - row * (D / 4)) * 4;
+        float m = -INFINITY, sum = 0.0f;
+        float4 o = make_float4(0, 0, 0, 0);
+        for (int c0 = 0; c0 < it.parts; c0 += 8) {                 // eight parts' loads in flight
+            float4 v[8];
+            float2 st[8];
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+                const float* p = base + (size_t)min(c0 + c, it.parts - 1) * G::PART;
+                v[c] = __ldcg(reinterpret_cast<const float4*>(p + row * D + e));
+                st[c] = __ldcg(reinterpret_cast<const float2*>(p + G::GROUP * D + 2 * row));
+                if (c0 + c >= it.parts) st[c] = make_float2(-INFINITY, 0.0f);
+            }
+            float big = m;
+#pragma unroll
+            for (int c = 0; c < 8; ++c) big = fmaxf(big, st[c].x);
+            const float ref = big == -INFINITY ? 0.0f : big, f = fast_exp2(m - ref);
+            sum *= f;
+            o.x *= f; o.y *= f; o.z *= f; o.w *= f;
+            m = big;
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+                if (c0 + c >= it.parts) break;
+                const float g = fast_exp2(st[c].x - ref);
+                sum += st[c].y * g;
+                o.x += v[c].x * g; o.y += v[c].y * g; o.z += v[c].z * g; o.w += v[c].w * g;
+            }
+        }
+        const long grow = (long)it.group * G::GROUP + row;
+        kv_store_out<DT, D>(a, KvaRow{it.row0 + (int)(grow / a.group), it.head * a.group + (int)(grow % a.group)}, e, o, sum);
+    }
+}
+
+template <int D, int DT>
+static tk_status go(tk_ctx* ctx, KvaArgs& a, cudaStream_t st) {
+    using G = Geo<D, DT == TK_DT_F32>;
+    static std::atomic<uint64_t> attr_done{0};
+    auto kern = kv_prompt_kernel<D, DT>;
+    cudaError_t e = smem_attr_once(kern, G::SMEM, ctx->device, attr_done);
+    if (e != cudaSuccess) return cuda_fail(e, "kv prompt smem attribute");
+    // no more row sets than whole groups of all rows and one begun per
+    // sequence; cut into parts only where there are at most as many as SMs
+    const long sets = (((long)a.s.n_tokens * a.group + G::GROUP - 1) / G::GROUP + a.s.n_seqs) * a.c.heads;
+    const long grid = sets > ctx->num_sms ? sets : ctx->num_sms;
+    if (grid > INT32_MAX) return fail(TK_ERR_INVALID, "tk_kv_attend: too many rows");
+    tk_status r = ws_ensure(ctx, (size_t)ctx->num_sms * G::PART * sizeof(float), st);
+    if (r == TK_OK) r = kv_count_ensure(ctx, (size_t)sets);
+    if (r != TK_OK) return r;
+    a.part = static_cast<float*>(ctx->ws);
+    a.count = ctx->kv_count;
+    ProfScope ps(ctx, st, PK_SERVE);
+    kern<<<(unsigned)grid, THREADS, G::SMEM, st>>>(a, ctx->num_sms);
+    ctx->launches++;
+    return cuda_fail(cudaGetLastError(), "kv prompt launch");
+}
+
+}  // namespace kt
+
+tk_status launch_kv_prompt(tk_ctx* ctx, KvaArgs& a, int dtype, cudaStream_t st) {
+    const bool wide = a.c.dim == 128;
+    if (dtype == TK_DT_F32) return wide ? kt::go<128, TK_DT_F32>(ctx, a, st) : kt::go<64, TK_DT_F32>(ctx, a, st);
+    if (dtype == TK_DT_F16) return wide ? kt::go<128, TK_DT_F16>(ctx, a, st) : kt::go<64, TK_DT_F16>(ctx, a, st);
+    return wide ? kt::go<128, TK_DT_BF16>(ctx, a, st) : kt::go<64, TK_DT_BF16>(ctx, a, st);
+}
+
+}  // namespace tk
