@@ -20,15 +20,18 @@
 // As in the streaming kernel the softmax's reference moves only when a row
 // passes it by 2^8, so that O in TMEM is rarely rescaled.
 //
-// Warps (416 threads, one block an SM): 0-3 and 4-7 the streams' softmax, 8-11
-// the converters, 12 issues the products.  A row set that would leave SMs idle
+// Warps (512 threads, one block an SM): 0-3 and 4-7 the streams' softmax, 8-11
+// the converters, 12 issues the products (13-15 idle: registers are divided by
+// groups of four warps).  A row set that would leave SMs idle
 // is cut along the keys, and its parts joined by the last block to finish.
 #include "tk_kv.cuh"
 
 namespace tk {
 namespace kt {
 
-constexpr int ROWS = 128, KEYS = 128, THREADS = 13 * 32;
+constexpr int ROWS = 128, KEYS = 128, THREADS = 512;
+// registers a thread of each warpgroup: 4 x 128 at launch, 184 + 184 + 88 + 56 = 512 after the split
+constexpr int REG_SOFTMAX = 184, REG_CONVERT = 88, REG_ISSUE = 56;
 
 template <int D, bool SPLIT>
 struct Geo {
@@ -141,17 +144,42 @@ __device__ __forceinline__ void tc_st_32x32b_x16(uint32_t taddr, const uint32_t 
         "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
         : "memory");
 }
-__device__ __forceinline__ void tc_st_32x32b_x32(uint32_t taddr, const uint32_t (&r)[32]) {
+__device__ __forceinline__ void tc_ld_32x32b_x16(uint32_t taddr, uint32_t (&r)[16]) {
     asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
-        "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
-        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
-        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
-        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
-        : "memory");
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
 }
 __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void reg_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void reg_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+// The two softmax warpgroups' own barrier.
+__device__ __forceinline__ void softmax_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pack2(float a, float b) {
+    f32x2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void unpack2(f32x2 v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+    f32x2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+    f32x2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
 // D[tmem] (+)= A[tmem] * B[smem desc], kind::f16.
 __device__ __forceinline__ void tc_mma_f16_ta(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc,
                                               uint32_t accumulate) {
@@ -161,6 +189,56 @@ __device__ __forceinline__ void tc_mma_f16_ta(uint32_t d_tmem, uint32_t a_tmem, 
         "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
         "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
         : "memory");
+}
+
+// The last part of a row set to finish joins them, in the order of the keys
+// (by the softmax warpgroups; parts lie by block).
+template <int D, int DT>
+__device__ __forceinline__ void join_parts(const KvaArgs& a, const Item& it, int* sh_last) {
+    using G = Geo<D, DT == TK_DT_F32>;
+    __threadfence();
+    softmax_sync();
+    if (threadIdx.x == 0) {
+        const int done = atomicAdd(a.count + it.id, 1) + 1;
+        *sh_last = done == it.parts;
+        if (*sh_last) a.count[it.id] = 0;
+    }
+    softmax_sync();
+    if (!*sh_last) return;
+    __threadfence();
+    const float* base = a.part + (size_t)(blockIdx.x - it.part) * G::PART;
+    for (int i = threadIdx.x; i < it.rows * (D / 4); i += 256) {
+        const int row = i / (D / 4), e = (i - row * (D / 4)) * 4;
+        float m = -INFINITY, sum = 0.0f;
+        float4 o = make_float4(0, 0, 0, 0);
+        for (int c0 = 0; c0 < it.parts; c0 += 8) {                 // eight parts' loads in flight
+            float4 v[8];
+            float2 st[8];
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+                const float* p = base + (size_t)min(c0 + c, it.parts - 1) * G::PART;
+                v[c] = __ldcg(reinterpret_cast<const float4*>(p + row * D + e));
+                st[c] = __ldcg(reinterpret_cast<const float2*>(p + G::GROUP * D + 2 * row));
+                if (c0 + c >= it.parts) st[c] = make_float2(-INFINITY, 0.0f);
+            }
+            float big = m;
+#pragma unroll
+            for (int c = 0; c < 8; ++c) big = fmaxf(big, st[c].x);
+            const float ref = big == -INFINITY ? 0.0f : big, f = fast_exp2(m - ref);
+            sum *= f;
+            o.x *= f; o.y *= f; o.z *= f; o.w *= f;
+            m = big;
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+                if (c0 + c >= it.parts) break;
+                const float g = fast_exp2(st[c].x - ref);
+                sum += st[c].y * g;
+                o.x += v[c].x * g; o.y += v[c].y * g; o.z += v[c].z * g; o.w += v[c].w * g;
+            }
+        }
+        const long grow = (long)it.group * G::GROUP + row;
+        kv_store_out<DT, D>(a, KvaRow{it.row0 + (int)(grow / a.group), it.head * a.group + (int)(grow % a.group)}, e, o, sum);
+    }
 }
 
 template <int D, int DT>
@@ -209,9 +287,10 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvaArgs a, 
     const int pos0 = it.kv - it.n_new;
     // lane address of a softmax warp's rows
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    float l = 0.0f, nm = INFINITY;                                 // minus the reference; +inf before the first
 
     if (warp < 8) {
+        reg_inc<REG_SOFTMAX>();
+        float l = 0.0f, nm = INFINITY;                             // nm: minus the reference; +inf before the first
         // ---------------- softmax: thread = row ----------------
         const int w = warp >> 2, r = (warp & 3) * 32 + lane, row = same ? r : w * ROWS + r;
         const long grow = (long)it.group * G::GROUP + row;         // row of the sequence
@@ -233,7 +312,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvaArgs a, 
                 }
             float back;
             const float up = copysignf(q_unit(mx, back), a.scale2);
-            sc = back * fabsf(a.scale2);
+            sc = fmaxf(back * fabsf(a.scale2), 1e-37f);            // above zero: masked scores stay -inf
             if (w == 0 || !same)
                 for (int c = 0; c < D / 8; ++c) {
                     float x[8] = {};
@@ -260,24 +339,29 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvaArgs a, 
             tc_fence_after();
             if (any_live) {
                 const bool edge = __any_sync(~0u, live && (key0 + KEYS > limit || key0 < from));
-                const unsigned width = max(limit - from, 0);
-                const int rel = key0 - from;
-                float mx = -INFINITY;
-#pragma unroll 1
-                for (int c = 0; c < 4; ++c) {
-                    uint32_t x[32];
-                    tc_ld_32x32b_x32(ts + c * 32, x);
-                    tc_wait_ld();
-                    if (edge) {
+                // S of the whole row in registers
+                float x[KEYS];
 #pragma unroll
-                        for (int i = 0; i < 32; ++i)
-                            if ((unsigned)(rel + c * 32 + i) < width) mx = fmaxf(mx, __uint_as_float(x[i]));
-                    } else {
+                for (int c = 0; c < 4; ++c) tc_ld_32x32b_x32(ts + c * 32, *reinterpret_cast<uint32_t(*)[32]>(x + c * 32));
+                tc_wait_ld();
+                if (edge) {                                        // what the row does not see
+                    const unsigned width = max(limit - from, 0);
+                    const int rel = key0 - from;
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) mx = fmaxf(mx, __uint_as_float(x[i]));
+                    for (int i = 0; i < KEYS; ++i)
+                        if ((unsigned)(rel + i) >= width) x[i] = -INFINITY;
+                }
+                float m0 = x[0], m1 = x[1], m2 = x[2], m3 = x[3];
+#pragma unroll
+                for (int i = 4; i < KEYS; i += 8) {
+                    m0 = max3(m0, x[i], x[i + 1]);
+                    m1 = max3(m1, x[i + 2], x[i + 3]);
+                    if (i + 4 < KEYS) {
+                        m2 = max3(m2, x[i + 4], x[i + 5]);
+                        m3 = max3(m3, x[i + 6], x[i + 7]);
                     }
                 }
-                mx *= sc;                                          // (-inf * 0 = NaN: no key and no scale)
+                const float mx = fmaxf(max3(m0, m1, m2), m3) * sc;
                 const bool move = mx + nm > 8.0f;
                 if (__any_sync(~0u, move)) {
                     const float now = move ? -mx : nm;
@@ -286,49 +370,38 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvaArgs a, 
                     l *= f;
                     if (j > 0) {
 #pragma unroll 1
-                        for (int c = 0; c < D; c += 32) {
-                            uint32_t x[32];
-                            tc_ld_32x32b_x32(to + c, x);
+                        for (int c = 0; c < D; c += 16) {
+                            uint32_t y[16];
+                            tc_ld_32x32b_x16(to + c, y);
                             tc_wait_ld();
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) * f);
-                            tc_st_32x32b_x32(to + c, x);
+                            for (int i = 0; i < 16; ++i) y[i] = __float_as_uint(__uint_as_float(y[i]) * f);
+                            tc_st_32x32b_x16(to + c, y);
                         }
                         tc_wait_st();
                     }
                 }
-                const float ref = nm == INFINITY ? 0.0f : nm;
-                uint32_t low[PARTS == 2 ? 64 : 1];                 // P's lo parts wait until S has been read
+                const f32x2 sc2 = pack2(sc, sc), ref2 = nm == INFINITY ? pack2(0.0f, 0.0f) : pack2(nm, nm);
+                f32x2 sum = pack2(l, 0.0f);
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
-                    uint32_t x[32], hi[16];
-                    tc_ld_32x32b_x32(ts + c * 32, x);
-                    tc_wait_ld();
+                    uint32_t hi[16], lo[16];
 #pragma unroll
                     for (int i = 0; i < 32; i += 2) {
-                        float v0 = fmaf(__uint_as_float(x[i]), sc, ref), v1 = fmaf(__uint_as_float(x[i + 1]), sc, ref);
-                        if (edge) {
-                            if ((unsigned)(rel + c * 32 + i) >= width) v0 = -INFINITY;
-                            if ((unsigned)(rel + c * 32 + i + 1) >= width) v1 = -INFINITY;
-                        }
+                        float v0, v1;
+                        unpack2(fma2(pack2(x[c * 32 + i], x[c * 32 + i + 1]), sc2, ref2), v0, v1);
                         const float p0 = fast_exp2(v0), p1 = fast_exp2(v1);
-                        l += p0 + p1;
+                        sum = add2(sum, pack2(p0, p1));
                         hi[i / 2] = pack_half2(p0, p1);
                         if constexpr (SPLIT)
-                            low[c * 16 + i / 2] = pack_half2(p0 - __low2float(as_half2(hi[i / 2])),
-                                                             p1 - __high2float(as_half2(hi[i / 2])));
+                            lo[i / 2] = pack_half2(p0 - __low2float(as_half2(hi[i / 2])), p1 - __high2float(as_half2(hi[i / 2])));
                     }
                     tc_st_32x32b_x16(ts + c * 16, hi);
+                    if constexpr (SPLIT) tc_st_32x32b_x16(ts + 64 + c * 16, lo);
                 }
-                if constexpr (SPLIT) {
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        uint32_t x[16];
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) x[i] = low[c * 16 + i];
-                        tc_st_32x32b_x16(ts + 64 + c * 16, x);
-                    }
-                }
+                float s0, s1;
+                unpack2(sum, s0, s1);
+                l = s0 + s1;
                 tc_wait_st();
             }
             tc_fence_before();
@@ -340,7 +413,63 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvaArgs a, 
         }
         ml[w][r][0] = -nm;
         ml[w][r][1] = l;
+        if (same) {                                                // the second stream's O of the same rows by way of smem
+            float* osh = reinterpret_cast<float*>(smem);           // [128][D + 4]
+            softmax_sync();                                        // (both streams' products are done: q, K and V are free)
+            if (w == 1 && steps)
+#pragma unroll 1
+                for (int c = 0; c < D; c += 32) {
+                    uint32_t x[32];
+                    tc_ld_32x32b_x32(to + c, x);
+                    tc_wait_ld();
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4)
+                        *reinterpret_cast<uint4*>(osh + r * (D + 4) + c + i) = make_uint4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+                }
+            softmax_sync();
+        }
+        float* part = it.parts > 1 ? a.part + (size_t)blockIdx.x * G::PART : nullptr;
+        if (!same || w == 0) {
+            const float* osh = reinterpret_cast<const float*>(smem);
+            float m = -nm, sum = l, f0 = 1.0f, f1 = 0.0f;
+            if (same) {
+                const float m1 = ml[1][r][0], big = fmaxf(m, m1), ref = big == -INFINITY ? 0.0f : big;
+                f0 = fast_exp2(m - ref);
+                f1 = fast_exp2(m1 - ref);
+                sum = sum * f0 + ml[1][r][1] * f1;
+                m = big;
+            }
+            const KvaRow out{it.row0 + tok, it.head * a.group + (int)(grow % a.group)};
+            if (part && live) {
+                part[G::GROUP * D + 2 * row] = m;
+                part[G::GROUP * D + 2 * row + 1] = sum;
+            }
+#pragma unroll 1
+            for (int c = 0; c < D; c += 32) {
+                uint32_t x[32];
+#pragma unroll
+                for (int i = 0; i < 32; ++i) x[i] = 0;
+                if (steps) {                                       // (uniform)
+                    tc_ld_32x32b_x32(to + c, x);
+                    tc_wait_ld();
+                }
+                if (!live) continue;
+#pragma unroll
+                for (int i = 0; i < 32; i += 4) {
+                    float4 o = make_float4(__uint_as_float(x[i]) * f0, __uint_as_float(x[i + 1]) * f0,
+                                           __uint_as_float(x[i + 2]) * f0, __uint_as_float(x[i + 3]) * f0);
+                    if (same && steps) {
+                        const float4 u = *reinterpret_cast<const float4*>(osh + r * (D + 4) + c + i);
+                        o.x += u.x * f1; o.y += u.y * f1; o.z += u.z * f1; o.w += u.w * f1;
+                    }
+                    if (part) *reinterpret_cast<float4*>(part + row * D + c + i) = o;
+                    else kv_store_out<DT, D>(a, out, c + i, o, sum);
+                }
+            }
+        }
+        if (part) join_parts<D, DT>(a, it, &sh_last);
     } else if (warp < 12) {
+        reg_dec<REG_CONVERT>();
         // ---------------- converters: thread = key of the tile ----------------
         const int t = threadIdx.x - 256;
         uint4 kr[D / 32], vr[D / 32];
@@ -396,7 +525,9 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvaArgs a, 
             mbar_arrive(&v_full[st]);
             fetch(i + 1);
         }
-    } else if (lane == 0 && steps) {
+    } else {
+        reg_dec<REG_ISSUE>();
+        if (warp == 12 && lane == 0 && steps) {
         // ---------------- products ----------------
         constexpr uint32_t id_s = idesc_f16(128, KEYS, 0, 0, 0), id_o = idesc_f16(128, D, 0, 0, 1);
         const uint32_t q0 = smem_u32(sq), k0 = smem_u32(sk), v0 = smem_u32(sv);
@@ -451,117 +582,14 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvaArgs a, 
             mbar_wait(&o_full[0], 0, a.status);
             mbar_wait(&o_full[1], 0, a.status);
         }
-    }
-    __syncwarp();
-    tc_fence_before();
-    __syncthreads();                                               // every product is done, ml is written
-    tc_fence_after();
-
-    // ---- output ----
-    const int w = warp >> 2, r = (warp & 3) * 32 + lane;
-    float* osh = reinterpret_cast<float*>(smem);                   // [128][D + 4]: the second stream's O of the same rows
-    if (same && warp >= 4 && warp < 8 && steps)
-#pragma unroll 1
-        for (int c = 0; c < D; c += 32) {
-            uint32_t x[32];
-            tc_ld_32x32b_x32(tmem + lanes + G::O + D + c, x);
-            tc_wait_ld();
-#pragma unroll
-            for (int i = 0; i < 32; i += 4)
-                *reinterpret_cast<uint4*>(osh + r * (D + 4) + c + i) = make_uint4(x[i], x[i + 1], x[i + 2], x[i + 3]);
         }
-    if (same) __syncthreads();
-    if (warp < (same ? 4 : 8)) {
-        const int row = same ? r : w * ROWS + r;
-        float m = ml[w][r][0], sum = ml[w][r][1], f0 = 1.0f, f1 = 0.0f;
-        if (same) {
-            const float m1 = ml[1][r][0], big = fmaxf(m, m1), ref = big == -INFINITY ? 0.0f : big;
-            f0 = fast_exp2(m - ref);
-            f1 = fast_exp2(m1 - ref);
-            sum = sum * f0 + ml[1][r][1] * f1;
-            m = big;
-        }
-        const long grow = (long)it.group * G::GROUP + row;
-        const bool live = row < it.rows;
-        const KvaRow to{it.row0 + (int)(grow / a.group), it.head * a.group + (int)(grow % a.group)};
-        float* part = it.parts > 1 ? a.part + (size_t)blockIdx.x * G::PART : nullptr;
-        if (part && live) {
-            part[G::GROUP * D + 2 * row] = m;
-            part[G::GROUP * D + 2 * row + 1] = sum;
-        }
-#pragma unroll 1
-        for (int c = 0; c < D; c += 32) {
-            uint32_t x[32];
-#pragma unroll
-            for (int i = 0; i < 32; ++i) x[i] = 0;
-            if (steps) {                                           // (uniform)
-                tc_ld_32x32b_x32(tmem + lanes + G::O + w * D + c, x);
-                tc_wait_ld();
-            }
-            if (!live) continue;
-#pragma unroll
-            for (int i = 0; i < 32; i += 4) {
-                float4 o = make_float4(__uint_as_float(x[i]) * f0, __uint_as_float(x[i + 1]) * f0,
-                                       __uint_as_float(x[i + 2]) * f0, __uint_as_float(x[i + 3]) * f0);
-                if (same && steps) {
-                    const float4 u = *reinterpret_cast<const float4*>(osh + r * (D + 4) + c + i);
-                    o.x += u.x * f1; o.y += u.y * f1; o.z += u.z * f1; o.w += u.w * f1;
-                }
-                if (part) *reinterpret_cast<float4*>(part + row * D + c + i) = o;
-                else kv_store_out<DT, D>(a, to, c + i, o, sum);
-            }
-        }
+        __syncwarp();
     }
     tc_fence_before();
     __syncthreads();
     if (warp == 12) {
         tc_fence_after();
         tmem_dealloc(tmem, 512);
-    }
-    if (it.parts == 1) return;
-    // ---- the last part of the rows to finish joins them, in the order of the keys ----
-    __threadfence();
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        const int done = atomicAdd(a.count + it.id, 1) + 1;
-        sh_last = done == it.parts;
-        if (sh_last) a.count[it.id] = 0;
-    }
-    __syncthreads();
-    if (!sh_last) return;
-    __threadfence();
-    const float* base = a.part + (size_t)(blockIdx.x - it.part) * G::PART;
-    for (int i = threadIdx.x; i < it.rows * (D / 4); i += THREADS) {
-        const int row = i / (D / 4), e = (i - row * (D / 4)) * 4;
-        float m = -INFINITY, sum = 0.0f;
-        float4 o = make_float4(0, 0, 0, 0);
-        for (int c0 = 0; c0 < it.parts; c0 += 8) {                 // eight parts' loads in flight
-            float4 v[8];
-            float2 st[8];
-#pragma unroll
-            for (int c = 0; c < 8; ++c) {
-                const float* p = base + (size_t)min(c0 + c, it.parts - 1) * G::PART;
-                v[c] = __ldcg(reinterpret_cast<const float4*>(p + row * D + e));
-                st[c] = __ldcg(reinterpret_cast<const float2*>(p + G::GROUP * D + 2 * row));
-                if (c0 + c >= it.parts) st[c] = make_float2(-INFINITY, 0.0f);
-            }
-            float big = m;
-#pragma unroll
-            for (int c = 0; c < 8; ++c) big = fmaxf(big, st[c].x);
-            const float ref = big == -INFINITY ? 0.0f : big, f = fast_exp2(m - ref);
-            sum *= f;
-            o.x *= f; o.y *= f; o.z *= f; o.w *= f;
-            m = big;
-#pragma unroll
-            for (int c = 0; c < 8; ++c) {
-                if (c0 + c >= it.parts) break;
-                const float g = fast_exp2(st[c].x - ref);
-                sum += st[c].y * g;
-                o.x += v[c].x * g; o.y += v[c].y * g; o.z += v[c].z * g; o.w += v[c].w * g;
-            }
-        }
-        const long grow = (long)it.group * G::GROUP + row;
-        kv_store_out<DT, D>(a, KvaRow{it.row0 + (int)(grow / a.group), it.head * a.group + (int)(grow % a.group)}, e, o, sum);
     }
 }
 
