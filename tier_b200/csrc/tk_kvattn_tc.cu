@@ -180,14 +180,39 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
-// D[tmem] (+)= A[tmem] * B[smem desc], kind::f16.
-__device__ __forceinline__ void tc_mma_f16_ta(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc,
-                                              uint32_t accumulate) {
+// The products' warp stays converged, so that descriptors live in uniform
+// registers: one lane (`one`) issues.  With the whole loop in one lane, moving
+// each product's operands into place took twice the product's own 64 cycles.
+__device__ __forceinline__ uint32_t elect_one() {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r;
+}
+// D[tmem] (+)= A[smem desc] * B[smem desc]^T, kind::f16.
+__device__ __forceinline__ void mma_ss(uint32_t one, uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                       uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
-        "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(one)
+        : "memory");
+}
+// D[tmem] (+)= A[tmem] * B[smem desc], kind::f16.
+__device__ __forceinline__ void mma_ts(uint32_t one, uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc,
+                                       uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(one)
+        : "memory");
+}
+__device__ __forceinline__ void commit(uint32_t one, uint64_t* bar) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)),
+        "r"(one)
         : "memory");
 }
 
@@ -527,61 +552,64 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvaArgs a, 
         }
     } else {
         reg_dec<REG_ISSUE>();
-        if (warp == 12 && lane == 0 && steps) {
-        // ---------------- products ----------------
-        constexpr uint32_t id_s = idesc_f16(128, KEYS, 0, 0, 0), id_o = idesc_f16(128, D, 0, 0, 1);
-        const uint32_t q0 = smem_u32(sq), k0 = smem_u32(sk), v0 = smem_u32(sv);
-        bool ok = mbar_wait(&q_full, 0, a.status);
-        auto product_s = [&](int w, int i) {                       // stream w, tile i of the ring
-            const uint32_t kb = k0 + (i & 1) * G::TILE;
+        if (warp == 12 && steps) {
+            // ---------------- products (the whole warp; one lane issues) ----------------
+            constexpr uint32_t id_s = idesc_f16(128, KEYS, 0, 0, 0), id_o = idesc_f16(128, D, 0, 0, 1);
+            constexpr uint64_t TILE = G::TILE >> 4;                // in a descriptor's address units
+            const uint32_t one = elect_one();
+            const uint64_t dq = sdesc_sw128(smem_u32(sq), 16, 1024), dk = sdesc_sw128(smem_u32(sk), 16, 1024);
+            const uint64_t dv = sdesc_sw128(smem_u32(sv), G::PANEL, 1024);
+            auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(~0u, mbar_wait(bar, parity, a.status)); };
+            auto product_s = [&](int w, int i) {                   // stream w, tile i of the ring
+                const uint64_t kd = dk + (i & 1) * TILE;
 #pragma unroll
-            for (int p = PARTS - 1; p >= 0; --p) {
-                const uint32_t qb = q0 + (SPLIT ? p : same ? 0 : w) * G::TILE;
+                for (int p = PARTS - 1; p >= 0; --p) {
+                    const uint64_t qd = dq + (SPLIT ? p : same ? 0 : w) * TILE;
 #pragma unroll
-                for (int kk = 0; kk < D / 16; ++kk) {
-                    const uint32_t off = (kk >> 2) * G::PANEL + (kk & 3) * 32;
-                    tc_mma_f16(tmem + G::S + w * 128, sdesc_sw128(qb + off, 16, 1024), sdesc_sw128(kb + off, 16, 1024), id_s,
-                               p != PARTS - 1 || kk > 0);
+                    for (int kk = 0; kk < D / 16; ++kk) {
+                        const uint32_t off = ((kk >> 2) * G::PANEL + (kk & 3) * 32) >> 4;
+                        mma_ss(one, tmem + G::S + w * 128, qd + off, kd + off, id_s, p != PARTS - 1 || kk > 0);
+                    }
                 }
-            }
-            tc_commit(&s_full[w]);
-            if (same || w == 1) tc_commit(&k_empty[i & 1]);
-        };
-        for (int w = 0; w < 2 && ok; ++w) {
-            const int i = same ? w : 0;
-            ok = mbar_wait(&k_full[i & 1], (i >> 1) & 1, a.status);
-            tc_fence_after();
-            if (ok) product_s(w, i);
-        }
-        for (int j = 0; j < steps && ok; ++j)
+                commit(one, &s_full[w]);
+                if (same || w == 1) commit(one, &k_empty[i & 1]);
+            };
+            bool ok = wait(&q_full, 0);
             for (int w = 0; w < 2 && ok; ++w) {
-                const int i = same ? 2 * j + w : j;
-                ok = mbar_wait(&v_full[i & 1], (i >> 1) & 1, a.status) && mbar_wait(&p_full[w], j & 1, a.status);
-                if (!ok) break;
+                const int i = same ? w : 0;
+                ok = wait(&k_full[i & 1], (i >> 1) & 1);
                 tc_fence_after();
-                const uint32_t vb = v0 + (i & 1) * G::TILE;
-#pragma unroll
-                for (int p = PARTS - 1; p >= 0; --p)
-#pragma unroll
-                    for (int kk = 0; kk < KEYS / 16; ++kk)
-                        tc_mma_f16_ta(tmem + G::O + w * D, tmem + G::S + w * 128 + p * 64 + kk * 8,
-                                      sdesc_sw128(vb + kk * 2048, G::PANEL, 1024), id_o, j > 0 || p != PARTS - 1 || kk > 0);
-                if (same || w == 1) tc_commit(&v_empty[i & 1]);
-                if (j + 1 < steps) {
-                    const int n = same ? i + 2 : j + 1;
-                    ok = mbar_wait(&k_full[n & 1], (n >> 1) & 1, a.status);
-                    tc_fence_after();
-                    if (ok) product_s(w, n);
-                } else {
-                    tc_commit(&o_full[w]);
-                }
+                if (ok) product_s(w, i);
             }
-        if (!ok) {      // reported; what was issued ends first
-            tc_commit(&o_full[0]);
-            tc_commit(&o_full[1]);
-            mbar_wait(&o_full[0], 0, a.status);
-            mbar_wait(&o_full[1], 0, a.status);
-        }
+            for (int j = 0; j < steps && ok; ++j)
+                for (int w = 0; w < 2 && ok; ++w) {
+                    const int i = same ? 2 * j + w : j;
+                    ok = wait(&v_full[i & 1], (i >> 1) & 1) && wait(&p_full[w], j & 1);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint64_t vd = dv + (i & 1) * TILE;
+#pragma unroll
+                    for (int p = PARTS - 1; p >= 0; --p)
+#pragma unroll
+                        for (int kk = 0; kk < KEYS / 16; ++kk)
+                            mma_ts(one, tmem + G::O + w * D, tmem + G::S + w * 128 + p * 64 + kk * 8, vd + (kk * 2048 >> 4), id_o,
+                                   j > 0 || p != PARTS - 1 || kk > 0);
+                    if (same || w == 1) commit(one, &v_empty[i & 1]);
+                    if (j + 1 < steps) {
+                        const int n = same ? i + 2 : j + 1;
+                        ok = wait(&k_full[n & 1], (n >> 1) & 1);
+                        tc_fence_after();
+                        if (ok) product_s(w, n);
+                    } else {
+                        commit(one, &o_full[w]);
+                    }
+                }
+            if (!ok) {  // reported; what was issued ends first
+                commit(one, &o_full[0]);
+                commit(one, &o_full[1]);
+                mbar_wait(&o_full[0], 0, a.status);
+                mbar_wait(&o_full[1], 0, a.status);
+            }
         }
         __syncwarp();
     }
