@@ -144,6 +144,11 @@ __device__ __forceinline__ void tc_st_32x32b_x16(uint32_t taddr, const uint32_t 
         "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
         : "memory");
 }
+__device__ __forceinline__ void tc_st_32x32b_x8(uint32_t taddr, const uint32_t (&r)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]),
+                 "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
+}
 __device__ __forceinline__ void tc_ld_32x32b_x16(uint32_t taddr, uint32_t (&r)[16]) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
@@ -408,22 +413,38 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvaArgs a, 
                 }
                 const f32x2 sc2 = pack2(sc, sc), ref2 = nm == INFINITY ? pack2(0.0f, 0.0f) : pack2(nm, nm);
                 f32x2 sum = pack2(l, 0.0f);
+                // in place and in three steps, eight pairs apart, so that no
+                // exponential waits for its own operand or its own use
+                auto exponent = [&](int i) {                       // pairs i .. i + 7
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    uint32_t hi[16], lo[16];
+                    for (int k = i; k < i + 8; ++k)
+                        unpack2(fma2(pack2(x[2 * k], x[2 * k + 1]), sc2, ref2), x[2 * k], x[2 * k + 1]);
+                };
+                auto power = [&](int i) {
 #pragma unroll
-                    for (int i = 0; i < 32; i += 2) {
-                        float v0, v1;
-                        unpack2(fma2(pack2(x[c * 32 + i], x[c * 32 + i + 1]), sc2, ref2), v0, v1);
-                        const float p0 = fast_exp2(v0), p1 = fast_exp2(v1);
+                    for (int k = 2 * i; k < 2 * i + 16; ++k) x[k] = fast_exp2(x[k]);
+                };
+                auto finish = [&](int i) {
+                    uint32_t hi[8], lo[8];
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        const float p0 = x[2 * (i + k)], p1 = x[2 * (i + k) + 1];
                         sum = add2(sum, pack2(p0, p1));
-                        hi[i / 2] = pack_half2(p0, p1);
+                        hi[k] = pack_half2(p0, p1);
                         if constexpr (SPLIT)
-                            lo[i / 2] = pack_half2(p0 - __low2float(as_half2(hi[i / 2])), p1 - __high2float(as_half2(hi[i / 2])));
+                            lo[k] = pack_half2(p0 - __low2float(as_half2(hi[k])), p1 - __high2float(as_half2(hi[k])));
                     }
-                    tc_st_32x32b_x16(ts + c * 16, hi);
-                    if constexpr (SPLIT) tc_st_32x32b_x16(ts + 64 + c * 16, lo);
+                    tc_st_32x32b_x8(ts + i, hi);
+                    if constexpr (SPLIT) tc_st_32x32b_x8(ts + 64 + i, lo);
+                };
+                exponent(0);
+#pragma unroll
+                for (int i = 0; i < KEYS / 2; i += 8) {
+                    power(i);
+                    if (i + 8 < KEYS / 2) exponent(i + 8);
+                    if (i >= 8) finish(i - 8);
                 }
+                finish(KEYS / 2 - 8);
                 float s0, s1;
                 unpack2(sum, s0, s1);
                 l = s0 + s1;
