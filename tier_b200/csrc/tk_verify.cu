@@ -16,6 +16,7 @@
 // that holds the draw searched again.
 #include <climits>
 #include "tk_device.cuh"
+#include "tk_f32x2.cuh"
 #include "tk_internal.h"
 
 namespace tk {
@@ -75,31 +76,6 @@ __device__ __forceinline__ float dv_weight(float x, float c, float top) {
 // shifted up are added to the exponent of 2^(y - i): the bits of dv_weight
 // without its conversions and comparisons.  Packed fp32 instructions take
 // both at once.
-typedef unsigned long long f32x2;
-__device__ __forceinline__ f32x2 dv_pack(float a, float b) {
-    f32x2 r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ void dv_unpack(f32x2 v, float& a, float& b) {
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
-}
-__device__ __forceinline__ f32x2 dv_add2(f32x2 a, f32x2 b) {
-    f32x2 r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ f32x2 dv_mul2(f32x2 a, f32x2 b) {
-    f32x2 r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ f32x2 dv_fma2(f32x2 a, f32x2 b, f32x2 c) {
-    f32x2 r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-__device__ __forceinline__ f32x2 dv_sub2(f32x2 a, f32x2 b) { return dv_fma2(b, dv_pack(-1.0f, -1.0f), a); }
 constexpr float DV_NEAR = 4194304.0f;              // |top| below this: dv_weight2
 struct DvFast {
     f32x2 c, bias, nbias;
@@ -107,17 +83,17 @@ struct DvFast {
 };
 __device__ __forceinline__ DvFast dv_fast(float c, float top) {
     const float m = 12582912.0f - top;
-    return DvFast{dv_pack(c, c), dv_pack(m, m), dv_pack(-m, -m), top - 110.0f};
+    return DvFast{pack2(c, c), pack2(m, m), pack2(-m, -m), top - 110.0f};
 }
 __device__ __forceinline__ f32x2 dv_weight2(float x0, float x1, const DvFast& k) {
     f32x2 y, t;
     float y0, y1, f0, f1, t0, t1;
-    dv_unpack(dv_mul2(dv_pack(x0, x1), k.c), y0, y1);
-    y = dv_pack(fmaxf(y0, k.low), fmaxf(y1, k.low));
-    asm("add.rm.f32x2 %0, %1, %2;" : "=l"(t) : "l"(y), "l"(k.bias));
-    dv_unpack(dv_sub2(y, dv_add2(t, k.nbias)), f0, f1);
-    dv_unpack(t, t0, t1);
-    return dv_pack(__uint_as_float((__float_as_uint(t0) << 23) + __float_as_uint(dv_exp2(f0))),
+    unpack2(mul2(pack2(x0, x1), k.c), y0, y1);
+    y = pack2(fmaxf(y0, k.low), fmaxf(y1, k.low));
+    t = add2_rm(y, k.bias);
+    unpack2(sub2(y, add2(t, k.nbias)), f0, f1);
+    unpack2(t, t0, t1);
+    return pack2(__uint_as_float((__float_as_uint(t0) << 23) + __float_as_uint(dv_exp2(f0))),
                    __uint_as_float((__float_as_uint(t1) << 23) + __float_as_uint(dv_exp2(f1))));
 }
 
@@ -132,12 +108,12 @@ struct DvProb {
 };
 __device__ __forceinline__ DvProb dv_prepare(const DvStat& st, float c) {
     const float s = (float)st.sum, r = __frcp_rn(s);
-    return DvProb{dv_fast(c, st.top), dv_pack(-s, -s), dv_pack(r, r),
+    return DvProb{dv_fast(c, st.top), pack2(-s, -s), pack2(r, r),
                   fabsf(st.top) < DV_NEAR && (__float_as_uint(s) & 0x7fffffu) != 0x7fffffu};
 }
 __device__ __forceinline__ f32x2 dv_prob2(float x0, float x1, const DvProb& k) {
-    const f32x2 w = dv_weight2(x0, x1, k.fast), q = dv_mul2(w, k.r);
-    return dv_fma2(dv_fma2(q, k.ns, w), k.r, q);
+    const f32x2 w = dv_weight2(x0, x1, k.fast), q = mul2(w, k.r);
+    return fma2(fma2(q, k.ns, w), k.r, q);
 }
 __device__ __forceinline__ float dv_prob(float x, float c, const DvStat& s) {
     return __fdiv_rn(dv_weight(x, c, s.top), (float)s.sum);
@@ -237,20 +213,20 @@ __global__ void __launch_bounds__(DV_THREADS, 4) dv_rows_kernel(const DvArgs a) 
     if (fabsf(top) < DV_NEAR) {
         // sums start above any weight, so that t - s2 and its difference to the weight are exact
         const DvFast fast = dv_fast(a.c, top);
-        f32x2 s2 = dv_pack(2.0f, 2.0f), err = dv_pack(0.0f, 0.0f);
+        f32x2 s2 = pack2(2.0f, 2.0f), err = pack2(0.0f, 0.0f);
 #pragma unroll
         for (int k = 0; k < QUADS; ++k) {
             if (k * DV_THREADS >= n) break;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const f32x2 w = h ? dv_weight2(v[k].z, v[k].w, fast) : dv_weight2(v[k].x, v[k].y, fast), t = dv_add2(s2, w);
-                err = dv_add2(err, dv_sub2(w, dv_sub2(t, s2)));
+                const f32x2 w = h ? dv_weight2(v[k].z, v[k].w, fast) : dv_weight2(v[k].x, v[k].y, fast), t = add2(s2, w);
+                err = add2(err, sub2(w, sub2(t, s2)));
                 s2 = t;
             }
         }
         float p0, p1, e0, e1;
-        dv_unpack(s2, p0, p1);
-        dv_unpack(err, e0, e1);
+        unpack2(s2, p0, p1);
+        unpack2(err, e0, e1);
         sum = (((double)p0 - 2.0) + ((double)p1 - 2.0)) + ((double)e0 + (double)e1);
     } else if (top > -3.402823466e38f) {           // logits of such size: one by one
 #pragma unroll 1
@@ -398,7 +374,7 @@ __global__ void __launch_bounds__(DP_THREADS, 2) dv_pick_kernel(const DvArgs a) 
     };
     // floor(p 2^38) = hi 2^19 + lo: adding 2^23 downwards leaves a whole number in the low bits (above DP_BIAS)
     constexpr uint32_t DP_BIAS = 0x4b000000u;
-    const f32x2 k19 = dv_pack(524288.0f, 524288.0f), k23 = dv_pack(8388608.0f, 8388608.0f), n23 = dv_pack(-8388608.0f, -8388608.0f);
+    const f32x2 k19 = pack2(524288.0f, 524288.0f), k23 = pack2(8388608.0f, 8388608.0f), n23 = pack2(-8388608.0f, -8388608.0f);
     auto weights = [&](long q, bool rest, const float4& tv, const float4& dv, uint32_t (&hi)[4], uint32_t (&lo)[4]) {
         const float e[4] = {tv.x, tv.y, tv.z, tv.w}, o[4] = {dv.x, dv.y, dv.z, dv.w};
 #pragma unroll
@@ -406,8 +382,8 @@ __global__ void __launch_bounds__(DP_THREADS, 2) dv_pick_kernel(const DvArgs a) 
             float p0, p1;
             if (quick) {
                 f32x2 p = dv_prob2(e[i], e[i + 1], pt);
-                if (rest && d) p = dv_sub2(p, dv_prob2(o[i], o[i + 1], pd));
-                dv_unpack(p, p0, p1);
+                if (rest && d) p = sub2(p, dv_prob2(o[i], o[i + 1], pd));
+                unpack2(p, p0, p1);
             } else {
                 p0 = dv_prob(e[i], a.c, st);
                 p1 = dv_prob(e[i + 1], a.c, st);
@@ -420,16 +396,13 @@ __global__ void __launch_bounds__(DP_THREADS, 2) dv_pick_kernel(const DvArgs a) 
                 if (4 * q - off + i == x) p0 = 0.0f;
                 if (4 * q - off + i + 1 == x) p1 = 0.0f;
             }
-            const f32x2 u = dv_mul2(dv_pack(fmaxf(p0, 0.0f), fmaxf(p1, 0.0f)), k19);
-            f32x2 h, l;
-            asm("add.rm.f32x2 %0, %1, %2;" : "=l"(h) : "l"(u), "l"(k23));
-            l = dv_sub2(u, dv_add2(h, n23));
-            asm("fma.rm.f32x2 %0, %1, %2, %3;" : "=l"(l) : "l"(l), "l"(k19), "l"(k23));
+            const f32x2 u = mul2(pack2(fmaxf(p0, 0.0f), fmaxf(p1, 0.0f)), k19);
+            const f32x2 h = add2_rm(u, k23), l = fma2_rm(sub2(u, add2(h, n23)), k19, k23);
             float v0, v1;
-            dv_unpack(h, v0, v1);
+            unpack2(h, v0, v1);
             hi[i] = __float_as_uint(v0) - DP_BIAS;
             hi[i + 1] = __float_as_uint(v1) - DP_BIAS;
-            dv_unpack(l, v0, v1);
+            unpack2(l, v0, v1);
             lo[i] = __float_as_uint(v0) - DP_BIAS;
             lo[i + 1] = __float_as_uint(v1) - DP_BIAS;
         }
