@@ -186,6 +186,69 @@ __device__ __forceinline__ void kv_store_out(const KvaArgs& a, KvaRow r, int e, 
     }
 }
 
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// Joins the parts of a row set, in the order of the keys, by all `threads` of a
+// group (`sync`: its barrier): a part is O of `rows` rows (D values each, of
+// ROWS), then (m, l) of each.  at(c): part c, out(r): row r.  Statistics and
+// factors go through shared memory (`bytes` of it, rows in batches that fit),
+// a warp a row; then 16 parts' O are in flight together.
+template <int D, int DT, int ROWS, class At, class Out, class Sync>
+__device__ __forceinline__ void kv_join(const KvaArgs& a, int parts, int all_rows, int thread, int threads, uint8_t* smem,
+                                        int bytes, At at, Out out, Sync sync) {
+    const int some = max(1, min(all_rows, bytes / (8 * parts + 4)));
+    const int warp = thread >> 5, lane = thread & 31;
+    for (int r0 = 0; r0 < all_rows; r0 += some) {
+        const int rows = min(some, all_rows - r0);
+        float* fac = reinterpret_cast<float*>(smem);               // [parts][rows] m, then the factor; the same of l; [rows] sums
+        float* ls = fac + parts * rows;
+        float* sum = ls + parts * rows;
+        for (int i = thread; i < parts * rows; i += threads) {
+            const int c = i / rows, r = i - c * rows;
+            const float2 ml = __ldcg(reinterpret_cast<const float2*>(at(c) + ROWS * D) + r0 + r);
+            fac[i] = ml.x;
+            ls[i] = ml.y;
+        }
+        sync();
+        for (int r = warp; r < rows; r += threads >> 5) {
+            float m = -INFINITY, l = 0.0f;
+            for (int c = lane; c < parts; c += 32) m = fmaxf(m, fac[c * rows + r]);
+            for (int i = 16; i; i >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, i));
+            const float ref = m == -INFINITY ? 0.0f : m;
+            for (int c = lane; c < parts; c += 32) {
+                const float f = fast_exp2(fac[c * rows + r] - ref);
+                fac[c * rows + r] = f;
+                l += ls[c * rows + r] * f;
+            }
+            for (int i = 16; i; i >>= 1) l += __shfl_xor_sync(~0u, l, i);
+            if (lane == 0) sum[r] = l;
+        }
+        sync();
+        for (int i = thread; i < rows * (D / 4); i += threads) {
+            const int r = i / (D / 4), e = (i - r * (D / 4)) * 4;
+            float4 o = make_float4(0, 0, 0, 0);
+            for (int c0 = 0; c0 < parts; c0 += 16) {               // whatever is left of 16
+                float4 v[16];
+#pragma unroll
+                for (int c = 0; c < 16; ++c)
+                    v[c] = __ldcg(reinterpret_cast<const float4*>(at(min(c0 + c, parts - 1)) + (r0 + r) * D + e));
+#pragma unroll
+                for (int c = 0; c < 16; ++c) {
+                    const float f = c0 + c < parts ? fac[(c0 + c) * rows + r] : 0.0f;
+                    o.x += v[c].x * f; o.y += v[c].y * f; o.z += v[c].z * f; o.w += v[c].w * f;
+                }
+            }
+            kv_store_out<DT, D>(a, out(r0 + r), e, o, sum[r]);
+        }
+        sync();
+    }
+}
+
 // tk_kvattn_tc.cu
 tk_status launch_kv_prompt(tk_ctx* ctx, KvaArgs& a, int dtype, cudaStream_t st);
 // Zeroed counters for joins (tk_kvattn.cu).

@@ -4,11 +4,11 @@
 
 namespace tk {
 
-// The last of a head's parts to finish joins them, in the order of the keys
-// (the result does not depend on which block that is): parts are [16 rows, D]
-// of O, then (m, l) of each row; smem holds a factor per part and row.  The counter is left at zero for the next call.
-template <int D, int DT, class Item>
-__device__ __forceinline__ void kv_join_last(const KvaArgs& a, const Item& it, int live, uint8_t* smem, int* sh_last) {
+// The last of a head's parts to finish joins them (the result does not depend
+// on which block that is).  The counter is left at zero for the next call.
+template <int D, int DT, int ROWS, class Item>
+__device__ __forceinline__ void kv_join_last(const KvaArgs& a, const Item& it, int live, uint8_t* smem, int bytes,
+                                             int* sh_last) {
     __threadfence();
     __syncthreads();
     if (threadIdx.x == 0) {
@@ -20,53 +20,14 @@ __device__ __forceinline__ void kv_join_last(const KvaArgs& a, const Item& it, i
     __syncthreads();
     if (!*sh_last) return;
     __threadfence();
-    constexpr int P = 16 * (D + 2);                                // floats of a part
-    auto part_of = [&](int c) { return a.part + (size_t)(2 * (it.c0 + c) + (c == 0 ? it.odd : 0)) * P; };
-    float* fac = reinterpret_cast<float*>(smem);                   // [chunks][live] m, then factor; the same of l; [live] sums
-    float* ls = fac + it.chunks * live;
-    float* sum = ls + it.chunks * live;
-    for (int i = threadIdx.x; i < it.chunks * live; i += blockDim.x) {
-        const int c = i / live, r = i - c * live;
-        const float2 ml = __ldcg(reinterpret_cast<const float2*>(part_of(c) + 16 * D + 2 * r));
-        fac[i] = ml.x;
-        ls[i] = ml.y;
-    }
-    __syncthreads();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    for (int r = warp; r < live; r += blockDim.x >> 5) {
-        float m = -INFINITY, l = 0.0f;
-        for (int c = lane; c < it.chunks; c += 32) m = fmaxf(m, fac[c * live + r]);
-        for (int i = 16; i; i >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, i));
-        const float ref = m == -INFINITY ? 0.0f : m;
-        for (int c = lane; c < it.chunks; c += 32) {
-            const float f = fast_exp2(fac[c * live + r] - ref);
-            fac[c * live + r] = f;
-            l += ls[c * live + r] * f;
-        }
-        for (int i = 16; i; i >>= 1) l += __shfl_xor_sync(~0u, l, i);
-        if (lane == 0) sum[r] = l;
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < live * (D / 4); i += blockDim.x) {
-        const int r = i / (D / 4), e = (i - r * (D / 4)) * 4;
-        float4 o = make_float4(0, 0, 0, 0);
-        for (int c0 = 0; c0 < it.chunks; c0 += 16) {               // 16 loads in flight, whatever is left of them
-            float4 v[16];
-#pragma unroll
-            for (int c = 0; c < 16; ++c)
-                v[c] = __ldcg(reinterpret_cast<const float4*>(part_of(min(c0 + c, it.chunks - 1)) + r * D + e));
-#pragma unroll
-            for (int c = 0; c < 16; ++c) {
-                const float f = c0 + c < it.chunks ? fac[(c0 + c) * live + r] : 0.0f;
-                o.x += v[c].x * f; o.y += v[c].y * f; o.z += v[c].z * f; o.w += v[c].w * f;
-            }
-        }
-        kv_store_out<DT, D>(a, KvaRow{it.row0 + r / a.group, it.head * a.group + r % a.group}, e, o, sum[r]);
-    }
+    kv_join<D, DT, ROWS>(
+        a, it.chunks, live, threadIdx.x, blockDim.x, smem, bytes,
+        [&](int c) { return a.part + (size_t)(2 * (it.c0 + c) + (c == 0 ? it.odd : 0)) * (ROWS * (D + 2)); },
+        [&](int r) { return KvaRow{it.row0 + r / a.group, it.head * a.group + r % a.group}; }, [] { __syncthreads(); });
 }
 
 // ---------------------------------------------------------------------------
-// Few rows per key/value head (new tokens x heads of the group <= 16): the
+// Few rows per key/value head (new tokens x heads of the group <= 32): the
 // cache is streamed once, divided among thread blocks.
 //
 // One warp takes units of 32 keys.  S^T = K Q^T and O^T += V^T P^T are
@@ -91,18 +52,18 @@ __device__ __forceinline__ void kv_join_last(const KvaArgs& a, const Item& it, i
 // barrier handling.  The keys' order within 8 (kd_key) and an exchange of
 // half rows of V keep the fragment loads free of bank conflicts.
 // ---------------------------------------------------------------------------
-#ifndef KD_CTAS
-#define KD_CTAS 3
-#endif
-constexpr int KD_WARPS = 4, KD_STAGES = KD_CTAS == 3 ? 3 : 2, KD_UNIT = 32;
+constexpr int KD_WARPS = 4, KD_STAGES = 3, KD_UNIT = 32, KD_MAX_ROWS = 32;
+// Blocks an SM: registers for 8 or 16 query rows allow three, for 24 or 32 two.
+constexpr int kd_blocks(int nt) { return nt <= 2 ? 3 : 2; }
 
-template <int D>
+template <int D, int NT>
 struct KdGeo {
     static constexpr int QB = KD_UNIT * D / 2, SB = KD_UNIT * D / 16;      // bytes of numbers, of scales
     static constexpr int STAGE = 2 * QB + 2 * SB;
     static constexpr int RING = KD_WARPS * KD_STAGES * STAGE;
-    static constexpr int JOIN = KD_WARPS * (16 * (D + 4) * 4 + 16 * 8);    // each warp's O rows, m and l
+    static constexpr int JOIN = KD_WARPS * 8 * NT * ((D + 4) * 4 + 8);     // each warp's O rows, m and l
     static constexpr int SMEM = RING > JOIN ? RING : JOIN;
+    static constexpr int PART = 8 * NT * (D + 2);                          // floats of a part: O, then (m, l) of each row
 };
 
 // How the units of all sequences and key/value heads are divided among the
@@ -222,12 +183,6 @@ __device__ __forceinline__ void kd_find(const KvaArgs& a, const KdPlan& plan, ui
     }
 }
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 // Key of matrix index i within its 8: 0 5 2 7 1 4 3 6.  Neighbours (one fp16
 // pair of P^T, two rows of K) differ in parity, so that 64-byte rows fall on
 // different banks; the even and the odd four are distinct modulo 4.
@@ -248,8 +203,8 @@ __device__ __forceinline__ uint32_t turn8x8(uint32_t x) {
     return r;
 }
 template <int D, int DT, int NT>
-__global__ void __launch_bounds__(KD_WARPS * 32, KD_CTAS) kv_decode_kernel(const KvaArgs a, uint32_t least) {
-    using G = KdGeo<D>;
+__global__ void __launch_bounds__(KD_WARPS * 32, kd_blocks(NT)) kv_decode_kernel(const KvaArgs a, uint32_t least) {
+    using G = KdGeo<D, NT>;
     constexpr bool SPLIT = DT == TK_DT_F32;
     constexpr int ROWS = 8 * NT, PARTS = SPLIT ? 2 : 1;            // query rows, fp16 parts of q and p
     constexpr int KW = D / 32, VW = D / 64;                        // 32-bit words of a lane's piece of a key / value row
@@ -596,15 +551,15 @@ __global__ void __launch_bounds__(KD_WARPS * 32, KD_CTAS) kv_decode_kernel(const
         }
         if (whole) kv_store_out<DT, D>(a, KvaRow{it.row0 + r / a.group, it.head * a.group + r % a.group}, e, acc, ll);
         else {
-            float* part = a.part + (size_t)it.slot * (16 * (D + 2));
+            float* part = a.part + (size_t)it.slot * G::PART;
             *reinterpret_cast<float4*>(part + r * D + e) = acc;
             if (e == 0) {
-                part[16 * D + 2 * r] = mm;
-                part[16 * D + 2 * r + 1] = ll;
+                part[ROWS * D + 2 * r] = mm;
+                part[ROWS * D + 2 * r + 1] = ll;
             }
         }
     }
-    if (!whole) kv_join_last<D, DT>(a, it, live, smem, &sh_last);
+    if (!whole) kv_join_last<D, DT, ROWS>(a, it, live, smem, G::SMEM, &sh_last);
     __syncthreads();
   }
 }
@@ -630,32 +585,39 @@ template <int D, int DT, int NT>
 static tk_status go_decode_t(tk_ctx* ctx, const KvaArgs& a, unsigned grid, int least, cudaStream_t st) {
     static std::atomic<uint64_t> attr_done{0};
     auto kern = kv_decode_kernel<D, DT, NT>;
-    cudaError_t e = smem_attr_once(kern, KdGeo<D>::SMEM, ctx->device, attr_done);
+    cudaError_t e = smem_attr_once(kern, KdGeo<D, NT>::SMEM, ctx->device, attr_done);
     if (e != cudaSuccess) return cuda_fail(e, "kv decode smem attribute");
     ProfScope ps(ctx, st, PK_SERVE);
-    kern<<<grid, KD_WARPS * 32, KdGeo<D>::SMEM, st>>>(a, least);
+    kern<<<grid, KD_WARPS * 32, KdGeo<D, NT>::SMEM, st>>>(a, least);
     ctx->launches++;
     return cuda_fail(cudaGetLastError(), "kv decode launch");
 }
 
-template <int D>
-static tk_status go_decode(tk_ctx* ctx, KvaArgs& a, int dtype, cudaStream_t st) {
+template <int D, int DT>
+static tk_status go_decode(tk_ctx* ctx, KvaArgs& a, cudaStream_t st) {
     const size_t pairs = (size_t)a.s.n_seqs * a.c.heads;
-    const unsigned grid = KD_CTAS * ctx->num_sms;   // what is resident at once
-    const int least = KD_WARPS;               // a unit for every warp
+    const int nt = ((int)a.s.max_new * a.group + 7) / 8;
+    const unsigned grid = kd_blocks(nt) * ctx->num_sms;   // what is resident at once
+    const int least = KD_WARPS;                           // a unit for every warp
     if (pairs * ((size_t)a.s.max_pages << a.c.page_shift) / KD_UNIT + pairs > (1ull << 31))
         return fail(TK_ERR_UNSUPPORTED, "tk_kv_attend: sequences x heads x table length beyond 2^36 tokens");
-    tk_status r = ws_ensure(ctx, (size_t)grid * 2 * (16 * (D + 2)) * sizeof(float), st);
+    tk_status r = ws_ensure(ctx, (size_t)grid * 2 * (8 * nt * (D + 2)) * sizeof(float), st);
     if (r == TK_OK) r = kv_count_ensure(ctx, pairs);
     if (r != TK_OK) return r;
     a.part = static_cast<float*>(ctx->ws);
     a.count = ctx->kv_count;
-    const bool two = (long)a.s.max_new * a.group > 8;
-    if (dtype == TK_DT_F32)
-        return two ? go_decode_t<D, TK_DT_F32, 2>(ctx, a, grid, least, st) : go_decode_t<D, TK_DT_F32, 1>(ctx, a, grid, least, st);
-    if (dtype == TK_DT_F16)
-        return two ? go_decode_t<D, TK_DT_F16, 2>(ctx, a, grid, least, st) : go_decode_t<D, TK_DT_F16, 1>(ctx, a, grid, least, st);
-    return two ? go_decode_t<D, TK_DT_BF16, 2>(ctx, a, grid, least, st) : go_decode_t<D, TK_DT_BF16, 1>(ctx, a, grid, least, st);
+    switch (nt) {
+        case 1: return go_decode_t<D, DT, 1>(ctx, a, grid, least, st);
+        case 2: return go_decode_t<D, DT, 2>(ctx, a, grid, least, st);
+        case 3: return go_decode_t<D, DT, 3>(ctx, a, grid, least, st);
+        default: return go_decode_t<D, DT, 4>(ctx, a, grid, least, st);
+    }
+}
+template <int D>
+static tk_status go_decode_d(tk_ctx* ctx, KvaArgs& a, int dtype, cudaStream_t st) {
+    if (dtype == TK_DT_F32) return go_decode<D, TK_DT_F32>(ctx, a, st);
+    if (dtype == TK_DT_F16) return go_decode<D, TK_DT_F16>(ctx, a, st);
+    return go_decode<D, TK_DT_BF16>(ctx, a, st);
 }
 
 tk_status launch_kv_attend(tk_ctx* ctx, const tk_kvcache& c, const tk_seqs& s, const void* q, int dtype, long ldq,
@@ -671,8 +633,8 @@ tk_status launch_kv_attend(tk_ctx* ctx, const tk_kvcache& c, const tk_seqs& s, c
     a.scale2 = (float)((double)scale * 1.4426950408889634);
     a.status = ctx->status;
     // few rows per key/value head are memory's work, many the tensor cores'
-    if ((long)s.max_new * a.group <= 16)
-        return c.head_dim == 64 ? go_decode<64>(ctx, a, dtype, st) : go_decode<128>(ctx, a, dtype, st);
+    if ((long)s.max_new * a.group <= KD_MAX_ROWS)
+        return c.head_dim == 64 ? go_decode_d<64>(ctx, a, dtype, st) : go_decode_d<128>(ctx, a, dtype, st);
     return launch_kv_prompt(ctx, a, dtype, st);
 }
 

@@ -208,7 +208,7 @@ __device__ __forceinline__ void commit(uint32_t one, uint64_t* bar) {
 // The last part of a row set to finish joins them, in the order of the keys
 // (by the softmax warpgroups; parts lie by block).
 template <int D, int DT>
-__device__ __forceinline__ void join_parts(const KvaArgs& a, const Item& it, int* sh_last) {
+__device__ __forceinline__ void join_parts(const KvaArgs& a, const Item& it, uint8_t* smem, int* sh_last) {
     using G = Geo<D, DT == TK_DT_F32>;
     __threadfence();
     softmax_sync();
@@ -221,38 +221,13 @@ __device__ __forceinline__ void join_parts(const KvaArgs& a, const Item& it, int
     if (!*sh_last) return;
     __threadfence();
     const float* base = a.part + (size_t)(blockIdx.x - it.part) * G::PART;
-    for (int i = threadIdx.x; i < it.rows * (D / 4); i += 256) {
-        const int row = i / (D / 4), e = (i - row * (D / 4)) * 4;
-        float m = -INFINITY, sum = 0.0f;
-        float4 o = make_float4(0, 0, 0, 0);
-        for (int c0 = 0; c0 < it.parts; c0 += 8) {                 // eight parts' loads in flight
-            float4 v[8];
-            float2 st[8];
-#pragma unroll
-            for (int c = 0; c < 8; ++c) {
-                const float* p = base + (size_t)min(c0 + c, it.parts - 1) * G::PART;
-                v[c] = __ldcg(reinterpret_cast<const float4*>(p + row * D + e));
-                st[c] = __ldcg(reinterpret_cast<const float2*>(p + G::GROUP * D + 2 * row));
-                if (c0 + c >= it.parts) st[c] = make_float2(-INFINITY, 0.0f);
-            }
-            float big = m;
-#pragma unroll
-            for (int c = 0; c < 8; ++c) big = fmaxf(big, st[c].x);
-            const float ref = big == -INFINITY ? 0.0f : big, f = fast_exp2(m - ref);
-            sum *= f;
-            o.x *= f; o.y *= f; o.z *= f; o.w *= f;
-            m = big;
-#pragma unroll
-            for (int c = 0; c < 8; ++c) {
-                if (c0 + c >= it.parts) break;
-                const float g = fast_exp2(st[c].x - ref);
-                sum += st[c].y * g;
-                o.x += v[c].x * g; o.y += v[c].y * g; o.z += v[c].z * g; o.w += v[c].w * g;
-            }
-        }
-        const long grow = (long)it.group * G::GROUP + row;
-        kv_store_out<DT, D>(a, KvaRow{it.row0 + (int)(grow / a.group), it.head * a.group + (int)(grow % a.group)}, e, o, sum);
-    }
+    kv_join<D, DT, G::GROUP>(
+        a, it.parts, it.rows, threadIdx.x, 256, smem, G::SMEM - 1024, [&](int c) { return base + (size_t)c * G::PART; },
+        [&](int row) {
+            const long grow = (long)it.group * G::GROUP + row;
+            return KvaRow{it.row0 + (int)(grow / a.group), it.head * a.group + (int)(grow % a.group)};
+        },
+        [] { softmax_sync(); });
 }
 
 template <int D, int DT>
@@ -497,7 +472,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvaArgs a, 
                 }
             }
         }
-        if (part) join_parts<D, DT>(a, it, &sh_last);
+        if (part) join_parts<D, DT>(a, it, smem, &sh_last);
     } else if (warp < 12) {
         reg_dec<REG_CONVERT>();
         // ---------------- converters: thread = key of the tile ----------------
