@@ -244,6 +244,49 @@ def test_attend_strided_rows_and_long_context(ctx, dtype, new, heads):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("new,heads,kv_heads", [(1, 24, 1), (3, 8, 1), (7, 8, 2), (8, 4, 1), (1, 31, 1)])
+def test_attend_all_row_counts_of_the_streaming_kernel(ctx, dtype, new, heads, kv_heads):
+    """17 to 32 rows per key/value head."""
+    attend_case(ctx, [new, max(1, new - 1), new], [2000, 33, new], heads, kv_heads, 128 if new == 3 else 64, 64, dtype, seed=heads)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("new", [1, 9])
+def test_attend_many_sequences_of_different_length(ctx, dtype, new):
+    """More sequences than a warp has lanes, and more heads than thread blocks: a few long, most short, some empty."""
+    rng = np.random.default_rng(21)
+    kv = [int(x) for x in rng.integers(new, 60, 70)]
+    for b in range(0, 70, 9):
+        kv[b] = 1500 + b
+    news = [0 if b % 13 == 5 else new for b in range(70)]
+    attend_case(ctx, news, kv, 16 if new == 9 else 8, 8 if new == 1 else 2, 64, 16, dtype, seed=22)
+
+
+def test_append_many_sequences(ctx):
+    """More than 32 and more than 1024 sequences: the places of their tokens."""
+    import torch
+    import tier_b200 as tk
+    for B in (33, 1100):
+        rng = np.random.default_rng(B)
+        new = [int(x) for x in rng.integers(0, 3, B)]
+        kv = [n + int(x) for n, x in zip(new, rng.integers(0, 20, B))]
+        q_start, kv_len, pages, total = ref.batch(rng, new, kv, 16)
+        kc = tk.alloc_kvcache(total, 16, 1, 64)
+        sq = device_seqs(q_start, kv_len, pages)
+        x = rng.standard_normal((sum(new), 64)).astype(np.float32)
+        ctx.kv_append(kc, sq, dev(x), dev(-x))
+        ctx.sync_status()
+        k_q, v_q = kc._owner[0].cpu().numpy(), kc._owner[2].cpu().numpy()
+        m, _ = ref.quantize(x)
+        w, _ = ref.quantize(-x)
+        for b in range(B):
+            for i in range(new[b]):
+                t, r = kv[b] - new[b] + i, int(q_start[b]) + i
+                assert np.array_equal(k_q[pages[b, t // 16], 0, t % 16], ref.pack(m[r]))
+                assert np.array_equal(v_q[pages[b, t // 16], 0, t % 16], ref.pack(w[r]))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_attend_a_value_far_above_the_rest(ctx, dtype):
     """Scores that climb along the context and one key far above all others, each way round."""
     rng = np.random.default_rng(11)
@@ -393,6 +436,24 @@ def test_attend_in_a_captured_graph(ctx):
         exact, reach = ref.attend(cache, q_start, np.array(lens), pages, q.double().cpu().numpy(), 8, 2, 128, 128 ** -0.5, 0)
         check_attend(out.double().cpu().numpy().reshape(exact.shape), exact, reach, "f32")
     ctx.sync_status()
+
+
+def test_drafted_decoding_example(ctx):
+    """The example's greedy text is the same with drafts and without (each step's tokens through all operators)."""
+    import importlib.util
+    from conftest import ROOT
+    spec = importlib.util.spec_from_file_location("draft_decode", ROOT / "examples" / "draft_decode.py")
+    ex = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(ex)
+    prompts = [[3, 14, 15, 92, 65, 3, 14], [2, 71, 82, 2, 71], [1] * 40]
+    plain, _, _ = ex.generate(ex.Decoder(ctx), prompts, 24, drafts=0)
+    texts, taken, offered = ex.generate(ex.Decoder(ctx), prompts, 24, drafts=4)
+    for a, b in zip(plain, texts):
+        n = min(len(a), len(b))
+        assert a[:n] == b[:n]
+    assert 0 <= taken <= offered and offered > 0
+    warm, _, _ = ex.generate(ex.Decoder(ctx), prompts, 4, drafts=4, temperature=1.0, seed=5)
+    assert all(0 <= t < 1000 for w in warm for t in w)
 
 
 def test_refusals(ctx):

@@ -93,6 +93,29 @@ def test_verify_large_vocabulary(ctx, V):
     ctx.sync_status()
 
 
+@pytest.mark.parametrize("B", [1, 7, 10, 30, 120, 300])
+def test_verify_batches_of_every_division(ctx, B):
+    """Few sequences are drawn by many thread blocks, many by one each."""
+    x = inputs(B, [1 + b % 3 for b in range(B)], 3001, B % 2 == 0, 0.9)
+    check(ctx, run(ctx, *x, 0.9), *x, 0.9)
+    ctx.sync_status()
+
+
+@pytest.mark.parametrize("shift", [-3e7, 3e7, -5e6, 1e9])
+def test_logits_far_from_zero(ctx, shift):
+    """Logits whose exponents pass the packed form's range (2^22): steps of an fp32 there, the same rule."""
+    rng = np.random.default_rng(8)
+    unit = np.float32(np.spacing(np.float32(abs(shift))))
+    t = (np.float32(shift) + unit * rng.integers(-3, 4, (6, 1500)).astype(np.float32)).astype(np.float32)
+    start, tokens = np.array([0, 2, 6], np.int32), np.array([0, 7, 0, 8, 9, 10], np.int32)
+    ua, us = np.array([0.9, 0.9, 1e-5, 1e-5, 1e-5, 0.5], np.float32), np.array([0.37, 0.81], np.float32)
+    for T in (0.0, 1.0):
+        acc, nxt, _ = run(ctx, start, t, None, tokens, ua, us, T)
+        want = ref.verify(t, tokens, start, ua, us, None, T)
+        assert np.array_equal(acc, want[0]) and np.array_equal(nxt, want[1])
+    ctx.sync_status()
+
+
 def test_every_draw_comes_from_its_weights(ctx):
     """8192 draws from one row: the tokens' frequencies fit the residual's within 5 deviations."""
     V, n = 16, 8192

@@ -75,6 +75,23 @@ inline cudaError_t smem_attr_once(K* kern, int bytes, int device, std::atomic<ui
     return e;
 }
 
+// Launch as a programmatic dependent: the kernel's blocks may start while the
+// one before it drains, and wait for it (pdl_wait) before they touch memory.
+template <class... P, class... A>
+inline cudaError_t launch_dependent(void (*kern)(P...), unsigned grid, unsigned block, size_t smem, cudaStream_t s, A&&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(block);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kern, static_cast<P>(args)...);
+}
+
 // Kernel families for tk_profile_read (TK_PROF_* in tierk.h).
 enum ProfKind { PK_GEMM = 0, PK_DEQUANT = 1, PK_SPLIT = 2, PK_GEMV = 3, PK_LMHEAD = 4, PK_COMM = 5, PK_SERVE = 6,
                 PK_COUNT = 7 };

@@ -162,6 +162,12 @@ __device__ __forceinline__ float q_unit(float max, float& back) {
     return __uint_as_float((uint32_t)(254 - (e - 13)) << 23);
 }
 
+// A row's softmax weights are 2^(score - reference).  The reference is set KV_UP
+// below the largest score seen and stays until a score passes it by KV_MOVE:
+// the largest weight lies between 2^7 and 2^15, inside fp16's range, with room
+// below: a weight of 2^-10 of it still has both its fp16 parts whole.
+constexpr float KV_UP = 7.0f, KV_MOVE = 15.0f;
+
 // Values e .. e + 3 of an output row (packed row, head): O / l, zero where nothing was seen.
 struct KvaRow {
     int row, head;

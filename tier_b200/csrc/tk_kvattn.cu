@@ -41,10 +41,10 @@ __device__ __forceinline__ void kv_join_last(const KvaArgs& a, const Item& it, i
 // of two rows of each 8 keys.  A key's scale multiplies its fp16
 // numbers exactly.  P^T's fragments are S^T's turned by movmatrix.
 //
-// The softmax keeps a reference per row that moves only when a unit exceeds
-// it by 2^8: p stays below 2^8 (fp16 rounds relatively), the rescaling of O is
-// rare, and otherwise no lane needs another's maximum.  l is summed per lane
-// in fp32 and joined at the end.
+// The softmax keeps a reference per row that moves only when a unit's largest
+// weight would pass 2^15 (KV_MOVE): the rescaling of O is rare, and otherwise
+// no lane needs another's maximum.  l is summed per lane in fp32 and joined at
+// the end.
 //
 // Rows are copied by 16-byte cp.async into each warp's own ring (no barrier
 // between warps), as far ahead as the ring is deep: nine instructions a unit,
@@ -70,7 +70,7 @@ struct KdGeo {
 // blocks, all of which are resident at once; each block works it out from the
 // lengths on the device.  With `per` the equal share of a block:
 //   whole parts: every head is cut into ceil(units / p) even parts, one a
-//     block, for the smallest p of per, 1.04, 1.09 and 1.15 per that leaves no
+//     block, for the smallest p of per, 1.03 per and 1.07 per that leaves no
 //     more parts than blocks.  A short batch (p = `least`) is always cut the
 //     same way, whatever else it holds.
 //   runs: otherwise (many heads of very different length) the units, one head
@@ -115,16 +115,16 @@ __device__ __forceinline__ KdPlan kd_plan(const KvaArgs& a, uint32_t least) {
     p.whole = false;
     p.per = max((p.total + gridDim.x - 1) / gridDim.x, least);
     const uint32_t room = gridDim.x / a.c.heads;                   // parts that a head may have, over all sequences
-    uint32_t tried[4] = {p.per, p.per + (p.per + 24) / 25, p.per + (p.per + 10) / 11, p.per + (p.per + 5) / 6};
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
+#pragma unroll 1
+    for (int k = 0; k < 3; ++k) {
+        const uint32_t tried = p.per + (k * p.per + 29) / 30;
         uint32_t parts = 0;
         for (int b0 = 0; b0 < a.s.n_seqs; b0 += 32) {
             const int n = a.s.n_seqs > 32 ? kd_seq(a, b0 + lane, nullptr).units : p.mine.units;
-            parts += __reduce_add_sync(~0u, (n + tried[k] - 1) / tried[k]);
+            parts += __reduce_add_sync(~0u, (n + tried - 1) / tried);
         }
         if (parts <= room) {
-            p.per = tried[k];
+            p.per = tried;
             p.whole = true;
             p.total = parts * a.c.heads;
             break;
@@ -214,6 +214,8 @@ __global__ void __launch_bounds__(KD_WARPS * 32, kd_blocks(NT)) kv_decode_kernel
     __shared__ int sh_last;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int kg = kd_key(g), k0 = kd_key(2 * t), k1 = kd_key(2 * t + 1);
+    pdl_trigger();
+    pdl_wait();
     const KdPlan plan = kd_plan(a, least);
     uint32_t x = plan.whole ? blockIdx.x : blockIdx.x * plan.per;
     const uint32_t end = min(x + (plan.whole ? 1 : plan.per), plan.total);
@@ -426,7 +428,7 @@ __global__ void __launch_bounds__(KD_WARPS * 32, kd_blocks(NT)) kv_decode_kernel
             for (int c = 0; c < 2; ++c)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) top = fmaxf(top, v[n][c][j]);
-        if (__any_sync(~0u, top > 8.0f)) {                         // a row's reference moves
+        if (__any_sync(~0u, top > KV_MOVE)) {                     // a row's reference moves
             float old[NT][2];
 #pragma unroll
             for (int n = 0; n < NT; ++n)
@@ -440,7 +442,7 @@ __global__ void __launch_bounds__(KD_WARPS * 32, kd_blocks(NT)) kv_decode_kernel
                     float mx = fmaxf(fmaxf(v[n][c][0], v[n][c][1]), fmaxf(v[n][c][2], v[n][c][3]));
 #pragma unroll
                     for (int i2 = 4; i2 < 32; i2 <<= 1) mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, i2));
-                    const float now = fminf(old[n][c], -mx), f = now == INFINITY ? 1.0f : fast_exp2(now - old[n][c]);
+                    const float now = fminf(old[n][c], KV_UP - mx), f = now == INFINITY ? 1.0f : fast_exp2(now - old[n][c]);
                     nm[n][c] = now;
                     l[n][c] *= f;
 #pragma unroll
@@ -588,9 +590,9 @@ static tk_status go_decode_t(tk_ctx* ctx, const KvaArgs& a, unsigned grid, int l
     cudaError_t e = smem_attr_once(kern, KdGeo<D, NT>::SMEM, ctx->device, attr_done);
     if (e != cudaSuccess) return cuda_fail(e, "kv decode smem attribute");
     ProfScope ps(ctx, st, PK_SERVE);
-    kern<<<grid, KD_WARPS * 32, KdGeo<D, NT>::SMEM, st>>>(a, least);
+    e = launch_dependent(kern, grid, KD_WARPS * 32, KdGeo<D, NT>::SMEM, st, a, (uint32_t)least);
     ctx->launches++;
-    return cuda_fail(cudaGetLastError(), "kv decode launch");
+    return cuda_fail(e, "kv decode launch");
 }
 
 template <int D, int DT>

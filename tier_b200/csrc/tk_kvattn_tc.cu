@@ -17,8 +17,8 @@
 // the 128-byte-swizzled operand layout (the same bytes serve K, whose
 // reduction index is the head's values, and V, where it is the keys).
 //
-// As in the streaming kernel the softmax's reference moves only when a row
-// passes it by 2^8, so that O in TMEM is rarely rescaled.
+// As in the streaming kernel the softmax's reference moves only when a weight
+// would pass 2^15 (KV_MOVE), so that O in TMEM is rarely rescaled.
 //
 // Warps (512 threads, one block an SM): 0-3 and 4-7 the streams' softmax, 8-11
 // the converters, 12 issues the products (13-15 idle: registers are divided by
@@ -244,6 +244,8 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvaArgs a, 
     uint8_t *sq = smem, *sk = smem + 2 * G::TILE, *sv = smem + 4 * G::TILE;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
+    pdl_trigger();
+    pdl_wait();
     Item it;
     if (!find<G::GROUP>(a, blockIdx.x, sms, it)) return;
     if (threadIdx.x == 0) {
@@ -351,9 +353,9 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvaArgs a, 
                     }
                 }
                 const float mx = fmaxf(max3(m0, m1, m2), m3) * sc;
-                const bool move = mx + nm > 8.0f;
+                const bool move = mx + nm > KV_MOVE;
                 if (__any_sync(~0u, move)) {
-                    const float now = move ? -mx : nm;
+                    const float now = move ? KV_UP - mx : nm;
                     const float f = now == INFINITY ? 1.0f : fast_exp2(now - nm);
                     nm = now;
                     l *= f;
@@ -619,9 +621,9 @@ static tk_status go(tk_ctx* ctx, KvaArgs& a, cudaStream_t st) {
     a.part = static_cast<float*>(ctx->ws);
     a.count = ctx->kv_count;
     ProfScope ps(ctx, st, PK_SERVE);
-    kern<<<(unsigned)grid, THREADS, G::SMEM, st>>>(a, ctx->num_sms);
+    e = launch_dependent(kern, (unsigned)grid, THREADS, G::SMEM, st, a, ctx->num_sms);
     ctx->launches++;
-    return cuda_fail(cudaGetLastError(), "kv prompt launch");
+    return cuda_fail(e, "kv prompt launch");
 }
 
 }  // namespace kt

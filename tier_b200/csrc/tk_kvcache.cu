@@ -128,6 +128,8 @@ __device__ __forceinline__ float group_extreme(const float (&x)[8]) {
 template <int DT, int ITEMS>
 __global__ void __launch_bounds__(KVC_THREADS) kv_append_kernel(const KvcArgs a) {
     constexpr int SIZE = DT == TK_DT_F32 ? 4 : 2;
+    pdl_trigger();
+    pdl_wait();
     Where w;
     if (!where_is<SIZE>(a, ITEMS * 32, w) || !w.ok) return;
     const bool holds_scale = (threadIdx.x & 3) == 0;
@@ -201,6 +203,8 @@ __global__ void __launch_bounds__(KVC_THREADS) kv_append_kernel(const KvcArgs a)
 template <int DT, int ITEMS>
 __global__ void __launch_bounds__(KVC_THREADS) kv_read_kernel(const KvcArgs a) {
     constexpr int SIZE = DT == TK_DT_F32 ? 4 : 2;
+    pdl_trigger();
+    pdl_wait();
     Where w;
     if (!where_is<SIZE>(a, ITEMS * 32, w)) return;
     uint32_t q[ITEMS];
@@ -244,16 +248,17 @@ __global__ void __launch_bounds__(KVC_THREADS) kv_read_kernel(const KvcArgs a) {
 }
 
 template <int ITEMS>
-static void go_kvc(const KvcArgs& a, int dtype, bool append, unsigned grid, cudaStream_t st) {
-    if (append) {
-        if (dtype == TK_DT_F32) kv_append_kernel<TK_DT_F32, ITEMS><<<grid, KVC_THREADS, 0, st>>>(a);
-        else if (dtype == TK_DT_F16) kv_append_kernel<TK_DT_F16, ITEMS><<<grid, KVC_THREADS, 0, st>>>(a);
-        else kv_append_kernel<TK_DT_BF16, ITEMS><<<grid, KVC_THREADS, 0, st>>>(a);
-    } else {
-        if (dtype == TK_DT_F32) kv_read_kernel<TK_DT_F32, ITEMS><<<grid, KVC_THREADS, 0, st>>>(a);
-        else if (dtype == TK_DT_F16) kv_read_kernel<TK_DT_F16, ITEMS><<<grid, KVC_THREADS, 0, st>>>(a);
-        else kv_read_kernel<TK_DT_BF16, ITEMS><<<grid, KVC_THREADS, 0, st>>>(a);
-    }
+static cudaError_t go_kvc(const KvcArgs& a, int dtype, bool append, unsigned grid, cudaStream_t st) {
+    void (*kern)(const KvcArgs);
+    if (append)
+        kern = dtype == TK_DT_F32   ? kv_append_kernel<TK_DT_F32, ITEMS>
+               : dtype == TK_DT_F16 ? kv_append_kernel<TK_DT_F16, ITEMS>
+                                    : kv_append_kernel<TK_DT_BF16, ITEMS>;
+    else
+        kern = dtype == TK_DT_F32   ? kv_read_kernel<TK_DT_F32, ITEMS>
+               : dtype == TK_DT_F16 ? kv_read_kernel<TK_DT_F16, ITEMS>
+                                    : kv_read_kernel<TK_DT_BF16, ITEMS>;
+    return launch_dependent(kern, grid, KVC_THREADS, 0, st, a);
 }
 
 static tk_status launch_kvc(tk_ctx* ctx, const tk_kvcache& c, const tk_seqs& s, void* k, void* v, int dtype, long ldk,
@@ -271,10 +276,9 @@ static tk_status launch_kvc(tk_ctx* ctx, const tk_kvcache& c, const tk_seqs& s, 
     const long grid = (2L * s.n_tokens * a.chunks + KVC_THREADS / 32 - 1) / (KVC_THREADS / 32);
     if (grid * (KVC_THREADS / 32) > INT32_MAX) return fail(TK_ERR_INVALID, "tk_kv_append / tk_kv_read: too many values");
     ProfScope ps(ctx, st, PK_SERVE);
-    if (many) go_kvc<4>(a, dtype, append, (unsigned)grid, st);
-    else go_kvc<1>(a, dtype, append, (unsigned)grid, st);
+    const cudaError_t e = many ? go_kvc<4>(a, dtype, append, (unsigned)grid, st) : go_kvc<1>(a, dtype, append, (unsigned)grid, st);
     ctx->launches++;
-    return cuda_fail(cudaGetLastError(), append ? "kv append launch" : "kv read launch");
+    return cuda_fail(e, append ? "kv append launch" : "kv read launch");
 }
 
 tk_status launch_kv_append(tk_ctx* ctx, const tk_kvcache& c, const tk_seqs& s, const void* k, const void* v, int dtype,
