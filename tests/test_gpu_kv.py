@@ -508,3 +508,35 @@ def test_refusals(ctx):
     with pytest.raises(ValueError):
         tk.make_seqs(seqs._owner[0].long(), seqs._owner[1], seqs._owner[2], 4, 4)
     ctx.sync_status()
+
+
+@pytest.mark.parametrize("rising", [False, True])
+@pytest.mark.parametrize("dtype,dim,new,seqs", [
+    ("f32", 128, 40, 90), ("f32", 64, 40, 90), ("f16", 128, 100, 90), ("f16", 64, 30, 150),   # row sets
+    ("f32", 128, 1, 330), ("f32", 64, 7, 330), ("f16", 128, 2, 330), ("bf16", 128, 1, 330),     # streamed
+])
+def test_attend_long_sums(ctx, dtype, dim, new, seqs, rising):
+    """One block or warp adds 20000 keys' values, all of one sign, in sequences enough that none is cut into short parts.
+
+    A sum that lost 2^-24 of itself with each of its 16-key products would be 7e-5 to 1.5e-4 off; what is allowed is 2e-5 of
+    sum p |v| (and the rounding of 16-bit outputs and weights), of which 128 such losses take 0.8e-5, 512 3.1e-5.
+    `rising`: scores grow by 2^60 along the keys, so that the reference moves in the midst of sums.
+    """
+    kv, page, heads = 20000, 256, 4
+    need = -(-kv // page)
+    rng = np.random.default_rng(11)
+    cache = ref.random_cache(rng, need, page, 1, dim)
+    cache["v_q"] = rng.integers(1, 8, cache["v_q"].shape, dtype=np.uint8) * 16 + rng.integers(1, 8, cache["v_q"].shape, dtype=np.uint8)
+    cache["v_s"] = np.abs(cache["v_s"]) + np.float16(2.0 ** -6)
+    cache["v_s"] = ref.round_bits(cache["v_s"].astype(np.float64), 8).astype(np.float16)
+    q = rng.standard_normal((new, heads * dim)) * 0.3
+    if rising:
+        cache["k_q"] = cache["k_q"] & 0x77                                  # 0 to 7
+        at = (np.arange(need * page).reshape(need, 1, page, 1) + 1) / (need * page)
+        cache["k_s"] = ref.round_bits(np.broadcast_to(0.1 * at, cache["k_s"].shape), 8).astype(np.float16)
+        q = np.abs(q) * 60 * np.log(2) * np.sqrt(dim) / (0.1 * 3.5 * np.abs(q).reshape(new, heads, dim).sum(-1).repeat(dim, -1))
+    pages = np.tile(np.arange(need, dtype=np.int32), (seqs, 1))
+    bat = (np.arange(seqs + 1, dtype=np.int32) * new, np.full(seqs, kv, np.int32), pages, need)
+    qr, out = run_attend(ctx, cache, bat, np.tile(q, (seqs, 1)), heads, dtype)
+    exact, reach = ref.attend(cache, bat[0][:2], bat[1][:1], pages[:1], qr[:new], heads, 1, dim, dim ** -0.5, 0)
+    check_attend(out.reshape(seqs, *exact.shape), exact[None], reach[None], dtype)

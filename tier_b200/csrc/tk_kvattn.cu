@@ -476,51 +476,45 @@ __global__ void __launch_bounds__(KD_WARPS * 32, kd_blocks(NT)) kv_decode_kernel
                 }
             }
         // O^T: matrix rows g and g + 8 of tile i are values (D / 8) g + 2 i and + 1 of the head. The tensor core cuts what
-        // it adds to an accumulator, which for fp32 rows shows (one accumulator for all keys: 2e-6 of the values off at
-        // 131071 keys): a unit's sum is made from zero and added to O here. 16-bit rows accumulate in place.
-        constexpr int HS = SPLIT ? 2 : 1;                          // 16-key halves whose fields are held together
+        // it adds to an accumulator: n products in one lose up to n 2^-24 of it. So the 32 keys' sum is made from zero and
+        // added to O here (fp32, 131071 keys: 54.2 us; 52.3 and 2e-6 off if all keys went to one accumulator).
+        uint32_t w[8][VW];                                         // the two keys of lane t, of each 8-key group
+        __half2 d[4];
 #pragma unroll
-        for (int h0 = 0; h0 < 2; h0 += HS) {
-            uint32_t w[4 * HS][VW];                                // the two keys of lane t, of each 8-key group
-            __half2 d[2 * HS];
+        for (int j = 0; j < 8; ++j) {
+            const int key = 8 * (j >> 1) + (j & 1 ? k1 : k0);
+            if constexpr (VW == 2) {
+                const uint2 u = *reinterpret_cast<const uint2*>(vq + key * (D / 2) + ((g * 8) ^ ((k0 & 2) << 4)));
+                w[j][0] = u.x; w[j][1] = u.y;
+            } else {
+                w[j][0] = *reinterpret_cast<const uint32_t*>(vq + key * (D / 2) + g * 4);
+            }
+            const __half dj = vs[key * (D / 32) + (g * D / 256)];
+            d[j >> 1] = j & 1 ? __halves2half2(__low2half(d[j >> 1]), dj) : __half2half2(dj);
+        }
 #pragma unroll
-            for (int j = 0; j < 4 * HS; ++j) {
-                const int key = 16 * h0 + 8 * (j >> 1) + (j & 1 ? k1 : k0);
-                if constexpr (VW == 2) {
-                    const uint2 u = *reinterpret_cast<const uint2*>(vq + key * (D / 2) + ((g * 8) ^ ((k0 & 2) << 4)));
-                    w[j][0] = u.x; w[j][1] = u.y;
-                } else {
-                    w[j][0] = *reinterpret_cast<const uint32_t*>(vq + key * (D / 2) + g * 4);
-                }
-                const __half dj = vs[key * (D / 32) + (g * D / 256)];
-                d[j >> 1] = j & 1 ? __halves2half2(__low2half(d[j >> 1]), dj) : __half2half2(dj);
+        for (int i2 = 0; i2 < VW; ++i2) {
+            uint32_t fl[8][4];                                     // fields 0..3: values 0 2 4 6; 4..7: 1 3 5 7
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                kv_fields(__byte_perm(w[2 * j][i2], w[2 * j + 1][i2], 0x5410u), d[j], fl[2 * j]);
+                kv_fields(__byte_perm(w[2 * j][i2], w[2 * j + 1][i2], 0x7632u), d[j], fl[2 * j + 1]);
             }
 #pragma unroll
-            for (int i2 = 0; i2 < VW; ++i2) {
-                uint32_t fl[4 * HS][4];                            // fields 0..3: values 0 2 4 6; 4..7: 1 3 5 7
+            for (int f = 0; f < 4; ++f)
 #pragma unroll
-                for (int j = 0; j < 2 * HS; ++j) {
-                    kv_fields(__byte_perm(w[2 * j][i2], w[2 * j + 1][i2], 0x5410u), d[j], fl[2 * j]);
-                    kv_fields(__byte_perm(w[2 * j][i2], w[2 * j + 1][i2], 0x7632u), d[j], fl[2 * j + 1]);
+                for (int n = 0; n < NT; ++n) {
+                    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int p = PARTS - 1; p >= 0; --p)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const uint32_t av[4] = {fl[4 * h][f], fl[4 * h + 1][f], fl[4 * h + 2][f], fl[4 * h + 3][f]};
+                            mma_16816(sum, av, pb[n][p][2 * h], pb[n][p][2 * h + 1]);
+                        }
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[n][4 * i2 + f][e] += sum[e];
                 }
-#pragma unroll
-                for (int f = 0; f < 4; ++f)
-#pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-                        float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                        float(&to)[4] = SPLIT ? acc : o[n][4 * i2 + f];
-#pragma unroll
-                        for (int p = PARTS - 1; p >= 0; --p)
-#pragma unroll
-                            for (int h = 0; h < HS; ++h) {
-                                const uint32_t av[4] = {fl[4 * h][f], fl[4 * h + 1][f], fl[4 * h + 2][f], fl[4 * h + 3][f]};
-                                mma_16816(to, av, pb[n][p][2 * (h0 + h)], pb[n][p][2 * (h0 + h) + 1]);
-                            }
-                        if constexpr (SPLIT)
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) o[n][4 * i2 + f][e] += acc[e];
-                    }
-            }
         }
         __syncwarp();                                              // the stage may be overwritten
         if (++stage == KD_STAGES) stage = 0;

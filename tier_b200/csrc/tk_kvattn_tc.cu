@@ -17,6 +17,11 @@
 // the 128-byte-swizzled operand layout (the same bytes serve K, whose
 // reduction index is the head's values, and V, where it is the keys).
 //
+// The tensor core cuts what it adds to an accumulator: n products in one lose
+// up to n 2^-24 of it (fp32, 30000 keys: 1.1e-4).  So every SEG steps O is
+// added to a sum in fp32, in memory that stays in L2, and begins from zero:
+// 128 products (7.6e-6) for fp32, 512 (3.1e-5, of a rounding of 4.9e-4) else.
+//
 // As in the streaming kernel the softmax's reference moves only when a weight
 // would pass 2^15 (KV_MOVE), so that O in TMEM is rarely rescaled.
 //
@@ -31,8 +36,9 @@ namespace tk {
 namespace kt {
 
 constexpr int ROWS = 128, KEYS = 128, THREADS = 512;
-// registers a thread of each warpgroup: 4 x 128 at launch, 184 + 184 + 88 + 56 = 512 after the split
-constexpr int REG_SOFTMAX = 184, REG_CONVERT = 88, REG_ISSUE = 56;
+// registers a thread of each warpgroup: 4 x 128 at launch, 192 + 192 + 80 + 48 = 512 after the split
+// (184 + 184 + 88 + 56 spills in the softmax: a prompt of 8192 takes 652 us, not 609)
+constexpr int REG_SOFTMAX = 192, REG_CONVERT = 80, REG_ISSUE = 48;
 
 template <int D, bool SPLIT>
 struct Geo {
@@ -42,6 +48,8 @@ struct Geo {
     static constexpr int SMEM = 6 * TILE + 1024;                   // q: 2 sets (or parts), K and V: 2 stages each
     static constexpr uint32_t S = 0, O = 256;                      // TMEM columns: S of stream w at 128 w, O at 256 + D w
     static constexpr int PART = GROUP * (D + 2);                   // floats of a part: O, then (m, l) of each row
+    static constexpr int SUM = 2 * ROWS * D;                       // floats of the two streams' sums
+    static constexpr int SEG = SPLIT ? 8 : 64;                     // steps between additions to them (a power of two)
 };
 
 struct Item {
@@ -205,6 +213,24 @@ __device__ __forceinline__ void commit(uint32_t one, uint64_t* bar) {
         : "memory");
 }
 
+// A place for the block's sums: one block an SM is resident, so that of `slots`
+// places one is free (its flag is zero between blocks).
+__device__ __forceinline__ int take_slot(int* busy, int slots, int* status) {
+    uint32_t s;
+    asm volatile("mov.u32 %0, %%smid;" : "=r"(s));
+    s %= (uint32_t)slots;
+    const uint64_t t0 = globaltimer();
+    do {
+        for (int i = 0; i < slots; ++i, s = s + 1 == (uint32_t)slots ? 0 : s + 1)
+            if (atomicCAS(busy + s, 0, 1) == 0) {
+                __threadfence();
+                return (int)s;
+            }
+    } while (globaltimer() - t0 < kWaitLimitNs);
+    raise_status(status, DEV_TIMEOUT);
+    return -1;
+}
+
 // The last part of a row set to finish joins them, in the order of the keys
 // (by the softmax warpgroups; parts lie by block).
 template <int D, int DT>
@@ -231,7 +257,7 @@ __device__ __forceinline__ void join_parts(const KvaArgs& a, const Item& it, uin
 }
 
 template <int D, int DT>
-__global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvaArgs a, int sms) {
+__global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvaArgs a, float* sums, int* busy, int sms) {
     constexpr bool SPLIT = DT == TK_DT_F32;
     constexpr int PARTS = SPLIT ? 2 : 1;                           // fp16 parts of q and of P
     using G = Geo<D, SPLIT>;
@@ -239,16 +265,23 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvaArgs a, 
     __shared__ uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], q_full, s_full[2], p_full[2], o_full[2];
     __shared__ uint32_t tmem_slot;
     __shared__ float ml[2][ROWS][2];
-    __shared__ int sh_last;
+    __shared__ int sh_last, sh_slot;
+    __shared__ Item it;                                            // (not in registers: the softmax needs them all)
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t *sq = smem, *sk = smem + 2 * G::TILE, *sv = smem + 4 * G::TILE;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     pdl_trigger();
     pdl_wait();
-    Item it;
-    if (!find<G::GROUP>(a, blockIdx.x, sms, it)) return;
+    Item found;
+    if (!find<G::GROUP>(a, blockIdx.x, sms, found)) return;
+    // both streams on the same rows, every other tile each
+    const bool same = SPLIT || found.rows <= ROWS;
+    const int tiles = found.t1 - found.t0;
+    const int steps = same ? (tiles + 1) / 2 : tiles;              // tiles of a stream
     if (threadIdx.x == 0) {
+        it = found;
+        sh_slot = steps > G::SEG ? take_slot(busy, sms, a.status) : -1;
         for (int i = 0; i < 2; ++i) {
             mbar_init(&k_full[i], 128);
             mbar_init(&v_full[i], 128);
@@ -270,10 +303,6 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvaArgs a, 
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
 
-    // both streams on the same rows, every other tile each
-    const bool same = SPLIT || it.rows <= ROWS;
-    const int tiles = it.t1 - it.t0;
-    const int steps = same ? (tiles + 1) / 2 : tiles;              // tiles of a stream
     const int made = same ? 2 * steps : steps;                     // tiles made (the last may have no keys)
     const int pos0 = it.kv - it.n_new;
     // lane address of a softmax warp's rows
@@ -324,95 +353,130 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvaArgs a, 
         }
         const uint32_t ts = tmem + lanes + G::S + w * 128, to = tmem + lanes + G::O + w * D;
         const bool any_live = __any_sync(~0u, live);
-        for (int j = 0; j < steps; ++j) {
-            const int key0 = (it.t0 + (same ? 2 * j + w : j)) * KEYS;
-            if (!__all_sync(~0u, mbar_wait(&s_full[w], j & 1, a.status))) break;
-            tc_fence_after();
-            if (any_live) {
-                const bool edge = __any_sync(~0u, live && (key0 + KEYS > limit || key0 < from));
-                // S of the whole row in registers
-                float x[KEYS];
-#pragma unroll
-                for (int c = 0; c < 4; ++c) tc_ld_32x32b_x32(ts + c * 32, *reinterpret_cast<uint32_t(*)[32]>(x + c * 32));
-                tc_wait_ld();
-                if (edge) {                                        // what the row does not see
-                    const unsigned width = max(limit - from, 0);
-                    const int rel = key0 - from;
-#pragma unroll
-                    for (int i = 0; i < KEYS; ++i)
-                        if ((unsigned)(rel + i) >= width) x[i] = -INFINITY;
-                }
-                float m0 = x[0], m1 = x[1], m2 = x[2], m3 = x[3];
-#pragma unroll
-                for (int i = 4; i < KEYS; i += 8) {
-                    m0 = max3(m0, x[i], x[i + 1]);
-                    m1 = max3(m1, x[i + 2], x[i + 3]);
-                    if (i + 4 < KEYS) {
-                        m2 = max3(m2, x[i + 4], x[i + 5]);
-                        m3 = max3(m3, x[i + 6], x[i + 7]);
-                    }
-                }
-                const float mx = fmaxf(max3(m0, m1, m2), m3) * sc;
-                const bool move = mx + nm > KV_MOVE;
-                if (__any_sync(~0u, move)) {
-                    const float now = move ? KV_UP - mx : nm;
-                    const float f = now == INFINITY ? 1.0f : fast_exp2(now - nm);
-                    nm = now;
-                    l *= f;
-                    if (j > 0) {
+        // this row's sum, chunks of four values 128 rows apart, and its factor
+        auto total = [&](int c) {
+            return reinterpret_cast<float4*>(sums + (size_t)sh_slot * G::SUM) + (w * (D / 4) + c / 4) * ROWS + r;
+        };
+        float ft = 1.0f;
+        const int seg = sh_slot >= 0 ? G::SEG : steps;
+        bool ok = true;
+        for (int j0 = 0; j0 < steps && ok; j0 += seg) {
+            if (j0 > 0 && any_live) {                              // (with S, the last O is there)
+                ok = __all_sync(~0u, mbar_wait(&s_full[w], j0 & 1, a.status));
+                tc_fence_after();
+                if (!ok) break;
 #pragma unroll 1
-                        for (int c = 0; c < D; c += 16) {
-                            uint32_t y[16];
-                            tc_ld_32x32b_x16(to + c, y);
-                            tc_wait_ld();
+                for (int c = 0; c < D; c += 32) {
+                    uint32_t y[32];
+                    float4 t[8];
 #pragma unroll
-                            for (int i = 0; i < 16; ++i) y[i] = __float_as_uint(__uint_as_float(y[i]) * f);
-                            tc_st_32x32b_x16(to + c, y);
-                        }
-                        tc_wait_st();
-                    }
+                    for (int i = 0; i < 8; ++i)
+                        t[i] = j0 > G::SEG ? __ldcg(total(c + 4 * i)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    tc_ld_32x32b_x32(to + c, y);
+                    tc_wait_ld();
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        __stcg(total(c + 4 * i),
+                               make_float4(fmaf(t[i].x, ft, __uint_as_float(y[4 * i])),
+                                           fmaf(t[i].y, ft, __uint_as_float(y[4 * i + 1])),
+                                           fmaf(t[i].z, ft, __uint_as_float(y[4 * i + 2])),
+                                           fmaf(t[i].w, ft, __uint_as_float(y[4 * i + 3]))));
                 }
-                const f32x2 sc2 = pack2(sc, sc), ref2 = nm == INFINITY ? pack2(0.0f, 0.0f) : pack2(nm, nm);
-                f32x2 sum = pack2(l, 0.0f);
-                // in place and in three steps, eight pairs apart, so that no
-                // exponential waits for its own operand or its own use
-                auto exponent = [&](int i) {                       // pairs i .. i + 7
-#pragma unroll
-                    for (int k = i; k < i + 8; ++k)
-                        unpack2(fma2(pack2(x[2 * k], x[2 * k + 1]), sc2, ref2), x[2 * k], x[2 * k + 1]);
-                };
-                auto power = [&](int i) {
-#pragma unroll
-                    for (int k = 2 * i; k < 2 * i + 16; ++k) x[k] = fast_exp2(x[k]);
-                };
-                auto finish = [&](int i) {
-                    uint32_t hi[8], lo[8];
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) {
-                        const float p0 = x[2 * (i + k)], p1 = x[2 * (i + k) + 1];
-                        sum = add2(sum, pack2(p0, p1));
-                        hi[k] = pack_half2(p0, p1);
-                        if constexpr (SPLIT)
-                            lo[k] = pack_half2(p0 - __low2float(as_half2(hi[k])), p1 - __high2float(as_half2(hi[k])));
-                    }
-                    tc_st_32x32b_x8(ts + i, hi);
-                    if constexpr (SPLIT) tc_st_32x32b_x8(ts + 64 + i, lo);
-                };
-                exponent(0);
-#pragma unroll
-                for (int i = 0; i < KEYS / 2; i += 8) {
-                    power(i);
-                    if (i + 8 < KEYS / 2) exponent(i + 8);
-                    if (i >= 8) finish(i - 8);
-                }
-                finish(KEYS / 2 - 8);
-                float s0, s1;
-                unpack2(sum, s0, s1);
-                l = s0 + s1;
-                tc_wait_st();
+                ft = 1.0f;
             }
-            tc_fence_before();
-            mbar_arrive(&p_full[w]);
+            const int j1 = min(j0 + seg, steps);
+            for (int j = j0; j < j1; ++j) {
+                const int key0 = (it.t0 + (same ? 2 * j + w : j)) * KEYS;
+                ok = __all_sync(~0u, mbar_wait(&s_full[w], j & 1, a.status));
+                if (!ok) break;
+                tc_fence_after();
+                if (any_live) {
+                    const bool edge = __any_sync(~0u, live && (key0 + KEYS > limit || key0 < from));
+                    // S of the whole row in registers
+                    float x[KEYS];
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) tc_ld_32x32b_x32(ts + c * 32, *reinterpret_cast<uint32_t(*)[32]>(x + c * 32));
+                    tc_wait_ld();
+                    if (edge) {                                        // what the row does not see
+                        const unsigned width = max(limit - from, 0);
+                        const int rel = key0 - from;
+#pragma unroll
+                        for (int i = 0; i < KEYS; ++i)
+                            if ((unsigned)(rel + i) >= width) x[i] = -INFINITY;
+                    }
+                    float m0 = x[0], m1 = x[1], m2 = x[2], m3 = x[3];
+#pragma unroll
+                    for (int i = 4; i < KEYS; i += 8) {
+                        m0 = max3(m0, x[i], x[i + 1]);
+                        m1 = max3(m1, x[i + 2], x[i + 3]);
+                        if (i + 4 < KEYS) {
+                            m2 = max3(m2, x[i + 4], x[i + 5]);
+                            m3 = max3(m3, x[i + 6], x[i + 7]);
+                        }
+                    }
+                    const float mx = fmaxf(max3(m0, m1, m2), m3) * sc;
+                    const bool move = mx + nm > KV_MOVE;
+                    if (__any_sync(~0u, move)) {
+                        const float now = move ? KV_UP - mx : nm;
+                        const float f = now == INFINITY ? 1.0f : fast_exp2(now - nm);
+                        nm = now;
+                        l *= f;
+                        ft *= f;
+                        if (j > j0) {
+#pragma unroll 1
+                            for (int c = 0; c < D; c += 16) {
+                                uint32_t y[16];
+                                tc_ld_32x32b_x16(to + c, y);
+                                tc_wait_ld();
+#pragma unroll
+                                for (int i = 0; i < 16; ++i) y[i] = __float_as_uint(__uint_as_float(y[i]) * f);
+                                tc_st_32x32b_x16(to + c, y);
+                            }
+                            tc_wait_st();
+                        }
+                    }
+                    const f32x2 sc2 = pack2(sc, sc), ref2 = nm == INFINITY ? pack2(0.0f, 0.0f) : pack2(nm, nm);
+                    f32x2 sum = pack2(l, 0.0f);
+                    // in place and in three steps, eight pairs apart, so that no
+                    // exponential waits for its own operand or its own use
+                    auto exponent = [&](int i) {                       // pairs i .. i + 7
+#pragma unroll
+                        for (int k = i; k < i + 8; ++k)
+                            unpack2(fma2(pack2(x[2 * k], x[2 * k + 1]), sc2, ref2), x[2 * k], x[2 * k + 1]);
+                    };
+                    auto power = [&](int i) {
+#pragma unroll
+                        for (int k = 2 * i; k < 2 * i + 16; ++k) x[k] = fast_exp2(x[k]);
+                    };
+                    auto finish = [&](int i) {
+                        uint32_t hi[8], lo[8];
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            const float p0 = x[2 * (i + k)], p1 = x[2 * (i + k) + 1];
+                            sum = add2(sum, pack2(p0, p1));
+                            hi[k] = pack_half2(p0, p1);
+                            if constexpr (SPLIT)
+                                lo[k] = pack_half2(p0 - __low2float(as_half2(hi[k])), p1 - __high2float(as_half2(hi[k])));
+                        }
+                        tc_st_32x32b_x8(ts + i, hi);
+                        if constexpr (SPLIT) tc_st_32x32b_x8(ts + 64 + i, lo);
+                    };
+                    exponent(0);
+#pragma unroll
+                    for (int i = 0; i < KEYS / 2; i += 8) {
+                        power(i);
+                        if (i + 8 < KEYS / 2) exponent(i + 8);
+                        if (i >= 8) finish(i - 8);
+                    }
+                    finish(KEYS / 2 - 8);
+                    float s0, s1;
+                    unpack2(sum, s0, s1);
+                    l = s0 + s1;
+                    tc_wait_st();
+                }
+                tc_fence_before();
+                mbar_arrive(&p_full[w]);
+            }
         }
         if (steps) {
             mbar_wait(&o_full[w], 0, a.status);
@@ -420,6 +484,17 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvaArgs a, 
         }
         ml[w][r][0] = -nm;
         ml[w][r][1] = l;
+        auto add_total = [&](int c, uint32_t (&x)[32]) {
+            if (sh_slot < 0 || !any_live) return;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float4 t = __ldcg(total(c + 4 * i));
+                x[4 * i] = __float_as_uint(fmaf(t.x, ft, __uint_as_float(x[4 * i])));
+                x[4 * i + 1] = __float_as_uint(fmaf(t.y, ft, __uint_as_float(x[4 * i + 1])));
+                x[4 * i + 2] = __float_as_uint(fmaf(t.z, ft, __uint_as_float(x[4 * i + 2])));
+                x[4 * i + 3] = __float_as_uint(fmaf(t.w, ft, __uint_as_float(x[4 * i + 3])));
+            }
+        };
         if (same) {                                                // the second stream's O of the same rows by way of smem
             float* osh = reinterpret_cast<float*>(smem);           // [128][D + 4]
             softmax_sync();                                        // (both streams' products are done: q, K and V are free)
@@ -429,6 +504,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvaArgs a, 
                     uint32_t x[32];
                     tc_ld_32x32b_x32(to + c, x);
                     tc_wait_ld();
+                    add_total(c, x);
 #pragma unroll
                     for (int i = 0; i < 32; i += 4)
                         *reinterpret_cast<uint4*>(osh + r * (D + 4) + c + i) = make_uint4(x[i], x[i + 1], x[i + 2], x[i + 3]);
@@ -446,7 +522,8 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvaArgs a, 
                 sum = sum * f0 + ml[1][r][1] * f1;
                 m = big;
             }
-            const KvaRow out{it.row0 + tok, it.head * a.group + (int)(grow % a.group)};
+            const long at = (long)it.group * G::GROUP + row;
+            const KvaRow out{it.row0 + (int)(at / a.group), it.head * a.group + (int)(at % a.group)};
             if (part && live) {
                 part[G::GROUP * D + 2 * row] = m;
                 part[G::GROUP * D + 2 * row + 1] = sum;
@@ -459,6 +536,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvaArgs a, 
                 if (steps) {                                       // (uniform)
                     tc_ld_32x32b_x32(to + c, x);
                     tc_wait_ld();
+                    add_total(c, x);
                 }
                 if (!live) continue;
 #pragma unroll
@@ -556,6 +634,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvaArgs a, 
                 commit(one, &s_full[w]);
                 if (same || w == 1) commit(one, &k_empty[i & 1]);
             };
+            const bool cut = sh_slot >= 0;
             bool ok = wait(&q_full, 0);
             for (int w = 0; w < 2 && ok; ++w) {
                 const int i = same ? w : 0;
@@ -570,12 +649,13 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvaArgs a, 
                     if (!ok) break;
                     tc_fence_after();
                     const uint64_t vd = dv + (i & 1) * TILE;
+                    const uint32_t more = cut ? j % G::SEG > 0 : j > 0;
 #pragma unroll
                     for (int p = PARTS - 1; p >= 0; --p)
 #pragma unroll
                         for (int kk = 0; kk < KEYS / 16; ++kk)
                             mma_ts(one, tmem + G::O + w * D, tmem + G::S + w * 128 + p * 64 + kk * 8, vd + (kk * 2048 >> 4), id_o,
-                                   j > 0 || p != PARTS - 1 || kk > 0);
+                                   more || p != PARTS - 1 || kk > 0);
                     if (same || w == 1) commit(one, &v_empty[i & 1]);
                     if (j + 1 < steps) {
                         const int n = same ? i + 2 : j + 1;
@@ -597,6 +677,10 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvaArgs a, 
     }
     tc_fence_before();
     __syncthreads();
+    if (threadIdx.x == 0 && sh_slot >= 0) {
+        __threadfence();
+        atomicExch(busy + sh_slot, 0);
+    }
     if (warp == 12) {
         tc_fence_after();
         tmem_dealloc(tmem, 512);
@@ -615,13 +699,15 @@ static tk_status go(tk_ctx* ctx, KvaArgs& a, cudaStream_t st) {
     const long sets = (((long)a.s.n_tokens * a.group + G::GROUP - 1) / G::GROUP + a.s.n_seqs) * a.c.heads;
     const long grid = sets > ctx->num_sms ? sets : ctx->num_sms;
     if (grid > INT32_MAX) return fail(TK_ERR_INVALID, "tk_kv_attend: too many rows");
-    tk_status r = ws_ensure(ctx, (size_t)ctx->num_sms * G::PART * sizeof(float), st);
-    if (r == TK_OK) r = kv_count_ensure(ctx, (size_t)sets);
+    tk_status r = ws_ensure(ctx, (size_t)ctx->num_sms * (G::PART + G::SUM) * sizeof(float), st);
+    if (r == TK_OK) r = kv_count_ensure(ctx, (size_t)(sets + ctx->num_sms));
     if (r != TK_OK) return r;
     a.part = static_cast<float*>(ctx->ws);
-    a.count = ctx->kv_count;
+    float* sums = a.part + (size_t)ctx->num_sms * G::PART;
+    int* busy = ctx->kv_count;                                     // num_sms flags, then the row sets' counters
+    a.count = busy + ctx->num_sms;
     ProfScope ps(ctx, st, PK_SERVE);
-    e = launch_dependent(kern, (unsigned)grid, THREADS, G::SMEM, st, a, ctx->num_sms);
+    e = launch_dependent(kern, (unsigned)grid, THREADS, G::SMEM, st, a, sums, busy, ctx->num_sms);
     ctx->launches++;
     return cuda_fail(e, "kv prompt launch");
 }
