@@ -29,6 +29,15 @@
 // the converters, 12 issues the products (13-15 idle: registers are divided by
 // groups of four warps).  A row set that would leave SMs idle
 // is cut along the keys, and its parts joined by the last block to finish.
+//
+// Bound: the softmax's instructions (an exponential, a product-sum, an addition
+// and half a conversion a score) beside the tensor core's 2 x 128 cycles a
+// tile; neither waits long for the other, under a power limit that holds the
+// clock at 1.47 GHz of 1.97 in long prompts.  Measured (32 query heads on 8
+// key/value heads of 128): a prompt of 8192, bf16, 609 us, 900 TFLOP/s; three
+// chunks of up to 1000 rows behind 6001 keys, window 1024, 16 heads on 4 of
+// 64, fp16, 33.6 us; two fp32 prompts of up to 1537 rows, 2000 keys, 176 us, 218
+// TFLOP/s (two parts of q and of P: twice that in the tensor core).
 #include "tk_f32x2.cuh"
 #include "tk_kv.cuh"
 

