@@ -90,8 +90,9 @@ __device__ __forceinline__ bool find(const KvaArgs& a, int x, int sms, Item& it)
     const int lane = threadIdx.x & 31;
     int sets = 0;
     long work = 0;                                                 // tiles of all row sets
+    const Need first = need<GROUP>(a, lane, a.status);             // kept: mostly there are no others
     for (int b0 = 0; b0 < a.s.n_seqs; b0 += 32) {
-        const Need n = need<GROUP>(a, b0 + lane, a.status);
+        const Need n = b0 ? need<GROUP>(a, b0 + lane, a.status) : first;
         sets += __reduce_add_sync(~0u, n.groups);
         long w = (long)n.groups * n.tiles;
         for (int i = 16; i; i >>= 1) w += __shfl_xor_sync(~0u, w, i);
@@ -105,7 +106,7 @@ __device__ __forceinline__ bool find(const KvaArgs& a, int x, int sms, Item& it)
         for (int step = 0; step < 6; ++step, per += (per + 7) / 8) {
             int parts = 0;
             for (int b0 = 0; b0 < a.s.n_seqs; b0 += 32) {
-                const Need n = need<GROUP>(a, b0 + lane, nullptr);
+                const Need n = b0 ? need<GROUP>(a, b0 + lane, nullptr) : first;
                 parts += __reduce_add_sync(~0u, n.groups * ((max(n.tiles, 1) + per - 1) / per));
             }
             if (parts * a.c.heads <= sms) break;
@@ -114,7 +115,7 @@ __device__ __forceinline__ bool find(const KvaArgs& a, int x, int sms, Item& it)
     }
     int before = 0, id = 0;
     for (int b0 = 0; b0 < a.s.n_seqs; b0 += 32) {
-        const Need n = need<GROUP>(a, b0 + lane, nullptr);
+        const Need n = b0 ? need<GROUP>(a, b0 + lane, nullptr) : first;
         const int parts = per == INT32_MAX ? 1 : (max(n.tiles, 1) + per - 1) / per;
         const int mine = n.groups * a.c.heads * parts;
         int sum = mine, ids = n.groups * a.c.heads;
@@ -139,10 +140,10 @@ __device__ __forceinline__ bool find(const KvaArgs& a, int x, int sms, Item& it)
             it.id = id + __shfl_sync(~0u, ids - n.groups * a.c.heads, src) + set;
             it.rows = (int)min((long)GROUP, (long)it.n_new * a.group - (long)it.group * GROUP);
             const int pos0 = it.kv - it.n_new;
-            const int first = pos0 + (int)((long)it.group * GROUP / a.group);
+            const int front = pos0 + (int)((long)it.group * GROUP / a.group);
             const int last = pos0 + (int)(((long)it.group * GROUP + it.rows - 1) / a.group);
             it.hi = max(last + 1, 0);
-            it.lo = a.window > 0 ? max(first + 1 - a.window, 0) : 0;
+            it.lo = a.window > 0 ? max(front + 1 - a.window, 0) : 0;
             const int t = it.lo / KEYS, n2 = it.hi > it.lo ? (it.hi + KEYS - 1) / KEYS - t : 0;
             it.t0 = t + (int)((long)n2 * it.part / it.parts);
             it.t1 = t + (int)((long)n2 * (it.part + 1) / it.parts);
@@ -327,36 +328,75 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvaArgs a, 
         const int tok = live ? (int)(grow / a.group) : 0;
         const int end = live ? max(pos0 + tok + 1, 0) : 0, from = a.window > 0 ? max(end - a.window, 0) : 0;
         const int limit = min(end, it.hi);                         // keys [from, limit) are this part's and seen
+        // packed row and head of a row of this block
+        const int tok0 = (int)((long)it.group * G::GROUP / a.group), sub0 = (int)((long)it.group * G::GROUP % a.group);
+        auto place = [&](int x) {
+            const unsigned g = (unsigned)(sub0 + x);
+            return KvaRow{it.row0 + tok0 + (int)(g / (unsigned)a.group), it.head * a.group + (int)(g % (unsigned)a.group)};
+        };
+        constexpr int LANES = D / 8, AT_ONCE = 32 / LANES;         // lanes of a row, rows of a warp's instruction
         float sc = 0.0f;
         if (steps) {
-            // q to fp16 in shared memory: set w (of a split: both parts, by the first stream)
-            const size_t at = (size_t)(it.row0 + tok) * a.ldq + (size_t)(it.head * a.group + (live ? grow % a.group : 0)) * D;
-            float mx = 0.0f;
-            if (live)
-                for (int c = 0; c < D / 8; ++c) {
-                    float x[8];
-                    load_pairs8<DT>(a.q, at + c * 8, x);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(x[e]));
-                }
-            float back;
-            const float up = copysignf(q_unit(mx, back), a.scale2);
-            sc = fmaxf(back * fabsf(a.scale2), 1e-37f);            // above zero: masked scores stay -inf
-            if (w == 0 || !same)
-                for (int c = 0; c < D / 8; ++c) {
-                    float x[8] = {};
-                    if (live) load_pairs8<DT>(a.q, at + c * 8, x);
-                    uint32_t hi[4], lo[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float u = x[2 * e] * up, v = x[2 * e + 1] * up;
-                        hi[e] = pack_half2(u, v);
-                        lo[e] = pack_half2(u - __low2float(as_half2(hi[e])), v - __high2float(as_half2(hi[e])));
+            // q to fp16 in shared memory: set w, or of a split both parts; the streams of `same` halve the rows. Rows come as
+            // they are, all at once, and are turned where they lie by the lanes that copied them, in loops that stay short:
+            // this runs once a block, and fetching its instructions is dear (a thread its own row 18000 cycles, a
+            // seventh of a prompt of 8192; LANES lanes a row by registers, unrolled, 21000; so 7000).
+            float(*unit)[2] = ml[same ? 0 : w];
+            const int n = same ? 16 : 32, r0 = (warp & 3) * 32 + (same ? 16 * w : 0) + lane / LANES, c = lane % LANES;
+            uint8_t* set = sq + (same ? 0 : w) * G::TILE + (c >> 3) * G::PANEL;
+#pragma unroll 1
+            for (int i = 0; i < n; i += AT_ONCE) {
+                const int at = r0 + i, row2 = at + (same ? 0 : w * ROWS);
+                uint8_t* to = set + at * 128 + (((c & 7) ^ (at & 7)) << 4);
+                if (row2 < it.rows) {
+                    const KvaRow p = place(row2);
+                    const size_t e = (size_t)p.row * a.ldq + (size_t)p.head * D + c * 8;
+                    if constexpr (SPLIT) {
+                        cp_async16(smem_u32(to), static_cast<const float*>(a.q) + e);
+                        cp_async16(smem_u32(to + G::TILE), static_cast<const float*>(a.q) + e + 4);
+                    } else {
+                        cp_async16(smem_u32(to), static_cast<const uint16_t*>(a.q) + e);
                     }
-                    uint8_t* to = sq + w * G::TILE + (c >> 3) * G::PANEL + r * 128 + (((c & 7) ^ (r & 7)) << 4);
-                    *reinterpret_cast<uint4*>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                    if constexpr (SPLIT) *reinterpret_cast<uint4*>(to + G::TILE) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                } else {
+                    *reinterpret_cast<uint4*>(to) = make_uint4(0, 0, 0, 0);
+                    if constexpr (SPLIT) *reinterpret_cast<uint4*>(to + G::TILE) = make_uint4(0, 0, 0, 0);
                 }
+            }
+            cp_async_commit();
+            cp_async_wait<0>();
+#pragma unroll 2
+            for (int i = 0; i < n; i += AT_ONCE) {
+                const int at = r0 + i;
+                uint8_t* to = set + at * 128 + (((c & 7) ^ (at & 7)) << 4);
+                float x[8];
+                if constexpr (SPLIT) {
+                    const float4 u = *reinterpret_cast<const float4*>(to), v = *reinterpret_cast<const float4*>(to + G::TILE);
+                    x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w;
+                    x[4] = v.x; x[5] = v.y; x[6] = v.z; x[7] = v.w;
+                } else {
+                    load_pairs8<DT>(to, 0, x);
+                }
+                float mx = 0.0f;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(x[e]));
+#pragma unroll
+                for (int e = 1; e < LANES; e <<= 1) mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, e));
+                float back;
+                const float up = copysignf(q_unit(mx, back), a.scale2);
+                if (c == 0) unit[at][0] = back;
+                uint32_t hi[4], lo[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float u = x[2 * e] * up, v = x[2 * e + 1] * up;
+                    hi[e] = pack_half2(u, v);
+                    lo[e] = pack_half2(u - __low2float(as_half2(hi[e])), v - __high2float(as_half2(hi[e])));
+                }
+                *reinterpret_cast<uint4*>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                if constexpr (SPLIT) *reinterpret_cast<uint4*>(to + G::TILE) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+            }
+            if (same) softmax_sync();
+            else __syncwarp();
+            sc = fmaxf(unit[r][0] * fabsf(a.scale2), 1e-37f);      // above zero: masked scores stay -inf
             fence_async_shared();
             mbar_arrive(&q_full);
         }
@@ -531,34 +571,49 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvaArgs a, 
                 sum = sum * f0 + ml[1][r][1] * f1;
                 m = big;
             }
-            const long at = (long)it.group * G::GROUP + row;
-            const KvaRow out{it.row0 + (int)(at / a.group), it.head * a.group + (int)(at % a.group)};
             if (part && live) {
                 part[G::GROUP * D + 2 * row] = m;
                 part[G::GROUP * D + 2 * row + 1] = sum;
             }
+            const bool none = sum == 0.0f && !part;                // sees nothing: zero
+            const float inv = part ? 1.0f : none ? 0.0f : __fdividef(1.0f, sum);
+            // by halves of the columns through shared memory nothing else uses now, so that whole rows are written
+            uint8_t* stage = (same ? sv : sq + w * G::TILE) + (warp & 3) * 32 * (2 * D);
 #pragma unroll 1
-            for (int c = 0; c < D; c += 32) {
-                uint32_t x[32];
+            for (int half = 0; half < D && any_live; half += D / 2) {
+#pragma unroll 1
+                for (int c = half; c < half + D / 2; c += 32) {
+                    uint32_t x[32];
 #pragma unroll
-                for (int i = 0; i < 32; ++i) x[i] = 0;
-                if (steps) {                                       // (uniform)
-                    tc_ld_32x32b_x32(to + c, x);
-                    tc_wait_ld();
-                    add_total(c, x);
-                }
-                if (!live) continue;
-#pragma unroll
-                for (int i = 0; i < 32; i += 4) {
-                    float4 o = make_float4(__uint_as_float(x[i]) * f0, __uint_as_float(x[i + 1]) * f0,
-                                           __uint_as_float(x[i + 2]) * f0, __uint_as_float(x[i + 3]) * f0);
-                    if (same && steps) {
-                        const float4 u = *reinterpret_cast<const float4*>(osh + r * (D + 4) + c + i);
-                        o.x += u.x * f1; o.y += u.y * f1; o.z += u.z * f1; o.w += u.w * f1;
+                    for (int i = 0; i < 32; ++i) x[i] = 0;
+                    if (steps) {                                   // (uniform)
+                        tc_ld_32x32b_x32(to + c, x);
+                        tc_wait_ld();
+                        add_total(c, x);
                     }
-                    if (part) *reinterpret_cast<float4*>(part + row * D + c + i) = o;
-                    else kv_store_out<DT, D>(a, out, c + i, o, sum);
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4) {
+                        float4 o = make_float4(__uint_as_float(x[i]) * f0, __uint_as_float(x[i + 1]) * f0,
+                                               __uint_as_float(x[i + 2]) * f0, __uint_as_float(x[i + 3]) * f0);
+                        if (same && steps) {
+                            const float4 u = *reinterpret_cast<const float4*>(osh + r * (D + 4) + c + i);
+                            o.x += u.x * f1; o.y += u.y * f1; o.z += u.z * f1; o.w += u.w * f1;
+                        }
+                        o = none ? make_float4(0, 0, 0, 0) : make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+                        *reinterpret_cast<float4*>(stage + lane * (2 * D) + ((((c - half + i) >> 2) ^ (lane & 7)) << 4)) = o;
+                    }
                 }
+                __syncwarp();
+#pragma unroll 1
+                for (int i = 0; i < 32; i += AT_ONCE) {
+                    const int from = i + lane / LANES, q4 = lane % LANES, at = row - lane + from;
+                    const float4 o = *reinterpret_cast<const float4*>(stage + from * (2 * D) + ((q4 ^ (from & 7)) << 4));
+                    if (at < it.rows) {
+                        if (part) *reinterpret_cast<float4*>(part + at * D + half + q4 * 4) = o;
+                        else kv_store_out<DT, D>(a, place(at), half + q4 * 4, o, 1.0f);
+                    }
+                }
+                __syncwarp();
             }
         }
         if (part) join_parts<D, DT>(a, it, smem, &sh_last);
