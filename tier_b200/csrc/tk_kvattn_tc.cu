@@ -328,13 +328,15 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvaArgs a, 
         const int tok = live ? (int)(grow / a.group) : 0;
         const int end = live ? max(pos0 + tok + 1, 0) : 0, from = a.window > 0 ? max(end - a.window, 0) : 0;
         const int limit = min(end, it.hi);                         // keys [from, limit) are this part's and seen
-        // packed row and head of a row of this block
-        const int tok0 = (int)((long)it.group * G::GROUP / a.group), sub0 = (int)((long)it.group * G::GROUP % a.group);
-        auto place = [&](int x) {
-            const unsigned g = (unsigned)(sub0 + x);
-            return KvaRow{it.row0 + tok0 + (int)(g / (unsigned)a.group), it.head * a.group + (int)(g % (unsigned)a.group)};
-        };
         constexpr int LANES = D / 8, AT_ONCE = 32 / LANES;         // lanes of a row, rows of a warp's instruction
+        // packed row and head (within the group) of a row of this block, and of the row AT_ONCE further
+        auto place = [&](int x) {
+            const long g = (long)it.group * G::GROUP + x;
+            return KvaRow{it.row0 + (int)(g / a.group), (int)(g % a.group)};
+        };
+        auto further = [&](KvaRow& p) {
+            for (p.head += AT_ONCE; p.head >= a.group; p.head -= a.group) ++p.row;
+        };
         float sc = 0.0f;
         if (steps) {
             // q to fp16 in shared memory: set w, or of a split both parts; the streams of `same` halve the rows. Rows come as
@@ -344,13 +346,13 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvaArgs a, 
             float(*unit)[2] = ml[same ? 0 : w];
             const int n = same ? 16 : 32, r0 = (warp & 3) * 32 + (same ? 16 * w : 0) + lane / LANES, c = lane % LANES;
             uint8_t* set = sq + (same ? 0 : w) * G::TILE + (c >> 3) * G::PANEL;
+            KvaRow p = place(r0 + (same ? 0 : w * ROWS));
 #pragma unroll 1
-            for (int i = 0; i < n; i += AT_ONCE) {
+            for (int i = 0; i < n; i += AT_ONCE, further(p)) {
                 const int at = r0 + i, row2 = at + (same ? 0 : w * ROWS);
                 uint8_t* to = set + at * 128 + (((c & 7) ^ (at & 7)) << 4);
                 if (row2 < it.rows) {
-                    const KvaRow p = place(row2);
-                    const size_t e = (size_t)p.row * a.ldq + (size_t)p.head * D + c * 8;
+                    const size_t e = (size_t)p.row * a.ldq + (size_t)(it.head * a.group + p.head) * D + c * 8;
                     if constexpr (SPLIT) {
                         cp_async16(smem_u32(to), static_cast<const float*>(a.q) + e);
                         cp_async16(smem_u32(to + G::TILE), static_cast<const float*>(a.q) + e + 4);
@@ -364,35 +366,45 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvaArgs a, 
             }
             cp_async_commit();
             cp_async_wait<0>();
-#pragma unroll 2
-            for (int i = 0; i < n; i += AT_ONCE) {
-                const int at = r0 + i;
-                uint8_t* to = set + at * 128 + (((c & 7) ^ (at & 7)) << 4);
-                float x[8];
-                if constexpr (SPLIT) {
-                    const float4 u = *reinterpret_cast<const float4*>(to), v = *reinterpret_cast<const float4*>(to + G::TILE);
-                    x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w;
-                    x[4] = v.x; x[5] = v.y; x[6] = v.z; x[7] = v.w;
-                } else {
-                    load_pairs8<DT>(to, 0, x);
+#pragma unroll 1
+            for (int i = 0; i < n; i += 2 * AT_ONCE) {             // two rows a lane at once
+                float x[2][8], mx[2] = {0.0f, 0.0f};
+                auto spot = [&](int k) {
+                    const int at = r0 + i + k * AT_ONCE;
+                    return set + at * 128 + (((c & 7) ^ (at & 7)) << 4);
+                };
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    if constexpr (SPLIT) {
+                        const float4 u = *reinterpret_cast<const float4*>(spot(k));
+                        const float4 v = *reinterpret_cast<const float4*>(spot(k) + G::TILE);
+                        x[k][0] = u.x; x[k][1] = u.y; x[k][2] = u.z; x[k][3] = u.w;
+                        x[k][4] = v.x; x[k][5] = v.y; x[k][6] = v.z; x[k][7] = v.w;
+                    } else {
+                        load_pairs8<DT>(spot(k), 0, x[k]);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) mx[k] = fmaxf(mx[k], fabsf(x[k][e]));
                 }
-                float mx = 0.0f;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(x[e]));
+                for (int e = 1; e < LANES; e <<= 1)
 #pragma unroll
-                for (int e = 1; e < LANES; e <<= 1) mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, e));
-                float back;
-                const float up = copysignf(q_unit(mx, back), a.scale2);
-                if (c == 0) unit[at][0] = back;
-                uint32_t hi[4], lo[4];
+                    for (int k = 0; k < 2; ++k) mx[k] = fmaxf(mx[k], __shfl_xor_sync(~0u, mx[k], e));
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float u = x[2 * e] * up, v = x[2 * e + 1] * up;
-                    hi[e] = pack_half2(u, v);
-                    lo[e] = pack_half2(u - __low2float(as_half2(hi[e])), v - __high2float(as_half2(hi[e])));
+                for (int k = 0; k < 2; ++k) {
+                    float back;
+                    const float up = copysignf(q_unit(mx[k], back), a.scale2);
+                    if (c == 0) unit[r0 + i + k * AT_ONCE][0] = back;
+                    uint32_t hi[4], lo[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float u = x[k][2 * e] * up, v = x[k][2 * e + 1] * up;
+                        hi[e] = pack_half2(u, v);
+                        lo[e] = pack_half2(u - __low2float(as_half2(hi[e])), v - __high2float(as_half2(hi[e])));
+                    }
+                    *reinterpret_cast<uint4*>(spot(k)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                    if constexpr (SPLIT) *reinterpret_cast<uint4*>(spot(k) + G::TILE) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
                 }
-                *reinterpret_cast<uint4*>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                if constexpr (SPLIT) *reinterpret_cast<uint4*>(to + G::TILE) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
             }
             if (same) softmax_sync();
             else __syncwarp();
@@ -578,6 +590,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvaArgs a, 
             const bool none = sum == 0.0f && !part;                // sees nothing: zero
             const float inv = part ? 1.0f : none ? 0.0f : __fdividef(1.0f, sum);
             // by halves of the columns through shared memory nothing else uses now, so that whole rows are written
+            const KvaRow first = place(row - lane + lane / LANES);
             uint8_t* stage = (same ? sv : sq + w * G::TILE) + (warp & 3) * 32 * (2 * D);
 #pragma unroll 1
             for (int half = 0; half < D && any_live; half += D / 2) {
@@ -604,13 +617,14 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvaArgs a, 
                     }
                 }
                 __syncwarp();
+                KvaRow p = first;
 #pragma unroll 1
-                for (int i = 0; i < 32; i += AT_ONCE) {
+                for (int i = 0; i < 32; i += AT_ONCE, further(p)) {
                     const int from = i + lane / LANES, q4 = lane % LANES, at = row - lane + from;
                     const float4 o = *reinterpret_cast<const float4*>(stage + from * (2 * D) + ((q4 ^ (from & 7)) << 4));
                     if (at < it.rows) {
                         if (part) *reinterpret_cast<float4*>(part + at * D + half + q4 * 4) = o;
-                        else kv_store_out<DT, D>(a, place(at), half + q4 * 4, o, 1.0f);
+                        else kv_store_out<DT, D>(a, KvaRow{p.row, it.head * a.group + p.head}, half + q4 * 4, o, 1.0f);
                     }
                 }
                 __syncwarp();
