@@ -64,6 +64,7 @@ struct Geo {
 struct Item {
     int b, head, group, part, parts, id;   // id: of the row set (its counter)
     int kv, n_new, row0, rows;             // rows: of this block, from row group * GROUP of the sequence
+    int tok0, sub0;                        // token of the first of them, and head of the group
     int lo, hi, t0, t1;                    // this part's tiles, and the keys [lo, hi) of them that some row may see
 };
 
@@ -140,8 +141,9 @@ __device__ __forceinline__ bool find(const KvaArgs& a, int x, int sms, Item& it)
             it.id = id + __shfl_sync(~0u, ids - n.groups * a.c.heads, src) + set;
             it.rows = (int)min((long)GROUP, (long)it.n_new * a.group - (long)it.group * GROUP);
             const int pos0 = it.kv - it.n_new;
-            const int front = pos0 + (int)((long)it.group * GROUP / a.group);
-            const int last = pos0 + (int)(((long)it.group * GROUP + it.rows - 1) / a.group);
+            it.tok0 = (int)((long)it.group * GROUP / a.group);
+            it.sub0 = (int)((long)it.group * GROUP - (long)it.tok0 * a.group);
+            const int front = pos0 + it.tok0, last = front + (int)((unsigned)(it.sub0 + it.rows - 1) / (unsigned)a.group);
             it.hi = max(last + 1, 0);
             it.lo = a.window > 0 ? max(front + 1 - a.window, 0) : 0;
             const int t = it.lo / KEYS, n2 = it.hi > it.lo ? (it.hi + KEYS - 1) / KEYS - t : 0;
@@ -323,16 +325,15 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvaArgs a, 
         float l = 0.0f, nm = INFINITY;                             // nm: minus the reference; +inf before the first
         // ---------------- softmax: thread = row ----------------
         const int w = warp >> 2, r = (warp & 3) * 32 + lane, row = same ? r : w * ROWS + r;
-        const long grow = (long)it.group * G::GROUP + row;         // row of the sequence
         const bool live = row < it.rows;
-        const int tok = live ? (int)(grow / a.group) : 0;
+        const int tok = it.tok0 + (int)((unsigned)(it.sub0 + row) / (unsigned)a.group);
         const int end = live ? max(pos0 + tok + 1, 0) : 0, from = a.window > 0 ? max(end - a.window, 0) : 0;
         const int limit = min(end, it.hi);                         // keys [from, limit) are this part's and seen
         constexpr int LANES = D / 8, AT_ONCE = 32 / LANES;         // lanes of a row, rows of a warp's instruction
         // packed row and head (within the group) of a row of this block, and of the row AT_ONCE further
         auto place = [&](int x) {
-            const long g = (long)it.group * G::GROUP + x;
-            return KvaRow{it.row0 + (int)(g / a.group), (int)(g % a.group)};
+            const unsigned g = (unsigned)(it.sub0 + x), t = g / (unsigned)a.group;
+            return KvaRow{it.row0 + it.tok0 + (int)t, (int)(g - t * (unsigned)a.group)};
         };
         auto further = [&](KvaRow& p) {
             for (p.head += AT_ONCE; p.head >= a.group; p.head -= a.group) ++p.row;
@@ -347,12 +348,13 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvaArgs a, 
             const int n = same ? 16 : 32, r0 = (warp & 3) * 32 + (same ? 16 * w : 0) + lane / LANES, c = lane % LANES;
             uint8_t* set = sq + (same ? 0 : w) * G::TILE + (c >> 3) * G::PANEL;
             KvaRow p = place(r0 + (same ? 0 : w * ROWS));
-#pragma unroll 1
+            const int rows = it.rows, head0 = it.head * a.group;
+#pragma unroll 2
             for (int i = 0; i < n; i += AT_ONCE, further(p)) {
                 const int at = r0 + i, row2 = at + (same ? 0 : w * ROWS);
                 uint8_t* to = set + at * 128 + (((c & 7) ^ (at & 7)) << 4);
-                if (row2 < it.rows) {
-                    const size_t e = (size_t)p.row * a.ldq + (size_t)(it.head * a.group + p.head) * D + c * 8;
+                if (row2 < rows) {
+                    const size_t e = (size_t)p.row * a.ldq + (size_t)(head0 + p.head) * D + c * 8;
                     if constexpr (SPLIT) {
                         cp_async16(smem_u32(to), static_cast<const float*>(a.q) + e);
                         cp_async16(smem_u32(to + G::TILE), static_cast<const float*>(a.q) + e + 4);
@@ -618,13 +620,22 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvaArgs a, 
                 }
                 __syncwarp();
                 KvaRow p = first;
+                const int rows = it.rows, head0 = it.head * a.group;
 #pragma unroll 1
-                for (int i = 0; i < 32; i += AT_ONCE, further(p)) {
-                    const int from = i + lane / LANES, q4 = lane % LANES, at = row - lane + from;
-                    const float4 o = *reinterpret_cast<const float4*>(stage + from * (2 * D) + ((q4 ^ (from & 7)) << 4));
-                    if (at < it.rows) {
-                        if (part) *reinterpret_cast<float4*>(part + at * D + half + q4 * 4) = o;
-                        else kv_store_out<DT, D>(a, KvaRow{p.row, it.head * a.group + p.head}, half + q4 * 4, o, 1.0f);
+                for (int i = 0; i < 32; i += 4 * AT_ONCE) {
+                    const int q4 = lane % LANES;
+                    float4 o[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const int from = i + k * AT_ONCE + lane / LANES;
+                        o[k] = *reinterpret_cast<const float4*>(stage + from * (2 * D) + ((q4 ^ (from & 7)) << 4));
+                    }
+#pragma unroll
+                    for (int k = 0; k < 4; ++k, further(p)) {
+                        const int at = row - lane + i + k * AT_ONCE + lane / LANES;
+                        if (at >= rows) continue;
+                        if (part) *reinterpret_cast<float4*>(part + at * D + half + q4 * 4) = o[k];
+                        else kv_store_out<DT, D>(a, KvaRow{p.row, head0 + p.head}, half + q4 * 4, o[k], 1.0f);
                     }
                 }
                 __syncwarp();
