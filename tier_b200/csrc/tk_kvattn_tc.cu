@@ -34,9 +34,9 @@
 // and half a conversion a score) beside the tensor core's 2 x 128 cycles a
 // tile; neither waits long for the other, under a power limit that holds the
 // clock at 1.47 GHz of 1.97 in long prompts.  Measured (32 query heads on 8
-// key/value heads of 128): a prompt of 8192, bf16, 609 us, 900 TFLOP/s; three
+// key/value heads of 128): a prompt of 8192, bf16, 563 us, 976 TFLOP/s; three
 // chunks of up to 1000 rows behind 6001 keys, window 1024, 16 heads on 4 of
-// 64, fp16, 33.6 us; two fp32 prompts of up to 1537 rows, 2000 keys, 176 us, 218
+// 64, fp16, 32.5 us; two fp32 prompts of up to 1537 rows, 2000 keys, 154 us, 249
 // TFLOP/s (two parts of q and of P: twice that in the tensor core).
 #include "tk_f32x2.cuh"
 #include "tk_kv.cuh"
@@ -46,7 +46,7 @@ namespace kt {
 
 constexpr int ROWS = 128, KEYS = 128, THREADS = 512;
 // registers a thread of each warpgroup: 4 x 128 at launch, 192 + 192 + 80 + 48 = 512 after the split
-// (184 + 184 + 88 + 56 spills in the softmax: a prompt of 8192 takes 652 us, not 609)
+// (184 + 184 + 88 + 56 spills in the softmax: a prompt of 8192 took 652 us, not 609)
 constexpr int REG_SOFTMAX = 192, REG_CONVERT = 80, REG_ISSUE = 48;
 
 template <int D, bool SPLIT>
@@ -343,7 +343,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvaArgs a, 
             // q to fp16 in shared memory: set w, or of a split both parts; the streams of `same` halve the rows. Rows come as
             // they are, all at once, and are turned where they lie by the lanes that copied them, in loops that stay short:
             // this runs once a block, and fetching its instructions is dear (a thread its own row 18000 cycles, a
-            // seventh of a prompt of 8192; LANES lanes a row by registers, unrolled, 21000; so 7000).
+            // seventh of a prompt of 8192; LANES lanes a row by registers, unrolled, 21000; so 9000).
             float(*unit)[2] = ml[same ? 0 : w];
             const int n = same ? 16 : 32, r0 = (warp & 3) * 32 + (same ? 16 * w : 0) + lane / LANES, c = lane % LANES;
             uint8_t* set = sq + (same ? 0 : w) * G::TILE + (c >> 3) * G::PANEL;
@@ -591,7 +591,8 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvaArgs a, 
             }
             const bool none = sum == 0.0f && !part;                // sees nothing: zero
             const float inv = part ? 1.0f : none ? 0.0f : __fdividef(1.0f, sum);
-            // by halves of the columns through shared memory nothing else uses now, so that whole rows are written
+            // by halves of the columns through shared memory nothing else uses now, so that whole rows are written, four
+            // at once (one at a time, each by a division, 14500 cycles a block; so 10000)
             const KvaRow first = place(row - lane + lane / LANES);
             uint8_t* stage = (same ? sv : sq + w * G::TILE) + (warp & 3) * 32 * (2 * D);
 #pragma unroll 1
