@@ -1,0 +1,73 @@
+"""GPU tests of the 4-bit cache and the attention over it at the edges of their
+contract: captured graphs and what is allocated after them.  Tolerances as in
+test_gpu_kv.py."""
+import numpy as np
+import pytest
+
+import kv_ref as ref
+from test_gpu_kv import check_attend, dev, device_cache, device_seqs
+
+pytestmark = pytest.mark.gpu
+
+
+class Replayed:
+    """Two sequences' drafted rows, long enough to be divided among blocks and joined, captured in a graph."""
+
+    def __init__(self, ctx):
+        import torch
+        rng = np.random.default_rng(31)
+        self.ctx, self.bat = ctx, ref.batch(rng, [2, 2], [3000, 1700], 32)
+        self.cache = ref.random_cache(rng, self.bat[3], 32, 2, 128)
+        self.q = dev(rng.standard_normal((4, 8 * 128)).astype(np.float32))
+        self.out = torch.zeros_like(self.q)
+        self.kc, self.sq = device_cache(self.cache), device_seqs(*self.bat[:3])
+        self.side = torch.cuda.Stream()
+        torch.cuda.synchronize()
+        self.call()                                        # sizes the workspace before the capture
+        torch.cuda.synchronize()
+        self.graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(self.graph, stream=self.side):
+            self.call()
+
+    def call(self):
+        self.ctx.kv_attend(self.kc, self.sq, self.q, 8, self.out, stream=self.side)
+
+    def check(self):
+        import torch
+        for _ in range(2):
+            self.out.zero_()
+            self.graph.replay()
+            torch.cuda.synchronize()
+            exact, reach = ref.attend(self.cache, *self.bat[:3], self.q.double().cpu().numpy(), 8, 2, 128, 128 ** -0.5, 0)
+            check_attend(self.out.double().cpu().numpy().reshape(exact.shape), exact, reach, "f32")
+        self.ctx.sync_status()
+
+
+def larger_calls(ctx):
+    """A prompt of many row sets, and decoding of more sequences than the graph's."""
+    import torch
+    import tier_b200 as tk
+    kc = tk.alloc_kvcache(128, 64, 8, 128)
+    pages = torch.arange(128, dtype=torch.int32, device="cuda").view(1, -1)
+    starts = torch.tensor([0, 8192], dtype=torch.int32, device="cuda")
+    q = torch.randn(8192, 32 * 128, device="cuda").bfloat16()
+    ctx.kv_attend(kc, tk.make_seqs(starts, starts[1:].clone(), pages, 8192, 8192), q, 32, torch.empty_like(q), x_dtype=tk.DT_BF16)
+    n = 300
+    sq = tk.make_seqs(torch.arange(n + 1, dtype=torch.int32, device="cuda"), torch.full((n,), 200, dtype=torch.int32, device="cuda"),
+                      pages.repeat(n, 1), n, 1)
+    ctx.kv_attend(kc, sq, q[:n], 32, torch.empty_like(q[:n]), x_dtype=tk.DT_BF16)
+    ctx.sync_status()
+
+
+def test_replay_after_larger_calls_with_the_workspace_reserved():
+    """tk_reserve covers all that a call needs: nothing that a captured graph uses moves afterwards."""
+    import tier_b200 as tk
+    ctx = tk.Context(0)
+    ctx.reserve(256 << 20)
+    r = Replayed(ctx)
+    r.check()
+    size = ctx.lib.tk_workspace_bytes(ctx.h)
+    larger_calls(ctx)
+    assert ctx.lib.tk_workspace_bytes(ctx.h) == size
+    r.check()
+    ctx.close()

@@ -441,6 +441,11 @@ tk_status tk_init(int device, tk_ctx** out) {
         e = cudaMalloc(&c->flags, sizeof(int) * c->flags_len);
         if (e == cudaSuccess) e = cudaMemset(c->flags, 0, sizeof(int) * c->flags_len);
     }
+    if (e == cudaSuccess) {
+        const size_t n = sizeof(int) * KV_SYNC_PER_SM * c->num_sms;
+        e = cudaMalloc(&c->kv_sync, n);
+        if (e == cudaSuccess) e = cudaMemset(c->kv_sync, 0, n);
+    }
     if (e != cudaSuccess) {
         delete c;
         return cuda_fail(e, "tk_init: status word");
@@ -458,7 +463,7 @@ void tk_destroy(tk_ctx* ctx) {
     if (ctx->flags) cudaFree(ctx->flags);
     if (ctx->iq_tab) cudaFree(ctx->iq_tab);
     if (ctx->sched) cudaFree(ctx->sched);
-    if (ctx->kv_count) cudaFree(ctx->kv_count);
+    if (ctx->kv_sync) cudaFree(ctx->kv_sync);
     comm_destroy(ctx);
     for (cudaEvent_t e : ctx->prof.ev) cudaEventDestroy(e);
     delete ctx;

@@ -44,12 +44,15 @@ struct tk_ctx {
     int* sched = nullptr;
     size_t sched_cap = 0;            // ints
     std::vector<long> sched_key;
-    // tk_kv_attend: finished parts per (sequence, key/value head), zero between calls
-    int* kv_count = nullptr;
-    size_t kv_count_len = 0;
+    // tk_kv_attend: num_sms flags, then finished parts by block, zero between
+    // calls.  KV_SYNC_PER_SM ints an SM whatever the batch: the pointer that a
+    // captured graph holds stays good.
+    int* kv_sync = nullptr;
 };
 
 namespace tk {
+
+constexpr int KV_SYNC_PER_SM = 4;   // tk_ctx::kv_sync
 
 // k-blocks (64 each) per fp32 accumulation segment for the split product sets.
 // The error of the tensor-core fp32 accumulation grows with the segment

@@ -124,7 +124,7 @@ struct KvaArgs {
     int n_heads, group, window;
     float scale2;         // scale * log2(e)
     float* part;          // parts of divided rows (workspace)
-    int* count;           // finished parts of each sequence and key/value head, zero between calls
+    int* count;           // finished parts of each divided set of rows, by the block of its first part; zero between calls
     int* status;
 };
 
@@ -257,7 +257,5 @@ __device__ __forceinline__ void kv_join(const KvaArgs& a, int parts, int all_row
 
 // tk_kvattn_tc.cu
 tk_status launch_kv_prompt(tk_ctx* ctx, KvaArgs& a, int dtype, cudaStream_t st);
-// Zeroed counters for joins (tk_kvattn.cu).
-tk_status kv_count_ensure(tk_ctx* ctx, size_t n);
 
 }  // namespace tk

@@ -12,7 +12,7 @@ __device__ __forceinline__ void kv_join_last(const KvaArgs& a, const Item& it, i
     __threadfence();
     __syncthreads();
     if (threadIdx.x == 0) {
-        int* n = a.count + (size_t)it.b * a.c.heads + it.head;
+        int* n = a.count + it.c0;                                  // no other head in parts begins in that block
         const int done = atomicAdd(n, 1) + 1;
         *sh_last = done == it.chunks;
         if (done == it.chunks) *n = 0;
@@ -63,6 +63,7 @@ __device__ __forceinline__ void kv_join_last(const KvaArgs& a, const Item& it, i
 constexpr int KD_WARPS = 4, KD_STAGES = 3, KD_UNIT = 32, KD_MAX_ROWS = 32;
 // Blocks an SM: registers for 8 or 16 query rows allow three, for 24 or 32 two.
 constexpr int kd_blocks(int nt) { return nt <= 2 ? 3 : 2; }
+static_assert(kd_blocks(1) < KV_SYNC_PER_SM, "a counter a block behind the flags");
 
 template <int D, int NT>
 struct KdGeo {
@@ -580,23 +581,6 @@ __global__ void __launch_bounds__(KD_WARPS * 32, kd_blocks(NT)) kv_decode_kernel
   }
 }
 
-// Zeroed counters for the join, grown on demand (synchronizes the device then).
-tk_status kv_count_ensure(tk_ctx* ctx, size_t n) {
-    if (n <= ctx->kv_count_len) return TK_OK;
-    cudaError_t e = cudaDeviceSynchronize();
-    if (e != cudaSuccess) return cuda_fail(e, "tk_kv_attend: counter growth");
-    if (ctx->kv_count) cudaFree(ctx->kv_count);
-    ctx->kv_count = nullptr;
-    ctx->kv_count_len = 0;
-    n = (n + 1023) / 1024 * 1024;
-    e = cudaMalloc(&ctx->kv_count, n * sizeof(int));
-    if (e == cudaSuccess) e = cudaMemset(ctx->kv_count, 0, n * sizeof(int));
-    if (e == cudaSuccess) e = cudaDeviceSynchronize();
-    if (e != cudaSuccess) return cuda_fail(e, "tk_kv_attend: counters");
-    ctx->kv_count_len = n;
-    return TK_OK;
-}
-
 template <int D, int DT, int NT>
 static tk_status go_decode_t(tk_ctx* ctx, const KvaArgs& a, unsigned grid, int least, cudaStream_t st) {
     static std::atomic<uint64_t> attr_done{0};
@@ -618,10 +602,9 @@ static tk_status go_decode(tk_ctx* ctx, KvaArgs& a, cudaStream_t st) {
     if (pairs * ((size_t)a.s.max_pages << a.c.page_shift) / KD_UNIT + pairs > (1ull << 31))
         return fail(TK_ERR_UNSUPPORTED, "tk_kv_attend: sequences x heads x table length beyond 2^36 tokens");
     tk_status r = ws_ensure(ctx, (size_t)grid * 2 * (8 * nt * (D + 2)) * sizeof(float), st);
-    if (r == TK_OK) r = kv_count_ensure(ctx, pairs);
     if (r != TK_OK) return r;
     a.part = static_cast<float*>(ctx->ws);
-    a.count = ctx->kv_count;
+    a.count = ctx->kv_sync + ctx->num_sms;
     switch (nt) {
         case 1: return go_decode_t<D, DT, 1>(ctx, a, grid, least, st);
         case 2: return go_decode_t<D, DT, 2>(ctx, a, grid, least, st);

@@ -62,7 +62,7 @@ struct Geo {
 };
 
 struct Item {
-    int b, head, group, part, parts, id;   // id: of the row set (its counter)
+    int b, head, group, part, parts;
     int kv, n_new, row0, rows;             // rows: of this block, from row group * GROUP of the sequence
     int tok0, sub0;                        // token of the first of them, and head of the group
     int lo, hi, t0, t1;                    // this part's tiles, and the keys [lo, hi) of them that some row may see
@@ -114,15 +114,15 @@ __device__ __forceinline__ bool find(const KvaArgs& a, int x, int sms, Item& it)
         }
         if (per < 2) per = 2;
     }
-    int before = 0, id = 0;
+    int before = 0;
     for (int b0 = 0; b0 < a.s.n_seqs; b0 += 32) {
         const Need n = b0 ? need<GROUP>(a, b0 + lane, nullptr) : first;
         const int parts = per == INT32_MAX ? 1 : (max(n.tiles, 1) + per - 1) / per;
         const int mine = n.groups * a.c.heads * parts;
-        int sum = mine, ids = n.groups * a.c.heads;
+        int sum = mine;
         for (int i = 1; i < 32; i <<= 1) {
-            const int o = __shfl_up_sync(~0u, sum, i), p = __shfl_up_sync(~0u, ids, i);
-            if (lane >= i) { sum += o; ids += p; }
+            const int o = __shfl_up_sync(~0u, sum, i);
+            if (lane >= i) sum += o;
         }
         const unsigned hit = __ballot_sync(~0u, x < before + sum);
         if (hit) {
@@ -138,7 +138,6 @@ __device__ __forceinline__ bool find(const KvaArgs& a, int x, int sms, Item& it)
             const int set = at / it.parts;
             it.head = set % a.c.heads;
             it.group = groups - 1 - set / a.c.heads;
-            it.id = id + __shfl_sync(~0u, ids - n.groups * a.c.heads, src) + set;
             it.rows = (int)min((long)GROUP, (long)it.n_new * a.group - (long)it.group * GROUP);
             const int pos0 = it.kv - it.n_new;
             it.tok0 = (int)((long)it.group * GROUP / a.group);
@@ -153,7 +152,6 @@ __device__ __forceinline__ bool find(const KvaArgs& a, int x, int sms, Item& it)
             return true;
         }
         before += __shfl_sync(~0u, sum, 31);
-        id += __shfl_sync(~0u, ids, 31);
     }
     return false;
 }
@@ -251,9 +249,10 @@ __device__ __forceinline__ void join_parts(const KvaArgs& a, const Item& it, uin
     __threadfence();
     softmax_sync();
     if (threadIdx.x == 0) {
-        const int done = atomicAdd(a.count + it.id, 1) + 1;
+        int* n = a.count + (blockIdx.x - it.part);                 // (sets in parts have no more blocks than SMs)
+        const int done = atomicAdd(n, 1) + 1;
         *sh_last = done == it.parts;
-        if (*sh_last) a.count[it.id] = 0;
+        if (*sh_last) *n = 0;
     }
     softmax_sync();
     if (!*sh_last) return;
@@ -790,11 +789,10 @@ static tk_status go(tk_ctx* ctx, KvaArgs& a, cudaStream_t st) {
     const long grid = sets > ctx->num_sms ? sets : ctx->num_sms;
     if (grid > INT32_MAX) return fail(TK_ERR_INVALID, "tk_kv_attend: too many rows");
     tk_status r = ws_ensure(ctx, (size_t)ctx->num_sms * (G::PART + G::SUM) * sizeof(float), st);
-    if (r == TK_OK) r = kv_count_ensure(ctx, (size_t)(sets + ctx->num_sms));
     if (r != TK_OK) return r;
     a.part = static_cast<float*>(ctx->ws);
     float* sums = a.part + (size_t)ctx->num_sms * G::PART;
-    int* busy = ctx->kv_count;                                     // num_sms flags, then the row sets' counters
+    int* busy = ctx->kv_sync;
     a.count = busy + ctx->num_sms;
     ProfScope ps(ctx, st, PK_SERVE);
     e = launch_dependent(kern, (unsigned)grid, THREADS, G::SMEM, st, a, sums, busy, ctx->num_sms);
