@@ -108,7 +108,11 @@ tk_status tk_init(int device, tk_ctx **out);
 void tk_destroy(tk_ctx *ctx);
 const char *tk_last_error_string(void);
 /* Grow the context workspace to at least `bytes` now (entry points grow it on
- * demand otherwise, which synchronizes the device). */
+ * demand otherwise, which synchronizes the device).  A captured graph keeps the
+ * workspace of its calls: growth inside a capture is refused (TK_ERR_INVALID;
+ * the capture stays valid), and a workspace that a captured call used and a
+ * later call outgrew is kept until tk_destroy.  Replays share that workspace
+ * with the context's other calls: order them as calls on several streams. */
 tk_status tk_reserve(tk_ctx *ctx, size_t bytes);
 size_t tk_workspace_bytes(const tk_ctx *ctx);
 /* Synchronize `stream` and report any device-side status (timeouts, invalid

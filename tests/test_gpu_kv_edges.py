@@ -71,3 +71,40 @@ def test_replay_after_larger_calls_with_the_workspace_reserved():
     assert ctx.lib.tk_workspace_bytes(ctx.h) == size
     r.check()
     ctx.close()
+
+
+def test_replay_after_the_workspace_has_grown():
+    """A graph captured before a larger call still computes in memory of its own context."""
+    import tier_b200 as tk
+    ctx = tk.Context(0)
+    r = Replayed(ctx)
+    size = ctx.lib.tk_workspace_bytes(ctx.h)
+    larger_calls(ctx)
+    assert ctx.lib.tk_workspace_bytes(ctx.h) > size
+    r.check()
+    ctx.close()
+
+
+def test_growth_inside_a_capture_is_refused():
+    import torch
+    import tier_b200 as tk
+    ctx = tk.Context(0)
+    side = torch.cuda.Stream()
+    kc = tk.alloc_kvcache(2, 16, 1, 64)
+    sq = device_seqs(np.array([0, 1], np.int32), np.array([20], np.int32), np.array([[0, 1]], np.int32))
+    q = torch.randn(1, 4 * 64, device="cuda")
+    out = torch.empty_like(q)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=side):
+        with pytest.raises(tk.TierkError) as e:
+            ctx.kv_attend(kc, sq, q, 4, out, stream=side)
+        out.fill_(3.0)                                     # the capture goes on
+    assert e.value.status == tk.TK_ERR_INVALID and "capture" in str(e.value)
+    g.replay()
+    torch.cuda.synchronize()
+    assert (out == 3).all()
+    ctx.kv_attend(kc, sq, q, 4, out)
+    ctx.sync_status()
+    assert (out != 3).any()
+    ctx.close()

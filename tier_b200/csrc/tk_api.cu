@@ -22,14 +22,30 @@ tk_status cuda_fail(cudaError_t e, const char* what) {
     return e == cudaErrorMemoryAllocation ? TK_ERR_NOMEM : TK_ERR_CUDA;
 }
 
+static bool capturing(cudaStream_t stream) {
+    cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(stream, &st) == cudaSuccess) return st != cudaStreamCaptureStatusNone;
+    cudaGetLastError();          // the legacy stream beside a capture: not in it
+    return false;
+}
+
 tk_status ws_ensure(tk_ctx* ctx, size_t bytes, cudaStream_t stream) {
     ctx->wexp_valid = false;     // the caller is about to carve the workspace
-    if (bytes <= ctx->ws_bytes) return TK_OK;
+    const bool in_capture = capturing(stream);
+    if (bytes <= ctx->ws_bytes) {
+        ctx->ws_in_graph |= in_capture;
+        return TK_OK;
+    }
+    if (in_capture)
+        return fail(TK_ERR_INVALID, "workspace growth inside a stream capture: make the call once before it, or tk_reserve");
     // Work queued on any stream may still use the old buffer.
     cudaError_t e = cudaDeviceSynchronize();
     if (e != cudaSuccess) return cuda_fail(e, "workspace growth sync");
-    (void)stream;
-    if (ctx->ws) cudaFree(ctx->ws);
+    if (ctx->ws) {
+        if (ctx->ws_in_graph) ctx->ws_kept.push_back(ctx->ws);   // a replay still uses it
+        else cudaFree(ctx->ws);
+    }
+    ctx->ws_in_graph = false;
     ctx->ws = nullptr;
     ctx->ws_bytes = 0;
     size_t want = align256(bytes + (bytes >> 3));
@@ -459,6 +475,7 @@ void tk_destroy(tk_ctx* ctx) {
     cudaSetDevice(ctx->device);
     cudaDeviceSynchronize();
     if (ctx->ws) cudaFree(ctx->ws);
+    for (void* p : ctx->ws_kept) cudaFree(p);
     if (ctx->status) cudaFree(ctx->status);
     if (ctx->flags) cudaFree(ctx->flags);
     if (ctx->iq_tab) cudaFree(ctx->iq_tab);

@@ -22,6 +22,8 @@ struct tk_ctx {
     int num_sms = 0;
     void* ws = nullptr;          // workspace (device)
     size_t ws_bytes = 0;
+    bool ws_in_graph = false;    // a captured call uses ws
+    std::vector<void*> ws_kept;  // outgrown workspaces of captured calls
     int* status = nullptr;       // device status word (tk::DEV_*)
     uint64_t launches = 0;       // kernels launched through this context
     int* flags = nullptr;        // split-K progress flags (device), flags_len ints
