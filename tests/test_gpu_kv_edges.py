@@ -1,11 +1,11 @@
 """GPU tests of the 4-bit cache and the attention over it at the edges of their
-contract: captured graphs and what is allocated after them.  Tolerances as in
-test_gpu_kv.py."""
+contract: captured graphs and what is allocated after them, windows of any
+size.  Tolerances as in test_gpu_kv.py."""
 import numpy as np
 import pytest
 
 import kv_ref as ref
-from test_gpu_kv import check_attend, dev, device_cache, device_seqs
+from test_gpu_kv import DTYPES, check_attend, dev, device_cache, device_seqs, run_attend
 
 pytestmark = pytest.mark.gpu
 
@@ -108,3 +108,33 @@ def test_growth_inside_a_capture_is_refused():
     ctx.sync_status()
     assert (out != 3).any()
     ctx.close()
+
+
+# ---- windows ---------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("new,kv", [([8, 5, 1], [2, 1, 40]), ([64, 200, 40], [2, 50, 90])])
+@pytest.mark.parametrize("window", [2 ** 30 - 1, 2 ** 30, 2 ** 31 - 4, 2 ** 31 - 1])
+def test_windows_as_large_as_an_int(ctx, dtype, new, kv, window):
+    """More new tokens than cached ones, so that rows have negative positions: a window that hides nothing is no window."""
+    rng = np.random.default_rng(41)
+    bat = ref.batch(rng, new, kv, 16)
+    cache = ref.random_cache(rng, bat[3], 16, 2, 64)
+    q = rng.standard_normal((sum(new), 4 * 64)) * 2
+    qr, none = run_attend(ctx, cache, bat, q, 4, dtype)
+    _, out = run_attend(ctx, cache, bat, q, 4, dtype, window=window)
+    exact, reach = ref.attend(cache, *bat[:3], qr, 4, 2, 64, 0.125, 0)
+    check_attend(out.reshape(exact.shape), exact, reach, dtype)
+    assert np.array_equal(out, none)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("new,kv", [([8, 5, 1], [2, 1, 40]), ([64, 200, 40], [2, 50, 90])])
+@pytest.mark.parametrize("window", [1, 7, 50])
+def test_windows_with_rows_before_the_cache(ctx, dtype, new, kv, window):
+    rng = np.random.default_rng(42)
+    bat = ref.batch(rng, new, kv, 16)
+    cache = ref.random_cache(rng, bat[3], 16, 2, 64)
+    q = rng.standard_normal((sum(new), 4 * 64)) * 2
+    qr, out = run_attend(ctx, cache, bat, q, 4, dtype, window=window)
+    exact, reach = ref.attend(cache, *bat[:3], qr, 4, 2, 64, 0.125, window)
+    check_attend(out.reshape(exact.shape), exact, reach, dtype)

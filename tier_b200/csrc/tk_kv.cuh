@@ -51,6 +51,14 @@ __device__ __forceinline__ SeqInfo seq_info(const SeqView& s, int page_shift, in
     return i;
 }
 
+// First key of rows at positions `pos` and on: 0 without a window.  (pos may be
+// negative, down to minus the new tokens, and a window of any size: from
+// position 0 back nothing can overflow, and no key lies before it.)
+__host__ __device__ __forceinline__ int kv_first_key(int pos, int window) {
+    const int p = pos > 0 ? pos : 0;
+    return window > 0 && p >= window ? p - window + 1 : 0;
+}
+
 // Last sequence whose q_start is at or before packed row r (q_start in global
 // or shared memory); the caller checks that r lies inside it.
 __device__ __forceinline__ int seq_of_row(const int32_t* q_start, int n_seqs, int r) {

@@ -105,8 +105,7 @@ __device__ __forceinline__ KdSeq kd_seq(const KvaArgs& a, int b, int* status) {
     const SeqInfo q = seq_info(a.s, a.c.page_shift, b, status);
     if (q.n_new == 0) return s;
     s.kv = q.kv; s.n_new = q.n_new; s.row0 = q.row0;
-    const int first = q.kv - q.n_new - a.window + 1;
-    if (a.window > 0 && first > 0) s.lo = first;
+    s.lo = kv_first_key(q.kv - q.n_new, a.window);
     // no key at all: one unit without keys, whose result is zero
     s.units = max((q.kv + KD_UNIT - 1) / KD_UNIT - s.lo / KD_UNIT, 1);
     return s;

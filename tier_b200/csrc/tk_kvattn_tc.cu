@@ -144,7 +144,7 @@ __device__ __forceinline__ bool find(const KvaArgs& a, int x, int sms, Item& it)
             it.sub0 = (int)((long)it.group * GROUP - (long)it.tok0 * a.group);
             const int front = pos0 + it.tok0, last = front + (int)((unsigned)(it.sub0 + it.rows - 1) / (unsigned)a.group);
             it.hi = max(last + 1, 0);
-            it.lo = a.window > 0 ? max(front + 1 - a.window, 0) : 0;
+            it.lo = kv_first_key(front, a.window);
             const int t = it.lo / KEYS, n2 = it.hi > it.lo ? (it.hi + KEYS - 1) / KEYS - t : 0;
             it.t0 = t + (int)((long)n2 * it.part / it.parts);
             it.t1 = t + (int)((long)n2 * (it.part + 1) / it.parts);
