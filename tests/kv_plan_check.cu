@@ -1,8 +1,17 @@
 // Host-side check of what the attention kernels work out from a batch's lengths
 // (no GPU needed).  Built and run by tests/test_kv_plans.py.
-#include "../tier_b200/csrc/tk_kv.cuh"
+#include "../tier_b200/csrc/tk_kvattn_tc.cu"
 
 #include <cstdio>
+
+// the library's other translation units, reduced to what the kernels link against
+namespace tk {
+tk_status fail(tk_status st, const std::string&) { return st; }
+tk_status cuda_fail(cudaError_t e, const char*) { return e == cudaSuccess ? TK_OK : TK_ERR_CUDA; }
+int prof_begin(tk_ctx*, cudaStream_t) { return -1; }
+void prof_end(tk_ctx*, cudaStream_t, int, int) {}
+tk_status ws_ensure(tk_ctx*, size_t, cudaStream_t) { return TK_OK; }
+}  // namespace tk
 
 using namespace tk;
 
@@ -32,8 +41,16 @@ static void first_keys() {
         }
 }
 
+// parts are only taken where all of them have a place in the workspace (one an SM), whatever the contents of q_start
+static void divisions() {
+    for (long sets : {0L, 1L, 2L, 9L, 10L, 74L, 75L, 1L << 20, 1L << 27, 1L << 28, (1L << 28) + 1, 1L << 29, 1L << 31, 1L << 40})
+        for (int heads : {1, 2, 8, 65535})
+            CHECK(kt::cuts(sets, heads, 148) == ((double)sets * heads <= 74.0), "%ld sets, %d heads", sets, heads);
+}
+
 int main() {
     first_keys();
+    divisions();
     printf("%d failures\n", g_bad);
     return g_bad != 0;
 }

@@ -83,14 +83,18 @@ __device__ __forceinline__ Need need(const KvaArgs& a, int b, int* status) {
     return n;
 }
 
+// Whether row sets are cut into parts: twice as many as there are would fill
+// the SMs at most.  (64 bits: packed rows that invalid contents name in many
+// sequences are counted in each.)
+__host__ __device__ __forceinline__ bool cuts(long sets, int heads, int sms) { return 2 * sets * heads <= sms; }
+
 // Item `x`: sequences in order, within one the last rows (most keys) first,
 // heads innermost.  Row sets are cut into parts only while that leaves no more
 // blocks than SMs.
 template <int GROUP>
 __device__ __forceinline__ bool find(const KvaArgs& a, int x, int sms, Item& it) {
     const int lane = threadIdx.x & 31;
-    int sets = 0;
-    long work = 0;                                                 // tiles of all row sets
+    long sets = 0, work = 0;                                       // row sets, their tiles
     const Need first = need<GROUP>(a, lane, a.status);             // kept: mostly there are no others
     for (int b0 = 0; b0 < a.s.n_seqs; b0 += 32) {
         const Need n = b0 ? need<GROUP>(a, b0 + lane, a.status) : first;
@@ -100,7 +104,7 @@ __device__ __forceinline__ bool find(const KvaArgs& a, int x, int sms, Item& it)
         work += w;
     }
     int per = INT32_MAX;                                           // tiles of a part
-    if (2 * sets * a.c.heads <= sms) {
+    if (cuts(sets, a.c.heads, sms)) {
         // at most sms / 2 parts are begun and not full, so that twice the even
         // share (six steps of an eighth) always fits
         per = max(1, (int)((work * a.c.heads + sms - 1) / sms));
