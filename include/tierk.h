@@ -266,7 +266,9 @@ typedef struct tk_kvcache {
  * that decreases or passes n_tokens, more than max_new new tokens, kv_len
  * beyond max_pages pages, a page outside the cache) make tk_sync_status report
  * TK_ERR_DEVICE; the affected sequence's results are then unspecified, but
- * nothing outside the caller's arrays is read or written. */
+ * nothing outside the caller's arrays is read or written.  A token whose page
+ * lies outside the cache is written nowhere (no other sequence's tokens are
+ * touched) and reads back as zeros. */
 typedef struct tk_seqs {
     int n_seqs, n_tokens, max_new, max_pages;
     const int32_t *q_start, *kv_len, *pages;

@@ -1,6 +1,6 @@
 """GPU tests of the 4-bit cache and the attention over it at the edges of their
 contract: captured graphs and what is allocated after them, windows of any
-size.  Tolerances as in test_gpu_kv.py."""
+size, page ids that do not fit.  Tolerances as in test_gpu_kv.py."""
 import numpy as np
 import pytest
 
@@ -138,3 +138,52 @@ def test_windows_with_rows_before_the_cache(ctx, dtype, new, kv, window):
     qr, out = run_attend(ctx, cache, bat, q, 4, dtype, window=window)
     exact, reach = ref.attend(cache, *bat[:3], qr, 4, 2, 64, 0.125, window)
     check_attend(out.reshape(exact.shape), exact, reach, dtype)
+
+
+# ---- pages -------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("many", [False, True])
+def test_append_to_a_page_outside_the_cache_is_skipped(ctx, dtype, many):
+    """Its tokens are reported, written nowhere and read back as zeros; every other byte of the cache is as it should be."""
+    import torch
+    import tier_b200 as tk
+    heads, dim, page = (8, 128, 16) if many else (2, 64, 16)
+    new = [1300, 40, 30] if many else [20, 40, 30]
+    kv = [n + 5 for n in new]
+    rng = np.random.default_rng(51)
+    q_start, kv_len, pages, total = ref.batch(rng, new, kv, page)
+    at0 = np.argwhere(pages[0] == 0)
+    if at0.size == 0:                                     # page 0 is some sequence's: here the first one's second page
+        pages[pages == 0], pages[0, 1] = pages[0, 1], 0
+    pages[1, 1], pages[2, 0] = total, -1
+    cache = ref.random_cache(rng, total, page, heads, dim)
+    tt, dt = {"f32": (torch.float32, tk.DT_F32), "f16": (torch.float16, tk.DT_F16), "bf16": (torch.bfloat16, tk.DT_BF16)}[dtype]
+    x = [dev(rng.standard_normal((sum(new), heads * dim)).astype(np.float32)).to(tt) for _ in "kv"]
+    kc, sq = device_cache(cache), device_seqs(q_start, kv_len, pages)
+    ctx.kv_append(kc, sq, *x, x_dtype=dt)
+    with pytest.raises(tk.TierkError) as e:
+        ctx.sync_status()
+    assert e.value.status == tk.TK_ERR_DEVICE
+    got = dict(zip(("k_q", "k_s", "v_q", "v_s"), (t.cpu().numpy() for t in kc._owner)))
+    want = []
+    for s, rows in zip("kv", x):
+        m, d = ref.quantize(rows.float().cpu().numpy().reshape(-1, heads, dim))
+        back = (m * np.repeat(d.astype(np.float64), 32, -1)).reshape(len(m), -1)
+        for b in range(3):
+            for i in range(new[b]):
+                t, r = kv[b] - new[b] + i, int(q_start[b]) + i
+                p = pages[b, t // page]
+                if not 0 <= p < total:
+                    back[r] = 0
+                    continue
+                cache[s + "_q"][p, :, t % page] = ref.pack(m[r])
+                cache[s + "_s"][p, :, t % page] = d[r]
+        want.append(back)
+    for name, a in got.items():
+        assert np.array_equal(a.view(np.uint8), cache[name].view(np.uint8)), name
+    out = [torch.full((sum(new), heads * dim), 5.0, device="cuda") for _ in "kv"]
+    ctx.kv_read(kc, sq, *out)
+    with pytest.raises(tk.TierkError):
+        ctx.sync_status()
+    for a, w in zip(out, want):
+        assert np.array_equal(a.double().cpu().numpy(), w)

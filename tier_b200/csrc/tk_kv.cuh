@@ -72,12 +72,19 @@ __device__ __forceinline__ int seq_of_row(const int32_t* q_start, int n_seqs, in
 }
 
 // Page holding a sequence's token `pos`: an id outside the cache is reported
-// and read as page 0.
-__device__ __forceinline__ int page_of(const SeqView& s, const KvView& c, int b, int pos, int* status) {
-    const int p = s.pages[(size_t)b * s.max_pages + (pos >> c.page_shift)];
-    if ((unsigned)p < (unsigned)c.n_pages) return p;
+// (false, page 0).
+__device__ __forceinline__ bool page_at(const SeqView& s, const KvView& c, int b, int pos, int* status, int& page) {
+    page = s.pages[(size_t)b * s.max_pages + (pos >> c.page_shift)];
+    if ((unsigned)page < (unsigned)c.n_pages) return true;
     raise_status(status, DEV_INVALID);
-    return 0;
+    page = 0;
+    return false;
+}
+// The same to read from: page 0 in place of one outside the cache.
+__device__ __forceinline__ int page_of(const SeqView& s, const KvView& c, int b, int pos, int* status) {
+    int page;
+    page_at(s, c, b, pos, status, page);
+    return page;
 }
 // Index of (page, key/value head, row) among the cache's rows.
 __device__ __forceinline__ size_t kv_row(const KvView& c, int page, int head, int pos) {

@@ -86,12 +86,13 @@ __device__ __forceinline__ bool where_is(const KvcArgs& a, int items_of_warp, Wh
     const int b = seq_of_row_warp(a.s.q_start, a.s.n_seqs, token);
     const SeqInfo q = seq_info(a.s, a.c.page_shift, b, a.status);
     const int at = (int)token - q.row0, pos = q.kv - q.n_new + at;
-    w.ok = at >= 0 && at < q.n_new && pos >= 0;
+    int page = 0;
+    w.ok = at >= 0 && at < q.n_new && pos >= 0 && page_at(a.s, a.c, b, pos, a.status, page);   // (alike in all lanes)
     const int shift = a.c.dim == 128 ? 4 : 3;                      // items of a head
     const uint32_t item = chunk * items_of_warp + lane, word = item & ((1u << shift) - 1);
     w.left = a.items - (int)item;
     w.x = static_cast<uint8_t*>(v ? a.v : a.k) + ((size_t)token * (v ? a.ldv : a.ldk) + (size_t)item * 8) * SIZE;
-    const size_t held = w.ok ? kv_row(a.c, page_of(a.s, a.c, b, pos, a.status), item >> shift, pos) : 0;
+    const size_t held = w.ok ? kv_row(a.c, page, item >> shift, pos) : 0;
     w.q = (v ? a.c.vq : a.c.kq) + held * (a.c.dim >> 1) + word * 4;
     w.s = reinterpret_cast<uint8_t*>(v ? a.c.vs : a.c.ks) + held * (a.c.dim >> 4) + (word >> 2) * 2;
     const uint32_t rows = (32u >> shift) << a.c.page_shift;
