@@ -187,3 +187,23 @@ def test_append_to_a_page_outside_the_cache_is_skipped(ctx, dtype, many):
         ctx.sync_status()
     for a, w in zip(out, want):
         assert np.array_equal(a.double().cpu().numpy(), w)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("page", [16, 32, 64])
+@pytest.mark.parametrize("new", [1, 5, 70])
+def test_pages_behind_a_window_are_not_looked_up(ctx, dtype, page, new):
+    """Entries of pages that no row sees may be anything: a caller frees those before the window."""
+    rng = np.random.default_rng(52)
+    kv = [400, 333, 96, 70 + new, 511]
+    for window in (1, 17, 40, 100):
+        bat = ref.batch(rng, [new] * 5, kv, page)
+        cache = ref.random_cache(rng, bat[3], page, 2, 64)
+        q = rng.standard_normal((5 * new, 4 * 64)) * 2
+        q_start, kv_len, pages = (a.copy() for a in bat[:3])
+        for b, c in enumerate(kv):
+            pages[b, : max(0, c - new - window + 1) // page] = -1
+            pages[b, -(-c // page):] = bat[3] + 7
+        qr, out = run_attend(ctx, cache, (q_start, kv_len, pages), q, 4, dtype, window=window)
+        exact, reach = ref.attend(cache, *bat[:3], qr, 4, 2, 64, 0.125, window)
+        check_attend(out.reshape(exact.shape), exact, reach, dtype)

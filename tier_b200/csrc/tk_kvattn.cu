@@ -272,8 +272,8 @@ __global__ void __launch_bounds__(KD_WARPS * 32, kd_blocks(NT)) kv_decode_kernel
             const int pos = (it.u0 + warp + i * KD_WARPS) * KD_UNIT;
             if ((i & 31) == 0) {                                   // page ids of the next 32 units, one a lane
                 const int p = pos + lane * (KD_WARPS * KD_UNIT);
-                if (i + lane < mine) {
-                    pid = page_of(a.s, a.c, it.b, p, a.status);
+                if (i + lane < mine) {                             // (of two pages the first may lie before every window)
+                    pid = small && p + 16 <= it.lo ? 0 : page_of(a.s, a.c, it.b, p, a.status);
                     if (small && p + 16 < it.kv) pid2 = page_of(a.s, a.c, it.b, p + 16, a.status);
                 }
             }
