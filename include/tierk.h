@@ -292,9 +292,13 @@ tk_status tk_kv_read(tk_ctx *ctx, const tk_kvcache *cache, const tk_seqs *seqs, 
  * tokens j that row i sees: j <= its position, and j > position - window when
  * window > 0.  q, out [n_tokens, n_heads * head_dim] in x_dtype; head h reads
  * key/value head h / (n_heads / n_kv_heads).  A row that sees nothing is zero.
- * fp32 rows are computed to fp32 accuracy (q and the probabilities as two fp16
- * parts), fp16 and bf16 rows with one fp16 part of the probabilities; all sums
- * are fp32.  Cached rows that no row sees do not matter, whatever they hold.
+ * q and the probabilities of fp32 rows enter as two fp16 parts, 22 bits:
+ * probabilities down to 2^-18 of a row's largest are off by 2^-21 of themselves
+ * at most, smaller ones by 2^-39 of the largest (2^-17 of themselves at 2^-22
+ * of it).  fp16 and bf16 rows have one part of the probabilities: off by 2^-12
+ * of themselves down to 2^-21 of the largest, below by 2^-32 of it.  All sums
+ * are fp32.  Cached rows that no row sees, and table entries of pages without
+ * others, do not matter, whatever they hold.
  * Replaces attn_cache (tier/tier.cpp:2240-2259). */
 tk_status tk_kv_attend(tk_ctx *ctx, const tk_kvcache *cache, const tk_seqs *seqs, const void *q, int x_dtype,
                        int ldq, int n_heads, float scale, int window, void *out, int ldo, void *stream);

@@ -1,6 +1,6 @@
 """GPU tests of the 4-bit cache and the attention over it at the edges of their
 contract: captured graphs and what is allocated after them, windows of any
-size, page ids that do not fit.  Tolerances as in test_gpu_kv.py."""
+size, page ids that do not fit, small weights of fp32 rows.  Tolerances as in test_gpu_kv.py."""
 import numpy as np
 import pytest
 
@@ -207,3 +207,31 @@ def test_pages_behind_a_window_are_not_looked_up(ctx, dtype, page, new):
         qr, out = run_attend(ctx, cache, (q_start, kv_len, pages), q, 4, dtype, window=window)
         exact, reach = ref.attend(cache, *bat[:3], qr, 4, 2, 64, 0.125, window)
         check_attend(out.reshape(exact.shape), exact, reach, dtype)
+
+
+# ---- fp32 rows -----------------------------------------------------------------------
+@pytest.mark.parametrize("where", [0, 700, 1999])
+@pytest.mark.parametrize("new,seqs", [(1, 1), (1, 330), (4, 330), (6, 330), (8, 330), (60, 1), (300, 1)])
+def test_fp32_rows_whose_mass_lies_on_a_key_of_no_value(ctx, new, seqs, where):
+    """One key weighs 2^5 to 2^22 times any other and its value is zero: the others' weights, alike and small, are the
+    whole output.  Their two fp16 parts end at 2^-25, the largest weight is 2^14 or more: 2^-17 of a weight that is 2^-22
+    of it, within the 2e-5 of every fp32 row.  (330 sequences: none is cut into short parts.)"""
+    rng = np.random.default_rng(53)
+    kv, page, dim, heads = 2000 + new, 64, 64, 4
+    bat = ref.batch(rng, [new], [kv], page)
+    cache = ref.random_cache(rng, bat[3], page, 1, dim)
+    cache["k_q"][:] = 0
+    cache["k_s"][:] = 0.0625
+    cache["v_q"] = rng.integers(1, 8, cache["v_q"].shape, dtype=np.uint8) * 17
+    cache["v_s"] = np.abs(cache["v_s"]) + np.float16(2.0 ** -6)
+    cache["v_s"] = ref.round_bits(cache["v_s"].astype(np.float64), 8).astype(np.float16)
+    p, r = bat[2][0, where // page], where % page
+    cache["k_q"][p, :, r] = ref.pack(np.full((1, dim), 7, np.int8))
+    cache["v_q"][p, :, r] = 0
+    gap = rng.uniform(5, 22, (new, heads))                 # of the weights' exponents
+    gap[0] = [21.9, 20.3, 18.6, 21.2]
+    q = np.repeat(gap * np.log(2) / (0.125 * dim * 7 * 0.0625), dim, -1)
+    many = (np.arange(seqs + 1, dtype=np.int32) * new, np.full(seqs, kv, np.int32), np.tile(bat[2], (seqs, 1)), bat[3])
+    qr, out = run_attend(ctx, cache, many, np.tile(q, (seqs, 1)), heads, "f32")
+    exact, reach = ref.attend(cache, *bat[:3], qr[:new], heads, 1, dim, 0.125, 0)
+    check_attend(out.reshape(seqs, *exact.shape), exact[None], reach[None], "f32")

@@ -177,11 +177,22 @@ __device__ __forceinline__ float q_unit(float max, float& back) {
     return __uint_as_float((uint32_t)(254 - (e - 13)) << 23);
 }
 
-// A row's softmax weights are 2^(score - reference).  The reference is set KV_UP
-// below the largest score seen and stays until a score passes it by KV_MOVE:
-// the largest weight lies between 2^7 and 2^15, inside fp16's range, with room
-// below: a weight of 2^-10 of it still has both its fp16 parts whole.
-constexpr float KV_UP = 7.0f, KV_MOVE = 15.0f;
+// A row's softmax weights are 2^(score - reference).  The reference is set `up`
+// below the largest score seen and stays until a score passes it by `move`:
+// the largest weight lies between 2^up and 2^move, inside fp16's range.  What
+// lies below decides how small weights are held, as fp16 ends at 2^-24.
+//   fp32 rows, 14 and 15.9: the two parts end at 2^-25, 2^-39 of the largest
+//   weight at most; a weight of 2^-22 of it is off by 2^-17 of itself.
+//   16-bit rows, 7 and 15: whole fp16 numbers (off by 2^-12 of themselves)
+//   down to 2^-21 of the largest, then off by 2^-32 of it.
+// A reference that may stay moves less often: 7 for fp32 rows too, off by
+// 2^-10 of a weight of 2^-22, took 67.4 us for 8 sequences of 5 rows at 8191
+// keys, not 69.4, and 151.4 for two prompts of up to 1537, not 152.3; 14 and 15 for
+// 16-bit rows 661 for a prompt of 8192, not 608.
+template <bool FP32>
+struct KvRef {
+    static constexpr float up = FP32 ? 14.0f : 7.0f, move = FP32 ? 15.9f : 15.0f;
+};
 
 // Values e .. e + 3 of an output row (packed row, head): O / l, zero where nothing was seen.
 struct KvaRow {

@@ -42,7 +42,7 @@ __device__ __forceinline__ void kv_join_last(const KvaArgs& a, const Item& it, i
 // numbers exactly.  P^T's fragments are S^T's turned by movmatrix.
 //
 // The softmax keeps a reference per row that moves only when a unit's largest
-// weight would pass 2^15 (KV_MOVE): the rescaling of O is rare, and otherwise
+// weight would near fp16's largest (KvRef): the rescaling of O is rare, and otherwise
 // no lane needs another's maximum.  l is summed per lane in fp32 and joined at
 // the end.
 //
@@ -436,7 +436,7 @@ __global__ void __launch_bounds__(KD_WARPS * 32, kd_blocks(NT)) kv_decode_kernel
             for (int c = 0; c < 2; ++c)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) top = fmaxf(top, v[n][c][j]);
-        if (__any_sync(~0u, top > KV_MOVE)) {                     // a row's reference moves
+        if (__any_sync(~0u, top > KvRef<SPLIT>::move)) {                     // a row's reference moves
             float old[NT][2];
 #pragma unroll
             for (int n = 0; n < NT; ++n)
@@ -450,7 +450,7 @@ __global__ void __launch_bounds__(KD_WARPS * 32, kd_blocks(NT)) kv_decode_kernel
                     float mx = fmaxf(fmaxf(v[n][c][0], v[n][c][1]), fmaxf(v[n][c][2], v[n][c][3]));
 #pragma unroll
                     for (int i2 = 4; i2 < 32; i2 <<= 1) mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, i2));
-                    const float now = fminf(old[n][c], KV_UP - mx), f = now == INFINITY ? 1.0f : fast_exp2(now - old[n][c]);
+                    const float now = fminf(old[n][c], KvRef<SPLIT>::up - mx), f = now == INFINITY ? 1.0f : fast_exp2(now - old[n][c]);
                     nm[n][c] = now;
                     l[n][c] *= f;
 #pragma unroll

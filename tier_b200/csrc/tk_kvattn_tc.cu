@@ -23,7 +23,7 @@
 // 128 products (7.6e-6) for fp32, 512 (3.1e-5, of a rounding of 4.9e-4) else.
 //
 // As in the streaming kernel the softmax's reference moves only when a weight
-// would pass 2^15 (KV_MOVE), so that O in TMEM is rarely rescaled.
+// would near fp16's largest (KvRef), so that O in TMEM is rarely rescaled.
 //
 // Warps (512 threads, one block an SM): 0-3 and 4-7 the streams' softmax, 8-11
 // the converters, 12 issues the products (13-15 idle: registers are divided by
@@ -481,9 +481,9 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvaArgs a, 
                         }
                     }
                     const float mx = fmaxf(max3(m0, m1, m2), m3) * sc;
-                    const bool move = mx + nm > KV_MOVE;
+                    const bool move = mx + nm > KvRef<SPLIT>::move;
                     if (__any_sync(~0u, move)) {
-                        const float now = move ? KV_UP - mx : nm;
+                        const float now = move ? KvRef<SPLIT>::up - mx : nm;
                         const float f = now == INFINITY ? 1.0f : fast_exp2(now - nm);
                         nm = now;
                         l *= f;
