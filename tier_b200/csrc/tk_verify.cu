@@ -450,6 +450,9 @@ __global__ void __launch_bounds__(DP_THREADS, 2) dv_pick_kernel(const DvArgs a) 
                 l += lo[0] + lo[1] + lo[2] + lo[3];
             }
             if (++k == each || i == mine - 1) {
+                // (a lane's low halves stay below 2^28; 32 lanes' would pass 2^32 in the largest vocabularies)
+                h += l >> 19;
+                l &= 0x7ffffu;
                 const unsigned long long s = ((unsigned long long)__reduce_add_sync(~0u, h) << 19) + __reduce_add_sync(~0u, l);
                 if (lane == 0) wsum[warp][e] = s;
                 own += s;
