@@ -1,6 +1,7 @@
 """GPU tests of the 4-bit cache and the attention over it at the edges of their
 contract: captured graphs and what is allocated after them, windows of any
-size, page ids that do not fit, small weights of fp32 rows.  Tolerances as in test_gpu_kv.py."""
+size, page ids that do not fit, small weights of fp32 rows, long appends.
+Tolerances as in test_gpu_kv.py."""
 import numpy as np
 import pytest
 
@@ -235,3 +236,71 @@ def test_fp32_rows_whose_mass_lies_on_a_key_of_no_value(ctx, new, seqs, where):
     qr, out = run_attend(ctx, cache, many, np.tile(q, (seqs, 1)), heads, "f32")
     exact, reach = ref.attend(cache, *bat[:3], qr[:new], heads, 1, dim, 0.125, 0)
     check_attend(out.reshape(seqs, *exact.shape), exact[None], reach[None], "f32")
+
+
+# ---- append and read back of many tokens ----------------------------------------------
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim,heads,page,n", [(128, 8, 64, 1500), (64, 3, 16, 7001), (128, 5, 128, 2200), (64, 17, 256, 1300)])
+def test_append_and_read_of_many_tokens(ctx, dtype, dim, heads, page, n):
+    """Calls long enough that a warp takes 128 groups of eight of a row; rows whose last warp is not full; every type."""
+    import torch
+    import tier_b200 as tk
+    assert n * heads * dim // 8 > 32 * 32 * 148
+    rng = np.random.default_rng(dim + heads)
+    new = [n // 3, 0, 1, n - n // 3 - 1]
+    kv = [new[0] + 9, 5, 1, new[3]]
+    q_start, kv_len, pages, total = ref.batch(rng, new, kv, page)
+    tt = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+    dt = {"f32": tk.DT_F32, "f16": tk.DT_F16, "bf16": tk.DT_BF16}
+    cache, w, x = ref.random_cache(rng, total, page, heads, dim), heads * dim, {}
+    for s in "kv":
+        a = rng.standard_normal((n, heads, dim // 32, 32)) * np.exp(rng.uniform(-4, 4, (n, heads, dim // 32, 1)))
+        a[rng.random(a.shape[:3]) < 0.05] = 0
+        a[rng.random(a.shape[:3]) < 0.05] *= 2.0 ** -24
+        a[rng.random(a.shape[:3]) < 0.02] *= 1e6 / 8
+        a[:: 97, 0, 0, :] = np.where(np.arange(32) % 2, -1.5, 1.5)
+        x[s] = torch.zeros(n, w + 8, dtype=tt[dtype], device="cuda")
+        x[s][:, :w] = dev(np.clip(a, -65504, 65504).reshape(n, w)).to(tt[dtype])
+    kc, sq = device_cache(cache), device_seqs(q_start, kv_len, pages)
+    ctx.kv_append(kc, sq, x["k"], x["v"], x_dtype=dt[dtype])
+    ctx.sync_status()
+    got = dict(zip(("k_q", "k_s", "v_q", "v_s"), (t.cpu().numpy() for t in kc._owner)))
+    seq = np.repeat(np.arange(4), new)
+    t = kv_len[seq] - (q_start[seq + 1] - np.arange(n))
+    place = (pages[seq, t // page], slice(None), t % page)
+    want = {}
+    for s in "kv":
+        m, d = ref.quantize(x[s][:, :w].float().cpu().numpy().reshape(n, heads, dim))
+        cache[s + "_q"][place], cache[s + "_s"][place] = ref.pack(m), d
+        want[s] = (m * np.repeat(d.astype(np.float64), 32, -1)).reshape(n, w)
+    for name, a in got.items():
+        assert np.array_equal(a.view(np.uint8), cache[name].view(np.uint8)), name
+    for out in DTYPES:
+        k, v = (torch.full((n, w + 8), 5.0, dtype=tt[out], device="cuda") for _ in "kv")
+        ctx.kv_read(kc, sq, k, v, out_dtype=dt[out])
+        ctx.sync_status()
+        for s, r in (("k", k), ("v", v)):
+            assert torch.equal(r[:, :w].cpu(), torch.from_numpy(want[s]).to(tt[out])), (s, out)
+            assert (r[:, w:] == 5).all()
+
+
+def test_read_back_in_bf16(ctx):
+    """Few tokens; a value n * d of 11 bits is rounded to bf16's 8, ties to even."""
+    import torch
+    import tier_b200 as tk
+    rng = np.random.default_rng(54)
+    new, kv = [3, 1, 40], [10, 1, 60]
+    q_start, kv_len, pages, total = ref.batch(rng, new, kv, 16)
+    cache = ref.random_cache(rng, total, 16, 3, 64)
+    kc, sq = device_cache(cache), device_seqs(q_start, kv_len, pages)
+    k, v = (torch.full((44, 3 * 64 + 8), 5.0, dtype=torch.bfloat16, device="cuda") for _ in "kv")
+    ctx.kv_read(kc, sq, k, v, out_dtype=tk.DT_BF16)
+    ctx.sync_status()
+    for s, r in (("k", k), ("v", v)):
+        values = ref.unpack(cache[s + "_q"], cache[s + "_s"])
+        for b in range(3):
+            for i in range(new[b]):
+                t = kv[b] - new[b] + i
+                want = torch.from_numpy(values[pages[b, t // 16], :, t % 16].reshape(-1)).to(torch.bfloat16)
+                assert torch.equal(r[q_start[b] + i, :192].cpu(), want)
+        assert (r[:, 192:] == 5).all()

@@ -28,3 +28,25 @@ def test_draws_of_the_largest_vocabulary(ctx):
     assert weight == (1 << 19) - 1
     want = [(weight * some * int(u * np.float32(2 ** 24)) >> 24) // weight for u in us]
     assert (acc == 0).all() and nxt.tolist() == want
+
+
+def test_rows_behind_a_refusal_may_hold_anything(ctx):
+    """Nothing of the rows after the refused one is needed, nor a sequence's last row of draft logits."""
+    V = 5000
+    rng = np.random.default_rng(61)
+    base = rng.standard_normal((5, V)).astype(np.float32)
+    start, tokens = np.array([0, 3, 5], np.int32), np.zeros(5, np.int32)
+    tokens[1:] = base.argmax(1)[:-1]
+    tokens[1] = base[0].argmin()
+    us = np.full(2, 0.5, np.float32)
+    for with_draft in (False, True):
+        t, d = base.copy(), base.copy()
+        d[0, tokens[1]] = 20.0                            # drafted far above its probability: refused
+        t[1:3] = np.nan
+        d[1:3] = np.nan
+        d[4] = np.nan
+        ua = np.array([0.999, 0.999, 0.999, 0.0, 0.999], np.float32)
+        acc, nxt, logp = run(ctx, start, t, d if with_draft else None, tokens, ua, us, 1.0)
+        ctx.sync_status()
+        assert acc.tolist() == [0, 1] and (nxt >= 0).all() and nxt[0] != tokens[1]
+        assert (logp[1:3] == 0).all() and np.isfinite(logp).all()
