@@ -71,6 +71,7 @@ class IqGrids(ctypes.Structure):
 
 class KvCache(ctypes.Structure):
     """tk_kvcache: one layer's 4-bit key/value cache on the device."""
+    _device = None         # where make_kvcache's tensors are
     _fields_ = [("n_pages", ctypes.c_int), ("page_tokens", ctypes.c_int), ("n_kv_heads", ctypes.c_int),
                 ("head_dim", ctypes.c_int), ("k_q", ctypes.c_void_p), ("k_s", ctypes.c_void_p),
                 ("v_q", ctypes.c_void_p), ("v_s", ctypes.c_void_p)]
@@ -78,6 +79,7 @@ class KvCache(ctypes.Structure):
 
 class Seqs(ctypes.Structure):
     """tk_seqs: a batch of sequences with packed new tokens."""
+    _device = None         # where make_seqs' tensors are
     _fields_ = [("n_seqs", ctypes.c_int), ("n_tokens", ctypes.c_int), ("max_new", ctypes.c_int),
                 ("max_pages", ctypes.c_int), ("q_start", ctypes.c_void_p), ("kv_len", ctypes.c_void_p),
                 ("pages", ctypes.c_void_p)]
@@ -211,15 +213,77 @@ def _ptr(t) -> int | None:
 
 def _current_stream() -> int:
     """The current stream's handle, without the Stream object (3 us a call) where torch offers that."""
-    import torch
-    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-    return raw(torch.cuda.current_device()) if raw else torch.cuda.current_stream().cuda_stream
+    global _raw_stream
+    if _raw_stream is None:
+        import torch
+        raw, device = (getattr(torch._C, n, None) for n in ("_cuda_getCurrentRawStream", "_cuda_getDevice"))
+        torch.cuda.init()
+        _raw_stream = (lambda: raw(device())) if raw and device else (lambda: torch.cuda.current_stream().cuda_stream)
+    return _raw_stream()
+
+
+_raw_stream = None
 
 
 def _stream(stream) -> int | None:
     if stream is None:
         return _current_stream()
     return getattr(stream, "cuda_stream", stream)
+
+
+def _reachable(t, device) -> bool:
+    return t.get_device() == device or (t.get_device() < 0 and t.is_pinned())
+
+
+def _row_stride(fn, name, t, code, n, width, ld, device):
+    """The stride in elements of n rows of `width` elements of DT_* code `code` (ld, or None: the tensor's own), which must
+    lie in t: the library sees an address and cannot tell where its memory ends.  What the library itself refuses (null
+    pointers, unknown codes, strides below the width, alignment) is left to it."""
+    if t is None:
+        return ld or 0
+    strides = t.stride()                                   # (each look at a tensor is 50 to 200 ns: as few as there may be)
+    if len(strides) == 2 and strides[1] == 1 and (not ld or ld == strides[0]) and t.dtype is _DTYPES.get(code):
+        rows, cols = t.shape
+        if rows >= n and cols >= width and t.get_device() == device:
+            return strides[0]
+    return _other_row_stride(fn, name, t, code, n, width, ld, device)
+
+
+def _other_row_stride(fn, name, t, code, n, width, ld, device):
+    """_row_stride of what is not a plain matrix of those rows."""
+    if not _DTYPES:
+        import torch
+        _DTYPES.update({DT_F32: torch.float32, DT_F16: torch.float16, DT_BF16: torch.bfloat16, _I32: torch.int32})
+    shaped, ld, want, bad = not ld, ld or t.stride(0), _DTYPES.get(code), None
+    if want is None:
+        return ld
+    if t.element_size() != want.itemsize or (t.dtype.is_floating_point and t.dtype is not want):   # (raw bits may pass)
+        bad = f"holds {t.dtype}, given as {want}"
+    elif not _reachable(t, device):
+        bad = f"is not on device {device}"
+    elif ld >= width > 0 and n > 0:
+        if t.dim() > 1 and t.size(0) > 0 and not t[0].is_contiguous():
+            bad = "has rows that are not contiguous"
+        elif (shaped and (t.size(0) < n or t[0].numel() < width)
+              or (n - 1) * ld + width > t.untyped_storage().nbytes() // want.itemsize - t.storage_offset()):
+            bad = f"holds no {n} rows of {width}, {ld} apart"
+    if bad:
+        raise TierkError(TK_ERR_INVALID, f"{fn}: {name} {bad}")
+    return ld
+
+
+def _check_vector(fn, name, t, n, code, device):
+    """n contiguous elements: fp32 (DT_F32) or 32-bit whole numbers (_I32)."""
+    if t is None or (t.dtype is _DTYPES.get(code) and t.numel() >= n and t.is_contiguous() and t.get_device() == device):
+        return
+    if not (t.numel() >= n and t.element_size() == 4 and t.is_floating_point() == (code == DT_F32) and t.is_contiguous()):
+        raise TierkError(TK_ERR_INVALID, f"{fn}: {name} must be {n} contiguous {'float32' if code == DT_F32 else 'int32'} elements")
+    if not _reachable(t, device):
+        raise TierkError(TK_ERR_INVALID, f"{fn}: {name} is not on device {device}")
+
+
+_I32 = -1
+_DTYPES: dict = {}         # the torch type of each DT_* code, once a tensor has been looked at; _I32's
 
 
 class Context:
@@ -338,15 +402,26 @@ class Context:
         return out
 
     # ---- 4-bit key/value cache, attention over it, drafted tokens ----
+    def _kv_strides(self, fn, cache, seqs, heads, code, names, a, lda, b, ldb):
+        """Row strides of a call's two packed arrays, which must lie in their tensors."""
+        device, width = self.device, heads * cache.head_dim
+        if cache._device not in (None, device) or seqs._device not in (None, device):
+            raise TierkError(TK_ERR_INVALID, f"{fn}: cache and batch must be on device {device}")
+        n = seqs.n_tokens if seqs.n_seqs > 0 and seqs.max_new > 0 else 0
+        return (_row_stride(fn, names[0], a, code, n, width, lda, device),
+                _row_stride(fn, names[1], b, code, n, width, ldb, device))
+
     def kv_append(self, cache: KvCache, seqs: Seqs, k, v, x_dtype=DT_F32, ldk=None, ldv=None, stream=None):
         """Round the batch's new keys and values to 4 bits into the cache (tk_kv_append)."""
+        ldk, ldv = self._kv_strides("tk_kv_append", cache, seqs, cache.n_kv_heads, x_dtype, "kv", k, ldk, v, ldv)
         _check(self.lib.tk_kv_append(self.h, ctypes.byref(cache), ctypes.byref(seqs), _ptr(k), _ptr(v), x_dtype,
-                                     ldk or k.stride(0), ldv or v.stride(0), _stream(stream)))
+                                     ldk, ldv, _stream(stream)))
 
     def kv_read(self, cache: KvCache, seqs: Seqs, k, v, out_dtype=DT_F32, ldk=None, ldv=None, stream=None):
         """k, v = the values that the cache holds for the batch's new tokens (tk_kv_read)."""
+        ldk, ldv = self._kv_strides("tk_kv_read", cache, seqs, cache.n_kv_heads, out_dtype, "kv", k, ldk, v, ldv)
         _check(self.lib.tk_kv_read(self.h, ctypes.byref(cache), ctypes.byref(seqs), _ptr(k), _ptr(v), out_dtype,
-                                   ldk or k.stride(0), ldv or v.stride(0), _stream(stream)))
+                                   ldk, ldv, _stream(stream)))
         return k, v
 
     def kv_attend(self, cache: KvCache, seqs: Seqs, q, n_heads, out, x_dtype=DT_F32, scale=None, window=0, ldq=None,
@@ -354,20 +429,29 @@ class Context:
         """out = attention of the batch's new tokens over the cache (tk_kv_attend);
         scale defaults to 1 / sqrt(head_dim)."""
         scale = cache.head_dim ** -0.5 if scale is None else scale
+        ldq, ldo = self._kv_strides("tk_kv_attend", cache, seqs, n_heads, x_dtype, ("q", "out"), q, ldq, out, ldo)
         _check(self.lib.tk_kv_attend(self.h, ctypes.byref(cache), ctypes.byref(seqs), _ptr(q), x_dtype,
-                                     ldq or q.stride(0), n_heads, scale, window, _ptr(out), ldo or out.stride(0),
-                                     _stream(stream)))
+                                     ldq, n_heads, scale, window, _ptr(out), ldo, _stream(stream)))
         return out
 
     def draft_verify(self, target, tokens, row_start, u_accept, u_sample, n_accept, next_token, logp=None, draft=None,
                      temperature=1.0, stream=None):
         """Accept drafted tokens against the target's logits and draw each
         sequence's next token (tk_draft_verify)."""
-        _check(self.lib.tk_draft_verify(self.h, n_accept.numel(), _ptr(row_start), target.shape[0], target.shape[1],
-                                        _ptr(target), target.stride(0), _ptr(draft),
-                                        draft.stride(0) if draft is not None else 0, _ptr(tokens), _ptr(u_accept),
-                                        _ptr(u_sample), temperature, _ptr(n_accept), _ptr(next_token), _ptr(logp),
-                                        _stream(stream)))
+        fn, dev, B, (n, V) = "tk_draft_verify", self.device, n_accept.numel(), target.shape
+        ldt = _row_stride(fn, "target", target, DT_F32, n, V, None, dev)
+        ldd = _row_stride(fn, "draft", draft, DT_F32, n, V, None, dev)
+        _check_vector(fn, "row_start", row_start, B + 1, _I32, dev)
+        _check_vector(fn, "tokens", tokens, n, _I32, dev)
+        if temperature:
+            _check_vector(fn, "u_accept", u_accept, n - 1, DT_F32, dev)     # (the last row judges no draft)
+            _check_vector(fn, "u_sample", u_sample, B, DT_F32, dev)
+        _check_vector(fn, "n_accept", n_accept, B, _I32, dev)
+        _check_vector(fn, "next_token", next_token, B, _I32, dev)
+        _check_vector(fn, "logp", logp, n, DT_F32, dev)
+        _check(self.lib.tk_draft_verify(self.h, B, _ptr(row_start), n, V, _ptr(target), ldt, _ptr(draft), ldd, _ptr(tokens),
+                                        _ptr(u_accept), _ptr(u_sample), temperature, _ptr(n_accept), _ptr(next_token),
+                                        _ptr(logp), _stream(stream)))
         return n_accept, next_token
 
     # ---- reduce-scatter over peer memory (multi-GPU) ----
@@ -479,6 +563,14 @@ def make_weight(qtype: int, rows: int, cols: int, data, scale_log2: int = 0) -> 
     return w
 
 
+def _one_device(what, tensors) -> int | None:
+    """The CUDA device of all tensors (None: pinned host memory, which every device reaches)."""
+    at = {None if t.get_device() < 0 and t.is_pinned() else t.get_device() for t in tensors}
+    if -1 in at or len(at - {None}) > 1:
+        raise ValueError(f"{what} must be on one CUDA device")
+    return next(iter(at - {None}), None)
+
+
 def make_kvcache(k_q, k_s, v_q, v_s) -> KvCache:
     """Describe a cache's four device tensors (layout: tk_kvcache in tierk.h):
     k_q, v_q uint8 [pages, kv_heads, page_tokens, head_dim / 2], k_s, v_s
@@ -490,6 +582,7 @@ def make_kvcache(k_q, k_s, v_q, v_s) -> KvCache:
             raise ValueError(f"cache tensor {tuple(t.shape)}: expected contiguous {shape} of {size}-byte elements")
     c = KvCache(n, p, h, 2 * half, k_q.data_ptr(), k_s.data_ptr(), v_q.data_ptr(), v_s.data_ptr())
     c._owner = (k_q, k_s, v_q, v_s)   # the descriptor keeps its device memory alive
+    c._device = _one_device("cache tensors", c._owner)
     return c
 
 
@@ -513,6 +606,7 @@ def make_seqs(q_start, kv_len, pages, n_tokens: int, max_new: int) -> Seqs:
         raise ValueError("q_start must have n_seqs + 1 entries and pages n_seqs rows")
     s = Seqs(B, n_tokens, max_new, pages.shape[1], q_start.data_ptr(), kv_len.data_ptr(), pages.data_ptr())
     s._owner = (q_start, kv_len, pages)
+    s._device = _one_device("q_start, kv_len and pages", s._owner)
     return s
 
 
