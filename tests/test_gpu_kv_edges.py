@@ -304,3 +304,20 @@ def test_read_back_in_bf16(ctx):
                 want = torch.from_numpy(values[pages[b, t // 16], :, t % 16].reshape(-1)).to(torch.bfloat16)
                 assert torch.equal(r[q_start[b] + i, :192].cpu(), want)
         assert (r[:, 192:] == 5).all()
+
+
+def test_scales_whose_power_of_two_overflows_are_refused(ctx):
+    """Scores are scale * log2(e) * q . k: such a scale made every score infinite or NaN."""
+    import torch
+    import tier_b200 as tk
+    kc = tk.alloc_kvcache(1, 16, 1, 64)
+    sq = device_seqs(np.array([0, 2], np.int32), np.array([9], np.int32), np.zeros((1, 1), np.int32))
+    q = torch.zeros(2, 64, device="cuda")
+    for scale in (2.5e38, -3.4e38, float("inf")):
+        with pytest.raises(tk.TierkError) as e:
+            ctx.kv_attend(kc, sq, q, 1, torch.empty_like(q), scale=scale)
+        assert e.value.status == tk.TK_ERR_INVALID
+    out = torch.full_like(q, 3.0)
+    ctx.kv_attend(kc, sq, q, 1, out, scale=2.3e38)
+    ctx.sync_status()
+    assert (out == 0).all()

@@ -709,7 +709,8 @@ tk_status tk_kv_attend(tk_ctx* ctx, const tk_kvcache* cache, const tk_seqs* seqs
     if (st != TK_OK) return st;
     if (n_heads <= 0 || n_heads % cache->n_kv_heads)
         return fail(TK_ERR_INVALID, "tk_kv_attend: n_heads must be a multiple of the cache's n_kv_heads");
-    if (!std::isfinite(scale)) return fail(TK_ERR_INVALID, "tk_kv_attend: scale must be finite");
+    if (!std::isfinite((float)(scale * 1.4426950408889634)))       // scores are taken in powers of two
+        return fail(TK_ERR_INVALID, "tk_kv_attend: scale * log2(e) must be finite");
     if (window < 0) return fail(TK_ERR_INVALID, "tk_kv_attend: negative window");
     if (kv_empty(seqs)) return TK_OK;
     return launch_kv_attend(ctx, *cache, *seqs, q, x_dtype, ldq, n_heads, scale, window, out, ldo,
