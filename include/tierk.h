@@ -112,7 +112,10 @@ const char *tk_last_error_string(void);
  * workspace of its calls: growth inside a capture is refused (TK_ERR_INVALID;
  * the capture stays valid), and a workspace that a captured call used and a
  * later call outgrew is kept until tk_destroy.  Replays share that workspace
- * with the context's other calls: order them as calls on several streams. */
+ * with the context's other calls: order them as calls on several streams.
+ * Not covered: tk_linear_fwd_dx and its _rs form keep one table of work per
+ * context, that of the last shape; a graph of them is captured anew after a
+ * call of another shape. */
 tk_status tk_reserve(tk_ctx *ctx, size_t bytes);
 size_t tk_workspace_bytes(const tk_ctx *ctx);
 /* Synchronize `stream` and report any device-side status (timeouts, invalid
@@ -314,15 +317,17 @@ tk_status tk_kv_attend(tk_ctx *ctx, const tk_kvcache *cache, const tk_seqs *seqs
  * tokens are accepted in turn while u_accept[i] * q(x) < p(x).  At the first
  * refusal the sequence's next token is drawn from max(p - q, 0), or from p at
  * its last row: the lowest token whose running sum of weights passes
- * u_sample[b] times their total.  Weights are whole multiples of 2^-38, so the
- * draw depends on no order of summation.  temperature == 0: accepted while the
+ * u_sample[b] times their total.  Weights are whole multiples of 2^-38, whose
+ * sum depends on no order.  vocab <= 2^23; temperature 0 or at least 1e-4.
+ * temperature == 0: accepted while the
  * drafted token is the row's largest logit (the lowest of several), which is
  * also the next token.
  * Out: n_accept[b] = drafted tokens accepted; next[b]; logp[i] (nullable) = log
  * p of the token that row i settled (accepted or drawn; at temperature 0 for
  * temperature 1), 0 for rows after the refusal.
  * Logits of -inf have probability 0.  Random numbers are in [0, 1).  A row that
- * is needed and holds NaN, +inf or only -inf ends its sequence with next = -1,
+ * is needed and holds NaN, +inf or only -inf, or whose largest logit times
+ * log2(e) / temperature passes fp32, ends its sequence with next = -1,
  * as does a row_start that does not fit, and tk_sync_status reports
  * TK_ERR_DEVICE.  A drafted token outside the vocabulary is refused.
  * No counterpart in the reference, which decodes one token at a time. */

@@ -91,20 +91,16 @@ __device__ __forceinline__ size_t kv_row(const KvView& c, int page, int head, in
     return ((((size_t)page * c.heads + head) << c.page_shift) + (pos & ((1 << c.page_shift) - 1)));
 }
 
-// The word's value e (0..7), -8..7: fields 0..3 hold values 0, 2, 4, 6 and
-// fields 4..7 values 1, 3, 5, 7, so that one mask takes the two fp16 halves of
-// a pair of neighbouring values (kv_pairs).
-__device__ __forceinline__ int kv_nibble(uint32_t w, int e) {
-    const int f = (e >> 1) + 4 * (e & 1);
-    return (int)(((w >> (4 * f)) & 15u) ^ 8u) - 8;
-}
-
 // ---- 4-bit numbers to fp16 -------------------------------------------------
-// x: four 4-bit fields of each 16-bit half.  An fp16 with exponent bits 0x6400
-// counts in ones from 1024, so OR-ing a field n + 8 into its low bits gives
-// 1024 + (n + 8), or 1024 + 16 (n + 8) for the second field; the XOR in the
-// same LOP3 turns two's complement n into n + 8.  Both are brought back to n
-// exactly (|n| <= 8), then scaled: n * d is exact for d of 8 significant bits.
+// A word's fields 0..3 hold values 0, 2, 4, 6 and fields 4..7 values 1, 3, 5, 7
+// (two's complement), so that one mask takes the two fp16 halves of a pair of
+// neighbouring values.  x: four fields of each 16-bit half.  The method is that
+// of Kim et al. (2022, "Who Says Elephants Can't Run") for integer weights: an
+// fp16 with exponent bits 0x6400 counts in ones from 1024, so OR-ing a field
+// n + 8 into its low bits gives 1024 + (n + 8), or 1024 + 16 (n + 8) for the
+// second field; the XOR in the same LOP3 turns two's complement n into n + 8.
+// Both are brought back to n exactly (|n| <= 8), then scaled: n * d is exact for
+// d of 8 significant bits.
 __device__ __forceinline__ uint32_t lop_and_xor(uint32_t x, uint32_t mask, uint32_t flip) {
     uint32_t r;
     asm("lop3.b32 %0, %1, %2, %3, 0x6a;" : "=r"(r) : "r"(x), "r"(mask), "r"(flip));   // (x & mask) ^ flip

@@ -55,9 +55,9 @@ __device__ __forceinline__ void kv_join_last(const KvaArgs& a, const Item& it, i
 // Bound: long caches by the instructions that turn 4 bits into fp16 fragments,
 // not by memory; few rows by the chain of one unit after another and the join.
 // Measured (32 query heads, 8 key/value heads of 128; us, TB/s of cache read):
-// one fp16 row at 4097 keys 10.8, 0.44; 32 bf16 rows at up to 16300 each 58.8,
-// 3.3; one fp32 row at 131071 54.0, 2.8; 8 sequences of 5 fp32 rows at 8191
-// 66.6, 1.2 (three column sets of two parts, 8 warps an SM: six products where
+// one fp16 row at 4097 keys 10.8, 0.44; 32 bf16 rows at up to 16300 each 58.7,
+// 3.3; one fp32 row at 131071 54.9, 2.8; 8 sequences of 5 fp32 rows at 8191
+// 69.3, 1.1 (three column sets of two parts, 8 warps an SM: six products where
 // a bf16 row has one, and few warps to hide their latency).
 // ---------------------------------------------------------------------------
 constexpr int KD_WARPS = 4, KD_STAGES = 3, KD_UNIT = 32, KD_MAX_ROWS = 32;
@@ -485,7 +485,7 @@ __global__ void __launch_bounds__(KD_WARPS * 32, kd_blocks(NT)) kv_decode_kernel
             }
         // O^T: matrix rows g and g + 8 of tile i are values (D / 8) g + 2 i and + 1 of the head. The tensor core cuts what
         // it adds to an accumulator: n products in one lose up to n 2^-24 of it. So the 32 keys' sum is made from zero and
-        // added to O here (fp32, 131071 keys: 54.2 us; 52.3 and 2e-6 off if all keys went to one accumulator).
+        // added to O here (fp32, 131071 keys: 2 us of 55, where one accumulator for all keys was 2e-6 off).
         uint32_t w[8][VW];                                         // the two keys of lane t, of each 8-key group
         __half2 d[4];
 #pragma unroll

@@ -34,10 +34,11 @@
 // and half a conversion a score) beside the tensor core's 2 x 128 cycles a
 // tile; neither waits long for the other, under a power limit that holds the
 // clock at 1.47 GHz of 1.97 in long prompts.  Measured (32 query heads on 8
-// key/value heads of 128): a prompt of 8192, bf16, 563 us, 976 TFLOP/s; three
-// chunks of up to 1000 rows behind 6001 keys, window 1024, 16 heads on 4 of
-// 64, fp16, 32.5 us; two fp32 prompts of up to 1537 rows, 2000 keys, 154 us, 249
-// TFLOP/s (two parts of q and of P: twice that in the tensor core).
+// key/value heads of 128; calls one after the other): a prompt of 8192, bf16,
+// 608 us, 904 TFLOP/s; three chunks of up to 1000 rows behind 6001 keys, window
+// 1024, 16 heads on 4 of 64, fp16, 31.5 us; two fp32 prompts of up to 1537 rows,
+// 2000 keys, 152 us, 252 TFLOP/s (two parts of q and of P: twice that in the
+// tensor core).
 #include "tk_f32x2.cuh"
 #include "tk_kv.cuh"
 

@@ -40,11 +40,12 @@ __device__ __forceinline__ void widen8(const Raw8<DT>& r, float (&x)[8]) {
 // a group of 32.  A warp takes up to ITEMS * 32 items of one such row: it
 // finds the token's place once, and its loads are in flight together.
 // Bound: long appends by instructions (issue 75 % busy, the integer pipe 67 %:
-// the extreme, the exact rounding, the packing), reading back by memory; single
+// the extreme, the exact rounding, the packing), reading back by the latency of
+// its loads (issue 65 %, stalls on them 7.8 an instruction); single
 // tokens by the launch.  Measured: 13 thousand bf16 rows of k and v (8
 // key/value heads of 128) appended and read back, 117 MB in 32 us, 3.65 TB/s,
-// where an item a thread took 79; 16 single fp32 tokens 4.5 us for both calls
-// on the device, 10.9 with their host side.
+// where an item a thread took 79; 16 single fp32 tokens 5.2 us for both calls
+// in a graph, 12.6 with their host side.
 struct KvcArgs {
     KvView c;
     SeqView s;
@@ -126,8 +127,7 @@ __device__ __forceinline__ float group_extreme(const float (&x)[8]) {
     return m;
 }
 
-// Bound: memory (each value read once, half a byte and a sixteenth of a scale
-// written); the arithmetic is kept near it: the extreme from the group's
+// The arithmetic is kept short, as it is the bound: the extreme from the group's
 // largest and smallest value (value by value only where both are as far from
 // zero, or not finite), whole numbers by adding 2^23 downwards, whose bits are
 // shifted together.  Four lanes share a group so that every load is 16 or 32

@@ -5,8 +5,10 @@
 // i.  Only whole exponents are subtracted, so a weight's bits do not depend on
 // which part of the row saw the largest logit: parts of a row are summed each
 // to its own largest exponent, brought together by exact powers of two, and
-// the row's sum S (64 bits, rounded once to fp32) and its probabilities
-// weight / S come out the same for any division.
+// the row's sum S is rounded once to fp32 from a sum of 2^-46.  Another division
+// into parts (a batch of another size) can turn that one rounding where the sum
+// lies within 2^-46 of the middle between two fp32 numbers; else S, and the
+// probabilities weight / S with it, come out the same.
 //
 // Two launches.  dv_rows reads every logit once (the bound: memory) and leaves
 // each part's exponent, sum and largest logit.  dv_pick, a cluster of blocks
@@ -16,11 +18,11 @@
 // that holds the draw searched again.
 //
 // Measured: 24 sequences of up to 8 rows, vocabulary 262144, with draft logits
-// (191 MB) 70.5 us, 2.7 TB/s: dv_rows about 40 (4.8 TB/s; an exponential a
+// (191 MB) 73.3 us, 2.6 TB/s: dv_rows about 40 (4.8 TB/s; an exponential a
 // logit and half a dozen packed instructions keep it from the memory's rate),
 // the draw the rest (it reads its two rows again in 192 blocks, and its chain
-// of sums, exchange and search is latency).  One sequence of 5 rows 16.9 us, 64
-// greedy ones of up to 5 rows of 50257 (40.8 MB) 16.6: two dependent launches.
+// of sums, exchange and search is latency).  One sequence of 5 rows 18.4 us, 64
+// greedy ones of up to 5 rows of 50257 (40.8 MB) 18.4: two dependent launches.
 #include <climits>
 #include "tk_device.cuh"
 #include "tk_f32x2.cuh"
@@ -528,9 +530,14 @@ __global__ void __launch_bounds__(DP_THREADS, 2) dv_pick_kernel(const DvArgs a) 
 constexpr int DP_SMEM = DP_AHEAD * 2 * DP_THREADS * (int)sizeof(float4);
 
 // Blocks of a sequence's draw: 16 at most, and 4/3 an SM over all sequences.
-// Two an SM would hide more latency, but clusters stay within a GPC: 24
-// sequences by 10 blocks (240 of 296 places) ran in two waves (whole call 79.7
-// us), by 8 in one (72.0; 70.5 now), by 6 with half the warps an SM (79.6).
+// Two an SM would hide more latency, but clusters stay within a GPC, and a size
+// whose last cluster finds no place takes two waves.  Measured (4 rows of 262144
+// a sequence with draft logits, whole call, us; first the rule's size):
+//    8 sequences: 16 blocks 37, 12 41, 8 46     24: 8 72, 7 74, 10 82, 6 79
+//   16: 12 65, 10 55, 16 59, 8 60               32: 6 89, 7 86, 8 93, 5 94
+//   48: 4 123, 5 117, 3 136, 6 130
+// The rule is within 6 % of the best but at 16 sequences (17 %): which sizes fill
+// the GPCs depends on the GPU's floor plan, which it does not ask.
 static int pick_cluster(const tk_ctx* ctx, int n_seqs, bool greedy) {
     if (greedy) return 1;                          // a greedy row draws nothing
     const int c = ctx->num_sms * 4 / 3 / n_seqs;
