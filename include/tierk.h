@@ -295,7 +295,8 @@ tk_status tk_kv_read(tk_ctx *ctx, const tk_kvcache *cache, const tk_seqs *seqs, 
  * tokens j that row i sees: j <= its position, and j > position - window when
  * window > 0.  q, out [n_tokens, n_heads * head_dim] in x_dtype; head h reads
  * key/value head h / (n_heads / n_kv_heads).  A row that sees nothing is zero.
- * scale * log2(e) is finite in fp32, window >= 0.
+ * scale * log2(e) is finite in fp32, window >= 0; scores times log2(e) are below
+ * 2^27 in size (fp32 steps of 8), or their row is unspecified.
  * q and the probabilities of fp32 rows enter as two fp16 parts, 22 bits:
  * probabilities down to 2^-18 of a row's largest are off by 2^-21 of themselves
  * at most, smaller ones by 2^-39 of the largest (2^-17 of themselves at 2^-22

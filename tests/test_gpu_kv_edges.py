@@ -1,14 +1,21 @@
 """GPU tests of the 4-bit cache and the attention over it at the edges of their
 contract: captured graphs and what is allocated after them, windows of any
-size, page ids that do not fit, small weights of fp32 rows, long appends.
+size, page ids that do not fit, small weights of fp32 rows, scores near the
+limits of fp32, long appends.
 Tolerances as in test_gpu_kv.py."""
 import numpy as np
 import pytest
 
 import kv_ref as ref
-from test_gpu_kv import DTYPES, check_attend, dev, device_cache, device_seqs, run_attend
+import test_gpu_kv
+from test_gpu_kv import DTYPES, dev, device_cache, device_seqs, run_attend
 
 pytestmark = pytest.mark.gpu
+
+
+def check_attend(out, exact, reach, dtype):
+    assert np.isfinite(out).all()                          # (a NaN is above no bound)
+    test_gpu_kv.check_attend(out, exact, reach, dtype)
 
 
 class Replayed:
@@ -321,3 +328,26 @@ def test_scales_whose_power_of_two_overflows_are_refused(ctx):
     ctx.kv_attend(kc, sq, q, 1, out, scale=2.3e38)
     ctx.sync_status()
     assert (out == 0).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("where", [0, 700, 1999])
+@pytest.mark.parametrize("new,seqs", [(1, 1), (4, 100), (8, 100), (60, 1), (300, 1)])
+def test_scores_so_large_that_their_rounding_is_whole_powers(ctx, dtype, new, seqs, where):
+    """Scores of 2^10 to 2^26.9 in powers of two, whose fp32 steps reach 8: weights stay finite, and the key that leads by
+    half a score or more is the output (its weight's one or two fp16 parts over their sum: the tolerance of every row)."""
+    rng = np.random.default_rng(55)
+    kv, page, dim, heads = 2000 + new, 64, 64, 4
+    bat = ref.batch(rng, [new], [kv], page)
+    cache = ref.random_cache(rng, bat[3], page, 1, dim)
+    cache["k_q"] = ref.pack(rng.integers(-8, 4, (*cache["k_q"].shape[:3], dim)).astype(np.int8))
+    cache["k_s"][:] = 500.0
+    p, r = bat[2][0, where // page], where % page
+    cache["k_q"][p, :, r] = ref.pack(np.full((1, dim), 7, np.int8))
+    size = 2.0 ** rng.uniform(10, 26.9, (new, heads))
+    size[0] = 2.0 ** np.array([26.9, 25.7, 24.8, 20.6])
+    q = np.repeat(size * np.log(2) / (0.125 * dim * 7 * 500.0), dim, -1)
+    many = (np.arange(seqs + 1, dtype=np.int32) * new, np.full(seqs, kv, np.int32), np.tile(bat[2], (seqs, 1)), bat[3])
+    qr, out = run_attend(ctx, cache, many, np.tile(q, (seqs, 1)), heads, dtype)
+    exact, reach = ref.attend(cache, *bat[:3], qr[:new], heads, 1, dim, 0.125, 0)
+    check_attend(out.reshape(seqs, *exact.shape), exact[None], reach[None], dtype)

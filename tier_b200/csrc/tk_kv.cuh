@@ -188,6 +188,12 @@ __device__ __forceinline__ float q_unit(float max, float& back) {
 template <bool FP32>
 struct KvRef {
     static constexpr float up = FP32 ? 14.0f : 7.0f, move = FP32 ? 15.9f : 15.0f;
+    // Minus the reference for a largest score mx, itself rounded: both roundings
+    // go down, so that the weight stays below 2^up where a step of fp32 is whole
+    // powers of two (from scores of 2^24 on; below 2^27 it is down to 2^20 lower).
+    static __device__ __forceinline__ float minus(float mx) {
+        return __fsub_rd(up, __fmaf_ru(fabsf(mx), 5.9604644775390625e-08f, mx));
+    }
 };
 
 // Values e .. e + 3 of an output row (packed row, head): O / l, zero where nothing was seen.

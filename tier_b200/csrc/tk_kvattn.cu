@@ -450,7 +450,7 @@ __global__ void __launch_bounds__(KD_WARPS * 32, kd_blocks(NT)) kv_decode_kernel
                     float mx = fmaxf(fmaxf(v[n][c][0], v[n][c][1]), fmaxf(v[n][c][2], v[n][c][3]));
 #pragma unroll
                     for (int i2 = 4; i2 < 32; i2 <<= 1) mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, i2));
-                    const float now = fminf(old[n][c], KvRef<SPLIT>::up - mx), f = now == INFINITY ? 1.0f : fast_exp2(now - old[n][c]);
+                    const float now = fminf(old[n][c], KvRef<SPLIT>::minus(mx)), f = now == INFINITY ? 1.0f : fast_exp2(now - old[n][c]);
                     nm[n][c] = now;
                     l[n][c] *= f;
 #pragma unroll

@@ -481,10 +481,10 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvaArgs a, 
                             m3 = max3(m3, x[i + 6], x[i + 7]);
                         }
                     }
-                    const float mx = fmaxf(max3(m0, m1, m2), m3) * sc;
-                    const bool move = mx + nm > KvRef<SPLIT>::move;
+                    m0 = fmaxf(max3(m0, m1, m2), m3);
+                    const bool move = fmaf(m0, sc, nm) > KvRef<SPLIT>::move;   // the largest exponent, as it is taken below
                     if (__any_sync(~0u, move)) {
-                        const float now = move ? KvRef<SPLIT>::up - mx : nm;
+                        const float now = move ? KvRef<SPLIT>::minus(m0 * sc) : nm;
                         const float f = now == INFINITY ? 1.0f : fast_exp2(now - nm);
                         nm = now;
                         l *= f;
