@@ -337,6 +337,59 @@ tk_status tk_draft_verify(tk_ctx *ctx, int n_seqs, const int32_t *row_start, int
                           const float *u_accept, const float *u_sample, float temperature, int32_t *n_accept,
                           int32_t *next, float *logp, void *stream);
 
+/* ---- rows of logits: log-probabilities, distillation ----------------------- */
+/* n_rows rows of `vocab` logits (<= 2^23; fp32, fp16 or bf16; row stride ldx in
+ * elements, of any alignment), T = temperature (1e-4 to 1e4).  Of a row: m its
+ * largest logit, S = sum_j exp((l_j - m) / T), p_j = exp((l_j - m) / T) / S.
+ * Logits of -inf have p = 0; results beyond fp32 are infinite.  A row that is
+ * needed and holds NaN, +inf or only -inf has NaN in all its results (places -1) and makes tk_sync_status report
+ * TK_ERR_DEVICE.  No counterpart in the reference, whose loss is the
+ * cross-entropy of one label a row. */
+enum { TK_TOP_MAX = 256 };   /* top_k, k at most */
+/* Log-probabilities of given tokens, entropy and the likeliest tokens:
+ * logp[i] = ln p(tokens[i]), entropy[i] = -sum_j p_j ln p_j, rmax[i] = m,
+ * rsum[i] = S (each nullable), and for top_k > 0 top_ids[i, :] = the places of
+ * the top_k largest logits, largest first, of equal ones the lowest place
+ * first, with top_logp[i, :] (nullable) = ln p there; both [n_rows, top_k].
+ * A row whose token is negative is left out (a batch's padding, a prompt's
+ * tokens): its logits are not read, its results are zeros and places -1; so is
+ * one whose token is not in the vocabulary, and tk_sync_status reports
+ * TK_ERR_DEVICE.  tokens == NULL: every row, without logp. */
+tk_status tk_logprobs(tk_ctx *ctx, int n_rows, int vocab, const void *logits, int x_dtype, long ldx, const int32_t *tokens,
+                      float temperature, float *logp, float *entropy, float *rmax, float *rsum, int top_k, int32_t *top_ids,
+                      float *top_logp, void *stream);
+/* dlogits[i, j] = d_logp[i] d logp[i] / dl_j + d_entropy[i] d entropy[i] / dl_j
+ *   = (d_logp[i] (j == tokens[i]) - p_j (d_logp[i] + d_entropy[i] (ln p_j + entropy[i]))) / T
+ * from tk_logprobs' rmax, rsum and (with d_entropy) entropy; one of d_logp and
+ * d_entropy may be NULL.  dlogits in d_dtype, row stride ldd; it may be logits
+ * itself (same address, type and stride), and overlap it in no other way.  Rows
+ * left out, and rows whose two gradients are both zero, are zero and their
+ * logits are not read. */
+tk_status tk_logprobs_grad(tk_ctx *ctx, int n_rows, int vocab, const void *logits, int x_dtype, long ldx, const int32_t *tokens,
+                           float temperature, const float *rmax, const float *rsum, const float *d_logp, const float *entropy,
+                           const float *d_entropy, void *dlogits, int d_dtype, long ldd, void *stream);
+/* Distillation from a teacher's top logits.  ids, teacher [n_rows, k]: places
+ * and the teacher's logits there (or its log-probabilities: q does not change);
+ * an entry whose place is negative or whose logit is -inf does not count, one
+ * beyond the vocabulary neither (tk_sync_status reports TK_ERR_DEVICE); a place
+ * may be listed twice.  With q = softmax(teacher[i, :] / T) over the row's
+ * entries (below 2^-126: 0):
+ *   loss[i] = sum_e q_e (ln q_e - ln p(ids[i, e]))      (nullable; +inf where
+ *             some p is 0 and q is not)
+ *   dlogits[i, j] = weight[i] / T (p_j - sum of q_e with ids[i, e] == j)
+ * (dlogits NULL: the loss alone; weight NULL: 1; dlogits as for
+ * tk_logprobs_grad).  A row without entries has loss 0, rmax and rsum 0 and
+ * gradient 0, and its logits are not read; the gradient of a row of weight 0 is
+ * 0.  Teacher logits of NaN or +inf are as such in the row itself.  rmax, rsum
+ * nullable. */
+tk_status tk_distill(tk_ctx *ctx, int n_rows, int vocab, const void *logits, int x_dtype, long ldx, int k, const int32_t *ids,
+                     const float *teacher, float temperature, const float *weight, float *loss, float *rmax, float *rsum,
+                     void *dlogits, int d_dtype, long ldd, void *stream);
+/* The gradient alone, from tk_distill's rmax and rsum. */
+tk_status tk_distill_grad(tk_ctx *ctx, int n_rows, int vocab, const void *logits, int x_dtype, long ldx, int k,
+                          const int32_t *ids, const float *teacher, float temperature, const float *rmax, const float *rsum,
+                          const float *weight, void *dlogits, int d_dtype, long ldd, void *stream);
+
 /* ---- linear layers (tensor cores) --------------------------------------- */
 /* Y[M, N] = X[M, K] . W^T (+ Y if beta == 1).  X dtype per x_dtype with row
  * stride ldx (elements); Y fp32 with row stride ldy.  Block-quantized W is

@@ -131,6 +131,10 @@ SIGNATURES = [
     ("tk_kv_read", _I, [_P, ctypes.POINTER(KvCache), ctypes.POINTER(Seqs), _P, _P, _I, _I, _I, _P]),
     ("tk_kv_attend", _I, [_P, ctypes.POINTER(KvCache), ctypes.POINTER(Seqs), _P, _I, _I, _I, _F, _I, _P, _I, _P]),
     ("tk_draft_verify", _I, [_P, _I, _P, _I, _I, _P, _L, _P, _L, _P, _P, _P, _F, _P, _P, _P, _P]),
+    ("tk_logprobs", _I, [_P, _I, _I, _P, _I, _L, _P, _F, _P, _P, _P, _P, _I, _P, _P, _P]),
+    ("tk_logprobs_grad", _I, [_P, _I, _I, _P, _I, _L, _P, _F, _P, _P, _P, _P, _P, _P, _I, _L, _P]),
+    ("tk_distill", _I, [_P, _I, _I, _P, _I, _L, _I, _P, _P, _F, _P, _P, _P, _P, _P, _I, _L, _P]),
+    ("tk_distill_grad", _I, [_P, _I, _I, _P, _I, _L, _I, _P, _P, _F, _P, _P, _P, _P, _I, _L, _P]),
     ("tk_linear_fwd", _I, [_P, ctypes.POINTER(Weight), _P, _I, _I, _I, _P, _I, _F, _I, _P]),
     ("tk_linear_dx", _I, [_P, ctypes.POINTER(Weight), _P, _I, _I, _I, _P, _I, _F, _I, _P]),
     ("tk_linear_fwd_noalloc", _I, [_P, ctypes.POINTER(Weight), _P, _I, _I, _I, _P, _I, _F, _I, _P]),
@@ -280,6 +284,15 @@ def _check_vector(fn, name, t, n, code, device):
         raise TierkError(TK_ERR_INVALID, f"{fn}: {name} must be {n} contiguous {'float32' if code == DT_F32 else 'int32'} elements")
     if not _reachable(t, device):
         raise TierkError(TK_ERR_INVALID, f"{fn}: {name} is not on device {device}")
+
+
+def _width(fn, name, t, n):
+    """The columns of a contiguous matrix of n rows (None: 0)."""
+    if t is None:
+        return 0
+    if t.dim() != 2 or t.size(0) != n:
+        raise TierkError(TK_ERR_INVALID, f"{fn}: {name} must be a matrix of {n} rows")
+    return t.size(1)
 
 
 _I32 = -1
@@ -453,6 +466,79 @@ class Context:
                                         _ptr(u_accept), _ptr(u_sample), temperature, _ptr(n_accept), _ptr(next_token),
                                         _ptr(logp), _stream(stream)))
         return n_accept, next_token
+
+    # ---- rows of logits ----
+    def logprobs(self, logits, tokens=None, logp=None, entropy=None, rmax=None, rsum=None, top_ids=None, top_logp=None,
+                 temperature=1.0, x_dtype=DT_F32, stream=None):
+        """Log-probabilities of given tokens, entropy and the likeliest tokens of
+        each row of logits [n, vocab] (tk_logprobs); top_ids, top_logp [n, k]."""
+        fn, dev, (n, V) = "tk_logprobs", self.device, logits.shape
+        k = _width(fn, "top_ids", top_ids, n)
+        ldx = _row_stride(fn, "logits", logits, x_dtype, n, V, None, dev)
+        _check_vector(fn, "tokens", tokens, n, _I32, dev)
+        _check_vector(fn, "logp", logp, n, DT_F32, dev)
+        _check_vector(fn, "entropy", entropy, n, DT_F32, dev)
+        _check_vector(fn, "rmax", rmax, n, DT_F32, dev)
+        _check_vector(fn, "rsum", rsum, n, DT_F32, dev)
+        _check_vector(fn, "top_ids", top_ids, n * k, _I32, dev)
+        _check_vector(fn, "top_logp", top_logp, n * k, DT_F32, dev)
+        _check(self.lib.tk_logprobs(self.h, n, V, _ptr(logits), x_dtype, ldx, _ptr(tokens), temperature, _ptr(logp),
+                                    _ptr(entropy), _ptr(rmax), _ptr(rsum), k, _ptr(top_ids), _ptr(top_logp), _stream(stream)))
+        return logp
+
+    def logprobs_grad(self, logits, tokens, rmax, rsum, dlogits, d_logp=None, entropy=None, d_entropy=None, temperature=1.0,
+                      x_dtype=DT_F32, d_dtype=None, stream=None):
+        """dlogits [n, vocab] of d_logp . logp + d_entropy . entropy
+        (tk_logprobs_grad); dlogits may be logits."""
+        fn, dev, (n, V) = "tk_logprobs_grad", self.device, logits.shape
+        d_dtype = x_dtype if d_dtype is None else d_dtype
+        ldx = _row_stride(fn, "logits", logits, x_dtype, n, V, None, dev)
+        ldd = _row_stride(fn, "dlogits", dlogits, d_dtype, n, V, None, dev)
+        _check_vector(fn, "tokens", tokens, n, _I32, dev)
+        _check_vector(fn, "rmax", rmax, n, DT_F32, dev)
+        _check_vector(fn, "rsum", rsum, n, DT_F32, dev)
+        _check_vector(fn, "d_logp", d_logp, n, DT_F32, dev)
+        _check_vector(fn, "entropy", entropy, n, DT_F32, dev)
+        _check_vector(fn, "d_entropy", d_entropy, n, DT_F32, dev)
+        _check(self.lib.tk_logprobs_grad(self.h, n, V, _ptr(logits), x_dtype, ldx, _ptr(tokens), temperature, _ptr(rmax),
+                                         _ptr(rsum), _ptr(d_logp), _ptr(entropy), _ptr(d_entropy), _ptr(dlogits), d_dtype, ldd,
+                                         _stream(stream)))
+        return dlogits
+
+    def distill(self, logits, ids, teacher, loss=None, weight=None, dlogits=None, rmax=None, rsum=None, temperature=1.0,
+                x_dtype=DT_F32, d_dtype=None, stream=None):
+        """Loss of each row of logits [n, vocab] against a teacher's top logits
+        ids, teacher [n, k], and its gradient (tk_distill); dlogits may be logits."""
+        fn, dev, (n, V) = "tk_distill", self.device, logits.shape
+        d_dtype, k = x_dtype if d_dtype is None else d_dtype, _width(fn, "ids", ids, n)
+        ldx = _row_stride(fn, "logits", logits, x_dtype, n, V, None, dev)
+        ldd = _row_stride(fn, "dlogits", dlogits, d_dtype, n, V, None, dev)
+        _check_vector(fn, "ids", ids, n * k, _I32, dev)
+        _check_vector(fn, "teacher", teacher, n * k, DT_F32, dev)
+        _check_vector(fn, "weight", weight, n, DT_F32, dev)
+        _check_vector(fn, "loss", loss, n, DT_F32, dev)
+        _check_vector(fn, "rmax", rmax, n, DT_F32, dev)
+        _check_vector(fn, "rsum", rsum, n, DT_F32, dev)
+        _check(self.lib.tk_distill(self.h, n, V, _ptr(logits), x_dtype, ldx, k, _ptr(ids), _ptr(teacher), temperature,
+                                   _ptr(weight), _ptr(loss), _ptr(rmax), _ptr(rsum), _ptr(dlogits), d_dtype, ldd,
+                                   _stream(stream)))
+        return loss
+
+    def distill_grad(self, logits, ids, teacher, rmax, rsum, dlogits, weight=None, temperature=1.0, x_dtype=DT_F32, d_dtype=None,
+                     stream=None):
+        """The gradient alone, from distill's rmax and rsum (tk_distill_grad)."""
+        fn, dev, (n, V) = "tk_distill_grad", self.device, logits.shape
+        d_dtype, k = x_dtype if d_dtype is None else d_dtype, _width(fn, "ids", ids, n)
+        ldx = _row_stride(fn, "logits", logits, x_dtype, n, V, None, dev)
+        ldd = _row_stride(fn, "dlogits", dlogits, d_dtype, n, V, None, dev)
+        _check_vector(fn, "ids", ids, n * k, _I32, dev)
+        _check_vector(fn, "teacher", teacher, n * k, DT_F32, dev)
+        _check_vector(fn, "rmax", rmax, n, DT_F32, dev)
+        _check_vector(fn, "rsum", rsum, n, DT_F32, dev)
+        _check_vector(fn, "weight", weight, n, DT_F32, dev)
+        _check(self.lib.tk_distill_grad(self.h, n, V, _ptr(logits), x_dtype, ldx, k, _ptr(ids), _ptr(teacher), temperature,
+                                        _ptr(rmax), _ptr(rsum), _ptr(weight), _ptr(dlogits), d_dtype, ldd, _stream(stream)))
+        return dlogits
 
     # ---- reduce-scatter over peer memory (multi-GPU) ----
     def comm_init(self, rank: int, world: int, recv_bytes: int) -> bytes:

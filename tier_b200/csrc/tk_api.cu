@@ -735,6 +735,104 @@ tk_status tk_draft_verify(tk_ctx* ctx, int n_seqs, const int32_t* row_start, int
                                temperature, n_accept, next, logp, static_cast<cudaStream_t>(stream));
 }
 
+// ---- rows of logits -------------------------------------------------------
+static int dt_bytes(int dtype) {
+    return dtype == TK_DT_F32 ? 4 : dtype == TK_DT_F16 || dtype == TK_DT_BF16 ? 2 : 0;
+}
+// The logits, and the gradient where there is one (d_dtype >= 0).  In place
+// means the very same rows; other rows may share memory with the logits' only
+// as other columns of one matrix.
+static tk_status rows_check(const std::string& fn, tk_ctx* ctx, int n_rows, int vocab, const void* x, int x_dtype, long ldx,
+                            float temperature, void* dx, int d_dtype, long ldd, RowArgs& r) {
+    const int xb = dt_bytes(x_dtype), db = dx ? dt_bytes(d_dtype) : 0;
+    if (vocab <= 0) return fail(TK_ERR_INVALID, fn + ": empty vocabulary");
+    if (vocab > (1 << 23)) return fail(TK_ERR_UNSUPPORTED, fn + ": vocabulary beyond 2^23");
+    if (!x) return fail(TK_ERR_INVALID, fn + ": null pointer");
+    if (!xb || (dx && !db)) return fail(TK_ERR_INVALID, fn + ": unknown element type");
+    if (!(temperature >= 1e-4f && temperature <= 1e4f)) return fail(TK_ERR_INVALID, fn + ": temperature must be 1e-4 to 1e4");
+    if (ldx < vocab || (dx && ldd < vocab)) return fail(TK_ERR_INVALID, fn + ": row stride too small");
+    const uintptr_t a = reinterpret_cast<uintptr_t>(x), b = reinterpret_cast<uintptr_t>(dx);
+    if (a % xb || (dx && b % db)) return fail(TK_ERR_INVALID, fn + ": rows off their elements' boundary");
+    const unsigned __int128 sa = (unsigned __int128)ldx * xb, wa = (unsigned __int128)vocab * xb;
+    const unsigned __int128 sb = (unsigned __int128)ldd * db, wb = (unsigned __int128)vocab * db;
+    if (sa * n_rows > INT64_MAX || sb * n_rows > INT64_MAX) return fail(TK_ERR_INVALID, fn + ": rows beyond any memory");
+    if (dx && a < b + sb * (n_rows - 1) + wb && b < a + sa * (n_rows - 1) + wa) {
+        const bool same = a == b && xb == db && x_dtype == d_dtype && (ldx == ldd || n_rows == 1);
+        const unsigned __int128 off = b >= a ? (b - a) % sa : (sa - (a - b) % sa) % sa;   // dx's column in the logits' rows
+        if (!same && !(sa == sb && off >= wa && off + wb <= sa)) return fail(TK_ERR_INVALID, fn + ": gradient overlaps the logits");
+    }
+    r = RowArgs{n_rows, vocab, x, ldx, (float)(1.4426950408889634 / (double)temperature), (float)(1.0 / (double)temperature), dx,
+                ldd, ctx->status};
+    return TK_OK;
+}
+
+tk_status tk_logprobs(tk_ctx* ctx, int n_rows, int vocab, const void* logits, int x_dtype, long ldx, const int32_t* tokens,
+                      float temperature, float* logp, float* entropy, float* rmax, float* rsum, int top_k, int32_t* top_ids,
+                      float* top_logp, void* stream) {
+    if (!ctx) return fail(TK_ERR_INVALID, "tk_logprobs: null context");
+    if (n_rows < 0) return fail(TK_ERR_INVALID, "tk_logprobs: bad row count");
+    if (n_rows == 0) return TK_OK;
+    RowArgs r;
+    tk_status st = rows_check("tk_logprobs", ctx, n_rows, vocab, logits, x_dtype, ldx, temperature, nullptr, -1, 0, r);
+    if (st != TK_OK) return st;
+    if (logp && !tokens) return fail(TK_ERR_INVALID, "tk_logprobs: log-probabilities of no tokens");
+    if (top_k < 0 || top_k > TK_TOP_MAX || top_k > vocab)
+        return fail(TK_ERR_INVALID, "tk_logprobs: top_k must be 0 to TK_TOP_MAX, and no more than the vocabulary");
+    if (top_k ? !top_ids : top_ids || top_logp) return fail(TK_ERR_INVALID, "tk_logprobs: top_ids and top_k do not fit");
+    return launch_logprobs(ctx, r, x_dtype, tokens, logp, entropy, rmax, rsum, top_k, top_ids, top_logp,
+                           static_cast<cudaStream_t>(stream));
+}
+
+tk_status tk_logprobs_grad(tk_ctx* ctx, int n_rows, int vocab, const void* logits, int x_dtype, long ldx, const int32_t* tokens,
+                           float temperature, const float* rmax, const float* rsum, const float* d_logp, const float* entropy,
+                           const float* d_entropy, void* dlogits, int d_dtype, long ldd, void* stream) {
+    if (!ctx) return fail(TK_ERR_INVALID, "tk_logprobs_grad: null context");
+    if (n_rows < 0) return fail(TK_ERR_INVALID, "tk_logprobs_grad: bad row count");
+    if (n_rows == 0) return TK_OK;
+    if (!dlogits || !rmax || !rsum) return fail(TK_ERR_INVALID, "tk_logprobs_grad: null pointer");
+    RowArgs r;
+    tk_status st = rows_check("tk_logprobs_grad", ctx, n_rows, vocab, logits, x_dtype, ldx, temperature, dlogits, d_dtype, ldd, r);
+    if (st != TK_OK) return st;
+    if (!d_logp && !d_entropy) return fail(TK_ERR_INVALID, "tk_logprobs_grad: neither gradient is given");
+    if (d_logp && !tokens) return fail(TK_ERR_INVALID, "tk_logprobs_grad: log-probabilities of no tokens");
+    if (d_entropy && !entropy) return fail(TK_ERR_INVALID, "tk_logprobs_grad: the entropy's gradient needs the entropy");
+    return launch_logprobs_grad(ctx, r, x_dtype, tokens, rmax, rsum, entropy, d_logp, d_entropy, d_dtype,
+                                static_cast<cudaStream_t>(stream));
+}
+
+static tk_status teacher_check(const std::string& fn, int k, const int32_t* ids, const float* teacher) {
+    if (k <= 0 || k > TK_TOP_MAX) return fail(TK_ERR_INVALID, fn + ": k must be 1 to TK_TOP_MAX");
+    if (!ids || !teacher) return fail(TK_ERR_INVALID, fn + ": null pointer");
+    return TK_OK;
+}
+
+tk_status tk_distill(tk_ctx* ctx, int n_rows, int vocab, const void* logits, int x_dtype, long ldx, int k, const int32_t* ids,
+                     const float* teacher, float temperature, const float* weight, float* loss, float* rmax, float* rsum,
+                     void* dlogits, int d_dtype, long ldd, void* stream) {
+    if (!ctx) return fail(TK_ERR_INVALID, "tk_distill: null context");
+    if (n_rows < 0) return fail(TK_ERR_INVALID, "tk_distill: bad row count");
+    if (n_rows == 0) return TK_OK;
+    RowArgs r;
+    tk_status st = rows_check("tk_distill", ctx, n_rows, vocab, logits, x_dtype, ldx, temperature, dlogits, d_dtype, ldd, r);
+    if (st == TK_OK) st = teacher_check("tk_distill", k, ids, teacher);
+    if (st != TK_OK) return st;
+    return launch_distill(ctx, r, x_dtype, k, ids, teacher, weight, loss, rmax, rsum, d_dtype, static_cast<cudaStream_t>(stream));
+}
+
+tk_status tk_distill_grad(tk_ctx* ctx, int n_rows, int vocab, const void* logits, int x_dtype, long ldx, int k,
+                          const int32_t* ids, const float* teacher, float temperature, const float* rmax, const float* rsum,
+                          const float* weight, void* dlogits, int d_dtype, long ldd, void* stream) {
+    if (!ctx) return fail(TK_ERR_INVALID, "tk_distill_grad: null context");
+    if (n_rows < 0) return fail(TK_ERR_INVALID, "tk_distill_grad: bad row count");
+    if (n_rows == 0) return TK_OK;
+    if (!dlogits || !rmax || !rsum) return fail(TK_ERR_INVALID, "tk_distill_grad: null pointer");
+    RowArgs r;
+    tk_status st = rows_check("tk_distill_grad", ctx, n_rows, vocab, logits, x_dtype, ldx, temperature, dlogits, d_dtype, ldd, r);
+    if (st == TK_OK) st = teacher_check("tk_distill_grad", k, ids, teacher);
+    if (st != TK_OK) return st;
+    return launch_distill_grad(ctx, r, x_dtype, k, ids, teacher, rmax, rsum, weight, d_dtype, static_cast<cudaStream_t>(stream));
+}
+
 tk_status tk_linear_fwd(tk_ctx* ctx, const tk_weight* W, const void* X, int x_dtype, int M, int ldx, float* Y, int ldy,
                         float beta, int products, void* stream) {
     return linear(ctx, W, X, x_dtype, M, ldx, Y, ldy, beta, products, static_cast<cudaStream_t>(stream), false);

@@ -209,6 +209,26 @@ tk_status launch_draft_verify(tk_ctx* ctx, int n_seqs, const int32_t* row_start,
                               const float* u_accept, const float* u_sample, float temperature, int32_t* n_accept,
                               int32_t* next, float* logp, cudaStream_t s);
 
+// ---- tk_logprobs.cu, tk_distill.cu: rows of logits (arguments checked) ----
+struct RowArgs {              // what they have in common
+    int n_rows, vocab;
+    const void* x;            // logits
+    long ldx;
+    float c, inv_t;           // log2(e) / temperature, 1 / temperature
+    void* dx;                 // their gradient
+    long ldd;
+    int* status;
+};
+tk_status launch_logprobs(tk_ctx* ctx, const RowArgs& r, int x_dtype, const int32_t* tokens, float* logp, float* entropy,
+                          float* rmax, float* rsum, int top_k, int32_t* top_ids, float* top_logp, cudaStream_t s);
+tk_status launch_logprobs_grad(tk_ctx* ctx, const RowArgs& r, int x_dtype, const int32_t* tokens, const float* rmax,
+                               const float* rsum, const float* entropy, const float* d_logp, const float* d_entropy,
+                               int d_dtype, cudaStream_t s);
+tk_status launch_distill(tk_ctx* ctx, const RowArgs& r, int x_dtype, int k, const int32_t* ids, const float* teacher,
+                         const float* weight, float* loss, float* rmax, float* rsum, int d_dtype, cudaStream_t s);
+tk_status launch_distill_grad(tk_ctx* ctx, const RowArgs& r, int x_dtype, int k, const int32_t* ids, const float* teacher,
+                              const float* rmax, const float* rsum, const float* weight, int d_dtype, cudaStream_t s);
+
 // ---- tk_quant.cu: quantizers byte-exact with the reference's CPU ones ----
 tk_status launch_quantize(tk_ctx* ctx, int qtype, const float* x, long ldx, int rows, int cols, uint8_t* out,
                           size_t rb, cudaStream_t s);
