@@ -2,6 +2,7 @@
 // the arguments of the operators on them (tk_logprobs.cu, tk_distill.cu).
 #pragma once
 #include "tk_device.cuh"
+#include "tk_f32x2.cuh"
 #include "tk_internal.h"
 
 namespace tk {
@@ -60,12 +61,172 @@ __device__ __forceinline__ float rw_block_max(float v, float* part) {   // NaN i
     return v;
 }
 
-// m, S = sum 2^y and, relative to it, A = sum 2^y y of a whole row (the same in
-// every thread); a row that holds NaN, +inf or nothing above -inf: S = NaN.
+// ---------------------------------------------------------------------------
+// A row in units of eight logits on their own boundary (32 bytes of fp32, 16
+// of the 16-bit types: one load each).  What lies before the first boundary
+// and behind the last unit, 14 logits at most, are the row's ends.
+// ---------------------------------------------------------------------------
+template <class XT> struct RwUnit {                // 16-bit types
+    static constexpr int WORDS = 4, BATCH = 8;     // registers of a unit; units that a thread holds at once
+    uint32_t w[4];
+    __device__ __forceinline__ void load(const XT* p) {
+        asm volatile("ld.global.L1::no_allocate.v4.b32 {%0,%1,%2,%3}, [%4];"
+                     : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "l"(p) : "memory");
+    }
+    __device__ __forceinline__ f32x2 two(int i) const;     // logits 2 i, 2 i + 1
+    __device__ __forceinline__ void lowest();              // all -inf
+    __device__ __forceinline__ float max() const;          // NaN is passed over
+};
+template <> struct RwUnit<float> {
+    static constexpr int WORDS = 8, BATCH = 4;
+    uint32_t w[8];
+    __device__ __forceinline__ void load(const float* p) {
+        asm volatile("ld.global.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                     : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+                     : "l"(p) : "memory");
+    }
+    __device__ __forceinline__ f32x2 two(int i) const { return pack2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1])); }
+    __device__ __forceinline__ void lowest() {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = 0xff800000u;
+    }
+    __device__ __forceinline__ float max() const {
+        float m = __uint_as_float(w[0]);
+#pragma unroll
+        for (int i = 1; i < 8; ++i) m = fmaxf(m, __uint_as_float(w[i]));
+        return m;
+    }
+};
+template <> __device__ __forceinline__ f32x2 RwUnit<__nv_bfloat16>::two(int i) const {
+    return pack2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+}
+template <> __device__ __forceinline__ f32x2 RwUnit<__half>::two(int i) const {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+    return pack2(f.x, f.y);
+}
+template <> __device__ __forceinline__ void RwUnit<__nv_bfloat16>::lowest() { w[0] = w[1] = w[2] = w[3] = 0xff80ff80u; }
+template <> __device__ __forceinline__ void RwUnit<__half>::lowest() { w[0] = w[1] = w[2] = w[3] = 0xfc00fc00u; }
+template <> __device__ __forceinline__ float RwUnit<__nv_bfloat16>::max() const {
+    uint32_t a, b;
+    asm("max.bf16x2 %0, %1, %2;" : "=r"(a) : "r"(w[0]), "r"(w[1]));
+    asm("max.bf16x2 %0, %1, %2;" : "=r"(b) : "r"(w[2]), "r"(w[3]));
+    asm("max.bf16x2 %0, %1, %2;" : "=r"(a) : "r"(a), "r"(b));
+    return fmaxf(__uint_as_float(a << 16), __uint_as_float(a & 0xffff0000u));
+}
+template <> __device__ __forceinline__ float RwUnit<__half>::max() const {
+    uint32_t a, b;
+    asm("max.f16x2 %0, %1, %2;" : "=r"(a) : "r"(w[0]), "r"(w[1]));
+    asm("max.f16x2 %0, %1, %2;" : "=r"(b) : "r"(w[2]), "r"(w[3]));
+    asm("max.f16x2 %0, %1, %2;" : "=r"(a) : "r"(a), "r"(b));
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&a));
+    return fmaxf(f.x, f.y);
+}
+
+// The part of a row that one block of a cluster takes: units [0, n) from x.
+template <class XT>
+struct RwPart {
+    const XT* x;              // its first unit
+    int first;                // that unit's place in the row
+    int n;
+    __device__ __forceinline__ RwPart(const XT* row, int vocab, int rank, int parts) {
+        const int off = (int)(reinterpret_cast<uintptr_t>(row) / sizeof(XT)) & 7, head = min((8 - off) & 7, vocab);
+        const int units = (vocab - head) / 8, each = ((units + parts - 1) / parts + 31) & ~31;   // (whole 128-byte lines)
+        const int u0 = min(rank * each, units);
+        first = head + 8 * u0;
+        x = row + first;
+        n = min(each, units - u0);
+    }
+};
+// The row's ends: places of them, end i's place.
+template <class XT>
+struct RwEnds {
+    int head, skip, n;
+    __device__ __forceinline__ RwEnds(const XT* row, int vocab) {
+        const int off = (int)(reinterpret_cast<uintptr_t>(row) / sizeof(XT)) & 7;
+        head = min((8 - off) & 7, vocab);
+        skip = (vocab - head) / 8 * 8;
+        n = vocab - skip;
+    }
+    __device__ __forceinline__ int place(int i) const { return i < head ? i : i + skip; }
+};
+
+// Running sums of one thread.  m moves only when a batch of logits holds a
+// larger one; s and a are sums of at most a few batches before they go, in 64
+// bits, to the totals, which have a reference of their own.
+template <bool ENT>
+struct RwSums {
+    float m = RW_LOWEST, s = 0.0f, a = 0.0f, M = RW_LOWEST;
+    double S = 0.0, A = 0.0;
+    __device__ __forceinline__ void raise(float to, float c) {
+        const float d = fmaxf((m - to) * c, RW_LOW), f = rw_exp2(d);
+        if (ENT) a = f * fmaf(s, d, a);
+        s *= f;
+        m = to;
+    }
+    __device__ __forceinline__ void flush(float c) {
+        const float d = fmaxf((M - m) * c, RW_LOW);
+        const double f = rw_exp2(d);
+        if (ENT) A = f * (A + S * d) + a;
+        S = f * S + s;
+        M = m;
+        s = a = 0.0f;
+    }
+    // Two logits: weights to s2, weight times exponent to a2.
+    static __device__ __forceinline__ void two(f32x2 x, f32x2 nm, f32x2 c, f32x2& s2, f32x2& a2) {
+        const f32x2 y = mul2(add2(x, nm), c);
+        float y0, y1;
+        unpack2(y, y0, y1);
+        if (ENT) {
+            y0 = rw_max_nan(y0, RW_LOW);
+            y1 = rw_max_nan(y1, RW_LOW);
+        }
+        const f32x2 e = pack2(rw_exp2(y0), rw_exp2(y1));
+        s2 = add2(s2, e);
+        if (ENT) a2 = fma2(e, pack2(y0, y1), a2);
+    }
+    template <class U, int N>
+    __device__ __forceinline__ void batch(const U (&u)[N], f32x2 c) {     // none above m
+        const f32x2 nm = pack2(-m, -m);
+        f32x2 s2[2] = {0, 0}, a2[2] = {0, 0};
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) two(u[j].two(i), nm, c, s2[i & 1], a2[i & 1]);
+        float p, q;
+        unpack2(add2(s2[0], s2[1]), p, q);
+        s += p + q;
+        if (ENT) {
+            unpack2(add2(a2[0], a2[1]), p, q);
+            a += p + q;
+        }
+    }
+};
+
+// m, S and A of all parts brought together: threads of a block, blocks of a
+// cluster.  A row that holds NaN or +inf has S = NaN by its arithmetic.
 struct RwStat {
     float m;
     double s, a;
 };
+__device__ __forceinline__ RwStat rw_to_max(const RwStat& v, float m, float c) {
+    const float d = fmaxf((v.m - m) * c, RW_LOW);
+    const double f = rw_exp2(d);
+    return RwStat{m, f * v.s, f * (v.a + v.s * d)};
+}
+template <bool ENT>
+__device__ __forceinline__ RwStat rw_warp_join(RwStat v, float c) {
+    float m = v.m;
+    for (int i = 16; i; i >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, i));
+    v = rw_to_max(v, m, c);
+    for (int i = 16; i; i >>= 1) {
+        v.s += __shfl_xor_sync(~0u, v.s, i);
+        if (ENT) v.a += __shfl_xor_sync(~0u, v.a, i);
+    }
+    return v;
+}
+
+// m, S = sum 2^y and, relative to it, A = sum 2^y y of a whole row (the same in
+// every thread); a row that holds NaN, +inf or nothing above -inf: S = NaN.
 template <class XT>
 __device__ __forceinline__ RwStat rw_stats(const XT* x, int vocab, float c, double* dpart, float* fpart) {
     float m = RW_LOWEST;
