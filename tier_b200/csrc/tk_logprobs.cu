@@ -5,10 +5,11 @@
 
 namespace tk {
 
-constexpr int LP_GROUPS = 8;          // groups of logits a thread keeps the largest of
+constexpr int LP_GROUPS = 16;         // groups of logits a thread keeps the largest of
 constexpr int LP_KEEP = 2048;         // candidates a block can hold
-constexpr int LP_MARGIN = 64;         // and hands on beyond top_k
-constexpr int LP_CLUSTER = 16;        // blocks of a row at most
+constexpr int LP_SORT = 2 * RW_THREADS;   // and puts in order by counting
+constexpr int LP_AHEAD = 4;           // units on their way when groups are looked through again
+constexpr int LP_CLUSTER = 8;         // blocks of a row at most
 
 struct LpArgs {
     RowArgs r;
@@ -18,7 +19,7 @@ struct LpArgs {
     int32_t* top_ids;
     float* top_logp;
     int parts;                // blocks of a row (a cluster)
-    int batches;              // batches of a group
+    int shift;                // 2^shift batches make a group
     bool fine;                // a group is one unit
 };
 
@@ -27,6 +28,7 @@ __device__ __forceinline__ uint32_t lp_order(float x) {
     const uint32_t b = __float_as_uint(x + 0.0f);
     return b ^ ((int)b < 0 ? ~0u : 0x80000000u);
 }
+constexpr uint32_t LP_NOTHING = 0x007fffffu;       // of -inf
 __device__ __forceinline__ float lp_value(uint32_t o) { return __uint_as_float(o ^ ((int)o < 0 ? 0x80000000u : ~0u)); }
 // Order of candidates: larger logits first, then lower places; no two alike.
 __device__ __forceinline__ unsigned long long lp_key(uint32_t order, int place) {
@@ -38,6 +40,9 @@ struct LpTop {
     float big[LP_GROUPS][RW_THREADS];              // each group's largest logit
     unsigned long long keep[LP_KEEP];              // candidates
     uint16_t list[LP_GROUPS * RW_THREADS];         // groups to look through again
+    uint32_t low[RW_WARPS], high[RW_WARPS];
+    int before[TK_TOP_MAX];                        // of each of the block's largest: how many of all are before it
+    int peers[LP_CLUSTER];                         // candidates of the cluster's blocks (which follow this)
     int part[2][RW_WARPS];
     int n, listed;
 };
@@ -83,73 +88,105 @@ __device__ __noinline__ unsigned long long lp_thin(LpTop& t, int k, int& turn) {
 }
 
 // The block's candidates: a set that holds the top_k largest logits of its part
-// (or all).  With each group's largest known, the top_k-th largest of these is
-// a bound that top_k logits reach: only groups that reach it are looked
-// through again, about top_k of them, whatever the row looks like; rows of
-// many equal logits can make it more.  Candidates that do not fit are thinned
-// on the way.
+// (or all).  With v0 and v1, the largest logits of two halves of each thread's,
+// a bound is found that top_k of these reach, so top_k logits do; only groups
+// that reach it are looked through again, little more than top_k of them for
+// logits in any order.  (256 or 512 numbers instead of every group's: one
+// counting barrier a bit.)  Rows of many equal logits can make it more:
+// candidates that do not fit are thinned on the way.
 template <class XT>
-__device__ void lp_search(LpTop& t, const LpArgs& a, const XT* row, const RwPart<XT>& p, bool ends) {
+__device__ __forceinline__ void lp_search(LpTop& t, const LpArgs& a, const XT* row, const RwPart<XT>& p, bool ends, float v0, float v1) {
     constexpr int NB = RwUnit<XT>::BATCH;
     const int tid = threadIdx.x, k = a.top_k;
     const int batches = (p.n + RW_THREADS * NB - 1) / (RW_THREADS * NB);
-    const int groups = a.fine ? batches * NB : (batches + a.batches - 1) / a.batches;   // a thread's
-    int turn = 0;
+    const int groups = a.fine ? batches * NB : (batches + (1 << a.shift) - 1) >> a.shift;   // a thread's
     if (tid == 0) t.n = t.listed = 0;
-    uint32_t o[LP_GROUPS];
-#pragma unroll
-    for (int g = 0; g < LP_GROUPS; ++g) o[g] = g < groups ? lp_order(t.big[g][tid]) : 0;
-    uint32_t bound = 0;                            // enough groups reach it, and not many too many
-    for (int bit = 31; bit >= 0; --bit) {
-        const uint32_t to = bound | 1u << bit;
-        int c = 0;
-#pragma unroll
-        for (int g = 0; g < LP_GROUPS; ++g) c += o[g] >= to;
-        c = lp_count(t, c, turn);
-        if (c >= k) bound = to;
-        if (c >= k && c <= k + k / 8 + 4) break;
+    const bool both = k > RW_THREADS / 2;          // (256 of 256 would be no bound)
+    const uint32_t o0 = lp_order(both ? v0 : fmaxf(v0, v1)), o1 = both ? lp_order(v1) : 0;
+    uint32_t low = __reduce_min_sync(~0u, min(o0 > LP_NOTHING ? o0 : ~0u, o1 > LP_NOTHING ? o1 : ~0u));
+    uint32_t high = __reduce_max_sync(~0u, max(o0, o1));
+    if ((tid & 31) == 0) {
+        t.low[tid >> 5] = low;
+        t.high[tid >> 5] = high;
     }
-#pragma unroll
-    for (int g = 0; g < LP_GROUPS; ++g)
-        if (g < groups && o[g] >= bound) t.list[atomicAdd(&t.listed, 1)] = (uint16_t)(g * RW_THREADS + tid);
     __syncthreads();
-    if (ends && tid < 16) {
-        const RwEnds<XT> e(row, a.r.vocab);
-        if (tid < e.n) {
-            const int j = e.place(tid);
-            t.keep[atomicAdd(&t.n, 1)] = lp_key(lp_order(rw_float(row[j])), j);
+#pragma unroll
+    for (int w = 0; w < RW_WARPS; ++w) {
+        low = min(low, t.low[w]);
+        high = max(high, t.high[w]);
+    }
+    const auto reach = [&](uint32_t to) {
+        const int c = __syncthreads_count(o0 >= to);
+        return both ? c + __syncthreads_count(o1 >= to) : c;
+    };
+    // from the highest bit in which they differ; 0 where those above -inf are few
+    uint32_t bound = 0;
+    if (low <= high && reach(low) >= k) {
+        const int bits = 32 - __clz(low ^ high);
+        bound = bits < 32 ? low >> bits << bits : 0;
+        for (int bit = bits - 1; bit >= 0; --bit) {
+            const uint32_t to = bound | 1u << bit;
+            const int c = reach(to);
+            if (c < k) continue;
+            bound = to;
+            if (c <= k + k / 8 + 4) break;
         }
     }
+    const float least_x = bound ? lp_value(bound) : -INFINITY;
+    uint32_t mine = 0;
+#pragma unroll
+    for (int g = 0; g < LP_GROUPS; ++g)
+        if (g < groups && t.big[g][tid] >= least_x) mine |= 1u << g;
+    if (mine) {
+        int at = atomicAdd(&t.listed, __popc(mine));
+        do {
+            t.list[at++] = (uint16_t)((__ffs(mine) - 1) * RW_THREADS + tid);
+        } while (mine &= mine - 1);
+    }
+    __syncthreads();
+    const RwEnds<XT> e(row, a.r.vocab);
+    if (ends && tid < e.n) t.keep[atomicAdd(&t.n, 1)] = lp_key(lp_order(rw_float(row[e.place(tid)])), e.place(tid));
     // unit i of the listed groups
-    const int each = a.fine ? 1 : a.batches * NB, total = t.listed * each;
+    const int step = a.fine ? 0 : a.shift + (NB == 4 ? 2 : 3), total = t.listed << step;
     const auto unit_of = [&](int i) {
-        const int g = t.list[i / each], who = g % RW_THREADS, part = g / RW_THREADS, in = i % each;
-        return (a.fine ? part : part * each + in) * RW_THREADS + who;
+        const int g = t.list[i >> step], who = g % RW_THREADS, part = g / RW_THREADS;
+        return ((part << step) + (i & ((1 << step) - 1))) * RW_THREADS + who;
     };
     bool full = false;
-    for (int i = tid; i < total && !full; i += RW_THREADS) {
-        const int u = unit_of(i);
-        if (u >= p.n) continue;
-        RwUnit<XT> w;
-        w.load(p.x + 8L * u);
+    for (int i0 = tid; i0 < total && !full; i0 += LP_AHEAD * RW_THREADS) {
+        RwUnit<XT> w[LP_AHEAD];
+        int u[LP_AHEAD];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            float x[2];
-            unpack2(w.two(e), x[0], x[1]);
+        for (int q = 0; q < LP_AHEAD; ++q) {
+            u[q] = i0 + q * RW_THREADS < total ? unit_of(i0 + q * RW_THREADS) : p.n;
+            if (u[q] < p.n) w[q].load(p.x + 8L * u[q]);
+        }
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-                if (lp_order(x[h]) >= bound) {
-                    const int at = atomicAdd(&t.n, 1);
-                    if (at < LP_KEEP) t.keep[at] = lp_key(lp_order(x[h]), p.first + 8 * u + 2 * e + h);
-                    full |= at >= LP_KEEP;
-                }
+        for (int q = 0; q < LP_AHEAD; ++q) {
+            if (u[q] >= p.n || !(w[q].max() >= least_x)) continue;
+            uint32_t reached = 0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                float x[2];
+                unpack2(w[q].two(j / 2), x[0], x[1]);
+                reached |= (x[j & 1] >= least_x ? 1u : 0u) << j;
+            }
+            int at = atomicAdd(&t.n, __popc(reached));
+            full |= at + __popc(reached) > LP_KEEP;
+            if (!full) {
+                const XT* from = p.x + 8L * u[q];
+                do {
+                    const int j = __ffs(reached) - 1;
+                    t.keep[at++] = lp_key(lp_order(rw_float(from[j])), p.first + 8 * u[q] + j);
+                } while (reached &= reached - 1);
+            }
         }
     }
     if (__syncthreads_or(full)) {                  // too many: once more, thinned on the way
         unsigned long long least = (unsigned long long)bound << 32;
+        int turn = 0;
         if (tid == 0) t.n = 0;
         __syncthreads();
-        const RwEnds<XT> e(row, a.r.vocab);
         if (ends && tid < e.n) t.keep[atomicAdd(&t.n, 1)] = lp_key(lp_order(rw_float(row[e.place(tid)])), e.place(tid));
         __syncthreads();
         for (int i0 = 0; i0 < total; i0 += RW_THREADS) {
@@ -165,7 +202,21 @@ __device__ void lp_search(LpTop& t, const LpArgs& a, const XT* row, const RwPart
             }
         }
     }
-    if (t.n > k + LP_MARGIN) lp_thin(t, k, turn);
+    if (t.n > LP_SORT) {
+        int turn = 0;
+        lp_thin(t, k, turn);
+    }
+}
+
+// How many of `list` (n, largest first) are before `key`.
+__device__ __forceinline__ int lp_before(const unsigned long long* list, int n, unsigned long long key) {
+    int lo = 0;
+    while (lo < n) {
+        const int mid = (lo + n) >> 1;
+        if (list[mid] > key) lo = mid + 1;
+        else n = mid;
+    }
+    return lo;
 }
 
 // The same variable of another block of the cluster.
@@ -183,7 +234,7 @@ template <class XT, bool ENT, bool TOP>
 __global__ void __launch_bounds__(RW_THREADS, 4) lp_kernel(const LpArgs a) {
     constexpr int NB = RwUnit<XT>::BATCH;
     extern __shared__ __align__(16) char lp_smem[];
-    __shared__ RwStat join[RW_WARPS], part;
+    __shared__ RwStat join[RW_WARPS], parts[LP_CLUSTER];
     LpTop& t = *reinterpret_cast<LpTop*>(lp_smem);                                       // TOP
     const size_t row = blockIdx.x / a.parts;
     const int tid = threadIdx.x, vocab = a.r.vocab, rank = blockIdx.x % a.parts, k = a.top_k;
@@ -204,6 +255,7 @@ __global__ void __launch_bounds__(RW_THREADS, 4) lp_kernel(const LpArgs a) {
         }
         return;
     }
+    if (a.parts > 1) cluster_arrive();
     const XT* x = static_cast<const XT*>(a.r.x) + row * a.r.ldx;
     const float given = a.logp ? rw_float(x[token]) : 0.0f;
     const RwPart<XT> p(x, vocab, rank, a.parts);
@@ -223,7 +275,7 @@ __global__ void __launch_bounds__(RW_THREADS, 4) lp_kernel(const LpArgs a) {
         }
     }
     const f32x2 c2 = pack2(c, c);
-    float big = -INFINITY;
+    float big = -INFINITY, v0 = -INFINITY, v1 = -INFINITY;
     int in = 0, g = 0;
     for (int u0 = 0; u0 < p.n; u0 += RW_THREADS * NB) {
         RwUnit<XT> u[NB];
@@ -242,41 +294,74 @@ __global__ void __launch_bounds__(RW_THREADS, 4) lp_kernel(const LpArgs a) {
 #pragma unroll
         for (int j = 0; j < NB; ++j) {
             const float v = u[j].max();
-            if (TOP && a.fine) t.big[g + j][tid] = v;
+            if (TOP && a.fine) {
+                t.big[g + j][tid] = v;
+                if (j & 1) v1 = fmaxf(v1, v);
+                else v0 = fmaxf(v0, v);
+            }
             top = fmaxf(top, v);
         }
         if (top > sums.m) sums.raise(top, c);
         sums.batch(u, c2);
         big = fmaxf(big, top);
-        if (++in == a.batches) {
-            if (TOP && !a.fine) t.big[g++][tid] = big;
-            if (TOP && a.fine) g += NB;
+        if (++in % 16 == 0) sums.flush(c);         // (at most 16 batches are added in fp32)
+        if (in == 1 << a.shift) {
+            if (TOP) {
+                if (a.fine) g += NB;
+                else {
+                    t.big[g][tid] = big;
+                    if (g++ & 1) v1 = fmaxf(v1, big);
+                    else v0 = fmaxf(v0, big);
+                }
+            }
             big = -INFINITY;
             in = 0;
             sums.flush(c);
         }
     }
-    if (TOP && !a.fine && in) t.big[g][tid] = big;
+    if (TOP && !a.fine && in) {
+        t.big[g][tid] = big;
+        if (g & 1) v1 = fmaxf(v1, big);
+        else v0 = fmaxf(v0, big);
+    }
     sums.flush(c);
     const RwStat w = rw_warp_join<ENT>(RwStat{sums.M, sums.S, sums.A}, c);
     if ((tid & 31) == 0) join[tid >> 5] = w;
     __syncthreads();
-    const auto joined = [&](auto get, int n) {     // n of them, the same in every thread
-        RwStat v{RW_LOWEST, 0.0, 0.0};
-        for (int i = 0; i < n; ++i) v.m = fmaxf(v.m, get(i).m);
-        for (int i = 0; i < n; ++i) {
-            const RwStat o = rw_to_max(get(i), v.m, c);
-            v.s += o.s;
-            v.a += o.a;
-        }
-        return v;
-    };
-    RwStat st = joined([&](int i) { return join[i]; }, RW_WARPS);
-    if (TOP) lp_search(t, a, x, p, ends);
+    const RwStat none{RW_LOWEST, 0.0, 0.0};
+    const int lane = tid & 31;
+    RwStat st = rw_warp_join<ENT>(lane < RW_WARPS ? join[lane] : none, c);   // (in every warp)
+    if (TOP) {
+        lp_search(t, a, x, p, ends, v0, v1);
+        // the block's largest, in order: a candidate's place is the number of those
+        // before it, counted by 1 to 8 threads
+        const int n = t.n, sh = n <= 32 ? 3 : n <= 64 ? 2 : n <= 128 ? 1 : 0, i = tid >> sh;
+        const unsigned long long key = i < n ? t.keep[i] : 0, key2 = tid + RW_THREADS < n ? t.keep[tid + RW_THREADS] : 0;
+        int at = 0, at2 = 0;
+#pragma unroll 4
+        for (int j = tid & ((1 << sh) - 1); j < n; j += 1 << sh) at += t.keep[j] > key;
+        for (int b = 1 << sh >> 1; b; b >>= 1) at += __shfl_xor_sync(~0u, at, b);
+        if (n > RW_THREADS)
+            for (int j = 0; j < n; ++j) at2 += t.keep[j] > key2;
+        __syncthreads();
+        if (key && at < k && (tid & ((1 << sh) - 1)) == 0) t.keep[at] = key;
+        if (key2 && at2 < k) t.keep[at2] = key2;
+        if (tid == 0) t.n = min(n, k);
+        if (tid < k) t.before[tid] = a.parts > 1 ? 0 : tid;
+        __syncthreads();
+    }
+    // every block gets all blocks' sums and lists
+    unsigned long long* lists = reinterpret_cast<unsigned long long*>(lp_smem + sizeof(LpTop));
     if (a.parts > 1) {
-        if (tid == 0) part = st;
+        cluster_wait();                            // (all have begun)
+        if (tid < a.parts) {
+            *lp_peer(&parts[rank], tid) = st;
+            if (TOP) *lp_peer(&t.peers[rank], tid) = t.n;
+        }
+        if (TOP && tid >> 5 < a.parts)
+            for (int i = lane; i < t.n; i += 32) lp_peer(lists + rank * k, tid >> 5)[i] = t.keep[i];
         cluster_sync();
-        st = joined([&](int i) { return *lp_peer(&part, i); }, a.parts);
+        st = rw_warp_join<ENT>(lane < a.parts ? parts[lane] : none, c);
     }
     if (st.s == 0.0) st.s = (double)NAN;           // nothing above -inf
     const bool bad = st.s != st.s;
@@ -297,35 +382,23 @@ __global__ void __launch_bounds__(RW_THREADS, 4) lp_kernel(const LpArgs a) {
                 if (lp) lp[i] = NAN;
             }
         } else {
-            // a candidate's place in the row's order: how many are before it, in all blocks
-            const unsigned long long* all = t.keep;
-            int n = t.n;
+            const int n = t.n;
             if (a.parts > 1) {
-                unsigned long long* got = reinterpret_cast<unsigned long long*>(lp_smem + sizeof(LpTop));
-                n = 0;
-                for (int r = 0; r < a.parts; ++r) {
-                    const LpTop& o = *lp_peer(&t, r);
-                    const int m = o.n;
-                    for (int i = tid; i < m; i += RW_THREADS) got[n + i] = o.keep[i];
-                    n += m;
+                // before[i]: the sum of what each block has before the own i-th
+                for (int i = tid; i < n * a.parts; i += RW_THREADS) {
+                    const int r = i / n, j = i - r * n;
+                    const int before = lp_before(lists + r * k, t.peers[r], t.keep[j]);
+                    if (before) atomicAdd(&t.before[j], before);
                 }
                 __syncthreads();
-                all = got;
             }
-            for (int i = tid >> 5; i < t.n; i += RW_WARPS) {
-                const unsigned long long key = t.keep[i];
-                int before = 0;
-                for (int j = tid & 31; j < n; j += 32) before += all[j] > key;
-                before = __reduce_add_sync(~0u, before);
-                if (before < k && (tid & 31) == 0) {
-                    ids[before] = (int)~(uint32_t)key;
-                    if (lp) lp[before] = (float)(((double)lp_value((uint32_t)(key >> 32)) - st.m) * a.r.inv_t - lns);
-                }
+            if (tid < n && t.before[tid] < k) {
+                const unsigned long long key = t.keep[tid];
+                ids[t.before[tid]] = (int)~(uint32_t)key;
+                if (lp) lp[t.before[tid]] = (float)(((double)lp_value((uint32_t)(key >> 32)) - st.m) * a.r.inv_t - lns);
             }
         }
     }
-    __syncwarp();
-    if (a.parts > 1) cluster_sync();               // no block ends while another reads its memory
 }
 
 struct LgArgs {
@@ -364,33 +437,27 @@ __global__ void __launch_bounds__(RW_THREADS) lg_kernel(const LgArgs a) {
     });
 }
 
-// Blocks of a row: enough that the batch fills the GPU, parts of 2^19 logits at
-// most and of a batch of units at least.
-static int lp_parts(const tk_ctx* ctx, int n_rows, int vocab) {
+// Blocks of a row, for few rows: 8192 logits each at least.
+static int lp_parts(const tk_ctx* ctx, int n_rows, int vocab, bool top) {
+    const long most = top ? ctx->num_sms : 4L * ctx->num_sms;
     int parts = 1;
-    while (parts < LP_CLUSTER && (vocab / parts > 1 << 19 || ((long)n_rows * parts < 4L * ctx->num_sms && vocab / parts > 8192)))
-        parts *= 2;
+    while (parts < LP_CLUSTER && 2L * n_rows * parts <= most && vocab / (2 * parts) >= 8192) parts *= 2;
     return parts;
 }
 
 template <class XT, bool ENT, bool TOP>
 static cudaError_t launch_lp(const tk_ctx* ctx, LpArgs& a, cudaStream_t s) {
-    a.parts = lp_parts(ctx, a.r.n_rows, a.r.vocab);
+    a.parts = lp_parts(ctx, a.r.n_rows, a.r.vocab, TOP);
     const int per = RW_THREADS * RwUnit<XT>::BATCH;
     const int units = ((a.r.vocab / 8 + a.parts - 1) / a.parts + 31) & ~31, batches = (units + per - 1) / per;
     a.fine = batches * RwUnit<XT>::BATCH <= LP_GROUPS;
-    a.batches = a.fine ? 1 : (batches + LP_GROUPS - 1) / LP_GROUPS;
+    while (!a.fine && batches > LP_GROUPS << a.shift) ++a.shift;
     int smem = TOP ? (int)sizeof(LpTop) : 0;
-    if (TOP && a.parts > 1) smem += a.parts * (a.top_k + LP_MARGIN) * (int)sizeof(unsigned long long);
+    if (TOP && a.parts > 1) smem += a.parts * a.top_k * (int)sizeof(unsigned long long);
     const auto kern = lp_kernel<XT, ENT, TOP>;
-    static std::atomic<uint64_t> attr_smem{0}, attr_size{0};
-    constexpr int MOST = (int)sizeof(LpTop) + LP_CLUSTER * (TK_TOP_MAX + LP_MARGIN) * (int)sizeof(unsigned long long);
-    cudaError_t e = smem_attr_once(kern, MOST, ctx->device, attr_smem);
-    const uint64_t bit = 1ull << (ctx->device & 63);
-    if (e == cudaSuccess && !(attr_size.load(std::memory_order_relaxed) & bit)) {   // more than 8 blocks: on request
-        e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-        if (e == cudaSuccess) attr_size.fetch_or(bit);
-    }
+    static std::atomic<uint64_t> attr_smem{0};
+    constexpr int MOST = (int)sizeof(LpTop) + LP_CLUSTER * TK_TOP_MAX * (int)sizeof(unsigned long long);
+    const cudaError_t e = TOP ? smem_attr_once(kern, MOST, ctx->device, attr_smem) : cudaSuccess;
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)((long)a.r.n_rows * a.parts));
@@ -407,7 +474,7 @@ static cudaError_t launch_lp(const tk_ctx* ctx, LpArgs& a, cudaStream_t s) {
 }
 tk_status launch_logprobs(tk_ctx* ctx, const RowArgs& r, int x_dtype, const int32_t* tokens, float* logp, float* entropy,
                           float* rmax, float* rsum, int top_k, int32_t* top_ids, float* top_logp, cudaStream_t s) {
-    LpArgs a{r, tokens, logp, entropy, rmax, rsum, top_k, top_ids, top_logp, 1, 1, false};
+    LpArgs a{r, tokens, logp, entropy, rmax, rsum, top_k, top_ids, top_logp, 1, 0, false};
     ProfScope ps(ctx, s, PK_LMHEAD);
     ctx->launches += 1;
     const auto with = [&](auto x) {

@@ -279,8 +279,6 @@ __device__ __forceinline__ unsigned long long ld_cluster_u64(uint32_t addr) {
     asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(addr) : "memory");
     return v;
 }
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
 // One row's parts joined by a warp (all lanes return it).
 __device__ __forceinline__ DvStat dv_row(const DvArgs& a, size_t row) {
