@@ -5,10 +5,11 @@
 
 namespace tk {
 
-constexpr int LP_GROUPS = 16;         // groups of logits a thread keeps the largest of
-constexpr int LP_KEEP = 2048;         // candidates a block can hold
+constexpr int LP_SLOTS = 16;          // for the largest logits of a thread's batches
+constexpr int LP_LIST = 1024;         // units that can be listed to be looked through again
+constexpr int LP_KEEP = 1024;         // candidates a block can hold
 constexpr int LP_SORT = 2 * RW_THREADS;   // and puts in order by counting
-constexpr int LP_AHEAD = 4;           // units on their way when groups are looked through again
+constexpr int LP_AHEAD = 2;           // units on their way when groups are looked through again
 constexpr int LP_CLUSTER = 8;         // blocks of a row at most
 
 struct LpArgs {
@@ -19,8 +20,7 @@ struct LpArgs {
     int32_t* top_ids;
     float* top_logp;
     int parts;                // blocks of a row (a cluster)
-    int shift;                // 2^shift batches make a group
-    bool fine;                // a group is one unit
+    int shift;                // 2^shift batches share a slot
 };
 
 // Order of logits as whole numbers (-0 and 0 are alike).
@@ -37,11 +37,10 @@ __device__ __forceinline__ unsigned long long lp_key(uint32_t order, int place) 
 
 // Shared memory of the search for the largest logits.
 struct LpTop {
-    float big[LP_GROUPS][RW_THREADS];              // each group's largest logit
+    uint2 big[LP_SLOTS][RW_THREADS];               // the largest logit of each unit of a batch, upper 16 bits
     unsigned long long keep[LP_KEEP];              // candidates
-    uint16_t list[LP_GROUPS * RW_THREADS];         // groups to look through again
+    uint16_t list[LP_LIST];                        // slots' units to look through again
     uint32_t low[RW_WARPS], high[RW_WARPS];
-    int before[TK_TOP_MAX];                        // of each of the block's largest: how many of all are before it
     int peers[LP_CLUSTER];                         // candidates of the cluster's blocks (which follow this)
     int part[2][RW_WARPS];
     int n, listed;
@@ -89,17 +88,15 @@ __device__ __noinline__ unsigned long long lp_thin(LpTop& t, int k, int& turn) {
 
 // The block's candidates: a set that holds the top_k largest logits of its part
 // (or all).  With v0 and v1, the largest logits of two halves of each thread's,
-// a bound is found that top_k of these reach, so top_k logits do; only groups
-// that reach it are looked through again, little more than top_k of them for
-// logits in any order.  (256 or 512 numbers instead of every group's: one
-// counting barrier a bit.)  Rows of many equal logits can make it more:
+// a bound is found that top_k of these reach, so top_k logits do (256 or 512
+// numbers, one counting barrier a bit); only units that reach it are read
+// again, little more than top_k of them for logits in any order, a sector of
+// memory each.  Where many logits are alike or the largest stand together,
 // candidates that do not fit are thinned on the way.
 template <class XT>
 __device__ __forceinline__ void lp_search(LpTop& t, const LpArgs& a, const XT* row, const RwPart<XT>& p, bool ends, float v0, float v1) {
-    constexpr int NB = RwUnit<XT>::BATCH;
+    constexpr int N = RwUnit<XT>::N;
     const int tid = threadIdx.x, k = a.top_k;
-    const int batches = (p.n + RW_THREADS * NB - 1) / (RW_THREADS * NB);
-    const int groups = a.fine ? batches * NB : (batches + (1 << a.shift) - 1) >> a.shift;   // a thread's
     if (tid == 0) t.n = t.listed = 0;
     const bool both = k > RW_THREADS / 2;          // (256 of 256 would be no bound)
     const uint32_t o0 = lp_order(both ? v0 : fmaxf(v0, v1)), o1 = both ? lp_order(v1) : 0;
@@ -129,56 +126,69 @@ __device__ __forceinline__ void lp_search(LpTop& t, const LpArgs& a, const XT* r
             const int c = reach(to);
             if (c < k) continue;
             bound = to;
-            if (c <= k + k / 8 + 4) break;
+            if (c <= k + k / 8 + 8) break;
         }
     }
     const float least_x = bound ? lp_value(bound) : -INFINITY;
-    uint32_t mine = 0;
+    if (fmaxf(v0, v1) >= least_x) {
+        const float least_16 = __uint_as_float(__float_as_uint(least_x) & 0xffff0000u);   // (cut off as the slots' numbers are)
+        const int batches = (p.n + RW_THREADS * RW_BATCH - 1) / (RW_THREADS * RW_BATCH);
+        const int slots = (batches + (1 << a.shift) - 1) >> a.shift;
+        unsigned long long hits = 0;               // a bit for each of the thread's numbers
+#pragma unroll 4
+        for (int g = 0; g < slots; ++g) {
+            const uint2 m = t.big[g][tid];
+            const float v[RW_BATCH] = {__uint_as_float(m.x << 16), __uint_as_float(m.x & 0xffff0000u), __uint_as_float(m.y << 16),
+                                       __uint_as_float(m.y & 0xffff0000u)};
+            uint32_t h = 0;
 #pragma unroll
-    for (int g = 0; g < LP_GROUPS; ++g)
-        if (g < groups && t.big[g][tid] >= least_x) mine |= 1u << g;
-    if (mine) {
-        int at = atomicAdd(&t.listed, __popc(mine));
-        do {
-            t.list[at++] = (uint16_t)((__ffs(mine) - 1) * RW_THREADS + tid);
-        } while (mine &= mine - 1);
+            for (int j = 0; j < RW_BATCH; ++j) h |= (v[j] >= least_16 ? 1u : 0u) << j;
+            hits |= (unsigned long long)h << RW_BATCH * g;
+        }
+        int at = atomicAdd(&t.listed, __popcll(hits));
+        for (; hits; hits &= hits - 1, ++at)
+            if (at < LP_LIST) t.list[at] = (uint16_t)((__ffsll(hits) - 1) * RW_THREADS + tid);
     }
     __syncthreads();
     const RwEnds<XT> e(row, a.r.vocab);
-    if (ends && tid < e.n) t.keep[atomicAdd(&t.n, 1)] = lp_key(lp_order(rw_float(row[e.place(tid)])), e.place(tid));
-    // unit i of the listed groups
-    const int step = a.fine ? 0 : a.shift + (NB == 4 ? 2 : 3), total = t.listed << step;
+    const bool end = ends && tid < e.n;
+    if (end) t.keep[atomicAdd(&t.n, 1)] = lp_key(lp_order(rw_float(row[e.place(tid)])), e.place(tid));
+    // the i-th unit to look through: of those listed, or (where they are too many) of all
+    const bool all = t.listed > LP_LIST;
+    const int total = all ? p.n : t.listed << a.shift;
     const auto unit_of = [&](int i) {
-        const int g = t.list[i >> step], who = g % RW_THREADS, part = g / RW_THREADS;
-        return ((part << step) + (i & ((1 << step) - 1))) * RW_THREADS + who;
+        if (all) return i;
+        const int g = t.list[i >> a.shift], who = g % RW_THREADS, j = g / RW_THREADS % RW_BATCH, slot = g / RW_THREADS / RW_BATCH;
+        return (((slot << a.shift) + (i & ((1 << a.shift) - 1))) * RW_BATCH + j) * RW_THREADS + who;
     };
-    bool full = false;
+    bool full = all;
     for (int i0 = tid; i0 < total && !full; i0 += LP_AHEAD * RW_THREADS) {
         RwUnit<XT> w[LP_AHEAD];
         int u[LP_AHEAD];
 #pragma unroll
         for (int q = 0; q < LP_AHEAD; ++q) {
             u[q] = i0 + q * RW_THREADS < total ? unit_of(i0 + q * RW_THREADS) : p.n;
-            if (u[q] < p.n) w[q].load(p.x + 8L * u[q]);
+            if (u[q] < p.n) w[q].load(p.x + (long)N * u[q]);
         }
 #pragma unroll
         for (int q = 0; q < LP_AHEAD; ++q) {
-            if (u[q] >= p.n || !(w[q].max() >= least_x)) continue;
+            if (u[q] >= p.n) continue;
             uint32_t reached = 0;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
+            for (int j = 0; j < N; ++j) {
                 float x[2];
                 unpack2(w[q].two(j / 2), x[0], x[1]);
                 reached |= (x[j & 1] >= least_x ? 1u : 0u) << j;
             }
+            if (!reached) continue;
             int at = atomicAdd(&t.n, __popc(reached));
             full |= at + __popc(reached) > LP_KEEP;
-            if (!full) {
-                const XT* from = p.x + 8L * u[q];
-                do {
-                    const int j = __ffs(reached) - 1;
-                    t.keep[at++] = lp_key(lp_order(rw_float(from[j])), p.first + 8 * u[q] + j);
-                } while (reached &= reached - 1);
+            if (full) continue;
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                float x[2];
+                unpack2(w[q].two(j / 2), x[0], x[1]);
+                if (reached >> j & 1) t.keep[at++] = lp_key(lp_order(x[j & 1]), p.first + N * u[q] + j);
             }
         }
     }
@@ -187,14 +197,18 @@ __device__ __forceinline__ void lp_search(LpTop& t, const LpArgs& a, const XT* r
         int turn = 0;
         if (tid == 0) t.n = 0;
         __syncthreads();
-        if (ends && tid < e.n) t.keep[atomicAdd(&t.n, 1)] = lp_key(lp_order(rw_float(row[e.place(tid)])), e.place(tid));
+        if (end) t.keep[atomicAdd(&t.n, 1)] = lp_key(lp_order(rw_float(row[e.place(tid)])), e.place(tid));
         __syncthreads();
         for (int i0 = 0; i0 < total; i0 += RW_THREADS) {
             const int u = i0 + tid < total ? unit_of(i0 + tid) : p.n;
+            RwUnit<XT> w;
+            w.lowest();
+            if (u < p.n) w.load(p.x + (long)N * u);
+            if (!__syncthreads_or(u < p.n && lp_key(lp_order(w.max()), p.first + N * u) >= least)) continue;
 #pragma unroll 1
-            for (int j = 0; j < 8; ++j) {
+            for (int j = 0; j < N; ++j) {
                 unsigned long long key = 0;
-                if (u < p.n) key = lp_key(lp_order(rw_float(p.x[8L * u + j])), p.first + 8 * u + j);
+                if (u < p.n) key = lp_key(lp_order(rw_float(p.x[(long)N * u + j])), p.first + N * u + j);
                 const int n = t.n, more = lp_count(t, key >= least, turn);     // (n before the barrier: pushes come after it)
                 if (n + more > LP_KEEP) least = lp_thin(t, k, turn);
                 if (key >= least) t.keep[atomicAdd(&t.n, 1)] = key;
@@ -208,15 +222,57 @@ __device__ __forceinline__ void lp_search(LpTop& t, const LpArgs& a, const XT* r
     }
 }
 
-// How many of `list` (n, largest first) are before `key`.
-__device__ __forceinline__ int lp_before(const unsigned long long* list, int n, unsigned long long key) {
-    int lo = 0;
-    while (lo < n) {
-        const int mid = (lo + n) >> 1;
-        if (list[mid] > key) lo = mid + 1;
-        else n = mid;
+// A warp's 32 keys in order, largest first, by compare and exchange.
+__device__ __forceinline__ unsigned long long lp_sort32(unsigned long long v) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int size = 2; size <= 32; size *= 2)
+#pragma unroll
+        for (int d = size / 2; d; d /= 2) {
+            const unsigned long long o = __shfl_xor_sync(~0u, v, d);
+            const bool larger = (lane & d) == 0 ? (lane & size) == 0 : (lane & size) != 0;
+            if ((o > v) == larger) v = o;
+        }
+    return v;
+}
+
+// The t.n <= LP_SORT candidates in order, and no more than k of them: runs of
+// 32 are sorted by a warp each, and a key's place is the sum of what the runs
+// have before it.
+__device__ __forceinline__ void lp_ordered(LpTop& t, int k) {
+    constexpr int EACH = LP_SORT / RW_THREADS;
+    const int tid = threadIdx.x, lane = tid & 31, n = t.n, runs = (n + 31) / 32;
+    unsigned long long key[EACH];
+    int at[EACH];
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+        const int j = i * RW_THREADS + tid;
+        key[i] = 0;
+        if (j - lane >= n) continue;
+        key[i] = lp_sort32(j < n ? t.keep[j] : 0);
+        t.keep[j] = key[i];
     }
-    return lo;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+        at[i] = 0;
+        if (i * RW_THREADS + tid - lane >= n) continue;
+#pragma unroll 4
+        for (int r = 0; r < runs; ++r) {
+            const unsigned long long* run = t.keep + 32 * r;
+            int b = 0;
+#pragma unroll
+            for (int d = 16; d; d /= 2)
+                if (run[b + d - 1] > key[i]) b += d;
+            at[i] += b + (run[b] > key[i] ? 1 : 0);
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < EACH; ++i)
+        if (key[i] && at[i] < k) t.keep[at[i]] = key[i];
+    if (tid == 0) t.n = min(n, k);
+    __syncthreads();
 }
 
 // The same variable of another block of the cluster.
@@ -232,7 +288,7 @@ __device__ __forceinline__ T* lp_peer(T* mine, int rank) {
 // sums and candidates meet in shared memory.
 template <class XT, bool ENT, bool TOP>
 __global__ void __launch_bounds__(RW_THREADS, 4) lp_kernel(const LpArgs a) {
-    constexpr int NB = RwUnit<XT>::BATCH;
+    constexpr int N = RwUnit<XT>::N;
     extern __shared__ __align__(16) char lp_smem[];
     __shared__ RwStat join[RW_WARPS], parts[LP_CLUSTER];
     LpTop& t = *reinterpret_cast<LpTop*>(lp_smem);                                       // TOP
@@ -275,55 +331,45 @@ __global__ void __launch_bounds__(RW_THREADS, 4) lp_kernel(const LpArgs a) {
         }
     }
     const f32x2 c2 = pack2(c, c);
-    float big = -INFINITY, v0 = -INFINITY, v1 = -INFINITY;
-    int in = 0, g = 0;
-    for (int u0 = 0; u0 < p.n; u0 += RW_THREADS * NB) {
-        RwUnit<XT> u[NB];
-        const XT* from = p.x + 8L * (u0 + tid);
-        if (u0 + RW_THREADS * NB <= p.n) {
+    float big[RW_BATCH] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, v0 = -INFINITY, v1 = -INFINITY;
+    int batch = 0, slot = 0;
+    const int share = (1 << a.shift) - 1;
+    const auto store = [&]() {
+        t.big[slot++][tid] = make_uint2(__byte_perm(__float_as_uint(big[0]), __float_as_uint(big[1]), 0x7632),
+                                        __byte_perm(__float_as_uint(big[2]), __float_as_uint(big[3]), 0x7632));
+        v0 = fmaxf(v0, fmaxf(big[0], big[1]));
+        v1 = fmaxf(v1, fmaxf(big[2], big[3]));
+    };
+    for (int u0 = 0; u0 < p.n; u0 += RW_THREADS * RW_BATCH) {
+        RwUnit<XT> u[RW_BATCH];
+        const XT* from = p.x + (long)N * (u0 + tid);
+        if (u0 + RW_THREADS * RW_BATCH <= p.n) {
 #pragma unroll
-            for (int j = 0; j < NB; ++j) u[j].load(from + 8 * RW_THREADS * j);
+            for (int j = 0; j < RW_BATCH; ++j) u[j].load(from + N * RW_THREADS * j);
         } else {
 #pragma unroll
-            for (int j = 0; j < NB; ++j) {
-                if (u0 + j * RW_THREADS + tid < p.n) u[j].load(from + 8 * RW_THREADS * j);
+            for (int j = 0; j < RW_BATCH; ++j) {
+                if (u0 + j * RW_THREADS + tid < p.n) u[j].load(from + N * RW_THREADS * j);
                 else u[j].lowest();
             }
         }
         float top = -INFINITY;
 #pragma unroll
-        for (int j = 0; j < NB; ++j) {
+        for (int j = 0; j < RW_BATCH; ++j) {
             const float v = u[j].max();
-            if (TOP && a.fine) {
-                t.big[g + j][tid] = v;
-                if (j & 1) v1 = fmaxf(v1, v);
-                else v0 = fmaxf(v0, v);
-            }
+            if (TOP) big[j] = fmaxf(big[j], v);
             top = fmaxf(top, v);
         }
         if (top > sums.m) sums.raise(top, c);
         sums.batch(u, c2);
-        big = fmaxf(big, top);
-        if (++in % 16 == 0) sums.flush(c);         // (at most 16 batches are added in fp32)
-        if (in == 1 << a.shift) {
-            if (TOP) {
-                if (a.fine) g += NB;
-                else {
-                    t.big[g][tid] = big;
-                    if (g++ & 1) v1 = fmaxf(v1, big);
-                    else v0 = fmaxf(v0, big);
-                }
-            }
-            big = -INFINITY;
-            in = 0;
-            sums.flush(c);
+        if (++batch % 16 == 0) sums.flush(c);      // (at most 16 batches are added in fp32)
+        if (TOP && (batch & share) == 0) {
+            store();
+#pragma unroll
+            for (int j = 0; j < RW_BATCH; ++j) big[j] = -INFINITY;
         }
     }
-    if (TOP && !a.fine && in) {
-        t.big[g][tid] = big;
-        if (g & 1) v1 = fmaxf(v1, big);
-        else v0 = fmaxf(v0, big);
-    }
+    if (TOP && (batch & share)) store();
     sums.flush(c);
     const RwStat w = rw_warp_join<ENT>(RwStat{sums.M, sums.S, sums.A}, c);
     if ((tid & 31) == 0) join[tid >> 5] = w;
@@ -333,22 +379,7 @@ __global__ void __launch_bounds__(RW_THREADS, 4) lp_kernel(const LpArgs a) {
     RwStat st = rw_warp_join<ENT>(lane < RW_WARPS ? join[lane] : none, c);   // (in every warp)
     if (TOP) {
         lp_search(t, a, x, p, ends, v0, v1);
-        // the block's largest, in order: a candidate's place is the number of those
-        // before it, counted by 1 to 8 threads
-        const int n = t.n, sh = n <= 32 ? 3 : n <= 64 ? 2 : n <= 128 ? 1 : 0, i = tid >> sh;
-        const unsigned long long key = i < n ? t.keep[i] : 0, key2 = tid + RW_THREADS < n ? t.keep[tid + RW_THREADS] : 0;
-        int at = 0, at2 = 0;
-#pragma unroll 4
-        for (int j = tid & ((1 << sh) - 1); j < n; j += 1 << sh) at += t.keep[j] > key;
-        for (int b = 1 << sh >> 1; b; b >>= 1) at += __shfl_xor_sync(~0u, at, b);
-        if (n > RW_THREADS)
-            for (int j = 0; j < n; ++j) at2 += t.keep[j] > key2;
-        __syncthreads();
-        if (key && at < k && (tid & ((1 << sh) - 1)) == 0) t.keep[at] = key;
-        if (key2 && at2 < k) t.keep[at2] = key2;
-        if (tid == 0) t.n = min(n, k);
-        if (tid < k) t.before[tid] = a.parts > 1 ? 0 : tid;
-        __syncthreads();
+        lp_ordered(t, k);
     }
     // every block gets all blocks' sums and lists
     unsigned long long* lists = reinterpret_cast<unsigned long long*>(lp_smem + sizeof(LpTop));
@@ -382,20 +413,28 @@ __global__ void __launch_bounds__(RW_THREADS, 4) lp_kernel(const LpArgs a) {
                 if (lp) lp[i] = NAN;
             }
         } else {
+            // a key's place in the row: the sum of what each block has before it
             const int n = t.n;
-            if (a.parts > 1) {
-                // before[i]: the sum of what each block has before the own i-th
-                for (int i = tid; i < n * a.parts; i += RW_THREADS) {
-                    const int r = i / n, j = i - r * n;
-                    const int before = lp_before(lists + r * k, t.peers[r], t.keep[j]);
-                    if (before) atomicAdd(&t.before[j], before);
+            const unsigned long long key = tid < n ? t.keep[tid] : 0;
+            int at = tid;
+            if (a.parts > 1 && tid < n) {
+                int b[LP_CLUSTER], m[LP_CLUSTER];
+#pragma unroll
+                for (int r = 0; r < LP_CLUSTER; ++r) {
+                    b[r] = 0;
+                    m[r] = r < a.parts ? t.peers[r] : 0;
                 }
-                __syncthreads();
+                for (int d = 1 << (31 - __clz(k)); d; d /= 2)
+#pragma unroll
+                    for (int r = 0; r < LP_CLUSTER; ++r)
+                        if ((lists[min(r, a.parts - 1) * k + min(b[r] + d, k) - 1] > key) & (b[r] + d <= m[r])) b[r] += d;
+                at = 0;
+#pragma unroll
+                for (int r = 0; r < LP_CLUSTER; ++r) at += b[r];
             }
-            if (tid < n && t.before[tid] < k) {
-                const unsigned long long key = t.keep[tid];
-                ids[t.before[tid]] = (int)~(uint32_t)key;
-                if (lp) lp[t.before[tid]] = (float)(((double)lp_value((uint32_t)(key >> 32)) - st.m) * a.r.inv_t - lns);
+            if (tid < n && at < k) {
+                ids[at] = (int)~(uint32_t)key;
+                if (lp) lp[at] = (float)(((double)lp_value((uint32_t)(key >> 32)) - st.m) * a.r.inv_t - lns);
             }
         }
     }
@@ -448,10 +487,9 @@ static int lp_parts(const tk_ctx* ctx, int n_rows, int vocab, bool top) {
 template <class XT, bool ENT, bool TOP>
 static cudaError_t launch_lp(const tk_ctx* ctx, LpArgs& a, cudaStream_t s) {
     a.parts = lp_parts(ctx, a.r.n_rows, a.r.vocab, TOP);
-    const int per = RW_THREADS * RwUnit<XT>::BATCH;
-    const int units = ((a.r.vocab / 8 + a.parts - 1) / a.parts + 31) & ~31, batches = (units + per - 1) / per;
-    a.fine = batches * RwUnit<XT>::BATCH <= LP_GROUPS;
-    while (!a.fine && batches > LP_GROUPS << a.shift) ++a.shift;
+    const int each = ((a.r.vocab / RwUnit<XT>::N + a.parts - 1) / a.parts + 31) & ~31;
+    const int batches = (each + RW_THREADS * RW_BATCH - 1) / (RW_THREADS * RW_BATCH);
+    while (batches > LP_SLOTS << a.shift) ++a.shift;
     int smem = TOP ? (int)sizeof(LpTop) : 0;
     if (TOP && a.parts > 1) smem += a.parts * a.top_k * (int)sizeof(unsigned long long);
     const auto kern = lp_kernel<XT, ENT, TOP>;
@@ -474,7 +512,7 @@ static cudaError_t launch_lp(const tk_ctx* ctx, LpArgs& a, cudaStream_t s) {
 }
 tk_status launch_logprobs(tk_ctx* ctx, const RowArgs& r, int x_dtype, const int32_t* tokens, float* logp, float* entropy,
                           float* rmax, float* rsum, int top_k, int32_t* top_ids, float* top_logp, cudaStream_t s) {
-    LpArgs a{r, tokens, logp, entropy, rmax, rsum, top_k, top_ids, top_logp, 1, 0, false};
+    LpArgs a{r, tokens, logp, entropy, rmax, rsum, top_k, top_ids, top_logp, 1, 0};
     ProfScope ps(ctx, s, PK_LMHEAD);
     ctx->launches += 1;
     const auto with = [&](auto x) {

@@ -62,41 +62,26 @@ __device__ __forceinline__ float rw_block_max(float v, float* part) {   // NaN i
 }
 
 // ---------------------------------------------------------------------------
-// A row in units of eight logits on their own boundary (32 bytes of fp32, 16
-// of the 16-bit types: one load each).  What lies before the first boundary
-// and behind the last unit, 14 logits at most, are the row's ends.
+// A row in units of 32 bytes (8 fp32 logits, 16 of the 16-bit types), one load
+// and one sector of memory each.  What lies before the first boundary and
+// behind the last unit, 30 logits at most, are the row's ends.
 // ---------------------------------------------------------------------------
-template <class XT> struct RwUnit {                // 16-bit types
-    static constexpr int WORDS = 4, BATCH = 8;     // registers of a unit; units that a thread holds at once
-    uint32_t w[4];
+template <class XT>
+struct RwUnit {
+    static constexpr int N = 32 / sizeof(XT);      // logits
+    uint32_t w[8];
     __device__ __forceinline__ void load(const XT* p) {
-        asm volatile("ld.global.L1::no_allocate.v4.b32 {%0,%1,%2,%3}, [%4];"
-                     : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "l"(p) : "memory");
+        asm volatile("ld.global.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                     : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+                     : "l"(p) : "memory");
     }
     __device__ __forceinline__ f32x2 two(int i) const;     // logits 2 i, 2 i + 1
     __device__ __forceinline__ void lowest();              // all -inf
     __device__ __forceinline__ float max() const;          // NaN is passed over
 };
-template <> struct RwUnit<float> {
-    static constexpr int WORDS = 8, BATCH = 4;
-    uint32_t w[8];
-    __device__ __forceinline__ void load(const float* p) {
-        asm volatile("ld.global.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-                     : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
-                     : "l"(p) : "memory");
-    }
-    __device__ __forceinline__ f32x2 two(int i) const { return pack2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1])); }
-    __device__ __forceinline__ void lowest() {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) w[i] = 0xff800000u;
-    }
-    __device__ __forceinline__ float max() const {
-        float m = __uint_as_float(w[0]);
-#pragma unroll
-        for (int i = 1; i < 8; ++i) m = fmaxf(m, __uint_as_float(w[i]));
-        return m;
-    }
-};
+template <> __device__ __forceinline__ f32x2 RwUnit<float>::two(int i) const {
+    return pack2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+}
 template <> __device__ __forceinline__ f32x2 RwUnit<__nv_bfloat16>::two(int i) const {
     return pack2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
 }
@@ -104,47 +89,63 @@ template <> __device__ __forceinline__ f32x2 RwUnit<__half>::two(int i) const {
     const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
     return pack2(f.x, f.y);
 }
-template <> __device__ __forceinline__ void RwUnit<__nv_bfloat16>::lowest() { w[0] = w[1] = w[2] = w[3] = 0xff80ff80u; }
-template <> __device__ __forceinline__ void RwUnit<__half>::lowest() { w[0] = w[1] = w[2] = w[3] = 0xfc00fc00u; }
+template <class XT> __device__ __forceinline__ void RwUnit<XT>::lowest() {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = sizeof(XT) == 4 ? 0xff800000u : 0xff80ff80u;
+}
+template <> __device__ __forceinline__ void RwUnit<__half>::lowest() {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = 0xfc00fc00u;
+}
+template <> __device__ __forceinline__ float RwUnit<float>::max() const {
+    float m = __uint_as_float(w[0]);
+#pragma unroll
+    for (int i = 1; i < 8; ++i) m = fmaxf(m, __uint_as_float(w[i]));
+    return m;
+}
 template <> __device__ __forceinline__ float RwUnit<__nv_bfloat16>::max() const {
-    uint32_t a, b;
-    asm("max.bf16x2 %0, %1, %2;" : "=r"(a) : "r"(w[0]), "r"(w[1]));
-    asm("max.bf16x2 %0, %1, %2;" : "=r"(b) : "r"(w[2]), "r"(w[3]));
-    asm("max.bf16x2 %0, %1, %2;" : "=r"(a) : "r"(a), "r"(b));
-    return fmaxf(__uint_as_float(a << 16), __uint_as_float(a & 0xffff0000u));
+    uint32_t m = w[0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) asm("max.bf16x2 %0, %1, %2;" : "=r"(m) : "r"(m), "r"(w[i]));
+    return fmaxf(__uint_as_float(m << 16), __uint_as_float(m & 0xffff0000u));
 }
 template <> __device__ __forceinline__ float RwUnit<__half>::max() const {
-    uint32_t a, b;
-    asm("max.f16x2 %0, %1, %2;" : "=r"(a) : "r"(w[0]), "r"(w[1]));
-    asm("max.f16x2 %0, %1, %2;" : "=r"(b) : "r"(w[2]), "r"(w[3]));
-    asm("max.f16x2 %0, %1, %2;" : "=r"(a) : "r"(a), "r"(b));
-    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&a));
+    uint32_t m = w[0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) asm("max.f16x2 %0, %1, %2;" : "=r"(m) : "r"(m), "r"(w[i]));
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&m));
     return fmaxf(f.x, f.y);
 }
+constexpr int RW_BATCH = 4;                        // units that a thread holds at once
 
 // The part of a row that one block of a cluster takes: units [0, n) from x.
+template <class XT>
+__device__ __forceinline__ int rw_head(const XT* row, int vocab) {      // logits before the first boundary
+    constexpr int N = RwUnit<XT>::N;
+    return min((int)(-(reinterpret_cast<uintptr_t>(row) / sizeof(XT)) & (N - 1)), vocab);
+}
 template <class XT>
 struct RwPart {
     const XT* x;              // its first unit
     int first;                // that unit's place in the row
     int n;
     __device__ __forceinline__ RwPart(const XT* row, int vocab, int rank, int parts) {
-        const int off = (int)(reinterpret_cast<uintptr_t>(row) / sizeof(XT)) & 7, head = min((8 - off) & 7, vocab);
-        const int units = (vocab - head) / 8, each = ((units + parts - 1) / parts + 31) & ~31;   // (whole 128-byte lines)
-        const int u0 = min(rank * each, units);
-        first = head + 8 * u0;
+        constexpr int N = RwUnit<XT>::N;
+        const int head = rw_head(row, vocab), units = (vocab - head) / N;
+        const int each = ((units + parts - 1) / parts + 31) & ~31, u0 = min(rank * each, units);   // (a warp's loads stay whole)
+        first = head + N * u0;
         x = row + first;
         n = min(each, units - u0);
     }
 };
-// The row's ends: places of them, end i's place.
+// The row's ends: how many, and the place of the i-th.
 template <class XT>
 struct RwEnds {
     int head, skip, n;
     __device__ __forceinline__ RwEnds(const XT* row, int vocab) {
-        const int off = (int)(reinterpret_cast<uintptr_t>(row) / sizeof(XT)) & 7;
-        head = min((8 - off) & 7, vocab);
-        skip = (vocab - head) / 8 * 8;
+        constexpr int N = RwUnit<XT>::N;
+        head = rw_head(row, vocab);
+        skip = (vocab - head) / N * N;
         n = vocab - skip;
     }
     __device__ __forceinline__ int place(int i) const { return i < head ? i : i + skip; }
@@ -184,14 +185,14 @@ struct RwSums {
         s2 = add2(s2, e);
         if (ENT) a2 = fma2(e, pack2(y0, y1), a2);
     }
-    template <class U, int N>
-    __device__ __forceinline__ void batch(const U (&u)[N], f32x2 c) {     // none above m
+    template <class XT>
+    __device__ __forceinline__ void batch(const RwUnit<XT> (&u)[RW_BATCH], f32x2 c) {     // none above m
         const f32x2 nm = pack2(-m, -m);
         f32x2 s2[2] = {0, 0}, a2[2] = {0, 0};
 #pragma unroll
-        for (int j = 0; j < N; ++j)
+        for (int j = 0; j < RW_BATCH; ++j)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) two(u[j].two(i), nm, c, s2[i & 1], a2[i & 1]);
+            for (int i = 0; i < RwUnit<XT>::N / 2; ++i) two(u[j].two(i), nm, c, s2[i & 1], a2[i & 1]);
         float p, q;
         unpack2(add2(s2[0], s2[1]), p, q);
         s += p + q;
