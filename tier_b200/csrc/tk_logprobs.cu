@@ -87,7 +87,7 @@ __device__ __noinline__ unsigned long long lp_thin(LpTop& t, int k, int& turn) {
 }
 
 // The block's candidates: a set that holds the top_k largest logits of its part
-// (or all).  With v0 and v1, the largest logits of two halves of each thread's,
+// (or all).  With v0 and v1, the largest logits of the thread's units' first and second halves,
 // a bound is found that top_k of these reach, so top_k logits do (256 or 512
 // numbers, one counting barrier a bit); only units that reach it are read
 // again, little more than top_k of them for logits in any order, a sector of
@@ -193,7 +193,7 @@ __device__ __forceinline__ void lp_search(LpTop& t, const LpArgs& a, const XT* r
         }
     }
     if (__syncthreads_or(full)) {                  // too many: once more, thinned on the way
-        unsigned long long least = (unsigned long long)bound << 32;
+        unsigned long long least = max((unsigned long long)bound << 32, 1ull);     // (0: no logit)
         int turn = 0;
         if (tid == 0) t.n = 0;
         __syncthreads();
@@ -204,7 +204,7 @@ __device__ __forceinline__ void lp_search(LpTop& t, const LpArgs& a, const XT* r
             RwUnit<XT> w;
             w.lowest();
             if (u < p.n) w.load(p.x + (long)N * u);
-            if (!__syncthreads_or(u < p.n && lp_key(lp_order(w.max()), p.first + N * u) >= least)) continue;
+            if (!__syncthreads_or(u < p.n && lp_key(lp_order(fmaxf(w.max(0), w.max(1))), p.first + N * u) >= least)) continue;
 #pragma unroll 1
             for (int j = 0; j < N; ++j) {
                 unsigned long long key = 0;
@@ -337,8 +337,6 @@ __global__ void __launch_bounds__(RW_THREADS, 4) lp_kernel(const LpArgs a) {
     const auto store = [&]() {
         t.big[slot++][tid] = make_uint2(__byte_perm(__float_as_uint(big[0]), __float_as_uint(big[1]), 0x7632),
                                         __byte_perm(__float_as_uint(big[2]), __float_as_uint(big[3]), 0x7632));
-        v0 = fmaxf(v0, fmaxf(big[0], big[1]));
-        v1 = fmaxf(v1, fmaxf(big[2], big[3]));
     };
     for (int u0 = 0; u0 < p.n; u0 += RW_THREADS * RW_BATCH) {
         RwUnit<XT> u[RW_BATCH];
@@ -356,8 +354,12 @@ __global__ void __launch_bounds__(RW_THREADS, 4) lp_kernel(const LpArgs a) {
         float top = -INFINITY;
 #pragma unroll
         for (int j = 0; j < RW_BATCH; ++j) {
-            const float v = u[j].max();
-            if (TOP) big[j] = fmaxf(big[j], v);
+            const float lo = u[j].max(0), hi = u[j].max(1), v = fmaxf(lo, hi);
+            if (TOP) {
+                v0 = fmaxf(v0, lo);
+                v1 = fmaxf(v1, hi);
+                big[j] = fmaxf(big[j], v);
+            }
             top = fmaxf(top, v);
         }
         if (top > sums.m) sums.raise(top, c);

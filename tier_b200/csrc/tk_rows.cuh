@@ -77,7 +77,7 @@ struct RwUnit {
     }
     __device__ __forceinline__ f32x2 two(int i) const;     // logits 2 i, 2 i + 1
     __device__ __forceinline__ void lowest();              // all -inf
-    __device__ __forceinline__ float max() const;          // NaN is passed over
+    __device__ __forceinline__ float max(int half) const;  // of its first or second half; NaN is passed over
 };
 template <> __device__ __forceinline__ f32x2 RwUnit<float>::two(int i) const {
     return pack2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
@@ -97,22 +97,20 @@ template <> __device__ __forceinline__ void RwUnit<__half>::lowest() {
 #pragma unroll
     for (int i = 0; i < 8; ++i) w[i] = 0xfc00fc00u;
 }
-template <> __device__ __forceinline__ float RwUnit<float>::max() const {
-    float m = __uint_as_float(w[0]);
-#pragma unroll
-    for (int i = 1; i < 8; ++i) m = fmaxf(m, __uint_as_float(w[i]));
-    return m;
+template <> __device__ __forceinline__ float RwUnit<float>::max(int half) const {
+    const float a = fmaxf(__uint_as_float(w[4 * half]), __uint_as_float(w[4 * half + 1]));
+    return fmaxf(fmaxf(a, __uint_as_float(w[4 * half + 2])), __uint_as_float(w[4 * half + 3]));
 }
-template <> __device__ __forceinline__ float RwUnit<__nv_bfloat16>::max() const {
-    uint32_t m = w[0];
+template <> __device__ __forceinline__ float RwUnit<__nv_bfloat16>::max(int half) const {
+    uint32_t m = w[4 * half];
 #pragma unroll
-    for (int i = 1; i < 8; ++i) asm("max.bf16x2 %0, %1, %2;" : "=r"(m) : "r"(m), "r"(w[i]));
+    for (int i = 1; i < 4; ++i) asm("max.bf16x2 %0, %1, %2;" : "=r"(m) : "r"(m), "r"(w[4 * half + i]));
     return fmaxf(__uint_as_float(m << 16), __uint_as_float(m & 0xffff0000u));
 }
-template <> __device__ __forceinline__ float RwUnit<__half>::max() const {
-    uint32_t m = w[0];
+template <> __device__ __forceinline__ float RwUnit<__half>::max(int half) const {
+    uint32_t m = w[4 * half];
 #pragma unroll
-    for (int i = 1; i < 8; ++i) asm("max.f16x2 %0, %1, %2;" : "=r"(m) : "r"(m), "r"(w[i]));
+    for (int i = 1; i < 4; ++i) asm("max.f16x2 %0, %1, %2;" : "=r"(m) : "r"(m), "r"(w[4 * half + i]));
     const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&m));
     return fmaxf(f.x, f.y);
 }
