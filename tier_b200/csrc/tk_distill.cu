@@ -1,8 +1,12 @@
 // tk_distill.cu -- tk_distill, tk_distill_grad: distillation from a teacher's
 // top logits.
+#include <climits>
+#include <type_traits>
 #include "tk_rows.cuh"
 
 namespace tk {
+
+constexpr int DS_CLUSTER = 8;         // blocks of a row at most
 
 struct DsArgs {
     RowArgs r;
@@ -11,103 +15,228 @@ struct DsArgs {
     const float *teacher, *weight;
     float *loss, *rmax, *rsum;
     const float *in_max, *in_sum;     // tk_distill_grad: of the forward pass
+    int parts;                        // blocks of a row
 };
 
-// The teacher's row: its entries' places (-1: none), q and (in the entry's own
-// thread) ln q.  Returns 0: no entry, 1: entries, 2: NaN or +inf among them.
-__device__ __forceinline__ int ds_teacher(const DsArgs& a, size_t row, int* ids, float* q, double& lnq, double* dpart,
-                                          float* fpart) {
+// The teacher's row in shared memory: an entry's place (-1: it does not
+// count) and logit, then q; m, s: of its softmax.
+struct DsTeacher {
+    __align__(16) int ids[TK_TOP_MAX];
+    float t[TK_TOP_MAX], q[TK_TOP_MAX];
+    float m, s;
+};
+// Entries to shared memory.  0: none counts, 1: some do, 2: NaN or +inf among them.
+__device__ __forceinline__ int ds_read(DsTeacher& s, const DsArgs& a, size_t row, bool report) {
     const int tid = threadIdx.x;
     int id = -1;
     float t = -INFINITY;
     if (tid < a.k) {
         id = a.ids[row * a.k + tid];
+        t = a.teacher[row * a.k + tid];
         if (id >= a.r.vocab) {
-            raise_status(a.r.status, DEV_INVALID);
+            if (report) raise_status(a.r.status, DEV_INVALID);
             id = -1;
         }
-        if (id >= 0) t = a.teacher[row * a.k + tid];
-    }
-    const bool bad = !(t < INFINITY);
-    const float m = rw_block_max(fmaxf(t, RW_LOWEST), fpart);
-    const float e = t == -INFINITY ? 0.0f : rw_exp2(rw_exponent(t, m, a.r.c));
-    const double s = rw_block_sum((double)e, dpart);
-    lnq = ((double)t - m) * a.r.inv_t - log(s);
-    if (tid < a.k) {
-        ids[tid] = id;
-        q[tid] = (float)(e / s);
-    }
-    const int any_bad = __syncthreads_or(bad), any = __syncthreads_or(e > 0.0f);
-    return any_bad ? 2 : any ? 1 : 0;
-}
-
-template <class XT, class DT>
-__global__ void __launch_bounds__(RW_THREADS) ds_kernel(const DsArgs a) {
-    __shared__ double dpart[RW_WARPS];
-    __shared__ float fpart[RW_WARPS];
-    __shared__ int ids[TK_TOP_MAX];
-    __shared__ float q[TK_TOP_MAX];
-    const size_t row = blockIdx.x;
-    const int tid = threadIdx.x, vocab = a.r.vocab;
-    const XT* x = static_cast<const XT*>(a.r.x) + row * a.r.ldx;
-    DT* dx = a.r.dx ? static_cast<DT*>(a.r.dx) + row * a.r.ldd : nullptr;
-    double lnq;
-    const int state = ds_teacher(a, row, ids, q, lnq, dpart, fpart);
-    const float w = state ? (a.weight ? a.weight[row] : 1.0f) * a.r.inv_t : 0.0f;
-    RwStat st{0.0f, 0.0, 0.0};
-    if (a.in_max) {
-        st.m = a.in_max[row];
-        st.s = a.in_sum[row];
-        if (state == 2) st.s = (double)NAN;
-        if (state == 2 && tid == 0) raise_status(a.r.status, DEV_INVALID);
-    } else {
-        if (state) st = rw_stats(x, vocab, a.r.c, dpart, fpart);
-        if (state == 2) st.s = (double)NAN;
-        const bool bad = st.s != st.s;
-        double part = 0.0;
-        if (state == 1 && tid < a.k && q[tid] > 0.0f)
-            part = q[tid] * (lnq - (((double)rw_float(x[ids[tid]]) - st.m) * a.r.inv_t - log(st.s)));
-        part = rw_block_sum(part, dpart);
-        if (tid == 0) {
-            if (bad) raise_status(a.r.status, DEV_INVALID);
-            const float none = bad ? NAN : 0.0f;
-            const bool no = !state || bad;
-            if (a.loss) a.loss[row] = no ? none : (float)part;
-            if (a.rmax) a.rmax[row] = no ? none : st.m;
-            if (a.rsum) a.rsum[row] = no ? none : (float)st.s;
+        if (id < 0 || t == -INFINITY) {
+            id = -1;
+            t = -INFINITY;
         }
     }
-    if (!dx) return;
-    if (w == 0.0f) {
-        rw_zero(dx, vocab);
-        return;
+    s.ids[tid] = id;
+    s.t[tid] = t;
+    if (!__syncthreads_or(id >= 0)) return 0;
+    return __syncthreads_or(id >= 0 && !(t < INFINITY)) ? 2 : 1;
+}
+// One warp: q = softmax(t / T).
+__device__ __forceinline__ void ds_softmax(DsTeacher& s, const DsArgs& a) {
+    constexpr int EACH = TK_TOP_MAX / 32;
+    const int lane = threadIdx.x & 31;
+    float t[EACH], m = RW_LOWEST, sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+        t[i] = 32 * i < a.k ? s.t[32 * i + lane] : -INFINITY;
+        m = fmaxf(m, t[i]);
     }
-    if (tid < a.k) q[tid] *= w;
-    __syncthreads();
-    const float f = (float)(w / st.s), m = st.m, c = a.r.c;
-    rw_gradient(x, dx, vocab, ids, q, a.k, [=](float v) { return rw_exp2(rw_exponent(v, m, c)) * f; });
+    for (int i = 16; i; i >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, i));
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+        t[i] = t[i] == -INFINITY ? 0.0f : rw_exp2((t[i] - m) * a.r.c);
+        sum += t[i];
+    }
+    for (int i = 16; i; i >>= 1) sum += __shfl_xor_sync(~0u, sum, i);
+    const float r = 1.0f / sum;
+#pragma unroll
+    for (int i = 0; i < EACH; ++i)
+        if (32 * i < a.k) s.q[32 * i + lane] = t[i] * r;
+    if (lane == 0) {
+        s.m = m;
+        s.s = sum;
+    }
 }
 
+// A cluster of blocks per row, each with one part of it: the sums of the
+// softmax over one reading, the blocks' sums brought together in shared memory;
+// then the gradient over a second, which finds the row in the L2.
 template <class XT, class DT>
-static cudaError_t launch_ds(const DsArgs& a, cudaStream_t s) {
-    ds_kernel<XT, DT><<<a.r.n_rows, RW_THREADS, 0, s>>>(a);
-    return cudaGetLastError();
+__global__ void __launch_bounds__(RW_THREADS, 4) ds_kernel(const DsArgs a) {
+    constexpr bool GRAD = !std::is_same<DT, void>::value;
+    __shared__ DsTeacher t;
+    __shared__ RwStat join[RW_WARPS], parts[DS_CLUSTER];
+    const size_t row = blockIdx.x / a.parts;
+    const int tid = threadIdx.x, lane = tid & 31, vocab = a.r.vocab, rank = blockIdx.x % a.parts;
+    const float c = a.r.c;
+    const XT* x = static_cast<const XT*>(a.r.x) + row * a.r.ldx;
+    const int state = ds_read(t, a, row, rank == 0);
+    if (state == 0) {                              // the whole cluster alike
+        if (rank == 0 && tid == 0) {
+            if (a.loss) a.loss[row] = 0.0f;
+            if (a.rmax) a.rmax[row] = 0.0f;
+            if (a.rsum) a.rsum[row] = 0.0f;
+        }
+        if constexpr (GRAD) rw_zero(static_cast<DT*>(a.r.dx) + row * a.r.ldd, vocab, rank, a.parts);
+        return;
+    }
+    if (a.parts > 1) cluster_arrive();
+    const RwPart<XT> p(x, vocab, rank, a.parts);
+    const bool ends = rank == a.parts - 1;
+    // the listed logits, for the loss: before any gradient is written
+    const float listed = rank == 0 && tid < a.k && t.ids[tid] >= 0 ? rw_float(x[t.ids[tid]]) : 0.0f;
+    RwSums<false> sums;
+    if (ends) {
+        const RwEnds<XT> e(x, vocab);
+        if (tid < e.n) sums.single(rw_float(x[e.place(tid)]), c);
+    }
+    const f32x2 c2 = pack2(c, c);
+    int batch = 0;
+    for (int u0 = 0; u0 < p.n; u0 += RW_THREADS * RW_BATCH) {
+        RwUnit<XT> u[RW_BATCH];
+        rw_batch<XT>(u, p, u0);
+        float top = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < RW_BATCH; ++j) top = fmaxf(top, fmaxf(u[j].max(0), u[j].max(1)));
+        if (top > sums.m) sums.raise(top, c);
+        sums.batch(u, c2);
+        if (++batch % 16 == 0) sums.flush(c);
+    }
+    sums.flush(c);
+    const RwStat w = rw_warp_join<false>(RwStat{sums.M, sums.S, 0.0}, c);
+    if (lane == 0) join[tid >> 5] = w;
+    if (tid < 32) ds_softmax(t, a);
+    __syncthreads();
+    const RwStat none{RW_LOWEST, 0.0, 0.0};
+    RwStat st = rw_warp_join<false>(lane < RW_WARPS ? join[lane] : none, c);   // (in every warp)
+    if (a.parts > 1) {
+        cluster_wait();                            // (all have begun)
+        if (tid < a.parts) *rw_peer(&parts[rank], tid) = st;
+        cluster_sync();
+        st = rw_warp_join<false>(lane < a.parts ? parts[lane] : none, c);
+    }
+    if (st.s == 0.0 || state == 2) st.s = (double)NAN;      // nothing above -inf
+    const bool bad = st.s != st.s;
+    if (rank == 0) {
+        if (tid < a.k) t.t[tid] = (float)(t.q[tid] > 0.0f
+            ? t.q[tid] * (((double)t.t[tid] - t.m) * a.r.inv_t - ((double)listed - st.m) * a.r.inv_t) : 0.0);
+        __syncthreads();
+        if (tid < 32) {
+            double sum = 0.0, qs = 0.0;            // (q adds up to 1 but for its roundings)
+            for (int i = lane; i < a.k; i += 32) {
+                sum += t.t[i];
+                qs += t.q[i];
+            }
+            for (int i = 16; i; i >>= 1) {
+                sum += __shfl_xor_sync(~0u, sum, i);
+                qs += __shfl_xor_sync(~0u, qs, i);
+            }
+            if (lane == 0) {
+                if (bad) raise_status(a.r.status, DEV_INVALID);
+                if (a.loss) a.loss[row] = (float)(sum + qs * (log(st.s) - log((double)t.s)));
+                if (a.rmax) a.rmax[row] = bad ? NAN : st.m;
+                if (a.rsum) a.rsum[row] = (float)st.s;
+            }
+        }
+    }
+    if constexpr (GRAD) {
+        DT* dx = static_cast<DT*>(a.r.dx) + row * a.r.ldd;
+        const float wt = (a.weight ? a.weight[row] : 1.0f) * a.r.inv_t;
+        if (wt == 0.0f) {
+            rw_zero(dx, vocab, rank, a.parts);
+            return;
+        }
+        __syncthreads();                           // (q has been added up)
+        if (tid < a.k) t.q[tid] *= wt;
+        __syncthreads();
+        rw_gradient<XT, DT, false>(x, dx, vocab, p, ends, t.ids, t.q, a.k, RwDense<false>{st.m, c, (float)(wt / st.s), 0.0f});
+    }
+}
+
+// The gradient alone: one pass.
+template <class XT, class DT>
+__global__ void __launch_bounds__(RW_THREADS, 4) dg_kernel(const DsArgs a) {
+    __shared__ DsTeacher t;
+    const size_t row = blockIdx.x / a.parts;
+    const int tid = threadIdx.x, vocab = a.r.vocab, rank = blockIdx.x % a.parts;
+    const XT* x = static_cast<const XT*>(a.r.x) + row * a.r.ldx;
+    DT* dx = static_cast<DT*>(a.r.dx) + row * a.r.ldd;
+    const float wt = (a.weight ? a.weight[row] : 1.0f) * a.r.inv_t, m = a.in_max[row], s = a.in_sum[row];
+    const int state = ds_read(t, a, row, rank == 0);
+    if (state == 2 && rank == 0 && tid == 0) raise_status(a.r.status, DEV_INVALID);
+    if (state == 0 || wt == 0.0f) {
+        rw_zero(dx, vocab, rank, a.parts);
+        return;
+    }
+    if (tid < 32) ds_softmax(t, a);
+    __syncthreads();
+    if (tid < a.k) t.q[tid] *= wt;
+    __syncthreads();
+    rw_gradient<XT, DT, false>(x, dx, vocab, RwPart<XT>(x, vocab, rank, a.parts), rank == a.parts - 1, t.ids, t.q, a.k,
+                               RwDense<false>{m, a.r.c, state == 2 ? NAN : wt / s, 0.0f});
+}
+
+// Blocks of a row: enough for few rows (8192 logits each at least); with a
+// gradient, enough that the rows at work together stay in the L2.
+static int ds_parts(const tk_ctx* ctx, int n_rows, int vocab, int row_bytes, bool grad) {
+    int parts = 1;
+    while (parts < DS_CLUSTER && vocab / (2 * parts) >= 8192 &&
+           (2L * n_rows * parts <= 4L * ctx->num_sms || (grad && 4L * ctx->num_sms / parts * row_bytes > 48L << 20)))
+        parts *= 2;
+    return parts;
+}
+template <class XT, class DT>
+static cudaError_t launch_ds(const tk_ctx* ctx, DsArgs& a, cudaStream_t s) {
+    a.parts = ds_parts(ctx, a.r.n_rows, a.r.vocab, a.r.vocab * (int)sizeof(XT), !std::is_same<DT, void>::value);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)((long)a.r.n_rows * a.parts));
+    cfg.blockDim = dim3(RW_THREADS);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = a.parts;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, ds_kernel<XT, DT>, a);
 }
 tk_status launch_distill(tk_ctx* ctx, const RowArgs& r, int x_dtype, int k, const int32_t* ids, const float* teacher,
                          const float* weight, float* loss, float* rmax, float* rsum, int d_dtype, cudaStream_t s) {
-    const DsArgs a{r, k, ids, teacher, weight, loss, rmax, rsum, nullptr, nullptr};
+    DsArgs a{r, k, ids, teacher, weight, loss, rmax, rsum, nullptr, nullptr, 1};
     ProfScope ps(ctx, s, PK_LMHEAD);
     ctx->launches += 1;
-    return cuda_fail(rw_types(x_dtype, d_dtype, [&](auto x, auto d) { return launch_ds<decltype(x), decltype(d)>(a, s); }),
-                     "distillation launch");
+    const cudaError_t e = r.dx ? rw_types(x_dtype, d_dtype, [&](auto x, auto d) { return launch_ds<decltype(x), decltype(d)>(ctx, a, s); })
+                        : x_dtype == TK_DT_F32 ? launch_ds<float, void>(ctx, a, s)
+                        : x_dtype == TK_DT_F16 ? launch_ds<__half, void>(ctx, a, s) : launch_ds<__nv_bfloat16, void>(ctx, a, s);
+    if (e != cudaSuccess) return cuda_fail(e, "distillation launch");
+    return cuda_fail(cudaGetLastError(), "distillation launch");
 }
 tk_status launch_distill_grad(tk_ctx* ctx, const RowArgs& r, int x_dtype, int k, const int32_t* ids, const float* teacher,
                               const float* rmax, const float* rsum, const float* weight, int d_dtype, cudaStream_t s) {
-    const DsArgs a{r, k, ids, teacher, weight, nullptr, nullptr, nullptr, rmax, rsum};
+    DsArgs a{r, k, ids, teacher, weight, nullptr, nullptr, nullptr, rmax, rsum, 1};
     ProfScope ps(ctx, s, PK_LMHEAD);
     ctx->launches += 1;
-    return cuda_fail(rw_types(x_dtype, d_dtype, [&](auto x, auto d) { return launch_ds<decltype(x), decltype(d)>(a, s); }),
-                     "distillation gradient launch");
+    return cuda_fail(rw_types(x_dtype, d_dtype, [&](auto x, auto d) {
+        a.parts = rw_grad_parts<decltype(x)>(ctx, a.r.n_rows, a.r.vocab);
+        dg_kernel<decltype(x), decltype(d)><<<(unsigned)((long)a.r.n_rows * a.parts), RW_THREADS, 0, s>>>(a);
+        return cudaGetLastError();
+    }), "distillation gradient launch");
 }
 
 }  // namespace tk

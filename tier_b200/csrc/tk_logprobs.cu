@@ -275,20 +275,11 @@ __device__ __forceinline__ void lp_ordered(LpTop& t, int k) {
     __syncthreads();
 }
 
-// The same variable of another block of the cluster.
-template <class T>
-__device__ __forceinline__ T* lp_peer(T* mine, int rank) {
-    T* p;
-    asm("mapa.u64 %0, %1, %2;" : "=l"(p) : "l"(mine), "r"(rank));
-    return p;
-}
-
 // A cluster of blocks per row, each with one part of it.  Every logit is read
 // once, for the sums and for the largest of each group of logits; the blocks'
 // sums and candidates meet in shared memory.
 template <class XT, bool ENT, bool TOP>
 __global__ void __launch_bounds__(RW_THREADS, 4) lp_kernel(const LpArgs a) {
-    constexpr int N = RwUnit<XT>::N;
     extern __shared__ __align__(16) char lp_smem[];
     __shared__ RwStat join[RW_WARPS], parts[LP_CLUSTER];
     LpTop& t = *reinterpret_cast<LpTop*>(lp_smem);                                       // TOP
@@ -319,16 +310,7 @@ __global__ void __launch_bounds__(RW_THREADS, 4) lp_kernel(const LpArgs a) {
     RwSums<ENT> sums;
     if (ends) {
         const RwEnds<XT> e(x, vocab);
-        if (tid < e.n) {
-            const float v = rw_float(x[e.place(tid)]);
-            if (v > sums.m) sums.raise(v, c);
-            f32x2 s2 = 0, a2 = 0;
-            sums.two(pack2(v, -INFINITY), pack2(-sums.m, -sums.m), pack2(c, c), s2, a2);
-            float lo, hi;
-            unpack2(s2, sums.s, hi);
-            unpack2(a2, lo, hi);
-            if (ENT) sums.a = lo;
-        }
+        if (tid < e.n) sums.single(rw_float(x[e.place(tid)]), c);
     }
     const f32x2 c2 = pack2(c, c);
     float big[RW_BATCH] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, v0 = -INFINITY, v1 = -INFINITY;
@@ -340,17 +322,7 @@ __global__ void __launch_bounds__(RW_THREADS, 4) lp_kernel(const LpArgs a) {
     };
     for (int u0 = 0; u0 < p.n; u0 += RW_THREADS * RW_BATCH) {
         RwUnit<XT> u[RW_BATCH];
-        const XT* from = p.x + (long)N * (u0 + tid);
-        if (u0 + RW_THREADS * RW_BATCH <= p.n) {
-#pragma unroll
-            for (int j = 0; j < RW_BATCH; ++j) u[j].load(from + N * RW_THREADS * j);
-        } else {
-#pragma unroll
-            for (int j = 0; j < RW_BATCH; ++j) {
-                if (u0 + j * RW_THREADS + tid < p.n) u[j].load(from + N * RW_THREADS * j);
-                else u[j].lowest();
-            }
-        }
+        rw_batch<XT>(u, p, u0);
         float top = -INFINITY;
 #pragma unroll
         for (int j = 0; j < RW_BATCH; ++j) {
@@ -388,11 +360,11 @@ __global__ void __launch_bounds__(RW_THREADS, 4) lp_kernel(const LpArgs a) {
     if (a.parts > 1) {
         cluster_wait();                            // (all have begun)
         if (tid < a.parts) {
-            *lp_peer(&parts[rank], tid) = st;
-            if (TOP) *lp_peer(&t.peers[rank], tid) = t.n;
+            *rw_peer(&parts[rank], tid) = st;
+            if (TOP) *rw_peer(&t.peers[rank], tid) = t.n;
         }
         if (TOP && tid >> 5 < a.parts)
-            for (int i = lane; i < t.n; i += 32) lp_peer(lists + rank * k, tid >> 5)[i] = t.keep[i];
+            for (int i = lane; i < t.n; i += 32) rw_peer(lists + rank * k, tid >> 5)[i] = t.keep[i];
         cluster_sync();
         st = rw_warp_join<ENT>(lane < a.parts ? parts[lane] : none, c);
     }
@@ -446,36 +418,36 @@ struct LgArgs {
     RowArgs r;
     const int32_t* tokens;
     const float *rmax, *rsum, *entropy, *d_logp, *d_entropy;
+    int parts;                // blocks of a row
 };
 
-template <class XT, class DT>
-__global__ void __launch_bounds__(RW_THREADS) lg_kernel(const LgArgs a) {
-    const size_t row = blockIdx.x;
-    const int vocab = a.r.vocab;
+// One pass: every logit is read once, every gradient written once.
+template <class XT, class DT, bool ENT>
+__global__ void __launch_bounds__(RW_THREADS, 4) lg_kernel(const LgArgs a) {
+    __shared__ __align__(16) int ids[4];
+    __shared__ float sub[4];
+    const size_t row = blockIdx.x / a.parts;
+    const int vocab = a.r.vocab, rank = blockIdx.x % a.parts;
     const XT* x = static_cast<const XT*>(a.r.x) + row * a.r.ldx;
     DT* dx = static_cast<DT*>(a.r.dx) + row * a.r.ldd;
     const int token = a.tokens ? a.tokens[row] : 0;
-    const float dl = a.d_logp ? a.d_logp[row] : 0.0f, de = a.d_entropy ? a.d_entropy[row] : 0.0f;
-    if (token >= vocab && threadIdx.x == 0) raise_status(a.r.status, DEV_INVALID);
+    const float dl = a.d_logp ? a.d_logp[row] : 0.0f, de = ENT ? a.d_entropy[row] : 0.0f;
+    const float m = a.rmax[row], s = a.rsum[row], h = ENT ? a.entropy[row] : 0.0f;
+    if (token >= vocab && rank == 0 && threadIdx.x == 0) raise_status(a.r.status, DEV_INVALID);
     if (token < 0 || token >= vocab || (dl == 0.0f && de == 0.0f)) {
-        rw_zero(dx, vocab);
+        rw_zero(dx, vocab, rank, a.parts);
         return;
     }
-    const float m = a.rmax[row], c = a.r.c, s = a.rsum[row];
-    // p (-dl - de (ln p + H)) / T = 2^y (f + g y)
-    const float h = a.d_entropy ? a.entropy[row] - logf(s) : 0.0f;
-    const float f = -(dl + de * h) / s * a.r.inv_t, g = -de * 0.69314718f / s * a.r.inv_t;
-    __shared__ int ids[1];
-    __shared__ float sub[1];
-    if (threadIdx.x == 0) {
-        ids[0] = a.d_logp ? token : -1;
-        sub[0] = -dl * a.r.inv_t;
+    // -p (dl + de (ln p + H)) / T with ln p = y ln 2 - ln S
+    const float r = a.r.inv_t / s;
+    const RwDense<ENT> dense{m, a.r.c, -(ENT ? fmaf(de, h - logf(s), dl) : dl) * r, -de * 0.69314718f * r};
+    if (threadIdx.x < 4) {
+        ids[threadIdx.x] = threadIdx.x == 0 && a.d_logp ? token : -1;
+        sub[threadIdx.x] = -dl * a.r.inv_t;
     }
     __syncthreads();
-    rw_gradient(x, dx, vocab, ids, sub, 1, [=](float v) {
-        const float y = rw_exponent(v, m, c);
-        return rw_exp2(y) * (f + g * y);
-    });
+    const RwPart<XT> p(x, vocab, rank, a.parts);
+    rw_gradient<XT, DT, ENT>(x, dx, vocab, p, rank == a.parts - 1, ids, sub, 1, dense);
 }
 
 // Blocks of a row, for few rows: 8192 logits each at least.
@@ -528,17 +500,20 @@ tk_status launch_logprobs(tk_ctx* ctx, const RowArgs& r, int x_dtype, const int3
 }
 
 template <class XT, class DT>
-static cudaError_t launch_lg(const LgArgs& a, cudaStream_t s) {
-    lg_kernel<XT, DT><<<a.r.n_rows, RW_THREADS, 0, s>>>(a);
+static cudaError_t launch_lg(const tk_ctx* ctx, LgArgs& a, cudaStream_t s) {
+    a.parts = rw_grad_parts<XT>(ctx, a.r.n_rows, a.r.vocab);
+    const unsigned grid = (unsigned)((long)a.r.n_rows * a.parts);
+    if (a.d_entropy) lg_kernel<XT, DT, true><<<grid, RW_THREADS, 0, s>>>(a);
+    else lg_kernel<XT, DT, false><<<grid, RW_THREADS, 0, s>>>(a);
     return cudaGetLastError();
 }
 tk_status launch_logprobs_grad(tk_ctx* ctx, const RowArgs& r, int x_dtype, const int32_t* tokens, const float* rmax,
                                const float* rsum, const float* entropy, const float* d_logp, const float* d_entropy,
                                int d_dtype, cudaStream_t s) {
-    const LgArgs a{r, tokens, rmax, rsum, entropy, d_logp, d_entropy};
+    LgArgs a{r, tokens, rmax, rsum, entropy, d_logp, d_entropy, 1};
     ProfScope ps(ctx, s, PK_LMHEAD);
     ctx->launches += 1;
-    return cuda_fail(rw_types(x_dtype, d_dtype, [&](auto x, auto d) { return launch_lg<decltype(x), decltype(d)>(a, s); }),
+    return cuda_fail(rw_types(x_dtype, d_dtype, [&](auto x, auto d) { return launch_lg<decltype(x), decltype(d)>(ctx, a, s); }),
                      "log-probability gradient launch");
 }
 

@@ -136,6 +136,22 @@ struct RwPart {
         n = min(each, units - u0);
     }
 };
+// A batch: units u0 + tid, and RW_THREADS apart; -inf beyond the part.
+template <class XT>
+__device__ __forceinline__ void rw_batch(RwUnit<XT> (&u)[RW_BATCH], const RwPart<XT>& p, int u0) {
+    constexpr int N = RwUnit<XT>::N;
+    const XT* from = p.x + (long)N * (u0 + (int)threadIdx.x);
+    if (u0 + RW_THREADS * RW_BATCH <= p.n) {
+#pragma unroll
+        for (int j = 0; j < RW_BATCH; ++j) u[j].load(from + N * RW_THREADS * j);
+    } else {
+#pragma unroll
+        for (int j = 0; j < RW_BATCH; ++j) {
+            if (u0 + j * RW_THREADS + (int)threadIdx.x < p.n) u[j].load(from + N * RW_THREADS * j);
+            else u[j].lowest();
+        }
+    }
+}
 // The row's ends: how many, and the place of the i-th.
 template <class XT>
 struct RwEnds {
@@ -183,6 +199,15 @@ struct RwSums {
         s2 = add2(s2, e);
         if (ENT) a2 = fma2(e, pack2(y0, y1), a2);
     }
+    // One logit, before any other.
+    __device__ __forceinline__ void single(float v, float c) {
+        if (v > m) raise(v, c);
+        f32x2 s2 = 0, a2 = 0;
+        float none;
+        two(pack2(v, -INFINITY), pack2(-m, -m), pack2(c, c), s2, a2);
+        unpack2(s2, s, none);
+        if (ENT) unpack2(a2, a, none);
+    }
     template <class XT>
     __device__ __forceinline__ void batch(const RwUnit<XT> (&u)[RW_BATCH], f32x2 c) {     // none above m
         const f32x2 nm = pack2(-m, -m);
@@ -200,6 +225,14 @@ struct RwSums {
         }
     }
 };
+
+// The same variable of another block of the cluster.
+template <class T>
+__device__ __forceinline__ T* rw_peer(T* mine, int rank) {
+    T* p;
+    asm("mapa.u64 %0, %1, %2;" : "=l"(p) : "l"(mine), "r"(rank));
+    return p;
+}
 
 // m, S and A of all parts brought together: threads of a block, blocks of a
 // cluster.  A row that holds NaN or +inf has S = NaN by its arithmetic.
@@ -226,47 +259,159 @@ __device__ __forceinline__ RwStat rw_warp_join(RwStat v, float c) {
 
 // m, S = sum 2^y and, relative to it, A = sum 2^y y of a whole row (the same in
 // every thread); a row that holds NaN, +inf or nothing above -inf: S = NaN.
-template <class XT>
-__device__ __forceinline__ RwStat rw_stats(const XT* x, int vocab, float c, double* dpart, float* fpart) {
-    float m = RW_LOWEST;
-    for (int j = threadIdx.x; j < vocab; j += RW_THREADS) m = fmaxf(m, rw_float(x[j]));
-    m = rw_block_max(m, fpart);
-    double s = 0.0, a = 0.0;
-    for (int j = threadIdx.x; j < vocab; j += RW_THREADS) {
-        const float v = rw_float(x[j]), y = rw_exponent(v, m, c), e = v == -INFINITY ? 0.0f : rw_exp2(y);
-        s += e;
-        a += e * y;
-    }
-    s = rw_block_sum(s, dpart);
-    a = rw_block_sum(a, dpart);
-    if (s == 0.0) s = (double)NAN;                 // nothing above -inf
-    return RwStat{m, s, a};
+// Two numbers, rounded once, as a pair of DT.
+template <class DT> __device__ __forceinline__ uint32_t rw_pair(f32x2 v);
+template <> __device__ __forceinline__ uint32_t rw_pair<__nv_bfloat16>(f32x2 v) {
+    float lo, hi;
+    uint32_t r;
+    unpack2(v, lo, hi);
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+template <> __device__ __forceinline__ uint32_t rw_pair<__half>(f32x2 v) {
+    float lo, hi;
+    uint32_t r;
+    unpack2(v, lo, hi);
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+__device__ __forceinline__ void rw_store(void* p, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("st.global.L1::no_allocate.v4.b32 [%4], {%0,%1,%2,%3};" ::"r"(a), "r"(b), "r"(c), "r"(d), "l"(p) : "memory");
+}
+__device__ __forceinline__ void rw_store(void* p, const uint32_t* w) {
+    asm volatile("st.global.L1::no_allocate.v8.b32 [%8], {%0,%1,%2,%3,%4,%5,%6,%7};" ::"r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
+                 "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]), "l"(p)
+                 : "memory");
 }
 
-// dx[j] = dense(x[j]), at the listed places less sub[]: entries of the same
-// place are added up in the list's order by the first of them.  dx may be x
-// itself: a listed logit is read before any place is written.
-template <class XT, class DT, class F>
-__device__ __forceinline__ void rw_gradient(const XT* x, DT* dx, int vocab, const int* ids, const float* sub, int k, F dense) {
+// The gradient of a row is, but for its own few places, 2^y (f + g y) / S with
+// factors of the row (1 / S among them): the dense part.
+template <bool LIN>
+struct RwDense {
+    float m, c, f, g;
+    __device__ __forceinline__ f32x2 two(f32x2 x) const {
+        const f32x2 y = mul2(add2(x, pack2(-m, -m)), pack2(c, c));
+        float y0, y1;
+        unpack2(y, y0, y1);
+        if (LIN) {
+            y0 = rw_max_nan(y0, RW_LOW);
+            y1 = rw_max_nan(y1, RW_LOW);
+        }
+        const f32x2 e = pack2(rw_exp2(y0), rw_exp2(y1));
+        return mul2(e, LIN ? fma2(pack2(y0, y1), pack2(g, g), pack2(f, f)) : pack2(f, f));
+    }
+    __device__ __forceinline__ float one(float x) const {
+        float lo, hi;
+        unpack2(two(pack2(x, x)), lo, hi);
+        return lo;
+    }
+};
+
+// dx of one part of a row = the dense part, at the listed places less sub[]
+// (entries of the same place are added up in the list's order by the first of
+// them).  ids: in shared memory, 16-byte aligned, -1 up to a multiple of four.
+// dx may be x itself: what a thread writes it has read, and a listed logit is
+// read before any is written.
+template <class XT, class DT, bool LIN>
+__device__ __forceinline__ void rw_gradient(const XT* row, DT* drow, int vocab, const RwPart<XT>& p, bool ends, const int* ids,
+                                            const float* sub, int k, const RwDense<LIN>& dense) {
+    constexpr int N = RwUnit<XT>::N, BYTES = N * sizeof(DT);
     const int tid = threadIdx.x;
-    bool first = tid < k && ids[tid] >= 0;
+    const RwEnds<XT> e(row, vocab);
+    bool first = false;
     float q = 0.0f, v = 0.0f;
+    int id = -1;
+    if (tid < k) {
+        id = ids[tid];
+        first = id >= p.first && id < p.first + N * p.n;
+        if (ends) first |= id >= 0 && (id < e.head || id >= e.head + e.skip);
+    }
     if (first) {
-        v = rw_float(x[ids[tid]]);
-        for (int j = 0; j < k; ++j)
-            if (ids[j] == ids[tid]) {
-                first &= j >= tid;
-                q += sub[j];
+        v = rw_float(row[id]);
+        for (int j = 0; j < k; j += 4) {
+            const int4 o = *reinterpret_cast<const int4*>(ids + j);
+            const int at[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (at[i] == id) {
+                    first &= j + i >= tid;
+                    q += sub[j + i];
+                }
+        }
+    }
+    float end = 0.0f;
+    const bool has_end = ends && tid < e.n;
+    if (has_end) end = rw_float(row[e.place(tid)]);
+    __syncthreads();
+    if (has_end) drow[e.place(tid)] = rw_to<DT>(dense.one(end));
+    DT* d = drow + p.first;
+    if ((reinterpret_cast<uintptr_t>(d) & (BYTES > 32 ? 31 : BYTES - 1)) == 0) {
+        for (int u0 = tid; u0 < p.n; u0 += RW_THREADS * RW_BATCH) {
+            RwUnit<XT> u[RW_BATCH];
+#pragma unroll
+            for (int j = 0; j < RW_BATCH; ++j)
+                if (u0 + j * RW_THREADS < p.n) u[j].load(p.x + (long)N * (u0 + j * RW_THREADS));
+#pragma unroll
+            for (int j = 0; j < RW_BATCH; ++j) {
+                if (u0 + j * RW_THREADS >= p.n) break;
+                DT* to = d + (long)N * (u0 + j * RW_THREADS);
+                uint32_t w[BYTES / 4];
+#pragma unroll
+                for (int i = 0; i < N / 2; ++i) {
+                    const f32x2 r = dense.two(u[j].two(i));
+                    if constexpr (sizeof(DT) == 4) {
+                        float lo, hi;
+                        unpack2(r, lo, hi);
+                        w[2 * i] = __float_as_uint(lo);
+                        w[2 * i + 1] = __float_as_uint(hi);
+                    } else
+                        w[i] = rw_pair<DT>(r);
+                }
+                if constexpr (BYTES == 16) rw_store(to, w[0], w[1], w[2], w[3]);
+                else
+#pragma unroll
+                    for (int i = 0; i < BYTES / 32; ++i) rw_store(reinterpret_cast<char*>(to) + 32 * i, w + 8 * i);
             }
+        }
+    } else {                                       // dx lies otherwise than x: element by element, a warp's side by side
+        const int n = N * p.n;
+        for (int j0 = tid; j0 < n; j0 += 8 * RW_THREADS) {
+            float x[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = j0 + i * RW_THREADS < n ? rw_float(p.x[j0 + i * RW_THREADS]) : 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; i += 2) {
+                float lo, hi;
+                unpack2(dense.two(pack2(x[i], x[i + 1])), lo, hi);
+                if (j0 + i * RW_THREADS < n) d[j0 + i * RW_THREADS] = rw_to<DT>(lo);
+                if (j0 + (i + 1) * RW_THREADS < n) d[j0 + (i + 1) * RW_THREADS] = rw_to<DT>(hi);
+            }
+        }
     }
     __syncthreads();
-    for (int j = tid; j < vocab; j += RW_THREADS) dx[j] = rw_to<DT>(dense(rw_float(x[j])));
-    __syncthreads();
-    if (first) dx[ids[tid]] = rw_to<DT>(dense(v) - q);
+    if (first) drow[id] = rw_to<DT>(dense.one(v) - q);
 }
+// A part of a row of zeros.
 template <class DT>
-__device__ __forceinline__ void rw_zero(DT* dx, int vocab) {
-    for (int j = threadIdx.x; j < vocab; j += RW_THREADS) dx[j] = rw_to<DT>(0.0f);
+__device__ __forceinline__ void rw_zero(DT* drow, int vocab, int rank, int parts) {
+    const RwPart<DT> p(drow, vocab, rank, parts);
+    const uint32_t w[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    for (int u = threadIdx.x; u < p.n; u += RW_THREADS)
+        rw_store(const_cast<DT*>(p.x) + (long)RwUnit<DT>::N * u, w);
+    if (rank == parts - 1) {
+        const RwEnds<DT> e(drow, vocab);
+        if ((int)threadIdx.x < e.n) drow[e.place(threadIdx.x)] = rw_to<DT>(0.0f);
+    }
+}
+
+// Blocks of a row of a gradient: a batch of each thread at least, more while the
+// GPU holds all blocks at once; rows of many batches are cut in the end.
+template <class XT>
+inline int rw_grad_parts(const tk_ctx* ctx, long n_rows, int vocab) {
+    const long batch = RW_THREADS * RW_BATCH * RwUnit<XT>::N, batches = (vocab + batch - 1) / batch;
+    long parts = 8L * ctx->num_sms / n_rows;
+    parts = parts > batches ? batches : parts < 1 ? 1 : parts;
+    return (int)parts;
 }
 
 // launch(x, d) with values of the logits' and the gradient's element types.
