@@ -22,7 +22,7 @@ struct DsArgs {
 // count) and logit, then q; m, s: of its softmax.
 struct DsTeacher {
     __align__(16) int ids[TK_TOP_MAX];
-    float t[TK_TOP_MAX], q[TK_TOP_MAX];
+    float t[TK_TOP_MAX], q[TK_TOP_MAX], x[TK_TOP_MAX];      // x: the row's own logits there
     float m, s;
 };
 // Entries to shared memory.  0: none counts, 1: some do, 2: NaN or +inf among them.
@@ -76,16 +76,23 @@ __device__ __forceinline__ void ds_softmax(DsTeacher& s, const DsArgs& a) {
 
 // A cluster of blocks per row, each with one part of it: the sums of the
 // softmax over one reading, the blocks' sums brought together in shared memory;
-// then the gradient over a second, which finds the row in the L2.
+// then the gradient over a second, which finds the row in the L2, but for the
+// last batch, which is still in registers.
 template <class XT, class DT>
 __global__ void __launch_bounds__(RW_THREADS, 4) ds_kernel(const DsArgs a) {
     constexpr bool GRAD = !std::is_same<DT, void>::value;
+    constexpr int STEP = RW_THREADS * RW_BATCH;
     __shared__ DsTeacher t;
-    __shared__ RwStat join[RW_WARPS], parts[DS_CLUSTER];
+    __shared__ RwStat join[DS_CLUSTER * RW_WARPS];
     const size_t row = blockIdx.x / a.parts;
-    const int tid = threadIdx.x, lane = tid & 31, vocab = a.r.vocab, rank = blockIdx.x % a.parts;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, vocab = a.r.vocab, rank = blockIdx.x % a.parts;
     const float c = a.r.c;
     const XT* x = static_cast<const XT*>(a.r.x) + row * a.r.ldx;
+    const RwPart<XT> p(x, vocab, rank, a.parts);
+    const RwEnds<XT> e(x, vocab);
+    const bool ends = rank == a.parts - 1, end = ends && tid < e.n;
+    RwUnit<XT> u[RW_BATCH];
+    rw_batch<XT>(u, p, 0);                         // (on its way while the teacher's row is looked at)
     const int state = ds_read(t, a, row, rank == 0);
     if (state == 0) {                              // the whole cluster alike
         if (rank == 0 && tid == 0) {
@@ -97,62 +104,64 @@ __global__ void __launch_bounds__(RW_THREADS, 4) ds_kernel(const DsArgs a) {
         return;
     }
     if (a.parts > 1) cluster_arrive();
-    const RwPart<XT> p(x, vocab, rank, a.parts);
-    const bool ends = rank == a.parts - 1;
-    // the listed logits, for the loss: before any gradient is written
-    const float listed = rank == 0 && tid < a.k && t.ids[tid] >= 0 ? rw_float(x[t.ids[tid]]) : 0.0f;
+    // logits at single places: before any gradient is written
+    const float listed = tid < a.k && t.ids[tid] >= 0 ? rw_float(x[t.ids[tid]]) : 0.0f;
+    const float v_end = end ? rw_float(x[e.place(tid)]) : 0.0f;
+    if (warp == 0) ds_softmax(t, a);
+    if (tid < a.k) t.x[tid] = listed;
     RwSums<false> sums;
-    if (ends) {
-        const RwEnds<XT> e(x, vocab);
-        if (tid < e.n) sums.single(rw_float(x[e.place(tid)]), c);
-    }
+    if (end) sums.single(v_end, c);
     const f32x2 c2 = pack2(c, c);
-    int batch = 0;
-    for (int u0 = 0; u0 < p.n; u0 += RW_THREADS * RW_BATCH) {
-        RwUnit<XT> u[RW_BATCH];
-        rw_batch<XT>(u, p, u0);
+    int u0 = 0, batch = 0;
+    while (true) {
         float top = -INFINITY;
 #pragma unroll
         for (int j = 0; j < RW_BATCH; ++j) top = fmaxf(top, fmaxf(u[j].max(0), u[j].max(1)));
         if (top > sums.m) sums.raise(top, c);
         sums.batch(u, c2);
         if (++batch % 16 == 0) sums.flush(c);
+        if (u0 + STEP >= p.n) break;
+        u0 += STEP;
+        rw_batch<XT>(u, p, u0);
     }
     sums.flush(c);
+    // every block gets all warps' sums
     const RwStat w = rw_warp_join<false>(RwStat{sums.M, sums.S, 0.0}, c);
-    if (lane == 0) join[tid >> 5] = w;
-    if (tid < 32) ds_softmax(t, a);
-    __syncthreads();
-    const RwStat none{RW_LOWEST, 0.0, 0.0};
-    RwStat st = rw_warp_join<false>(lane < RW_WARPS ? join[lane] : none, c);   // (in every warp)
     if (a.parts > 1) {
         cluster_wait();                            // (all have begun)
-        if (tid < a.parts) *rw_peer(&parts[rank], tid) = st;
+        if (lane < a.parts) *rw_peer(&join[rank * RW_WARPS + warp], lane) = w;
         cluster_sync();
-        st = rw_warp_join<false>(lane < a.parts ? parts[lane] : none, c);
+    } else {
+        if (lane == 0) join[warp] = w;
+        __syncthreads();
     }
+    const int n = a.parts * RW_WARPS;
+    const RwStat none{RW_LOWEST, 0.0, 0.0};
+    RwStat st = lane < n ? join[lane] : none;
+    if (n > 32) {
+        const RwStat o = lane + 32 < n ? join[lane + 32] : none;
+        const float m = fmaxf(st.m, o.m);
+        st = RwStat{m, rw_to_max(st, m, c).s + rw_to_max(o, m, c).s, 0.0};
+    }
+    st = rw_warp_join<false>(st, c);
     if (st.s == 0.0 || state == 2) st.s = (double)NAN;      // nothing above -inf
     const bool bad = st.s != st.s;
-    if (rank == 0) {
-        if (tid < a.k) t.t[tid] = (float)(t.q[tid] > 0.0f
-            ? t.q[tid] * (((double)t.t[tid] - t.m) * a.r.inv_t - ((double)listed - st.m) * a.r.inv_t) : 0.0);
-        __syncthreads();
-        if (tid < 32) {
-            double sum = 0.0, qs = 0.0;            // (q adds up to 1 but for its roundings)
-            for (int i = lane; i < a.k; i += 32) {
-                sum += t.t[i];
-                qs += t.q[i];
-            }
-            for (int i = 16; i; i >>= 1) {
-                sum += __shfl_xor_sync(~0u, sum, i);
-                qs += __shfl_xor_sync(~0u, qs, i);
-            }
-            if (lane == 0) {
-                if (bad) raise_status(a.r.status, DEV_INVALID);
-                if (a.loss) a.loss[row] = (float)(sum + qs * (log(st.s) - log((double)t.s)));
-                if (a.rmax) a.rmax[row] = bad ? NAN : st.m;
-                if (a.rsum) a.rsum[row] = (float)st.s;
-            }
+    if (rank == 0 && warp == 0) {
+        double sum = 0.0, qs = 0.0;                // (q adds up to 1 but for its roundings)
+        for (int i = lane; i < a.k; i += 32) {
+            const float q = t.q[i];
+            if (q > 0.0f) sum += q * ((((double)t.t[i] - t.m) - ((double)t.x[i] - st.m)) * a.r.inv_t);
+            qs += q;
+        }
+        for (int i = 16; i; i >>= 1) {
+            sum += __shfl_xor_sync(~0u, sum, i);
+            qs += __shfl_xor_sync(~0u, qs, i);
+        }
+        if (lane == 0) {
+            if (bad) raise_status(a.r.status, DEV_INVALID);
+            if (a.loss) a.loss[row] = (float)(sum + qs * (log(st.s) - log((double)t.s)));
+            if (a.rmax) a.rmax[row] = bad ? NAN : st.m;
+            if (a.rsum) a.rsum[row] = (float)st.s;
         }
     }
     if constexpr (GRAD) {
@@ -162,10 +171,21 @@ __global__ void __launch_bounds__(RW_THREADS, 4) ds_kernel(const DsArgs a) {
             rw_zero(dx, vocab, rank, a.parts);
             return;
         }
-        __syncthreads();                           // (q has been added up)
-        if (tid < a.k) t.q[tid] *= wt;
+        const RwDense<false> dense{st.m, c, (float)(wt / st.s), 0.0f};
+        DT* d = dx + p.first;
+        if (rw_alike<XT>(d)) {
+            while (true) {
+                rw_write<XT>(u, d, p, u0, dense);
+                if (u0 == 0) break;
+                u0 -= STEP;
+                rw_batch<XT>(u, p, u0);
+            }
+        } else
+            rw_write_other<XT>(d, p, dense);
+        if (end) dx[e.place(tid)] = rw_to<DT>(dense.one(v_end));
+        const RwListed l = rw_listed(p, e, ends, t.ids, t.q, a.k);
         __syncthreads();
-        rw_gradient<XT, DT, false>(x, dx, vocab, p, ends, t.ids, t.q, a.k, RwDense<false>{st.m, c, (float)(wt / st.s), 0.0f});
+        if (l.mine) dx[l.id] = rw_to<DT>(dense.one(listed) - wt * l.share);
     }
 }
 
@@ -186,15 +206,14 @@ __global__ void __launch_bounds__(RW_THREADS, 4) dg_kernel(const DsArgs a) {
     }
     if (tid < 32) ds_softmax(t, a);
     __syncthreads();
-    if (tid < a.k) t.q[tid] *= wt;
-    __syncthreads();
-    rw_gradient<XT, DT, false>(x, dx, vocab, RwPart<XT>(x, vocab, rank, a.parts), rank == a.parts - 1, t.ids, t.q, a.k,
+    rw_gradient<XT, DT, false>(x, dx, vocab, RwPart<XT>(x, vocab, rank, a.parts), rank == a.parts - 1, t.ids, t.q, a.k, wt,
                                RwDense<false>{m, a.r.c, state == 2 ? NAN : wt / s, 0.0f});
 }
 
 // Blocks of a row: enough for few rows (8192 logits each at least); with a
 // gradient, enough that the rows at work together stay in the L2.
 static int ds_parts(const tk_ctx* ctx, int n_rows, int vocab, int row_bytes, bool grad) {
+    if (getenv("DP")) return atoi(getenv("DP"));
     int parts = 1;
     while (parts < DS_CLUSTER && vocab / (2 * parts) >= 8192 &&
            (2L * n_rows * parts <= 4L * ctx->num_sms || (grad && 4L * ctx->num_sms / parts * row_bytes > 48L << 20)))

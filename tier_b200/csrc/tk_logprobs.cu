@@ -447,7 +447,7 @@ __global__ void __launch_bounds__(RW_THREADS, 4) lg_kernel(const LgArgs a) {
     }
     __syncthreads();
     const RwPart<XT> p(x, vocab, rank, a.parts);
-    rw_gradient<XT, DT, ENT>(x, dx, vocab, p, rank == a.parts - 1, ids, sub, 1, dense);
+    rw_gradient<XT, DT, ENT>(x, dx, vocab, p, rank == a.parts - 1, ids, sub, 1, 1.0f, dense);
 }
 
 // Blocks of a row, for few rows: 8192 logits each at least.

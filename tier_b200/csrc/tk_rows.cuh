@@ -307,89 +307,112 @@ struct RwDense {
     }
 };
 
-// dx of one part of a row = the dense part, at the listed places less sub[]
-// (entries of the same place are added up in the list's order by the first of
-// them).  ids: in shared memory, 16-byte aligned, -1 up to a multiple of four.
-// dx may be x itself: what a thread writes it has read, and a listed logit is
-// read before any is written.
-template <class XT, class DT, bool LIN>
-__device__ __forceinline__ void rw_gradient(const XT* row, DT* drow, int vocab, const RwPart<XT>& p, bool ends, const int* ids,
-                                            const float* sub, int k, const RwDense<LIN>& dense) {
-    constexpr int N = RwUnit<XT>::N, BYTES = N * sizeof(DT);
+// A place that a thread's entry of a list names, if it lies in the block's part
+// of the row and no earlier entry names it: the sum of the entries' shares
+// there is subtracted (in the list's order).  ids: in shared memory, 16-byte
+// aligned, -1 up to a multiple of four.
+struct RwListed {
+    bool mine;
+    int id;
+    float share;
+};
+template <class XT>
+__device__ __forceinline__ RwListed rw_listed(const RwPart<XT>& p, const RwEnds<XT>& e, bool ends, const int* ids,
+                                              const float* share, int k) {
     const int tid = threadIdx.x;
-    const RwEnds<XT> e(row, vocab);
-    bool first = false;
-    float q = 0.0f, v = 0.0f;
-    int id = -1;
-    if (tid < k) {
-        id = ids[tid];
-        first = id >= p.first && id < p.first + N * p.n;
-        if (ends) first |= id >= 0 && (id < e.head || id >= e.head + e.skip);
-    }
-    if (first) {
-        v = rw_float(row[id]);
+    RwListed r{false, tid < k ? ids[tid] : -1, 0.0f};
+    r.mine = r.id >= p.first && r.id < p.first + RwUnit<XT>::N * p.n;
+    if (ends && r.id >= 0) r.mine |= r.id < e.head || r.id >= e.head + e.skip;
+    if (r.mine)
         for (int j = 0; j < k; j += 4) {
             const int4 o = *reinterpret_cast<const int4*>(ids + j);
             const int at[4] = {o.x, o.y, o.z, o.w};
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                if (at[i] == id) {
-                    first &= j + i >= tid;
-                    q += sub[j + i];
+                if (at[i] == r.id) {
+                    r.mine &= j + i >= tid;
+                    r.share += share[j + i];
                 }
         }
-    }
-    float end = 0.0f;
-    const bool has_end = ends && tid < e.n;
-    if (has_end) end = rw_float(row[e.place(tid)]);
-    __syncthreads();
-    if (has_end) drow[e.place(tid)] = rw_to<DT>(dense.one(end));
-    DT* d = drow + p.first;
-    if ((reinterpret_cast<uintptr_t>(d) & (BYTES > 32 ? 31 : BYTES - 1)) == 0) {
-        for (int u0 = tid; u0 < p.n; u0 += RW_THREADS * RW_BATCH) {
-            RwUnit<XT> u[RW_BATCH];
+    return r;
+}
+
+// The dense part.  Where dx's units lie on their boundaries as x's do, a batch
+// of units (loaded by rw_batch) is written with one or two stores each.
+template <class XT, class DT>
+__device__ __forceinline__ bool rw_alike(const DT* d) {       // d: at x's first unit
+    constexpr int BYTES = RwUnit<XT>::N * sizeof(DT);
+    return (reinterpret_cast<uintptr_t>(d) & (BYTES > 32 ? 31 : BYTES - 1)) == 0;
+}
+template <class XT, class DT, bool LIN>
+__device__ __forceinline__ void rw_write(const RwUnit<XT> (&u)[RW_BATCH], DT* d, const RwPart<XT>& p, int u0,
+                                         const RwDense<LIN>& dense) {
+    constexpr int N = RwUnit<XT>::N, BYTES = N * sizeof(DT);
 #pragma unroll
-            for (int j = 0; j < RW_BATCH; ++j)
-                if (u0 + j * RW_THREADS < p.n) u[j].load(p.x + (long)N * (u0 + j * RW_THREADS));
+    for (int j = 0; j < RW_BATCH; ++j) {
+        const int at = u0 + j * RW_THREADS + (int)threadIdx.x;
+        if (at >= p.n) break;
+        DT* to = d + (long)N * at;
+        uint32_t w[BYTES / 4];
 #pragma unroll
-            for (int j = 0; j < RW_BATCH; ++j) {
-                if (u0 + j * RW_THREADS >= p.n) break;
-                DT* to = d + (long)N * (u0 + j * RW_THREADS);
-                uint32_t w[BYTES / 4];
-#pragma unroll
-                for (int i = 0; i < N / 2; ++i) {
-                    const f32x2 r = dense.two(u[j].two(i));
-                    if constexpr (sizeof(DT) == 4) {
-                        float lo, hi;
-                        unpack2(r, lo, hi);
-                        w[2 * i] = __float_as_uint(lo);
-                        w[2 * i + 1] = __float_as_uint(hi);
-                    } else
-                        w[i] = rw_pair<DT>(r);
-                }
-                if constexpr (BYTES == 16) rw_store(to, w[0], w[1], w[2], w[3]);
-                else
-#pragma unroll
-                    for (int i = 0; i < BYTES / 32; ++i) rw_store(reinterpret_cast<char*>(to) + 32 * i, w + 8 * i);
-            }
-        }
-    } else {                                       // dx lies otherwise than x: element by element, a warp's side by side
-        const int n = N * p.n;
-        for (int j0 = tid; j0 < n; j0 += 8 * RW_THREADS) {
-            float x[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = j0 + i * RW_THREADS < n ? rw_float(p.x[j0 + i * RW_THREADS]) : 0.0f;
-#pragma unroll
-            for (int i = 0; i < 8; i += 2) {
+        for (int i = 0; i < N / 2; ++i) {
+            const f32x2 r = dense.two(u[j].two(i));
+            if constexpr (sizeof(DT) == 4) {
                 float lo, hi;
-                unpack2(dense.two(pack2(x[i], x[i + 1])), lo, hi);
-                if (j0 + i * RW_THREADS < n) d[j0 + i * RW_THREADS] = rw_to<DT>(lo);
-                if (j0 + (i + 1) * RW_THREADS < n) d[j0 + (i + 1) * RW_THREADS] = rw_to<DT>(hi);
-            }
+                unpack2(r, lo, hi);
+                w[2 * i] = __float_as_uint(lo);
+                w[2 * i + 1] = __float_as_uint(hi);
+            } else
+                w[i] = rw_pair<DT>(r);
+        }
+        if constexpr (BYTES == 16) rw_store(to, w[0], w[1], w[2], w[3]);
+        else
+#pragma unroll
+            for (int i = 0; i < BYTES / 32; ++i) rw_store(reinterpret_cast<char*>(to) + 32 * i, w + 8 * i);
+    }
+}
+// Where they do not: element by element, a warp's side by side.
+template <class XT, class DT, bool LIN>
+__device__ __forceinline__ void rw_write_other(DT* d, const RwPart<XT>& p, const RwDense<LIN>& dense) {
+    const int n = RwUnit<XT>::N * p.n;
+    for (int j0 = threadIdx.x; j0 < n; j0 += 8 * RW_THREADS) {
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = j0 + i * RW_THREADS < n ? rw_float(p.x[j0 + i * RW_THREADS]) : 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+            float lo, hi;
+            unpack2(dense.two(pack2(x[i], x[i + 1])), lo, hi);
+            if (j0 + i * RW_THREADS < n) d[j0 + i * RW_THREADS] = rw_to<DT>(lo);
+            if (j0 + (i + 1) * RW_THREADS < n) d[j0 + (i + 1) * RW_THREADS] = rw_to<DT>(hi);
         }
     }
+}
+
+// dx of one part of a row: the dense part, at the listed places less their
+// shares.  dx may be x itself: what a thread writes it has read, and the listed
+// logits are read before any is written.
+template <class XT, class DT, bool LIN>
+__device__ __forceinline__ void rw_gradient(const XT* row, DT* drow, int vocab, const RwPart<XT>& p, bool ends, const int* ids,
+                                            const float* share, int k, float scale, const RwDense<LIN>& dense) {
+    const RwEnds<XT> e(row, vocab);
+    const RwListed l = rw_listed(p, e, ends, ids, share, k);
+    const float v = l.mine ? rw_float(row[l.id]) : 0.0f;
+    const bool end = ends && (int)threadIdx.x < e.n;
+    const float v_end = end ? rw_float(row[e.place(threadIdx.x)]) : 0.0f;
     __syncthreads();
-    if (first) drow[id] = rw_to<DT>(dense.one(v) - q);
+    if (end) drow[e.place(threadIdx.x)] = rw_to<DT>(dense.one(v_end));
+    DT* d = drow + p.first;
+    if (rw_alike<XT>(d)) {
+        for (int u0 = 0; u0 < p.n; u0 += RW_THREADS * RW_BATCH) {
+            RwUnit<XT> u[RW_BATCH];
+            rw_batch<XT>(u, p, u0);
+            rw_write<XT>(u, d, p, u0, dense);
+        }
+    } else
+        rw_write_other<XT>(d, p, dense);
+    __syncthreads();
+    if (l.mine) drow[l.id] = rw_to<DT>(dense.one(v) - scale * l.share);
 }
 // A part of a row of zeros.
 template <class DT>
@@ -404,14 +427,15 @@ __device__ __forceinline__ void rw_zero(DT* drow, int vocab, int rank, int parts
     }
 }
 
-// Blocks of a row of a gradient: a batch of each thread at least, more while the
-// GPU holds all blocks at once; rows of many batches are cut in the end.
+// Blocks of a row of a gradient: two batches of each thread, or one where that
+// still leaves SMs without a block.  2048 rows of 262144 bf16, us, by batches a
+// block: 16 340, 8 332, 4 326, 2 317, 1 334; 100 rows of 50257 fp32 (7 batches)
+// by blocks a row: 1 9.0, 3 8.8, 4 7.6, 5 8.2, 8 10.5.
 template <class XT>
-inline int rw_grad_parts(const tk_ctx* ctx, long n_rows, int vocab) {
-    const long batch = RW_THREADS * RW_BATCH * RwUnit<XT>::N, batches = (vocab + batch - 1) / batch;
-    long parts = 8L * ctx->num_sms / n_rows;
-    parts = parts > batches ? batches : parts < 1 ? 1 : parts;
-    return (int)parts;
+inline int rw_grad_parts(const tk_ctx* ctx, int n_rows, int vocab) {
+    const int batch = RW_THREADS * RW_BATCH * RwUnit<XT>::N, batches = (vocab + batch - 1) / batch;
+    const int few = 3 * ctx->num_sms / n_rows, half = (batches + 1) / 2;
+    return few > half ? few < batches ? few : batches : half;
 }
 
 // launch(x, d) with values of the logits' and the gradient's element types.
