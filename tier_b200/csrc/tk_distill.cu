@@ -19,60 +19,70 @@ struct DsArgs {
 };
 
 // The teacher's row in shared memory: an entry's place (-1: it does not
-// count) and logit, then q; m, s: of its softmax.
+// count), logit and q = softmax(t / T); the row's own logits there; maximum and
+// sum of the teacher's softmax.  state 0: no entry counts, 1: some do, 2: NaN or
+// +inf among them.
 struct DsTeacher {
     __align__(16) int ids[TK_TOP_MAX];
-    float t[TK_TOP_MAX], q[TK_TOP_MAX], x[TK_TOP_MAX];      // x: the row's own logits there
+    float t[TK_TOP_MAX], q[TK_TOP_MAX], x[TK_TOP_MAX];
     float m, s;
+    int state;
 };
-// Entries to shared memory.  0: none counts, 1: some do, 2: NaN or +inf among them.
-__device__ __forceinline__ int ds_read(DsTeacher& s, const DsArgs& a, size_t row, bool report) {
-    const int tid = threadIdx.x;
-    int id = -1;
-    float t = -INFINITY;
-    if (tid < a.k) {
-        id = a.ids[row * a.k + tid];
-        t = a.teacher[row * a.k + tid];
-        if (id >= a.r.vocab) {
-            if (report) raise_status(a.r.status, DEV_INVALID);
-            id = -1;
-        }
-        if (id < 0 || t == -INFINITY) {
-            id = -1;
-            t = -INFINITY;
+// One warp's registers: entries lane, lane + 32, ...
+struct DsEntries {
+    static constexpr int EACH = TK_TOP_MAX / 32;
+    int id[EACH];
+    float t[EACH];
+    __device__ __forceinline__ void load(const DsArgs& a, size_t row) {
+        const int lane = threadIdx.x & 31;
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+            const bool in = 32 * i + lane < a.k;
+            id[i] = in ? a.ids[row * a.k + 32 * i + lane] : -1;
+            t[i] = in ? a.teacher[row * a.k + 32 * i + lane] : 0.0f;
         }
     }
-    s.ids[tid] = id;
-    s.t[tid] = t;
-    if (!__syncthreads_or(id >= 0)) return 0;
-    return __syncthreads_or(id >= 0 && !(t < INFINITY)) ? 2 : 1;
-}
-// One warp: q = softmax(t / T).
-__device__ __forceinline__ void ds_softmax(DsTeacher& s, const DsArgs& a) {
-    constexpr int EACH = TK_TOP_MAX / 32;
-    const int lane = threadIdx.x & 31;
-    float t[EACH], m = RW_LOWEST, sum = 0.0f;
+    __device__ __forceinline__ void softmax(DsTeacher& s, const DsArgs& a, bool report) {
+        const int lane = threadIdx.x & 31;
+        float m = RW_LOWEST, sum = 0.0f;
+        bool some = false, bad = false, beyond = false;
 #pragma unroll
-    for (int i = 0; i < EACH; ++i) {
-        t[i] = 32 * i < a.k ? s.t[32 * i + lane] : -INFINITY;
-        m = fmaxf(m, t[i]);
-    }
-    for (int i = 16; i; i >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, i));
+        for (int i = 0; i < EACH; ++i) {
+            beyond |= id[i] >= a.r.vocab;
+            if (id[i] < 0 || id[i] >= a.r.vocab || t[i] == -INFINITY) {
+                id[i] = -1;
+                t[i] = -INFINITY;
+            }
+            some |= id[i] >= 0;
+            bad |= !(t[i] < INFINITY);
+            m = fmaxf(m, t[i]);
+        }
+        for (int i = 16; i; i >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, i));
 #pragma unroll
-    for (int i = 0; i < EACH; ++i) {
-        t[i] = t[i] == -INFINITY ? 0.0f : rw_exp2((t[i] - m) * a.r.c);
-        sum += t[i];
-    }
-    for (int i = 16; i; i >>= 1) sum += __shfl_xor_sync(~0u, sum, i);
-    const float r = 1.0f / sum;
+        for (int i = 0; i < EACH; ++i) {
+            if (32 * i >= a.k) break;
+            s.ids[32 * i + lane] = id[i];
+            s.t[32 * i + lane] = t[i];
+            t[i] = rw_exp2((t[i] - m) * a.r.c);
+            sum += t[i];
+        }
+        for (int i = 16; i; i >>= 1) sum += __shfl_xor_sync(~0u, sum, i);
+        const float r = 1.0f / sum;
 #pragma unroll
-    for (int i = 0; i < EACH; ++i)
-        if (32 * i < a.k) s.q[32 * i + lane] = t[i] * r;
-    if (lane == 0) {
-        s.m = m;
-        s.s = sum;
+        for (int i = 0; i < EACH; ++i) {
+            if (32 * i >= a.k) break;
+            s.q[32 * i + lane] = t[i] * r;
+        }
+        some = __any_sync(~0u, some);
+        bad = __any_sync(~0u, bad);
+        if (report && beyond) raise_status(a.r.status, DEV_INVALID);
+        if (lane == 0) {
+            s.m = m;
+            s.s = sum;
+            s.state = bad ? 2 : some;
+        }
     }
-}
+};
 
 // A cluster of blocks per row, each with one part of it: the sums of the
 // softmax over one reading, the blocks' sums brought together in shared memory;
@@ -91,9 +101,27 @@ __global__ void __launch_bounds__(RW_THREADS, 4) ds_kernel(const DsArgs a) {
     const RwPart<XT> p(x, vocab, rank, a.parts);
     const RwEnds<XT> e(x, vocab);
     const bool ends = rank == a.parts - 1, end = ends && tid < e.n;
+    const float weight = a.weight ? a.weight[row] : 1.0f;
+    const f32x2 c2 = pack2(c, c);
+    RwSums<false> sums;
     RwUnit<XT> u[RW_BATCH];
-    rw_batch<XT>(u, p, 0);                         // (on its way while the teacher's row is looked at)
-    const int state = ds_read(t, a, row, rank == 0);
+    const auto add = [&]() {
+        float top = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < RW_BATCH; ++j) top = fmaxf(top, fmaxf(u[j].max(0), u[j].max(1)));
+        if (top > sums.m) sums.raise(top, c);
+        sums.batch(u, c2);
+    };
+    // the first batch and the teacher's row together
+    rw_batch<XT>(u, p, 0);
+    if (warp == RW_WARPS - 1) {
+        DsEntries entries;
+        entries.load(a, row);
+        entries.softmax(t, a, rank == 0);
+    }
+    add();
+    __syncthreads();
+    const int state = t.state;
     if (state == 0) {                              // the whole cluster alike
         if (rank == 0 && tid == 0) {
             if (a.loss) a.loss[row] = 0.0f;
@@ -105,25 +133,18 @@ __global__ void __launch_bounds__(RW_THREADS, 4) ds_kernel(const DsArgs a) {
     }
     if (a.parts > 1) cluster_arrive();
     // logits at single places: before any gradient is written
-    const float listed = tid < a.k && t.ids[tid] >= 0 ? rw_float(x[t.ids[tid]]) : 0.0f;
-    const float v_end = end ? rw_float(x[e.place(tid)]) : 0.0f;
-    if (warp == 0) ds_softmax(t, a);
-    if (tid < a.k) t.x[tid] = listed;
-    RwSums<false> sums;
-    if (end) sums.single(v_end, c);
-    const f32x2 c2 = pack2(c, c);
-    int u0 = 0, batch = 0;
-    while (true) {
-        float top = -INFINITY;
-#pragma unroll
-        for (int j = 0; j < RW_BATCH; ++j) top = fmaxf(top, fmaxf(u[j].max(0), u[j].max(1)));
-        if (top > sums.m) sums.raise(top, c);
-        sums.batch(u, c2);
-        if (++batch % 16 == 0) sums.flush(c);
-        if (u0 + STEP >= p.n) break;
+    const int entry = RW_THREADS - 1 - tid, id = entry < a.k ? t.ids[entry] : -1;    // (the first warp has the loss)
+    const float listed = id >= 0 ? rw_float(x[id]) : 0.0f;
+    const float v_end = end ? rw_float(x[e.place(tid)]) : -INFINITY;
+    int u0 = 0, batch = 1;
+    while (u0 + STEP < p.n) {
         u0 += STEP;
         rw_batch<XT>(u, p, u0);
+        add();
+        if (++batch % 16 == 0) sums.flush(c);
     }
+    if (entry < a.k) t.x[entry] = listed;
+    sums.single(v_end, c);
     sums.flush(c);
     // every block gets all warps' sums
     const RwStat w = rw_warp_join<false>(RwStat{sums.M, sums.S, 0.0}, c);
@@ -166,12 +187,12 @@ __global__ void __launch_bounds__(RW_THREADS, 4) ds_kernel(const DsArgs a) {
     }
     if constexpr (GRAD) {
         DT* dx = static_cast<DT*>(a.r.dx) + row * a.r.ldd;
-        const float wt = (a.weight ? a.weight[row] : 1.0f) * a.r.inv_t;
+        const float wt = weight * a.r.inv_t;
         if (wt == 0.0f) {
             rw_zero(dx, vocab, rank, a.parts);
             return;
         }
-        const RwDense<false> dense{st.m, c, (float)(wt / st.s), 0.0f};
+        const RwDense<false> dense{st.m, c, wt / (float)st.s, 0.0f};
         DT* d = dx + p.first;
         if (rw_alike<XT>(d)) {
             while (true) {
@@ -183,7 +204,7 @@ __global__ void __launch_bounds__(RW_THREADS, 4) ds_kernel(const DsArgs a) {
         } else
             rw_write_other<XT>(d, p, dense);
         if (end) dx[e.place(tid)] = rw_to<DT>(dense.one(v_end));
-        const RwListed l = rw_listed(p, e, ends, t.ids, t.q, a.k);
+        const RwListed l = rw_listed(p, e, ends, t.ids, t.q, a.k, entry);
         __syncthreads();
         if (l.mine) dx[l.id] = rw_to<DT>(dense.one(listed) - wt * l.share);
     }
@@ -198,14 +219,18 @@ __global__ void __launch_bounds__(RW_THREADS, 4) dg_kernel(const DsArgs a) {
     const XT* x = static_cast<const XT*>(a.r.x) + row * a.r.ldx;
     DT* dx = static_cast<DT*>(a.r.dx) + row * a.r.ldd;
     const float wt = (a.weight ? a.weight[row] : 1.0f) * a.r.inv_t, m = a.in_max[row], s = a.in_sum[row];
-    const int state = ds_read(t, a, row, rank == 0);
+    if (tid < 32) {
+        DsEntries entries;
+        entries.load(a, row);
+        entries.softmax(t, a, rank == 0);
+    }
+    __syncthreads();
+    const int state = t.state;
     if (state == 2 && rank == 0 && tid == 0) raise_status(a.r.status, DEV_INVALID);
     if (state == 0 || wt == 0.0f) {
         rw_zero(dx, vocab, rank, a.parts);
         return;
     }
-    if (tid < 32) ds_softmax(t, a);
-    __syncthreads();
     rw_gradient<XT, DT, false>(x, dx, vocab, RwPart<XT>(x, vocab, rank, a.parts), rank == a.parts - 1, t.ids, t.q, a.k, wt,
                                RwDense<false>{m, a.r.c, state == 2 ? NAN : wt / s, 0.0f});
 }

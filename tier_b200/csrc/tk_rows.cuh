@@ -199,14 +199,17 @@ struct RwSums {
         s2 = add2(s2, e);
         if (ENT) a2 = fma2(e, pack2(y0, y1), a2);
     }
-    // One logit, before any other.
     __device__ __forceinline__ void single(float v, float c) {
         if (v > m) raise(v, c);
         f32x2 s2 = 0, a2 = 0;
-        float none;
+        float e, none;
         two(pack2(v, -INFINITY), pack2(-m, -m), pack2(c, c), s2, a2);
-        unpack2(s2, s, none);
-        if (ENT) unpack2(a2, a, none);
+        unpack2(s2, e, none);
+        s += e;
+        if (ENT) {
+            unpack2(a2, e, none);
+            a += e;
+        }
     }
     template <class XT>
     __device__ __forceinline__ void batch(const RwUnit<XT> (&u)[RW_BATCH], f32x2 c) {     // none above m
@@ -318,9 +321,8 @@ struct RwListed {
 };
 template <class XT>
 __device__ __forceinline__ RwListed rw_listed(const RwPart<XT>& p, const RwEnds<XT>& e, bool ends, const int* ids,
-                                              const float* share, int k) {
-    const int tid = threadIdx.x;
-    RwListed r{false, tid < k ? ids[tid] : -1, 0.0f};
+                                              const float* share, int k, int entry) {
+    RwListed r{false, entry < k ? ids[entry] : -1, 0.0f};
     r.mine = r.id >= p.first && r.id < p.first + RwUnit<XT>::N * p.n;
     if (ends && r.id >= 0) r.mine |= r.id < e.head || r.id >= e.head + e.skip;
     if (r.mine)
@@ -330,7 +332,7 @@ __device__ __forceinline__ RwListed rw_listed(const RwPart<XT>& p, const RwEnds<
 #pragma unroll
             for (int i = 0; i < 4; ++i)
                 if (at[i] == r.id) {
-                    r.mine &= j + i >= tid;
+                    r.mine &= j + i >= entry;
                     r.share += share[j + i];
                 }
         }
@@ -396,7 +398,7 @@ template <class XT, class DT, bool LIN>
 __device__ __forceinline__ void rw_gradient(const XT* row, DT* drow, int vocab, const RwPart<XT>& p, bool ends, const int* ids,
                                             const float* share, int k, float scale, const RwDense<LIN>& dense) {
     const RwEnds<XT> e(row, vocab);
-    const RwListed l = rw_listed(p, e, ends, ids, share, k);
+    const RwListed l = rw_listed(p, e, ends, ids, share, k, (int)threadIdx.x);
     const float v = l.mine ? rw_float(row[l.id]) : 0.0f;
     const bool end = ends && (int)threadIdx.x < e.n;
     const float v_end = end ? rw_float(row[e.place(threadIdx.x)]) : 0.0f;
