@@ -84,14 +84,77 @@ struct DsEntries {
     }
 };
 
+// n sums brought together, in every lane of a warp.
+template <class F>
+__device__ __forceinline__ RwStat ds_join(F from, int n, float c) {
+    RwStat st{RW_LOWEST, 0.0, 0.0};
+    for (int i = threadIdx.x & 31; i < n; i += 32) {
+        const RwStat o = from(i);
+        const float m = fmaxf(st.m, o.m);
+        st = RwStat{m, rw_to_max(st, m, c).s + rw_to_max(o, m, c).s, 0.0};
+    }
+    return rw_warp_join<false>(st, c);
+}
+// One warp: the row's loss, maximum and sum.
+__device__ __forceinline__ void ds_loss(const DsTeacher& t, const DsArgs& a, size_t row, const RwStat& st) {
+    const int lane = threadIdx.x & 31;
+    const bool bad = st.s != st.s;
+    double sum = 0.0, qs = 0.0;                    // (q adds up to 1 but for its roundings)
+    for (int i = lane; i < a.k; i += 32) {
+        const float q = t.q[i];
+        if (q > 0.0f) sum += q * ((((double)t.t[i] - t.m) - ((double)t.x[i] - st.m)) * a.r.inv_t);
+        qs += q;
+    }
+    for (int i = 16; i; i >>= 1) {
+        sum += __shfl_xor_sync(~0u, sum, i);
+        qs += __shfl_xor_sync(~0u, qs, i);
+    }
+    if (lane == 0) {
+        if (bad) raise_status(a.r.status, DEV_INVALID);
+        if (a.loss) a.loss[row] = (float)(sum + qs * (log(st.s) - log((double)t.s)));
+        if (a.rmax) a.rmax[row] = bad ? NAN : st.m;
+        if (a.rsum) a.rsum[row] = (float)st.s;
+    }
+}
+
+// A thread's first batch stays in shared memory between the passes: its own
+// units, which no other thread reads (16 bytes of a warp's threads side by
+// side).  More of them would not help: 6 units instead of 4 left the L1 too
+// little room for the loads on their way (384 -> 437 us; 1 unit 413, 2 398).
+struct DsHeld {
+    uint4 part[RW_BATCH][2][RW_THREADS];
+    template <class XT>
+    __device__ __forceinline__ void hold(const RwUnit<XT> (&u)[RW_BATCH]) {
+#pragma unroll
+        for (int j = 0; j < RW_BATCH; ++j)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                part[j][h][threadIdx.x] = make_uint4(u[j].w[4 * h], u[j].w[4 * h + 1], u[j].w[4 * h + 2], u[j].w[4 * h + 3]);
+    }
+    template <class XT>
+    __device__ __forceinline__ void take(RwUnit<XT> (&u)[RW_BATCH]) const {
+#pragma unroll
+        for (int j = 0; j < RW_BATCH; ++j)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const uint4 q = part[j][h][threadIdx.x];
+                u[j].w[4 * h] = q.x;
+                u[j].w[4 * h + 1] = q.y;
+                u[j].w[4 * h + 2] = q.z;
+                u[j].w[4 * h + 3] = q.w;
+            }
+    }
+};
+
 // A cluster of blocks per row, each with one part of it: the sums of the
 // softmax over one reading, the blocks' sums brought together in shared memory;
-// then the gradient over a second, which finds the row in the L2, but for the
-// last batch, which is still in registers.
+// then the gradient over a second, which has the first batch in shared memory
+// and the last one in registers and finds the others in the L2.
 template <class XT, class DT>
 __global__ void __launch_bounds__(RW_THREADS, 4) ds_kernel(const DsArgs a) {
     constexpr bool GRAD = !std::is_same<DT, void>::value;
     constexpr int STEP = RW_THREADS * RW_BATCH;
+    __shared__ typename std::conditional<GRAD, DsHeld, int>::type held;
     __shared__ DsTeacher t;
     __shared__ RwStat join[DS_CLUSTER * RW_WARPS];
     const size_t row = blockIdx.x / a.parts;
@@ -138,6 +201,8 @@ __global__ void __launch_bounds__(RW_THREADS, 4) ds_kernel(const DsArgs a) {
     const float v_end = end ? rw_float(x[e.place(tid)]) : -INFINITY;
     int u0 = 0, batch = 1;
     while (u0 + STEP < p.n) {
+        if constexpr (GRAD)
+            if (u0 == 0) held.hold(u);
         u0 += STEP;
         rw_batch<XT>(u, p, u0);
         add();
@@ -156,35 +221,9 @@ __global__ void __launch_bounds__(RW_THREADS, 4) ds_kernel(const DsArgs a) {
         if (lane == 0) join[warp] = w;
         __syncthreads();
     }
-    const int n = a.parts * RW_WARPS;
-    const RwStat none{RW_LOWEST, 0.0, 0.0};
-    RwStat st = lane < n ? join[lane] : none;
-    if (n > 32) {
-        const RwStat o = lane + 32 < n ? join[lane + 32] : none;
-        const float m = fmaxf(st.m, o.m);
-        st = RwStat{m, rw_to_max(st, m, c).s + rw_to_max(o, m, c).s, 0.0};
-    }
-    st = rw_warp_join<false>(st, c);
+    RwStat st = ds_join([&](int i) { return join[i]; }, a.parts * RW_WARPS, c);
     if (st.s == 0.0 || state == 2) st.s = (double)NAN;      // nothing above -inf
-    const bool bad = st.s != st.s;
-    if (rank == 0 && warp == 0) {
-        double sum = 0.0, qs = 0.0;                // (q adds up to 1 but for its roundings)
-        for (int i = lane; i < a.k; i += 32) {
-            const float q = t.q[i];
-            if (q > 0.0f) sum += q * ((((double)t.t[i] - t.m) - ((double)t.x[i] - st.m)) * a.r.inv_t);
-            qs += q;
-        }
-        for (int i = 16; i; i >>= 1) {
-            sum += __shfl_xor_sync(~0u, sum, i);
-            qs += __shfl_xor_sync(~0u, qs, i);
-        }
-        if (lane == 0) {
-            if (bad) raise_status(a.r.status, DEV_INVALID);
-            if (a.loss) a.loss[row] = (float)(sum + qs * (log(st.s) - log((double)t.s)));
-            if (a.rmax) a.rmax[row] = bad ? NAN : st.m;
-            if (a.rsum) a.rsum[row] = (float)st.s;
-        }
-    }
+    if (rank == 0 && warp == 0) ds_loss(t, a, row, st);
     if constexpr (GRAD) {
         DT* dx = static_cast<DT*>(a.r.dx) + row * a.r.ldd;
         const float wt = weight * a.r.inv_t;
@@ -199,7 +238,8 @@ __global__ void __launch_bounds__(RW_THREADS, 4) ds_kernel(const DsArgs a) {
                 rw_write<XT>(u, d, p, u0, dense);
                 if (u0 == 0) break;
                 u0 -= STEP;
-                rw_batch<XT>(u, p, u0);
+                if (u0) rw_batch<XT>(u, p, u0);
+                else held.take(u);
             }
         } else
             rw_write_other<XT>(d, p, dense);
@@ -235,19 +275,22 @@ __global__ void __launch_bounds__(RW_THREADS, 4) dg_kernel(const DsArgs a) {
                                RwDense<false>{m, a.r.c, state == 2 ? NAN : wt / s, 0.0f});
 }
 
-// Blocks of a row: enough for few rows (8192 logits each at least); with a
-// gradient, enough that the rows at work together stay in the L2.
-static int ds_parts(const tk_ctx* ctx, int n_rows, int vocab, int row_bytes, bool grad) {
-    if (getenv("DP")) return atoi(getenv("DP"));
+// Blocks of a row: enough for few rows (of 8192 logits each at least); with a
+// gradient, one for every 128 KB of it: two batches of a block are then read
+// again, and the 148 rows that four blocks an SM hold of 512 KB each stay in the
+// L2.  us by blocks a row 1, 2, 4, 8: 2048 rows of 512 KB (bf16) 470, 440, 384,
+// 433; 512 of 1 MB (fp32) 207, 196, 177, 150; 300 of 256 KB 41.6, 39.7, 41.6,
+// 46.7; 1024 of 64 KB 31, 37, 59, 109; few: 100 of 50257 fp32 13.7, 13.3, 10.9, 15.8.
+static int ds_parts(const tk_ctx* ctx, int n_rows, int vocab, long row_bytes, bool grad) {
     int parts = 1;
     while (parts < DS_CLUSTER && vocab / (2 * parts) >= 8192 &&
-           (2L * n_rows * parts <= 4L * ctx->num_sms || (grad && 4L * ctx->num_sms / parts * row_bytes > 48L << 20)))
+           (2L * n_rows * parts <= 4L * ctx->num_sms || (grad && row_bytes / parts > 128 << 10)))
         parts *= 2;
     return parts;
 }
 template <class XT, class DT>
 static cudaError_t launch_ds(const tk_ctx* ctx, DsArgs& a, cudaStream_t s) {
-    a.parts = ds_parts(ctx, a.r.n_rows, a.r.vocab, a.r.vocab * (int)sizeof(XT), !std::is_same<DT, void>::value);
+    a.parts = ds_parts(ctx, a.r.n_rows, a.r.vocab, (long)a.r.vocab * sizeof(XT), !std::is_same<DT, void>::value);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)((long)a.r.n_rows * a.parts));
     cfg.blockDim = dim3(RW_THREADS);

@@ -211,12 +211,12 @@ struct RwSums {
             a += e;
         }
     }
-    template <class XT>
-    __device__ __forceinline__ void batch(const RwUnit<XT> (&u)[RW_BATCH], f32x2 c) {     // none above m
+    template <class XT, int NB>
+    __device__ __forceinline__ void batch(const RwUnit<XT> (&u)[NB], f32x2 c) {     // none above m
         const f32x2 nm = pack2(-m, -m);
         f32x2 s2[2] = {0, 0}, a2[2] = {0, 0};
 #pragma unroll
-        for (int j = 0; j < RW_BATCH; ++j)
+        for (int j = 0; j < NB; ++j)
 #pragma unroll
             for (int i = 0; i < RwUnit<XT>::N / 2; ++i) two(u[j].two(i), nm, c, s2[i & 1], a2[i & 1]);
         float p, q;
@@ -282,7 +282,7 @@ __device__ __forceinline__ void rw_store(void* p, uint32_t a, uint32_t b, uint32
     asm volatile("st.global.L1::no_allocate.v4.b32 [%4], {%0,%1,%2,%3};" ::"r"(a), "r"(b), "r"(c), "r"(d), "l"(p) : "memory");
 }
 __device__ __forceinline__ void rw_store(void* p, const uint32_t* w) {
-    asm volatile("st.global.L1::no_allocate.v8.b32 [%8], {%0,%1,%2,%3,%4,%5,%6,%7};" ::"r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
+    asm volatile("st.global.L1::no_allocate.L2::evict_first.v8.b32 [%8], {%0,%1,%2,%3,%4,%5,%6,%7};" ::"r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
                  "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]), "l"(p)
                  : "memory");
 }
@@ -346,12 +346,12 @@ __device__ __forceinline__ bool rw_alike(const DT* d) {       // d: at x's first
     constexpr int BYTES = RwUnit<XT>::N * sizeof(DT);
     return (reinterpret_cast<uintptr_t>(d) & (BYTES > 32 ? 31 : BYTES - 1)) == 0;
 }
-template <class XT, class DT, bool LIN>
-__device__ __forceinline__ void rw_write(const RwUnit<XT> (&u)[RW_BATCH], DT* d, const RwPart<XT>& p, int u0,
+template <class XT, class DT, bool LIN, int NB>
+__device__ __forceinline__ void rw_write(const RwUnit<XT> (&u)[NB], DT* d, const RwPart<XT>& p, int u0,
                                          const RwDense<LIN>& dense) {
     constexpr int N = RwUnit<XT>::N, BYTES = N * sizeof(DT);
 #pragma unroll
-    for (int j = 0; j < RW_BATCH; ++j) {
+    for (int j = 0; j < NB; ++j) {
         const int at = u0 + j * RW_THREADS + (int)threadIdx.x;
         if (at >= p.n) break;
         DT* to = d + (long)N * at;
