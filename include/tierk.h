@@ -341,10 +341,12 @@ tk_status tk_draft_verify(tk_ctx *ctx, int n_seqs, const int32_t *row_start, int
 /* n_rows rows of `vocab` logits (<= 2^23; fp32, fp16 or bf16; row stride ldx in
  * elements, of any alignment), T = temperature (1e-4 to 1e4).  Of a row: m its
  * largest logit, S = sum_j exp((l_j - m) / T), p_j = exp((l_j - m) / T) / S.
- * Logits of -inf have p = 0; results beyond fp32 are infinite.  A row that is
- * needed and holds NaN, +inf or only -inf has NaN in all its results (places -1) and makes tk_sync_status report
- * TK_ERR_DEVICE.  No counterpart in the reference, whose loss is the
- * cross-entropy of one label a row. */
+ * Logits of -inf, and those whose exponential is below 2^-126, have p = 0;
+ * results beyond fp32 are infinite.  A row that is needed and holds NaN, +inf or
+ * only -inf has NaN in all its results (places -1) and makes tk_sync_status
+ * report TK_ERR_DEVICE.  These four calls use no workspace: on several streams
+ * they need no order but that of their own data.  No counterpart in the
+ * reference, whose loss is the cross-entropy of one label a row. */
 enum { TK_TOP_MAX = 256 };   /* top_k, k at most */
 /* Log-probabilities of given tokens, entropy and the likeliest tokens:
  * logp[i] = ln p(tokens[i]), entropy[i] = -sum_j p_j ln p_j, rmax[i] = m,
@@ -352,7 +354,7 @@ enum { TK_TOP_MAX = 256 };   /* top_k, k at most */
  * the top_k largest logits, largest first, of equal ones the lowest place
  * first, with top_logp[i, :] (nullable) = ln p there; both [n_rows, top_k].
  * A row whose token is negative is left out (a batch's padding, a prompt's
- * tokens): its logits are not read, its results are zeros and places -1; so is
+ * tokens): whatever its logits hold, its results are zeros and places -1; so is
  * one whose token is not in the vocabulary, and tk_sync_status reports
  * TK_ERR_DEVICE.  tokens == NULL: every row, without logp. */
 tk_status tk_logprobs(tk_ctx *ctx, int n_rows, int vocab, const void *logits, int x_dtype, long ldx, const int32_t *tokens,
@@ -363,8 +365,8 @@ tk_status tk_logprobs(tk_ctx *ctx, int n_rows, int vocab, const void *logits, in
  * from tk_logprobs' rmax, rsum and (with d_entropy) entropy; one of d_logp and
  * d_entropy may be NULL.  dlogits in d_dtype, row stride ldd; it may be logits
  * itself (same address, type and stride), and overlap it in no other way.  Rows
- * left out, and rows whose two gradients are both zero, are zero and their
- * logits are not read. */
+ * left out, and rows whose two gradients are both zero, are zero, whatever
+ * their logits hold. */
 tk_status tk_logprobs_grad(tk_ctx *ctx, int n_rows, int vocab, const void *logits, int x_dtype, long ldx, const int32_t *tokens,
                            float temperature, const float *rmax, const float *rsum, const float *d_logp, const float *entropy,
                            const float *d_entropy, void *dlogits, int d_dtype, long ldd, void *stream);
@@ -379,8 +381,7 @@ tk_status tk_logprobs_grad(tk_ctx *ctx, int n_rows, int vocab, const void *logit
  *   dlogits[i, j] = weight[i] / T (p_j - sum of q_e with ids[i, e] == j)
  * (dlogits NULL: the loss alone; weight NULL: 1; dlogits as for
  * tk_logprobs_grad).  A row without entries has loss 0, rmax and rsum 0 and
- * gradient 0, and its logits are not read; the gradient of a row of weight 0 is
- * 0.  Teacher logits of NaN or +inf are as such in the row itself.  rmax, rsum
+ * gradient 0, whatever its logits hold; the gradient of a row of weight 0 is 0.  Teacher logits of NaN or +inf are as such in the row itself.  rmax, rsum
  * nullable. */
 tk_status tk_distill(tk_ctx *ctx, int n_rows, int vocab, const void *logits, int x_dtype, long ldx, int k, const int32_t *ids,
                      const float *teacher, float temperature, const float *weight, float *loss, float *rmax, float *rsum,

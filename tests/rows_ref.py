@@ -6,6 +6,9 @@ exponential's own error) and by 2^-22 ln 2 |y| (the difference, c and the
 product, each rounded); a sum of weights by their mean error and by its own
 roundings, of which no path to it has more than 64 (2^-24 each: 2^-18).  So the
 sum is off by e_S = 2^-18 + 2^-22 + 2^-22 E with E = sum p |y| ln 2 at most.
+Weights below 2^-126 are 0 in fp32 without subnormal numbers: as S is 1 or
+more, a p is off by 2^-126 besides, and what it is multiplied by counts (the
+weight over the temperature can be 1e10).
 """
 import torch
 
@@ -119,5 +122,5 @@ def distill(logits, ids, t, T, weight, dtype):
     places = torch.zeros_like(p).scatter_add_(1, ids.clamp(0, V - 1).long(), q)
     g = (p - places) * w[:, None]
     y = (m[:, None] / T - logits.double() / T).clamp(max=200.0)
-    off = p * (2.0 ** -21 + 2.0 ** -22 * y + e[:, None]) + torch.zeros_like(p).scatter_add_(1, ids.clamp(0, V - 1).long(), q * qrel)
+    off = p * (2.0 ** -21 + 2.0 ** -22 * y + e[:, None]) + 2.0 ** -126 + torch.zeros_like(p).scatter_add_(1, ids.clamp(0, V - 1).long(), q * qrel)
     return val + [g], tol + [_rounded(g, off * w.abs()[:, None], dtype)]

@@ -1,0 +1,152 @@
+"""GPU tests of the operators on rows of logits at the edges of their contract:
+calls at once, many short rows, rows of every place in memory, the same inputs
+through different divisions."""
+import math
+
+import pytest
+
+import rows_ref as ref
+from test_gpu_distill import blank, inputs as distill_inputs, run
+from test_gpu_logprobs import TYPES, check, code, dt, forward, gradient, inputs, put
+
+pytestmark = pytest.mark.gpu
+
+
+def test_two_calls_at_once(ctx):
+    """The operators share nothing but the status word: calls on two streams of one context do not disturb each other."""
+    import torch
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    sides = []
+    for seed in range(2):
+        x, tokens = inputs(seed, 60, 50257, "f32")
+        _, ids, t, w = distill_inputs(seed, 60, 50257, 40, "f32")
+        n = x.shape[0]
+        f = lambda *s: torch.zeros(*s, device="cuda")  # noqa: E731
+        sides.append(dict(x=x, gx=put(x), tokens=tokens, tok=tokens.cuda(), ids=ids, gi=ids.cuda(), t=t, gt=t.cuda(), w=w, gw=w.cuda(),
+                          f=[f(n) for _ in range(4)], top=torch.zeros(n, 30, dtype=torch.int32, device="cuda"), lp=f(n, 30),
+                          loss=[f(n) for _ in range(3)], dx=f(n, 50257), dy=f(n, 50257), one=torch.ones(n, device="cuda")))
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for s, d in zip(streams, sides):
+            ctx.logprobs(d["gx"], d["tok"], *d["f"], d["top"], d["lp"], stream=s)
+            ctx.distill(d["gx"], d["gi"], d["gt"], d["loss"][0], d["gw"], d["dx"], d["loss"][1], d["loss"][2], stream=s)
+            ctx.logprobs_grad(d["gx"], d["tok"], d["f"][2], d["f"][3], d["dy"], d["one"], d["f"][1], d["one"], stream=s)
+    torch.cuda.synchronize()
+    for d in sides:
+        check(d["f"] + [d["top"], d["lp"]], *ref.logprobs(d["x"], d["tokens"], 1.0, 30))
+        check(d["loss"] + [d["dx"]], *ref.distill(d["x"], d["ids"], d["t"], 1.0, d["w"], torch.float32))
+        want, tol = ref.logprobs_grad(d["x"], d["tokens"], 1.0, torch.ones(60), torch.ones(60), torch.float32)
+        check([d["dy"]], [want], [tol])
+    ctx.sync_status()
+
+
+@pytest.mark.parametrize("V", [1, 3, 40])
+def test_many_short_rows(ctx, V):
+    """More rows than a grid's y or z dimension holds."""
+    import torch
+    n = 100003
+    x, tokens = inputs(V, n, V, "bf16", left=0.1)
+    check(forward(ctx, put(x), tokens, 1.0, min(V, 2)), *ref.logprobs(x, tokens, 1.0, min(V, 2)))
+    dl = torch.ones(n)
+    want, tol = ref.logprobs_grad(x, tokens, 1.0, dl, dl, torch.float16)
+    check([gradient(ctx, put(x), tokens, 1.0, dl, dl, "f16")], [want], [tol])
+    ids = torch.randint(-1, V, (n, 3), generator=torch.Generator().manual_seed(1)).to(torch.int32)
+    t = torch.randn(n, 3, generator=torch.Generator().manual_seed(2))
+    want, tol = ref.distill(x, ids, t, 1.0, None, torch.bfloat16)
+    check(run(ctx, put(x), ids, t, 1.0, None, blank(x, "bf16")), want, tol)
+    ctx.sync_status()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_every_place_in_memory(ctx, dtype):
+    """Rows and gradients that begin at each place of a 32-byte unit, alike and differently; rows shorter than a unit."""
+    import torch
+    for V in (5, 33, 700):
+        x, tokens = inputs(V, 2, V, dtype)
+        _, ids, t, w = distill_inputs(V, 2, V, 4, dtype, empty=0.0)
+        dl = torch.tensor([1.0, -0.5])
+        lp = ref.logprobs(x, tokens, 1.3, min(V, 5))
+        for at in range(17):
+            gx = put(x, 1, at)
+            check(forward(ctx, gx, tokens, 1.3, min(V, 5)), *lp)
+            for d in TYPES:
+                for at2 in (at, at + 1, 0):
+                    want, tol = ref.logprobs_grad(x, tokens, 1.3, dl, dl, dt(d))
+                    out = blank(x, d, 1, at2)
+                    check([gradient(ctx, gx, tokens, 1.3, dl, dl, d, out=out)], [want], [tol])
+                    want, tol = ref.distill(x, ids, t, 1.3, w, dt(d))
+                    other = blank(x, d, 1, at2)
+                    check(run(ctx, gx, ids, t, 1.3, w, other), want, tol)
+                    for o in (out, other):               # what lies between the rows and behind them stays
+                        assert (o.as_strided((1,), (1,), o.storage_offset() + V) == 7.0).all()
+                        assert (o.as_strided((8,), (1,), o.storage_offset() + 2 * V + 1) == 7.0).all()
+    ctx.sync_status()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_alternatives_do_not_depend_on_the_batch(ctx, dtype):
+    """One row alone (eight blocks), in a small batch and in a large one (one block): the same places, the same logits there."""
+    import torch
+    V = 90001
+    x, tokens = inputs(3, 1, V, dtype)
+    x = x.float().round().to(dt(dtype)) if dtype == "f32" else x        # ties in every type
+    first = None
+    for n in (1, 4, 30, 160):
+        got = forward(ctx, put(x.expand(n, V)), tokens.expand(n).contiguous(), 1.0, 200)
+        assert (got[4] == got[4][:1]).all() and (got[2] == got[2][0]).all()
+        first = first or got
+        assert torch.equal(got[4][0], first[4][0])
+        assert (got[5][0] - first[5][0]).abs().max() < 2.0 ** -17        # two sums, each within 2^-18
+    ctx.sync_status()
+
+
+def test_sorted_rows_of_many_batches(ctx):
+    """The largest logits all in one place, more of them than a block's candidates hold: every group of them is looked through."""
+    import torch
+    V = 200000
+    i = torch.arange(V, dtype=torch.float32)
+    rows = torch.stack([i * 1e-4, -i * 1e-4, torch.where(i > V - 5000, 1.0, 0.0), torch.where((i // 16) % 3 == 0, 2.0, 1.0),
+                        torch.full((V,), -2.5), torch.where(i < 3000, 3.0 - i * 1e-5, -i)])
+    for n in (6, 240):
+        x = rows.repeat(n // 6, 1)
+        for k in (1, 100, 256):
+            got = forward(ctx, put(x), torch.full((n,), 5, dtype=torch.int32), 1.0, k)
+            want, tol = ref.logprobs(rows, torch.full((6,), 5, dtype=torch.int32), 1.0, k)
+            for at in range(0, n, 6):
+                if at in (0, n - 6):
+                    check([g[at:at + 6] for g in got], want, tol)
+                else:
+                    assert torch.equal(got[4][at:at + 6], got[4][:6])
+    ctx.sync_status()
+
+
+def test_loss_of_a_teacher_that_is_the_student(ctx):
+    """All of a small vocabulary listed, the teacher's logits the row's own: the loss is 0 and so is the gradient."""
+    import torch
+    n, V = 20, 200
+    x, _ = inputs(1, n, V, "f32")
+    ids = torch.stack([torch.randperm(V, generator=torch.Generator().manual_seed(i)) for i in range(n)]).to(torch.int32)
+    t = x.gather(1, ids.long())
+    got = run(ctx, put(x), ids, t, 1.0, None, blank(x, "f32"))
+    # p and q are each within 2^-18 of the same number, and differ from it by no more
+    assert got[0].abs().max() < 2.0 ** -17 * 12 and got[3].abs().max() < 2.0 ** -17
+    ctx.sync_status()
+
+
+def test_large_weights_and_temperatures(ctx):
+    import torch
+    x, ids, t, w = distill_inputs(4, 9, 3001, 12, "f32", empty=0.0)
+    for T in (1e-4, 0.01, 100.0, 1e4):
+        want, tol = ref.distill(x, ids, t, T, w * 1e6, torch.float32)
+        check(run(ctx, put(x), ids, t, T, w * 1e6, blank(x, "f32")), want, tol)
+    assert math.isfinite(float(want[0].max()))
+    ctx.sync_status()
+
+
+def test_too_many_rows_are_refused(ctx):
+    import tier_b200 as tk
+    import torch
+    x = torch.zeros(64, device="cuda")
+    for n, V in ((2 ** 31 - 1, 1 << 14), (1 << 24, 1 << 23)):
+        st = ctx.lib.tk_logprobs(ctx.h, n, V, x.data_ptr(), 0, V, None, 1.0, None, x.data_ptr(), None, None, 0, None, None, None)
+        assert st == tk.TK_ERR_INVALID

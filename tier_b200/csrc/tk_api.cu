@@ -742,24 +742,24 @@ static int dt_bytes(int dtype) {
 // The logits, and the gradient where there is one (d_dtype >= 0).  In place
 // means the very same rows; other rows may share memory with the logits' only
 // as other columns of one matrix.
-static tk_status rows_check(const std::string& fn, tk_ctx* ctx, int n_rows, int vocab, const void* x, int x_dtype, long ldx,
+static tk_status rows_check(const char* fn, tk_ctx* ctx, int n_rows, int vocab, const void* x, int x_dtype, long ldx,
                             float temperature, void* dx, int d_dtype, long ldd, RowArgs& r) {
     const int xb = dt_bytes(x_dtype), db = dx ? dt_bytes(d_dtype) : 0;
-    if (vocab <= 0) return fail(TK_ERR_INVALID, fn + ": empty vocabulary");
-    if (vocab > (1 << 23)) return fail(TK_ERR_UNSUPPORTED, fn + ": vocabulary beyond 2^23");
-    if (!x) return fail(TK_ERR_INVALID, fn + ": null pointer");
-    if (!xb || (dx && !db)) return fail(TK_ERR_INVALID, fn + ": unknown element type");
-    if (!(temperature >= 1e-4f && temperature <= 1e4f)) return fail(TK_ERR_INVALID, fn + ": temperature must be 1e-4 to 1e4");
-    if (ldx < vocab || (dx && ldd < vocab)) return fail(TK_ERR_INVALID, fn + ": row stride too small");
+    if (vocab <= 0) return fail(TK_ERR_INVALID, std::string(fn) + ": empty vocabulary");
+    if (vocab > (1 << 23)) return fail(TK_ERR_UNSUPPORTED, std::string(fn) + ": vocabulary beyond 2^23");
+    if (!x) return fail(TK_ERR_INVALID, std::string(fn) + ": null pointer");
+    if (!xb || (dx && !db)) return fail(TK_ERR_INVALID, std::string(fn) + ": unknown element type");
+    if (!(temperature >= 1e-4f && temperature <= 1e4f)) return fail(TK_ERR_INVALID, std::string(fn) + ": temperature must be 1e-4 to 1e4");
+    if (ldx < vocab || (dx && ldd < vocab)) return fail(TK_ERR_INVALID, std::string(fn) + ": row stride too small");
     const uintptr_t a = reinterpret_cast<uintptr_t>(x), b = reinterpret_cast<uintptr_t>(dx);
-    if (a % xb || (dx && b % db)) return fail(TK_ERR_INVALID, fn + ": rows off their elements' boundary");
+    if (a % xb || (dx && b % db)) return fail(TK_ERR_INVALID, std::string(fn) + ": rows off their elements' boundary");
     const unsigned __int128 sa = (unsigned __int128)ldx * xb, wa = (unsigned __int128)vocab * xb;
     const unsigned __int128 sb = (unsigned __int128)ldd * db, wb = (unsigned __int128)vocab * db;
-    if (sa * n_rows > INT64_MAX || sb * n_rows > INT64_MAX) return fail(TK_ERR_INVALID, fn + ": rows beyond any memory");
+    if (sa * n_rows > INT64_MAX || sb * n_rows > INT64_MAX || n_rows * (vocab / 8192 + 1L) > INT32_MAX) return fail(TK_ERR_INVALID, std::string(fn) + ": rows beyond any memory");
     if (dx && a < b + sb * (n_rows - 1) + wb && b < a + sa * (n_rows - 1) + wa) {
         const bool same = a == b && xb == db && x_dtype == d_dtype && (ldx == ldd || n_rows == 1);
         const unsigned __int128 off = b >= a ? (b - a) % sa : (sa - (a - b) % sa) % sa;   // dx's column in the logits' rows
-        if (!same && !(sa == sb && off >= wa && off + wb <= sa)) return fail(TK_ERR_INVALID, fn + ": gradient overlaps the logits");
+        if (!same && !(sa == sb && off >= wa && off + wb <= sa)) return fail(TK_ERR_INVALID, std::string(fn) + ": gradient overlaps the logits");
     }
     r = RowArgs{n_rows, vocab, x, ldx, (float)(1.4426950408889634 / (double)temperature), (float)(1.0 / (double)temperature), dx,
                 ldd, ctx->status};
@@ -800,9 +800,9 @@ tk_status tk_logprobs_grad(tk_ctx* ctx, int n_rows, int vocab, const void* logit
                                 static_cast<cudaStream_t>(stream));
 }
 
-static tk_status teacher_check(const std::string& fn, int k, const int32_t* ids, const float* teacher) {
-    if (k <= 0 || k > TK_TOP_MAX) return fail(TK_ERR_INVALID, fn + ": k must be 1 to TK_TOP_MAX");
-    if (!ids || !teacher) return fail(TK_ERR_INVALID, fn + ": null pointer");
+static tk_status teacher_check(const char* fn, int k, const int32_t* ids, const float* teacher) {
+    if (k <= 0 || k > TK_TOP_MAX) return fail(TK_ERR_INVALID, std::string(fn) + ": k must be 1 to TK_TOP_MAX");
+    if (!ids || !teacher) return fail(TK_ERR_INVALID, std::string(fn) + ": null pointer");
     return TK_OK;
 }
 

@@ -29,37 +29,17 @@ __device__ __forceinline__ float rw_max_nan(float a, float b) {
     return r;
 }
 
-// A logit's exponent to the base 2 below the row's largest, m.  The difference
-// comes first: it is exact where it matters, however large the logits are, and
-// a mask of fp32's lowest value only makes it -inf.  Clamped at -200, where the
-// weight 2^y is zero in fp32, so that y may be multiplied by the weight; a NaN
-// stays one (a row that holds NaN or +inf has the sum NaN).
+// Weights.  A logit's exponent to the base 2 below the row's largest, m, is
+// y = (x - m) * c, c = log2(e) / temperature.  The difference comes first: it is
+// exact where it matters, however large the logits are, and a mask of fp32's
+// lowest value only makes it -inf, whose weight 2^y is 0.  Where y is also a
+// factor it is clamped at RW_LOW, where the weight is 0 too; a NaN stays one (a
+// row that holds NaN or +inf has the sum NaN).
 constexpr float RW_LOW = -200.0f;
-__device__ __forceinline__ float rw_exponent(float x, float m, float c) { return rw_max_nan((x - m) * c, RW_LOW); }
 
 // What a row's sums are relative to before a logit was seen: the lowest
 // finite number, so that -inf has the weight 0 and not NaN.
 constexpr float RW_LOWEST = -3.402823466e38f;
-
-template <class T>
-__device__ __forceinline__ T rw_block_sum(T v, T* part) {             // the same in every thread
-    for (int i = 16; i; i >>= 1) v += __shfl_xor_sync(~0u, v, i);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = part[0];
-    for (int w = 1; w < RW_WARPS; ++w) v += part[w];
-    return v;
-}
-__device__ __forceinline__ float rw_block_max(float v, float* part) {   // NaN is passed over
-    for (int i = 16; i; i >>= 1) v = fmaxf(v, __shfl_xor_sync(~0u, v, i));
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = part[0];
-    for (int w = 1; w < RW_WARPS; ++w) v = fmaxf(v, part[w]);
-    return v;
-}
 
 // ---------------------------------------------------------------------------
 // A row in units of 32 bytes (8 fp32 logits, 16 of the 16-bit types), one load
