@@ -286,13 +286,23 @@ def _check_vector(fn, name, t, n, code, device):
         raise TierkError(TK_ERR_INVALID, f"{fn}: {name} is not on device {device}")
 
 
+def _vector(fn, name, t, n, code, device):
+    """_check_vector, and the address."""
+    if t is None:
+        return None
+    if not (t.dtype is _DTYPES.get(code) and t.get_device() == device and t.numel() >= n and t.is_contiguous()):
+        _check_vector(fn, name, t, n, code, device)
+    return t.data_ptr()
+
+
 def _width(fn, name, t, n):
     """The columns of a contiguous matrix of n rows (None: 0)."""
     if t is None:
         return 0
-    if t.dim() != 2 or t.size(0) != n:
+    shape = t.shape
+    if len(shape) != 2 or shape[0] != n:
         raise TierkError(TK_ERR_INVALID, f"{fn}: {name} must be a matrix of {n} rows")
-    return t.size(1)
+    return shape[1]
 
 
 _I32 = -1
@@ -475,15 +485,12 @@ class Context:
         fn, dev, (n, V) = "tk_logprobs", self.device, logits.shape
         k = _width(fn, "top_ids", top_ids, n)
         ldx = _row_stride(fn, "logits", logits, x_dtype, n, V, None, dev)
-        _check_vector(fn, "tokens", tokens, n, _I32, dev)
-        _check_vector(fn, "logp", logp, n, DT_F32, dev)
-        _check_vector(fn, "entropy", entropy, n, DT_F32, dev)
-        _check_vector(fn, "rmax", rmax, n, DT_F32, dev)
-        _check_vector(fn, "rsum", rsum, n, DT_F32, dev)
-        _check_vector(fn, "top_ids", top_ids, n * k, _I32, dev)
-        _check_vector(fn, "top_logp", top_logp, n * k, DT_F32, dev)
-        _check(self.lib.tk_logprobs(self.h, n, V, _ptr(logits), x_dtype, ldx, _ptr(tokens), temperature, _ptr(logp),
-                                    _ptr(entropy), _ptr(rmax), _ptr(rsum), k, _ptr(top_ids), _ptr(top_logp), _stream(stream)))
+        _check(self.lib.tk_logprobs(self.h, n, V, _ptr(logits), x_dtype, ldx, _vector(fn, "tokens", tokens, n, _I32, dev),
+                                    temperature, _vector(fn, "logp", logp, n, DT_F32, dev),
+                                    _vector(fn, "entropy", entropy, n, DT_F32, dev), _vector(fn, "rmax", rmax, n, DT_F32, dev),
+                                    _vector(fn, "rsum", rsum, n, DT_F32, dev), k,
+                                    _vector(fn, "top_ids", top_ids, n * k, _I32, dev),
+                                    _vector(fn, "top_logp", top_logp, n * k, DT_F32, dev), _stream(stream)))
         return logp
 
     def logprobs_grad(self, logits, tokens, rmax, rsum, dlogits, d_logp=None, entropy=None, d_entropy=None, temperature=1.0,
@@ -494,14 +501,12 @@ class Context:
         d_dtype = x_dtype if d_dtype is None else d_dtype
         ldx = _row_stride(fn, "logits", logits, x_dtype, n, V, None, dev)
         ldd = _row_stride(fn, "dlogits", dlogits, d_dtype, n, V, None, dev)
-        _check_vector(fn, "tokens", tokens, n, _I32, dev)
-        _check_vector(fn, "rmax", rmax, n, DT_F32, dev)
-        _check_vector(fn, "rsum", rsum, n, DT_F32, dev)
-        _check_vector(fn, "d_logp", d_logp, n, DT_F32, dev)
-        _check_vector(fn, "entropy", entropy, n, DT_F32, dev)
-        _check_vector(fn, "d_entropy", d_entropy, n, DT_F32, dev)
-        _check(self.lib.tk_logprobs_grad(self.h, n, V, _ptr(logits), x_dtype, ldx, _ptr(tokens), temperature, _ptr(rmax),
-                                         _ptr(rsum), _ptr(d_logp), _ptr(entropy), _ptr(d_entropy), _ptr(dlogits), d_dtype, ldd,
+        _check(self.lib.tk_logprobs_grad(self.h, n, V, _ptr(logits), x_dtype, ldx, _vector(fn, "tokens", tokens, n, _I32, dev),
+                                         temperature, _vector(fn, "rmax", rmax, n, DT_F32, dev),
+                                         _vector(fn, "rsum", rsum, n, DT_F32, dev),
+                                         _vector(fn, "d_logp", d_logp, n, DT_F32, dev),
+                                         _vector(fn, "entropy", entropy, n, DT_F32, dev),
+                                         _vector(fn, "d_entropy", d_entropy, n, DT_F32, dev), _ptr(dlogits), d_dtype, ldd,
                                          _stream(stream)))
         return dlogits
 
@@ -513,15 +518,11 @@ class Context:
         d_dtype, k = x_dtype if d_dtype is None else d_dtype, _width(fn, "ids", ids, n)
         ldx = _row_stride(fn, "logits", logits, x_dtype, n, V, None, dev)
         ldd = _row_stride(fn, "dlogits", dlogits, d_dtype, n, V, None, dev)
-        _check_vector(fn, "ids", ids, n * k, _I32, dev)
-        _check_vector(fn, "teacher", teacher, n * k, DT_F32, dev)
-        _check_vector(fn, "weight", weight, n, DT_F32, dev)
-        _check_vector(fn, "loss", loss, n, DT_F32, dev)
-        _check_vector(fn, "rmax", rmax, n, DT_F32, dev)
-        _check_vector(fn, "rsum", rsum, n, DT_F32, dev)
-        _check(self.lib.tk_distill(self.h, n, V, _ptr(logits), x_dtype, ldx, k, _ptr(ids), _ptr(teacher), temperature,
-                                   _ptr(weight), _ptr(loss), _ptr(rmax), _ptr(rsum), _ptr(dlogits), d_dtype, ldd,
-                                   _stream(stream)))
+        _check(self.lib.tk_distill(self.h, n, V, _ptr(logits), x_dtype, ldx, k, _vector(fn, "ids", ids, n * k, _I32, dev),
+                                   _vector(fn, "teacher", teacher, n * k, DT_F32, dev), temperature,
+                                   _vector(fn, "weight", weight, n, DT_F32, dev), _vector(fn, "loss", loss, n, DT_F32, dev),
+                                   _vector(fn, "rmax", rmax, n, DT_F32, dev), _vector(fn, "rsum", rsum, n, DT_F32, dev),
+                                   _ptr(dlogits), d_dtype, ldd, _stream(stream)))
         return loss
 
     def distill_grad(self, logits, ids, teacher, rmax, rsum, dlogits, weight=None, temperature=1.0, x_dtype=DT_F32, d_dtype=None,
@@ -531,13 +532,11 @@ class Context:
         d_dtype, k = x_dtype if d_dtype is None else d_dtype, _width(fn, "ids", ids, n)
         ldx = _row_stride(fn, "logits", logits, x_dtype, n, V, None, dev)
         ldd = _row_stride(fn, "dlogits", dlogits, d_dtype, n, V, None, dev)
-        _check_vector(fn, "ids", ids, n * k, _I32, dev)
-        _check_vector(fn, "teacher", teacher, n * k, DT_F32, dev)
-        _check_vector(fn, "rmax", rmax, n, DT_F32, dev)
-        _check_vector(fn, "rsum", rsum, n, DT_F32, dev)
-        _check_vector(fn, "weight", weight, n, DT_F32, dev)
-        _check(self.lib.tk_distill_grad(self.h, n, V, _ptr(logits), x_dtype, ldx, k, _ptr(ids), _ptr(teacher), temperature,
-                                        _ptr(rmax), _ptr(rsum), _ptr(weight), _ptr(dlogits), d_dtype, ldd, _stream(stream)))
+        _check(self.lib.tk_distill_grad(self.h, n, V, _ptr(logits), x_dtype, ldx, k, _vector(fn, "ids", ids, n * k, _I32, dev),
+                                        _vector(fn, "teacher", teacher, n * k, DT_F32, dev), temperature,
+                                        _vector(fn, "rmax", rmax, n, DT_F32, dev), _vector(fn, "rsum", rsum, n, DT_F32, dev),
+                                        _vector(fn, "weight", weight, n, DT_F32, dev), _ptr(dlogits), d_dtype, ldd,
+                                        _stream(stream)))
         return dlogits
 
     # ---- reduce-scatter over peer memory (multi-GPU) ----

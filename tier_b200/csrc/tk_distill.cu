@@ -291,17 +291,7 @@ static int ds_parts(const tk_ctx* ctx, int n_rows, int vocab, long row_bytes, bo
 template <class XT, class DT>
 static cudaError_t launch_ds(const tk_ctx* ctx, DsArgs& a, cudaStream_t s) {
     a.parts = ds_parts(ctx, a.r.n_rows, a.r.vocab, (long)a.r.vocab * sizeof(XT), !std::is_same<DT, void>::value);
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)((long)a.r.n_rows * a.parts));
-    cfg.blockDim = dim3(RW_THREADS);
-    cfg.stream = s;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = a.parts;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, ds_kernel<XT, DT>, a);
+    return rw_launch(ds_kernel<XT, DT>, a.r.n_rows, a.parts, true, 0, a, s);
 }
 tk_status launch_distill(tk_ctx* ctx, const RowArgs& r, int x_dtype, int k, const int32_t* ids, const float* teacher,
                          const float* weight, float* loss, float* rmax, float* rsum, int d_dtype, cudaStream_t s) {
@@ -321,8 +311,7 @@ tk_status launch_distill_grad(tk_ctx* ctx, const RowArgs& r, int x_dtype, int k,
     ctx->launches += 1;
     return cuda_fail(rw_types(x_dtype, d_dtype, [&](auto x, auto d) {
         a.parts = rw_grad_parts<decltype(x)>(ctx, a.r.n_rows, a.r.vocab);
-        dg_kernel<decltype(x), decltype(d)><<<(unsigned)((long)a.r.n_rows * a.parts), RW_THREADS, 0, s>>>(a);
-        return cudaGetLastError();
+        return rw_launch(dg_kernel<decltype(x), decltype(d)>, a.r.n_rows, a.parts, false, 0, a, s);
     }), "distillation gradient launch");
 }
 

@@ -471,18 +471,7 @@ static cudaError_t launch_lp(const tk_ctx* ctx, LpArgs& a, cudaStream_t s) {
     constexpr int MOST = (int)sizeof(LpTop) + LP_CLUSTER * TK_TOP_MAX * (int)sizeof(unsigned long long);
     const cudaError_t e = TOP ? smem_attr_once(kern, MOST, ctx->device, attr_smem) : cudaSuccess;
     if (e != cudaSuccess) return e;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)((long)a.r.n_rows * a.parts));
-    cfg.blockDim = dim3(RW_THREADS);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = s;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = a.parts;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kern, a);
+    return rw_launch(kern, a.r.n_rows, a.parts, true, smem, a, s);
 }
 tk_status launch_logprobs(tk_ctx* ctx, const RowArgs& r, int x_dtype, const int32_t* tokens, float* logp, float* entropy,
                           float* rmax, float* rsum, int top_k, int32_t* top_ids, float* top_logp, cudaStream_t s) {
@@ -502,10 +491,7 @@ tk_status launch_logprobs(tk_ctx* ctx, const RowArgs& r, int x_dtype, const int3
 template <class XT, class DT>
 static cudaError_t launch_lg(const tk_ctx* ctx, LgArgs& a, cudaStream_t s) {
     a.parts = rw_grad_parts<XT>(ctx, a.r.n_rows, a.r.vocab);
-    const unsigned grid = (unsigned)((long)a.r.n_rows * a.parts);
-    if (a.d_entropy) lg_kernel<XT, DT, true><<<grid, RW_THREADS, 0, s>>>(a);
-    else lg_kernel<XT, DT, false><<<grid, RW_THREADS, 0, s>>>(a);
-    return cudaGetLastError();
+    return rw_launch(a.d_entropy ? lg_kernel<XT, DT, true> : lg_kernel<XT, DT, false>, a.r.n_rows, a.parts, false, 0, a, s);
 }
 tk_status launch_logprobs_grad(tk_ctx* ctx, const RowArgs& r, int x_dtype, const int32_t* tokens, const float* rmax,
                                const float* rsum, const float* entropy, const float* d_logp, const float* d_entropy,

@@ -420,6 +420,25 @@ inline int rw_grad_parts(const tk_ctx* ctx, int n_rows, int vocab) {
     return few > half ? few < batches ? few : batches : half;
 }
 
+// Launch of n_rows * parts blocks, in clusters of `parts` where they meet.  (As
+// programmatic dependents, whose blocks wait in their places for the call
+// before: calls in a row 9.4 -> 10.5 us, 29 -> 31, 10.2 -> 10.0, large ones alike.)
+template <class A>
+inline cudaError_t rw_launch(void (*kern)(A), long n_rows, int parts, bool cluster, size_t smem, const A& a, cudaStream_t s) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(n_rows * parts));
+    cfg.blockDim = dim3(RW_THREADS);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = parts;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = cluster && parts > 1 ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, kern, a);
+}
+
 // launch(x, d) with values of the logits' and the gradient's element types.
 template <class F>
 inline cudaError_t rw_types(int x_dtype, int d_dtype, F launch) {
