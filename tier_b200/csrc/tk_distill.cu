@@ -132,17 +132,15 @@ struct DsHeld {
                 part[j][h][threadIdx.x] = make_uint4(u[j].w[4 * h], u[j].w[4 * h + 1], u[j].w[4 * h + 2], u[j].w[4 * h + 3]);
     }
     template <class XT>
-    __device__ __forceinline__ void take(RwUnit<XT> (&u)[RW_BATCH]) const {
+    __device__ __forceinline__ void take(RwUnit<XT>& u, int j) const {
 #pragma unroll
-        for (int j = 0; j < RW_BATCH; ++j)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const uint4 q = part[j][h][threadIdx.x];
-                u[j].w[4 * h] = q.x;
-                u[j].w[4 * h + 1] = q.y;
-                u[j].w[4 * h + 2] = q.z;
-                u[j].w[4 * h + 3] = q.w;
-            }
+        for (int h = 0; h < 2; ++h) {
+            const uint4 q = part[j][h][threadIdx.x];
+            u.w[4 * h] = q.x;
+            u.w[4 * h + 1] = q.y;
+            u.w[4 * h + 2] = q.z;
+            u.w[4 * h + 3] = q.w;
+        }
     }
 };
 
@@ -234,13 +232,28 @@ __global__ void __launch_bounds__(RW_THREADS, 4) ds_kernel(const DsArgs a) {
         const RwDense<false> dense{st.m, c, wt / (float)st.s, 0.0f};
         DT* d = dx + p.first;
         if (rw_alike<XT>(d)) {
-            while (true) {
+            rw_write<XT>(u, d, p, u0, dense);
+            const bool first = u0 > 0;             // there is a held batch
+            u0 -= STEP;
+            if (u0 > 0) rw_batch<XT>(u, p, u0);
+            const auto write_held = [&]() {
+#pragma unroll 2
+                for (int j = 0; j < RW_BATCH; ++j) {
+                    RwUnit<XT> w[1];
+                    held.take(w[0], j);
+                    rw_write<XT>(w, d, p, j * RW_THREADS, dense);
+                }
+            };
+            // fp32 rows: while the others are on their way (512 x 262144 to bf16 151 ->
+            // 144 us; 16-bit rows, whose conversions need the registers, 2048 x 262144
+            // 385 -> 392)
+            constexpr bool early = sizeof(XT) == 4;
+            if (early && first) write_held();
+            for (; u0 > 0; u0 -= STEP) {
                 rw_write<XT>(u, d, p, u0, dense);
-                if (u0 == 0) break;
-                u0 -= STEP;
-                if (u0) rw_batch<XT>(u, p, u0);
-                else held.take(u);
+                if (u0 > STEP) rw_batch<XT>(u, p, u0 - STEP);
             }
+            if (!early && first) write_held();
         } else
             rw_write_other<XT>(d, p, dense);
         if (end) dx[e.place(tid)] = rw_to<DT>(dense.one(v_end));
