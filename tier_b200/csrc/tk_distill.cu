@@ -1,6 +1,25 @@
 // tk_distill.cu -- tk_distill, tk_distill_grad: distillation from a teacher's
 // top logits.
-#include <climits>
+//
+// loss = sum q (ln q - ln p), of which sum q ln q and sum q l need the listed
+// places alone and ln S a reading of the row; the gradient (w / T) (p - q) is
+// dense but for q, which a second write puts in at the listed places.
+//
+// Loss and gradient in one call read the row from memory once and write the
+// gradient once; the row's second reading is served on the chip.  The bound is
+// memory; what keeps the call from it is the second reading (without it 331 us
+// where the call took 409, before a batch was held), blocks that meet between the
+// passes, and two exponentials a logit (without them 50 of 753 us, 100 where
+// long runs lower the clock).  Tried and slower: blocks that stay and take rows in
+// turn (498 to 604 us where this took 425: all read, meet and write at the same
+// time), both passes as tasks of a queue, gradients some rows behind the sums
+// (485: the rows between them pass the L2), a part's whole length in shared
+// memory (no room in the L1 for loads on their way: 506 and more), 512 or 1024
+// threads a block (427, 426).
+//
+// Measured (us; calls in a graph): 4096 x 262144 bf16 760 (5.5 TB/s of floor
+// bytes), 512 x 262144 fp32 to bf16 144, 16 x 50257 fp16 8.2; the loss of 300 x
+// 131072 fp32 29; the gradient alone 2048 x 262144 bf16 317 (6.8 TB/s).
 #include <type_traits>
 #include "tk_rows.cuh"
 

@@ -1,6 +1,28 @@
 // tk_logprobs.cu -- tk_logprobs, tk_logprobs_grad: log-probabilities of given
 // tokens, entropy, the likeliest tokens, and the gradient of the first two.
-#include <climits>
+//
+// With y = (l - m) / T and weights e^y, S = sum e^y and A = sum e^y y:
+// ln p = y - ln S and the entropy is ln S - A / S, two positive terms.  Both sums
+// come from one reading: m is a running maximum of each thread, to which its
+// sums are scaled again when it moves, and parts are brought together in 64
+// bits.  The bound is memory; for 16-bit rows an exponential a logit (16 a
+// clock and SM, 62 % of them busy) and six other instructions come near it.
+//
+// The largest logits cost little beside that reading: of each 32-byte unit its
+// maximum is kept, cut to 16 bits, a bound is found that enough logits reach,
+// and only units that reach it are read again.  (Kept per thread and batch
+// instead, a list of 128 read a fifth of a bf16 row again: 1024 rows of 262144
+// 129 us, now 103; every alternative by a pass of its own 27 ms.)  What the
+// search holds in shared memory is small on purpose: loads on their way need
+// the L1 (53 KB a block instead of 43: 1024 rows 112 us, 4096 404 instead of 369).
+//
+// The gradient reads every logit and writes every gradient once.
+//
+// Measured (us; calls in a graph, L2 warm): 1 row of 262144 fp32, 20
+// alternatives 10.0 (of them launch 3, the reading 3, the search 3, the meeting
+// of 8 blocks 1); 48 of 50257, 5 alternatives 10.0; 4095 x 262144 fp32, none 534
+// (7.2 TB/s); 1024 x 262144 bf16 without 85 (6.3 TB/s), 20 97, 128 103, 256 112.
+// Gradients of 2048 x 131072 bf16, 30 % of the rows left out, 141 (6.5 TB/s).
 #include "tk_rows.cuh"
 
 namespace tk {
@@ -8,8 +30,8 @@ namespace tk {
 constexpr int LP_SLOTS = 16;          // for the largest logits of a thread's batches
 constexpr int LP_LIST = 1024;         // units that can be listed to be looked through again
 constexpr int LP_KEEP = 1024;         // candidates a block can hold
-constexpr int LP_SORT = 2 * RW_THREADS;   // and puts in order by counting
-constexpr int LP_AHEAD = 2;           // units on their way when groups are looked through again
+constexpr int LP_SORT = 2 * RW_THREADS;   // and puts in order
+constexpr int LP_AHEAD = 2;           // units on their way when they are looked through again
 constexpr int LP_CLUSTER = 8;         // blocks of a row at most
 
 struct LpArgs {
@@ -87,14 +109,15 @@ __device__ __noinline__ unsigned long long lp_thin(LpTop& t, int k, int& turn) {
 }
 
 // The block's candidates: a set that holds the top_k largest logits of its part
-// (or all).  With v0 and v1, the largest logits of the thread's units' first and second halves,
-// a bound is found that top_k of these reach, so top_k logits do (256 or 512
-// numbers, one counting barrier a bit); only units that reach it are read
-// again, little more than top_k of them for logits in any order, a sector of
-// memory each.  Where many logits are alike or the largest stand together,
+// (or all).  With v0 and v1, the largest logits of the first and the second
+// halves of each thread's units, a bound is found that top_k of these reach, so
+// top_k logits do (256 or 512 numbers, one counting barrier a bit); only units
+// that reach it are read again, little more than top_k of them for logits in
+// any order, a sector of memory each.  Where many logits are alike or the largest stand together,
 // candidates that do not fit are thinned on the way.
 template <class XT>
-__device__ __forceinline__ void lp_search(LpTop& t, const LpArgs& a, const XT* row, const RwPart<XT>& p, bool ends, float v0, float v1) {
+__device__ __forceinline__ void lp_search(LpTop& t, const LpArgs& a, const XT* row, const RwPart<XT>& p, bool ends,
+                                          float v0, float v1) {
     constexpr int N = RwUnit<XT>::N;
     const int tid = threadIdx.x, k = a.top_k;
     if (tid == 0) t.n = t.listed = 0;
@@ -276,8 +299,8 @@ __device__ __forceinline__ void lp_ordered(LpTop& t, int k) {
 }
 
 // A cluster of blocks per row, each with one part of it.  Every logit is read
-// once, for the sums and for the largest of each group of logits; the blocks'
-// sums and candidates meet in shared memory.
+// once, for the sums and for the largest of each unit; the blocks' sums and
+// candidates meet in shared memory.
 template <class XT, bool ENT, bool TOP>
 __global__ void __launch_bounds__(RW_THREADS, 4) lp_kernel(const LpArgs a) {
     extern __shared__ __align__(16) char lp_smem[];
@@ -450,17 +473,22 @@ __global__ void __launch_bounds__(RW_THREADS, 4) lg_kernel(const LgArgs a) {
     rw_gradient<XT, DT, ENT>(x, dx, vocab, p, rank == a.parts - 1, ids, sub, 1, 1.0f, dense);
 }
 
-// Blocks of a row, for few rows: 8192 logits each at least.
-static int lp_parts(const tk_ctx* ctx, int n_rows, int vocab, bool top) {
-    const long most = top ? ctx->num_sms : 4L * ctx->num_sms;
+// Blocks of a row: for few rows as many as the GPU holds at once, of 8192
+// logits each at least.  us by blocks a row 1, 2, 4, 8, without and with 20
+// alternatives, whose search each block does: 1 row of 262144 fp32 19, 12, 8.4,
+// 6.1 and 25, 18, 12.9, 10.4; 32 of them 20, 13, 9.2, 7.8 and 26, 19, 13.5, 12.1;
+// 48 of 50257 7.2, 6.6, 6.1, 5.7 and 11.3, 10.9, 10.4, 10.9; 100 of 131072 bf16
+// 10.4, 10.7, 9.4, 10.9 and 14.8, 15.6, 14.1, 20.9; 256 of 262144 bf16 32, 30,
+// 32, 37 and 38, 37, 43, 57.
+static int lp_parts(const tk_ctx* ctx, int n_rows, int vocab) {
     int parts = 1;
-    while (parts < LP_CLUSTER && 2L * n_rows * parts <= most && vocab / (2 * parts) >= 8192) parts *= 2;
+    while (parts < LP_CLUSTER && 2L * n_rows * parts <= 4L * ctx->num_sms && vocab / (2 * parts) >= 8192) parts *= 2;
     return parts;
 }
 
 template <class XT, bool ENT, bool TOP>
 static cudaError_t launch_lp(const tk_ctx* ctx, LpArgs& a, cudaStream_t s) {
-    a.parts = lp_parts(ctx, a.r.n_rows, a.r.vocab, TOP);
+    a.parts = lp_parts(ctx, a.r.n_rows, a.r.vocab);
     const int each = ((a.r.vocab / RwUnit<XT>::N + a.parts - 1) / a.parts + 31) & ~31;
     const int batches = (each + RW_THREADS * RW_BATCH - 1) / (RW_THREADS * RW_BATCH);
     while (batches > LP_SLOTS << a.shift) ++a.shift;
