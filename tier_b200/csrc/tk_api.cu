@@ -762,7 +762,7 @@ static tk_status rows_check(const char* fn, tk_ctx* ctx, int n_rows, int vocab, 
         if (!same && !(sa == sb && off >= wa && off + wb <= sa)) return fail(TK_ERR_INVALID, std::string(fn) + ": gradient overlaps the logits");
     }
     r = RowArgs{n_rows, vocab, x, ldx, (float)(1.4426950408889634 / (double)temperature), (float)(1.0 / (double)temperature), dx,
-                ldd, ctx->status};
+                ldd, ctx->status, false};
     return TK_OK;
 }
 

@@ -174,6 +174,7 @@ __global__ void __launch_bounds__(RW_THREADS, 4) ds_kernel(const DsArgs a) {
     __shared__ typename std::conditional<GRAD, DsHeld, int>::type held;
     __shared__ DsTeacher t;
     __shared__ RwStat join[DS_CLUSTER * RW_WARPS];
+    pdl_wait();
     const size_t row = blockIdx.x / a.parts;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, vocab = a.r.vocab, rank = blockIdx.x % a.parts;
     const float c = a.r.c;
@@ -225,6 +226,7 @@ __global__ void __launch_bounds__(RW_THREADS, 4) ds_kernel(const DsArgs a) {
         add();
         if (++batch % 16 == 0) sums.flush(c);
     }
+    if (a.r.few) pdl_trigger();
     if (entry < a.k) t.x[entry] = listed;
     sums.single(v_end, c);
     sums.flush(c);
@@ -286,6 +288,8 @@ __global__ void __launch_bounds__(RW_THREADS, 4) ds_kernel(const DsArgs a) {
 template <class XT, class DT>
 __global__ void __launch_bounds__(RW_THREADS, 4) dg_kernel(const DsArgs a) {
     __shared__ DsTeacher t;
+    if (a.r.few) pdl_trigger();
+    pdl_wait();
     const size_t row = blockIdx.x / a.parts;
     const int tid = threadIdx.x, vocab = a.r.vocab, rank = blockIdx.x % a.parts;
     const XT* x = static_cast<const XT*>(a.r.x) + row * a.r.ldx;
@@ -323,6 +327,7 @@ static int ds_parts(const tk_ctx* ctx, int n_rows, int vocab, long row_bytes, bo
 template <class XT, class DT>
 static cudaError_t launch_ds(const tk_ctx* ctx, DsArgs& a, cudaStream_t s) {
     a.parts = ds_parts(ctx, a.r.n_rows, a.r.vocab, (long)a.r.vocab * sizeof(XT), !std::is_same<DT, void>::value);
+    a.r.few = rw_few(ctx, a.r.n_rows, a.parts);
     return rw_launch(ds_kernel<XT, DT>, a.r.n_rows, a.parts, true, 0, a, s);
 }
 tk_status launch_distill(tk_ctx* ctx, const RowArgs& r, int x_dtype, int k, const int32_t* ids, const float* teacher,
@@ -343,6 +348,7 @@ tk_status launch_distill_grad(tk_ctx* ctx, const RowArgs& r, int x_dtype, int k,
     ctx->launches += 1;
     return cuda_fail(rw_types(x_dtype, d_dtype, [&](auto x, auto d) {
         a.parts = rw_grad_parts<decltype(x)>(ctx, a.r.n_rows, a.r.vocab);
+        a.r.few = rw_few(ctx, a.r.n_rows, a.parts);
         return rw_launch(dg_kernel<decltype(x), decltype(d)>, a.r.n_rows, a.parts, false, 0, a, s);
     }), "distillation gradient launch");
 }

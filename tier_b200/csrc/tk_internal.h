@@ -218,6 +218,7 @@ struct RowArgs {              // what they have in common
     void* dx;                 // their gradient
     long ldd;
     int* status;
+    bool few;                 // the GPU holds all blocks at once (set at the launch)
 };
 tk_status launch_logprobs(tk_ctx* ctx, const RowArgs& r, int x_dtype, const int32_t* tokens, float* logp, float* entropy,
                           float* rmax, float* rsum, int top_k, int32_t* top_ids, float* top_logp, cudaStream_t s);

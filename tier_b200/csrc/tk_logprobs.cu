@@ -306,6 +306,7 @@ __global__ void __launch_bounds__(RW_THREADS, 4) lp_kernel(const LpArgs a) {
     extern __shared__ __align__(16) char lp_smem[];
     __shared__ RwStat join[RW_WARPS], parts[LP_CLUSTER];
     LpTop& t = *reinterpret_cast<LpTop*>(lp_smem);                                       // TOP
+    pdl_wait();
     const size_t row = blockIdx.x / a.parts;
     const int tid = threadIdx.x, vocab = a.r.vocab, rank = blockIdx.x % a.parts, k = a.top_k;
     const float c = a.r.c;
@@ -336,37 +337,42 @@ __global__ void __launch_bounds__(RW_THREADS, 4) lp_kernel(const LpArgs a) {
         if (tid < e.n) sums.single(rw_float(x[e.place(tid)]), c);
     }
     const f32x2 c2 = pack2(c, c);
-    float big[RW_BATCH] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, v0 = -INFINITY, v1 = -INFINITY;
-    int batch = 0, slot = 0;
-    const int share = (1 << a.shift) - 1;
-    const auto store = [&]() {
-        t.big[slot++][tid] = make_uint2(__byte_perm(__float_as_uint(big[0]), __float_as_uint(big[1]), 0x7632),
-                                        __byte_perm(__float_as_uint(big[2]), __float_as_uint(big[3]), 0x7632));
+    float v0 = -INFINITY, v1 = -INFINITY;
+    int batch = 0;
+    // (several batches may share a slot)
+    const auto keep = [&](const float (&v)[RW_BATCH]) {
+        uint2& slot = t.big[batch >> a.shift][tid];
+        float m[RW_BATCH] = {v[0], v[1], v[2], v[3]};
+        if (batch & ((1 << a.shift) - 1)) {
+            const uint2 o = slot;
+            m[0] = fmaxf(m[0], __uint_as_float(o.x << 16));
+            m[1] = fmaxf(m[1], __uint_as_float(o.x & 0xffff0000u));
+            m[2] = fmaxf(m[2], __uint_as_float(o.y << 16));
+            m[3] = fmaxf(m[3], __uint_as_float(o.y & 0xffff0000u));
+        }
+        slot = make_uint2(__byte_perm(__float_as_uint(m[0]), __float_as_uint(m[1]), 0x7632),
+                          __byte_perm(__float_as_uint(m[2]), __float_as_uint(m[3]), 0x7632));
     };
     for (int u0 = 0; u0 < p.n; u0 += RW_THREADS * RW_BATCH) {
         RwUnit<XT> u[RW_BATCH];
         rw_batch<XT>(u, p, u0);
-        float top = -INFINITY;
+        float v[RW_BATCH], top = -INFINITY;
 #pragma unroll
         for (int j = 0; j < RW_BATCH; ++j) {
-            const float lo = u[j].max(0), hi = u[j].max(1), v = fmaxf(lo, hi);
+            const float lo = u[j].max(0), hi = u[j].max(1);
+            v[j] = fmaxf(lo, hi);
             if (TOP) {
                 v0 = fmaxf(v0, lo);
                 v1 = fmaxf(v1, hi);
-                big[j] = fmaxf(big[j], v);
             }
-            top = fmaxf(top, v);
+            top = fmaxf(top, v[j]);
         }
+        if (TOP) keep(v);
         if (top > sums.m) sums.raise(top, c);
         sums.batch(u, c2);
         if (++batch % 16 == 0) sums.flush(c);      // (at most 16 batches are added in fp32)
-        if (TOP && (batch & share) == 0) {
-            store();
-#pragma unroll
-            for (int j = 0; j < RW_BATCH; ++j) big[j] = -INFINITY;
-        }
     }
-    if (TOP && (batch & share)) store();
+    if (a.r.few) pdl_trigger();                    // (earlier, the next call's blocks would take cache from the loads)
     sums.flush(c);
     const RwStat w = rw_warp_join<ENT>(RwStat{sums.M, sums.S, sums.A}, c);
     if ((tid & 31) == 0) join[tid >> 5] = w;
@@ -449,6 +455,8 @@ template <class XT, class DT, bool ENT>
 __global__ void __launch_bounds__(RW_THREADS, 4) lg_kernel(const LgArgs a) {
     __shared__ __align__(16) int ids[4];
     __shared__ float sub[4];
+    if (a.r.few) pdl_trigger();
+    pdl_wait();
     const size_t row = blockIdx.x / a.parts;
     const int vocab = a.r.vocab, rank = blockIdx.x % a.parts;
     const XT* x = static_cast<const XT*>(a.r.x) + row * a.r.ldx;
@@ -489,6 +497,7 @@ static int lp_parts(const tk_ctx* ctx, int n_rows, int vocab) {
 template <class XT, bool ENT, bool TOP>
 static cudaError_t launch_lp(const tk_ctx* ctx, LpArgs& a, cudaStream_t s) {
     a.parts = lp_parts(ctx, a.r.n_rows, a.r.vocab);
+    a.r.few = rw_few(ctx, a.r.n_rows, a.parts);
     const int each = ((a.r.vocab / RwUnit<XT>::N + a.parts - 1) / a.parts + 31) & ~31;
     const int batches = (each + RW_THREADS * RW_BATCH - 1) / (RW_THREADS * RW_BATCH);
     while (batches > LP_SLOTS << a.shift) ++a.shift;
@@ -519,6 +528,7 @@ tk_status launch_logprobs(tk_ctx* ctx, const RowArgs& r, int x_dtype, const int3
 template <class XT, class DT>
 static cudaError_t launch_lg(const tk_ctx* ctx, LgArgs& a, cudaStream_t s) {
     a.parts = rw_grad_parts<XT>(ctx, a.r.n_rows, a.r.vocab);
+    a.r.few = rw_few(ctx, a.r.n_rows, a.parts);
     return rw_launch(a.d_entropy ? lg_kernel<XT, DT, true> : lg_kernel<XT, DT, false>, a.r.n_rows, a.parts, false, 0, a, s);
 }
 tk_status launch_logprobs_grad(tk_ctx* ctx, const RowArgs& r, int x_dtype, const int32_t* tokens, const float* rmax,

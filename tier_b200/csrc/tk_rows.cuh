@@ -420,9 +420,12 @@ inline int rw_grad_parts(const tk_ctx* ctx, int n_rows, int vocab) {
     return few > half ? few < batches ? few : batches : half;
 }
 
-// Launch of n_rows * parts blocks, in clusters of `parts` where they meet.  (As
-// programmatic dependents, whose blocks wait in their places for the call
-// before: calls in a row 9.4 -> 10.5 us, 29 -> 31, 10.2 -> 10.0, large ones alike.)
+inline bool rw_few(const tk_ctx* ctx, long n_rows, int parts) { return n_rows * parts <= 4L * ctx->num_sms; }
+
+// Launch of n_rows * parts blocks, in clusters of `parts` where they meet, as a
+// programmatic dependent: every block waits, first of all, for the kernel before
+// to end, and is in its place by then.  Only calls of few blocks let the next
+// one's come early; large ones gain nothing.
 template <class A>
 inline cudaError_t rw_launch(void (*kern)(A), long n_rows, int parts, bool cluster, size_t smem, const A& a, cudaStream_t s) {
     cudaLaunchConfig_t cfg = {};
@@ -430,12 +433,14 @@ inline cudaError_t rw_launch(void (*kern)(A), long n_rows, int parts, bool clust
     cfg.blockDim = dim3(RW_THREADS);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = parts;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = parts;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = cluster && parts > 1 ? 1 : 0;
+    cfg.numAttrs = cluster && parts > 1 ? 2 : 1;
     return cudaLaunchKernelEx(&cfg, kern, a);
 }
 
