@@ -18,7 +18,7 @@
 // threads a block (427, 426).
 //
 // Measured (us; calls in a graph): 4096 x 262144 bf16 760 (5.5 TB/s of floor
-// bytes), 512 x 262144 fp32 to bf16 144, 16 x 50257 fp16 8.2; the loss of 300 x
+// bytes), 512 x 262144 fp32 to bf16 144, 16 x 50257 fp16 7.8; the loss of 300 x
 // 131072 fp32 29; the gradient alone 2048 x 262144 bf16 317 (6.8 TB/s).
 #include <type_traits>
 #include "tk_rows.cuh"

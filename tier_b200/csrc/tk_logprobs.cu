@@ -19,10 +19,10 @@
 // The gradient reads every logit and writes every gradient once.
 //
 // Measured (us; calls in a graph, L2 warm): 1 row of 262144 fp32, 20
-// alternatives 10.0 (of them launch 3, the reading 3, the search 3, the meeting
-// of 8 blocks 1); 48 of 50257, 5 alternatives 10.0; 4095 x 262144 fp32, none 534
-// (7.2 TB/s); 1024 x 262144 bf16 without 85 (6.3 TB/s), 20 97, 128 103, 256 112.
-// Gradients of 2048 x 131072 bf16, 30 % of the rows left out, 141 (6.5 TB/s).
+// alternatives 9.9 (of them the reading 3, the search 3, the meeting of 8 blocks
+// 1); 48 of 50257, 5 alternatives 9.8; 4095 x 262144 fp32, none 533 (7.2 TB/s);
+// 1024 x 262144 bf16 without 85 (6.3 TB/s), 20 97, 128 103, 256 112. Gradients
+// of 2048 x 131072 bf16, 30 % of the rows left out, 141 (6.5 TB/s).
 #include "tk_rows.cuh"
 
 namespace tk {
