@@ -135,7 +135,8 @@ uint64_t tk_launch_count(const tk_ctx *ctx);
  * (ms) and number of recorded launches of one kernel family.  TK_PROF_COMM:
  * the reduce-scatter's owner reduce (with its wait for the peers' tiles) and
  * the peer collectives' kernels.  TK_PROF_SERVE: the key/value cache, the
- * attention over it and the verification of drafted tokens. */
+ * attention over it and the verification of drafted tokens.  TK_PROF_LMHEAD:
+ * the head's own kernels and the calls on rows of logits. */
 enum { TK_PROF_GEMM = 0, TK_PROF_DEQUANT = 1, TK_PROF_SPLIT = 2, TK_PROF_GEMV = 3, TK_PROF_LMHEAD = 4,
        TK_PROF_COMM = 5, TK_PROF_SERVE = 6 };
 tk_status tk_profile(tk_ctx *ctx, int enable);
@@ -341,8 +342,8 @@ tk_status tk_draft_verify(tk_ctx *ctx, int n_seqs, const int32_t *row_start, int
 /* n_rows rows of `vocab` logits (<= 2^23; fp32, fp16 or bf16; row stride ldx in
  * elements, of any alignment), T = temperature (1e-4 to 1e4).  Of a row: m its
  * largest logit, S = sum_j exp((l_j - m) / T), p_j = exp((l_j - m) / T) / S.
- * Logits of -inf, and those whose exponential is below 2^-126, have p = 0;
- * results beyond fp32 are infinite.  A row that is needed and holds NaN, +inf or
+ * Logits of -inf have p = 0, and so, in sums and gradients, have those whose
+ * exponential is below 2^-126; results beyond fp32 are infinite.  A row that is needed and holds NaN, +inf or
  * only -inf has NaN in all its results (places -1) and makes tk_sync_status
  * report TK_ERR_DEVICE.  These four calls use no workspace: on several streams
  * they need no order but that of their own data.  No counterpart in the
@@ -377,11 +378,12 @@ tk_status tk_logprobs_grad(tk_ctx *ctx, int n_rows, int vocab, const void *logit
  * may be listed twice.  With q = softmax(teacher[i, :] / T) over the row's
  * entries (below 2^-126: 0):
  *   loss[i] = sum_e q_e (ln q_e - ln p(ids[i, e]))      (nullable; +inf where
- *             some p is 0 and q is not)
+ *             a listed logit of the row is -inf and q is not 0)
  *   dlogits[i, j] = weight[i] / T (p_j - sum of q_e with ids[i, e] == j)
  * (dlogits NULL: the loss alone; weight NULL: 1; dlogits as for
  * tk_logprobs_grad).  A row without entries has loss 0, rmax and rsum 0 and
- * gradient 0, whatever its logits hold; the gradient of a row of weight 0 is 0.  Teacher logits of NaN or +inf are as such in the row itself.  rmax, rsum
+ * gradient 0, whatever its logits hold; the gradient of a row of weight 0 is 0.
+ * Teacher logits of NaN or +inf are as such in the row itself.  rmax, rsum
  * nullable. */
 tk_status tk_distill(tk_ctx *ctx, int n_rows, int vocab, const void *logits, int x_dtype, long ldx, int k, const int32_t *ids,
                      const float *teacher, float temperature, const float *weight, float *loss, float *rmax, float *rsum,

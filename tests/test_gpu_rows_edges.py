@@ -150,3 +150,34 @@ def test_too_many_rows_are_refused(ctx):
     for n, V in ((2 ** 31 - 1, 1 << 14), (1 << 24, 1 << 23)):
         st = ctx.lib.tk_logprobs(ctx.h, n, V, x.data_ptr(), 0, V, None, 1.0, None, x.data_ptr(), None, None, 0, None, None, None)
         assert st == tk.TK_ERR_INVALID
+
+
+def test_calls_that_follow_each_other_at_once(ctx):
+    """A chain of short calls, each on what the one before left: the next call's blocks come early and wait for it."""
+    import torch
+    n, V, k = 6, 9001, 16
+    x, tokens = inputs(5, n, V, "f32")
+    gx, tok = put(x), tokens.cuda()
+    f = [torch.zeros(n, device="cuda") for _ in range(4)]
+    ids, lp = torch.zeros(n, k, dtype=torch.int32, device="cuda"), torch.zeros(n, k, device="cuda")
+    one, loss, buf = torch.ones(n, device="cuda"), torch.zeros(n, device="cuda"), torch.zeros(n, V, device="cuda")
+    for turn in range(40):
+        ids.fill_(-1)                                     # (what a call that did not wait would see)
+        f[2].fill_(1e30)
+        ctx.logprobs(gx, tok, *f, ids, lp)
+        ctx.distill(gx, ids, lp, loss, one, buf)          # its own ids and values: just written
+        ctx.distill(gx, ids, lp, loss)
+        ctx.logprobs_grad(gx, tok, f[2], f[3], buf, one, f[1], one)
+        ctx.logprobs(buf, None, top_ids=ids, top_logp=lp)  # of the gradient: just written over the other one
+        if turn % 13:
+            continue
+        torch.cuda.synchronize()
+        want, tol = ref.logprobs_grad(x, tokens, 1.0, torch.ones(n), torch.ones(n), torch.float32)
+        check([buf], [want], [tol])
+        top = ref.logprobs(buf.cpu(), None, 1.0, k)
+        check([ids, lp], top[0][4:], top[1][4:])
+        t = ref.logprobs(x, None, 1.0, k)[0]
+        want, tol = ref.distill(x, t[4].to(torch.int32), t[5].float(), 1.0, None, None)
+        # (the teacher's values are fp32 log-probabilities, off by 2^-18 and their rounding: q and the loss follow them)
+        assert (loss.cpu().double() - want[0]).abs().max() <= tol[0].max() + 2.0 ** -17 * (1 + want[0].max())
+    ctx.sync_status()
