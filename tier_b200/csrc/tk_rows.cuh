@@ -1,5 +1,5 @@
-// tk_rows.cuh -- rows of logits: element types, the weights of a softmax, and
-// the arguments of the operators on them (tk_logprobs.cu, tk_distill.cu).
+// tk_rows.cuh -- rows of logits: units of access, the sums of a softmax, its
+// dense gradient, and the launch (tk_logprobs.cu, tk_distill.cu).
 #pragma once
 #include "tk_device.cuh"
 #include "tk_f32x2.cuh"
@@ -145,7 +145,7 @@ struct RwEnds {
     __device__ __forceinline__ int place(int i) const { return i < head ? i : i + skip; }
 };
 
-// Running sums of one thread.  m moves only when a batch of logits holds a
+// Running sums of one thread: S of the weights 2^y and A of 2^y y.  m moves only when a batch of logits holds a
 // larger one; s and a are sums of at most a few batches before they go, in 64
 // bits, to the totals, which have a reference of their own.
 template <bool ENT>
@@ -218,7 +218,8 @@ __device__ __forceinline__ T* rw_peer(T* mine, int rank) {
 }
 
 // m, S and A of all parts brought together: threads of a block, blocks of a
-// cluster.  A row that holds NaN or +inf has S = NaN by its arithmetic.
+// cluster.  A row that holds NaN or +inf has S = NaN by its arithmetic, one of
+// nothing above -inf S = 0.
 struct RwStat {
     float m;
     double s, a;
@@ -240,8 +241,6 @@ __device__ __forceinline__ RwStat rw_warp_join(RwStat v, float c) {
     return v;
 }
 
-// m, S = sum 2^y and, relative to it, A = sum 2^y y of a whole row (the same in
-// every thread); a row that holds NaN, +inf or nothing above -inf: S = NaN.
 // Two numbers, rounded once, as a pair of DT.
 template <class DT> __device__ __forceinline__ uint32_t rw_pair(f32x2 v);
 template <> __device__ __forceinline__ uint32_t rw_pair<__nv_bfloat16>(f32x2 v) {
