@@ -64,6 +64,25 @@ def test_tensors_that_do_not_hold_the_rows_are_refused():
         ctx.device = -1
 
 
+def test_what_belongs_to_the_places_has_their_shape():
+    """A teacher's values, or the buffer for the alternatives', wider than the places or turned: their numbers would be
+    taken for other rows'."""
+    import tier_b200 as tk
+    ctx = tk.Context.__new__(tk.Context)
+    ctx.lib, ctx.h, ctx.device = tk.load(), None, -1
+    x, v, ids = torch.zeros(5, 100), torch.zeros(5), torch.zeros(5, 3, dtype=torch.int32)
+    calls = {"top_logp": [lambda t: ctx.logprobs(x, top_ids=ids, top_logp=t, stream=0)],
+             "teacher": [lambda t: ctx.distill(x, ids, t, v, stream=0), lambda t: ctx.distill_grad(x, ids, t, v, v, x.clone(), stream=0)]}
+    for name, fns in calls.items():
+        for fn in fns:
+            for shape in ((5, 6), (3, 5), (6, 3), (15,), (5, 3, 1), (5, 2), (1, 5, 3)):
+                with pytest.raises(tk.TierkError) as e:
+                    fn(torch.zeros(shape))
+                assert e.value.status == tk.TK_ERR_INVALID and f"{name} must be a matrix of" in str(e.value), str(e.value)
+            with pytest.raises(tk.TierkError, match="null context"):
+                fn(torch.zeros(5, 3))
+
+
 def test_plain_forms_agree_with_automatic_gradients():
     g = torch.Generator().manual_seed(0)
     x = torch.randn(6, 40, generator=g, dtype=torch.float64) * 2

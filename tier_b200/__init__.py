@@ -305,6 +305,18 @@ def _width(fn, name, t, n):
     return shape[1]
 
 
+def _beside(fn, name, t, ids, shape, code, device):
+    """The address of what belongs to the places in ids, entry by entry: of their very shape (the library goes by the
+    places' columns alone, and would take a wider or turned matrix's numbers for other rows')."""
+    if t is None:
+        return None
+    if not (t.shape == shape and t.dtype is _DTYPES.get(code) and t.get_device() == device and t.is_contiguous()):
+        if ids is not None and t.shape != shape:
+            raise TierkError(TK_ERR_INVALID, f"{fn}: {name} must be a matrix of {shape[0]} rows of {shape[1]}, as the places")
+        _check_vector(fn, name, t, shape[0] * shape[1], code, device)
+    return t.data_ptr()
+
+
 _I32 = -1
 _DTYPES: dict = {}         # the torch type of each DT_* code, once a tensor has been looked at; _I32's
 
@@ -490,7 +502,7 @@ class Context:
                                     _vector(fn, "entropy", entropy, n, DT_F32, dev), _vector(fn, "rmax", rmax, n, DT_F32, dev),
                                     _vector(fn, "rsum", rsum, n, DT_F32, dev), k,
                                     _vector(fn, "top_ids", top_ids, n * k, _I32, dev),
-                                    _vector(fn, "top_logp", top_logp, n * k, DT_F32, dev), _stream(stream)))
+                                    _beside(fn, "top_logp", top_logp, top_ids, (n, k), DT_F32, dev), _stream(stream)))
         return logp
 
     def logprobs_grad(self, logits, tokens, rmax, rsum, dlogits, d_logp=None, entropy=None, d_entropy=None, temperature=1.0,
@@ -519,7 +531,7 @@ class Context:
         ldx = _row_stride(fn, "logits", logits, x_dtype, n, V, None, dev)
         ldd = _row_stride(fn, "dlogits", dlogits, d_dtype, n, V, None, dev)
         _check(self.lib.tk_distill(self.h, n, V, _ptr(logits), x_dtype, ldx, k, _vector(fn, "ids", ids, n * k, _I32, dev),
-                                   _vector(fn, "teacher", teacher, n * k, DT_F32, dev), temperature,
+                                   _beside(fn, "teacher", teacher, ids, (n, k), DT_F32, dev), temperature,
                                    _vector(fn, "weight", weight, n, DT_F32, dev), _vector(fn, "loss", loss, n, DT_F32, dev),
                                    _vector(fn, "rmax", rmax, n, DT_F32, dev), _vector(fn, "rsum", rsum, n, DT_F32, dev),
                                    _ptr(dlogits), d_dtype, ldd, _stream(stream)))
@@ -533,7 +545,7 @@ class Context:
         ldx = _row_stride(fn, "logits", logits, x_dtype, n, V, None, dev)
         ldd = _row_stride(fn, "dlogits", dlogits, d_dtype, n, V, None, dev)
         _check(self.lib.tk_distill_grad(self.h, n, V, _ptr(logits), x_dtype, ldx, k, _vector(fn, "ids", ids, n * k, _I32, dev),
-                                        _vector(fn, "teacher", teacher, n * k, DT_F32, dev), temperature,
+                                        _beside(fn, "teacher", teacher, ids, (n, k), DT_F32, dev), temperature,
                                         _vector(fn, "rmax", rmax, n, DT_F32, dev), _vector(fn, "rsum", rsum, n, DT_F32, dev),
                                         _vector(fn, "weight", weight, n, DT_F32, dev), _ptr(dlogits), d_dtype, ldd,
                                         _stream(stream)))
