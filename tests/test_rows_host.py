@@ -83,6 +83,25 @@ def test_what_belongs_to_the_places_has_their_shape():
                 fn(torch.zeros(5, 3))
 
 
+def test_a_refused_launch_leaves_no_error_behind(tmp_path):
+    """The next call would launch, and return the old error as its own."""
+    import subprocess
+    from pathlib import Path
+    from tier_b200 import build
+    if not Path(build.NVCC).exists():
+        pytest.skip("nvcc not available")
+    objs = [build.BUILD / (s.stem + ".o") for s in build.sources()]
+    build.build(force=not all(o.exists() and o.stat().st_mtime >= s.stat().st_mtime for o, s in zip(objs, build.sources())))
+    src, exe = Path(__file__).parent / "refused_launch.cu", tmp_path / "refused_launch"
+    r = subprocess.run([build.NVCC, *build.ARCH, "-std=c++17", "-I", str(build.PKG.parent / "include"), "-I", str(build.CSRC), str(src),
+                        *map(str, objs), "-o", str(exe), "-ldl", "-lpthread", "-lrt",
+                        *(f"-Xlinker=--wrap={f}" for f in ("cudaLaunchKernelExC", "cudaGetLastError", "cudaFuncSetAttribute"))],
+                       capture_output=True, text=True, timeout=600)
+    assert r.returncode == 0, r.stdout + r.stderr
+    r = subprocess.run([str(exe)], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0 and "0 failures" in r.stdout, r.stdout + r.stderr
+
+
 def test_plain_forms_agree_with_automatic_gradients():
     g = torch.Generator().manual_seed(0)
     x = torch.randn(6, 40, generator=g, dtype=torch.float64) * 2

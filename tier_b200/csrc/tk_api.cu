@@ -18,6 +18,7 @@ tk_status fail(tk_status st, const std::string& msg) {
 }
 tk_status cuda_fail(cudaError_t e, const char* what) {
     if (e == cudaSuccess) return TK_OK;
+    cudaGetLastError();          // reported here: not to be found, and returned again, by the next call
     g_last_error = std::string(what) + ": " + cudaGetErrorString(e);
     return e == cudaErrorMemoryAllocation ? TK_ERR_NOMEM : TK_ERR_CUDA;
 }

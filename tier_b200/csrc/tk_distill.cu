@@ -338,8 +338,7 @@ tk_status launch_distill(tk_ctx* ctx, const RowArgs& r, int x_dtype, int k, cons
     const cudaError_t e = r.dx ? rw_types(x_dtype, d_dtype, [&](auto x, auto d) { return launch_ds<decltype(x), decltype(d)>(ctx, a, s); })
                         : x_dtype == TK_DT_F32 ? launch_ds<float, void>(ctx, a, s)
                         : x_dtype == TK_DT_F16 ? launch_ds<__half, void>(ctx, a, s) : launch_ds<__nv_bfloat16, void>(ctx, a, s);
-    const cudaError_t last = cudaGetLastError();
-    return cuda_fail(e != cudaSuccess ? e : last, "distillation launch");
+    return cuda_fail(e, "distillation launch");
 }
 tk_status launch_distill_grad(tk_ctx* ctx, const RowArgs& r, int x_dtype, int k, const int32_t* ids, const float* teacher,
                               const float* rmax, const float* rsum, const float* weight, int d_dtype, cudaStream_t s) {

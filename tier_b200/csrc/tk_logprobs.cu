@@ -520,9 +520,8 @@ tk_status launch_logprobs(tk_ctx* ctx, const RowArgs& r, int x_dtype, const int3
         return entropy ? top_k ? launch_lp<XT, true, true>(ctx, a, s) : launch_lp<XT, true, false>(ctx, a, s)
                        : top_k ? launch_lp<XT, false, true>(ctx, a, s) : launch_lp<XT, false, false>(ctx, a, s);
     };
-    const cudaError_t e = x_dtype == TK_DT_F32 ? with(float()) : x_dtype == TK_DT_F16 ? with(__half()) : with(__nv_bfloat16());
-    const cudaError_t last = cudaGetLastError();
-    return cuda_fail(e != cudaSuccess ? e : last, "log-probabilities launch");
+    return cuda_fail(x_dtype == TK_DT_F32 ? with(float()) : x_dtype == TK_DT_F16 ? with(__half()) : with(__nv_bfloat16()),
+                     "log-probabilities launch");
 }
 
 template <class XT, class DT>
