@@ -372,11 +372,12 @@ tk_status tk_logprobs_grad(tk_ctx *ctx, int n_rows, int vocab, const void *logit
                            float temperature, const float *rmax, const float *rsum, const float *d_logp, const float *entropy,
                            const float *d_entropy, void *dlogits, int d_dtype, long ldd, void *stream);
 /* Distillation from a teacher's top logits.  ids, teacher [n_rows, k]: places
- * and the teacher's logits there (or its log-probabilities: q does not change);
- * an entry whose place is negative or whose logit is -inf does not count, one
- * beyond the vocabulary neither (tk_sync_status reports TK_ERR_DEVICE); a place
- * may be listed twice.  With q = softmax(teacher[i, :] / T) over the row's
- * entries (below 2^-126: 0):
+ * and the teacher's logits there, or its log-probabilities at temperature 1 (q
+ * is the same; those of another temperature are divided already); an entry
+ * whose place is negative or whose logit is -inf does not count, one beyond the
+ * vocabulary neither (tk_sync_status reports TK_ERR_DEVICE); a place may be
+ * listed twice.  With q = softmax(teacher[i, :] / T) over the row's entries
+ * (below 2^-126: 0):
  *   loss[i] = sum_e q_e (ln q_e - ln p(ids[i, e]))      (nullable; +inf where
  *             a listed logit of the row is -inf and q is not 0)
  *   dlogits[i, j] = weight[i] / T (p_j - sum of q_e with ids[i, e] == j)
