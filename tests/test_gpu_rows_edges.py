@@ -181,3 +181,32 @@ def test_calls_that_follow_each_other_at_once(ctx):
         # (the teacher's values are fp32 log-probabilities, off by 2^-18 and their rounding: q and the loss follow them)
         assert (loss.cpu().double() - want[0]).abs().max() <= tol[0].max() + 2.0 ** -17 * (1 + want[0].max())
     ctx.sync_status()
+
+
+def test_entries_below_the_least_number_do_not_count(ctx):
+    """A q below 2^-126 is 0, though its weight before the division by their sum is above: a row of -inf there has a loss."""
+    import torch
+    n, V, k = 3, 5000, 256
+    x, _ = inputs(2, n, V, "f32")
+    ids = torch.arange(k, dtype=torch.int32).repeat(n, 1)
+    t = torch.zeros(n, k)
+    t[0, 200], t[1, 255], t[2, 7] = -85.0, -87.0, -83.0       # the others' sum is 255: q = 2^-130.6, 2^-133.5 and 2^-127.7
+    for r, at in enumerate((200, 255, 7)):
+        x[r, at] = -math.inf
+    want, tol = ref.distill(x, ids, t, 1.0, None, torch.float32)
+    assert want[0].isfinite().all()
+    got = run(ctx, put(x), ids, t, 1.0, None, blank(x, "f32"))
+    check(got, want, tol)
+    check(run(ctx, put(x), ids, t, 1.0, None), want[:3], tol[:3])
+    dx = blank(x, "f32")
+    ctx.distill_grad(put(x), ids.cuda(), t.cuda(), got[1], got[2], dx)
+    check([dx], want[3:], tol[3:])
+    for o in (got[3].cpu(), dx.cpu()):
+        assert all(o[r, at] == 0 for r, at in enumerate((200, 255, 7)))
+    t[:, 100] = -74.0                                         # 2^-114.8: counts
+    x[:, 100] = -math.inf
+    want, tol = ref.distill(x, ids, t, 1.0, None, torch.float32)
+    got = run(ctx, put(x), ids, t, 1.0, None, blank(x, "f32"))
+    assert (got[0] == math.inf).all()
+    check(got, want, tol)
+    ctx.sync_status()

@@ -90,7 +90,7 @@ struct DsEntries {
 #pragma unroll
         for (int i = 0; i < EACH; ++i) {
             if (32 * i >= a.k) break;
-            s.q[32 * i + lane] = t[i] * r;
+            asm("mul.ftz.f32 %0, %1, %2;" : "=f"(s.q[32 * i + lane]) : "f"(t[i]), "f"(r));   // (below 2^-126: 0)
         }
         some = __any_sync(~0u, some);
         bad = __any_sync(~0u, bad);
