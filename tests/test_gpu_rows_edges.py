@@ -210,3 +210,29 @@ def test_entries_below_the_least_number_do_not_count(ctx):
     assert (got[0] == math.inf).all()
     check(got, want, tol)
     ctx.sync_status()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,V", [(300, 40001), (200, 65536)])
+def test_gradients_of_many_batches_a_block(ctx, n, V, dtype):
+    """Rows enough that a block takes several batches of one, whole ones and a last one that is not: in place, into another
+    type's rows on other boundaries (element by element), with and without the entropy."""
+    import torch
+    x, tokens = inputs(n, n, V, dtype, left=0.1)
+    g = torch.Generator().manual_seed(n)
+    dl, de = torch.randn(n, generator=g), 0.1 * torch.randn(n, generator=g)
+    other = {"f32": "bf16", "f16": "f32", "bf16": "f16"}[dtype]
+    for a, b, d, at in ((dl, de, dtype, 0), (dl, de, other, 0), (dl, None, other, 3), (None, de, dtype, 1)):
+        want, tol = ref.logprobs_grad(x, tokens, 0.8, a, b, dt(d))
+        gx = put(x)
+        check([gradient(ctx, gx, tokens, 0.8, a, b, d, out=gx if a is dl and d == dtype else blank(x, d, at, at))], [want], [tol])
+    _, ids, t, w = distill_inputs(n, n, V, 40, dtype, twice=0.2)
+    for d, at in ((dtype, 0), (other, 0), (other, 3)):
+        want, tol = ref.distill(x, ids, t, 1.5, w, dt(d))
+        gx = put(x)
+        st = run(ctx, gx, ids, t, 1.5, w)
+        check(run(ctx, gx, ids, t, 1.5, w, blank(x, d, at, at)), want, tol)
+        dx = gx if d == dtype else blank(x, d, at, at)
+        ctx.distill_grad(gx, ids.cuda(), t.cuda(), st[1], st[2], dx, w.cuda(), temperature=1.5, x_dtype=code(gx), d_dtype=code(dx))
+        check([dx], want[3:], tol[3:])
+    ctx.sync_status()
