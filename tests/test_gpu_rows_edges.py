@@ -236,3 +236,35 @@ def test_gradients_of_many_batches_a_block(ctx, n, V, dtype):
         ctx.distill_grad(gx, ids.cuda(), t.cuda(), st[1], st[2], dx, w.cuda(), temperature=1.5, x_dtype=code(gx), d_dtype=code(dx))
         check([dx], want[3:], tol[3:])
     ctx.sync_status()
+
+
+def test_gradients_of_rows_that_hold_no_distribution(ctx):
+    """They are reported as the forward pass reports them; where no gradient is asked for, they are zero and are not."""
+    import tier_b200 as tk
+    import torch
+    n, V = 7, 9001
+    x, tokens = inputs(7, n, V, "f32")
+    x[0, 77], x[2, 8999], x[4] = math.nan, math.inf, -math.inf
+    _, ids, t, w = distill_inputs(7, n, V, 10, "f32", empty=0.0, short=0.0)
+    gx, tok, one = put(x), tokens.cuda(), torch.ones(n, device="cuda")
+    f = [torch.zeros(n, device="cuda") for _ in range(4)]
+    ctx.logprobs(gx, tok, *f)
+    loss = run(ctx, gx, ids, t, 1.0, None)
+    with pytest.raises(tk.TierkError):
+        ctx.sync_status()
+    none, good = [0, 2, 4], [1, 3, 5, 6]
+    calls = [lambda d, g: ctx.logprobs_grad(gx, tok, f[2], f[3], d, g, f[1], None),
+             lambda d, g: ctx.logprobs_grad(gx, None, f[2], f[3], d, None, f[1], g),
+             lambda d, g: ctx.distill_grad(gx, ids.cuda(), t.cuda(), loss[1], loss[2], d, g)]
+    for call in calls:
+        dx = blank(x, "f32")
+        call(dx, one)
+        with pytest.raises(tk.TierkError) as e:
+            ctx.sync_status()
+        assert e.value.status == tk.TK_ERR_DEVICE
+        assert dx[none].isnan().all() and dx[good].isfinite().all()
+        some = one.clone()
+        some[none] = 0.0
+        call(dx, some)
+        ctx.sync_status()
+        assert (dx[none] == 0).all() and dx[good].isfinite().all()

@@ -302,7 +302,7 @@ __global__ void __launch_bounds__(RW_THREADS, 4) dg_kernel(const DsArgs a) {
     }
     __syncthreads();
     const int state = t.state;
-    if (state == 2 && rank == 0 && tid == 0) raise_status(a.r.status, DEV_INVALID);
+    if (rank == 0 && tid == 0 && (state == 2 || (state == 1 && wt != 0.0f && s != s))) raise_status(a.r.status, DEV_INVALID);
     if (state == 0 || wt == 0.0f) {
         rw_zero(dx, vocab, rank, a.parts);
         return;

@@ -469,6 +469,7 @@ __global__ void __launch_bounds__(RW_THREADS, 4) lg_kernel(const LgArgs a) {
         rw_zero(dx, vocab, rank, a.parts);
         return;
     }
+    if (s != s && rank == 0 && threadIdx.x == 0) raise_status(a.r.status, DEV_INVALID);
     // -p (dl + de (ln p + H)) / T with ln p = y ln 2 - ln S
     const float r = a.r.inv_t / s;
     const RwDense<ENT> dense{m, a.r.c, -(ENT ? fmaf(de, h - logf(s), dl) : dl) * r, -de * 0.69314718f * r};
