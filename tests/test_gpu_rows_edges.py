@@ -268,3 +268,60 @@ def test_gradients_of_rows_that_hold_no_distribution(ctx):
         call(dx, some)
         ctx.sync_status()
         assert (dx[none] == 0).all() and dx[good].isfinite().all()
+
+
+@pytest.mark.parametrize("T", [1.0, 0.37])
+def test_rows_that_rise_slowly(ctx, T):
+    """One block a row, whose maximum moves in each of 256 batches by little: no weight decays, and each is scaled again and
+    again.  The sums keep the bound of 64 roundings."""
+    import torch
+    n, batches = 320, 256
+    rise = 2.0 ** torch.linspace(-13, 1, n, dtype=torch.float64)
+    v = (rise[:, None] * torch.arange(batches, dtype=torch.float64) * T / batches).float()       # by 2^-13 to 2 from end to end
+    v[::2] += rise[::2, None].float() * torch.arange(batches) * T                                # and a batch
+    x = torch.empty(n, batches, 8192, device="cuda")
+    x.copy_(v[:, :, None])
+    x = x.view(n, -1)
+    y = (v.double() - v.double()[:, -1:]) / T                # sums over the batches, 8192 logits alike in each
+    S = 8192 * y.exp().sum(1)
+    Y = -(8192 * y.exp() * y).sum(1) / S                     # mean |y|
+    e = 2.0 ** -18 + 2.0 ** -22 + 2.0 ** -22 * Y
+    logp, ent = y[:, 5] - S.log(), S.log() + Y
+    tokens = torch.full((n,), 5 * 8192 + 9, dtype=torch.int32)
+    want = [logp, ent, v[:, -1].double(), S]
+    tol = [e + 2.0 ** -23 * logp.abs(), (e + 2.0 ** -22) * (2 + 2 * ent + S.log()), torch.zeros(n, dtype=torch.float64), (e + 2.0 ** -24) * S]
+    for k in (0, 20):
+        got = forward(ctx, x, tokens, T, k)
+        check(got[:4], want, tol)
+    out = [torch.zeros(n, device="cuda") for _ in range(3)]
+    ids, t = tokens[:, None].cuda(), torch.zeros(n, 1, device="cuda")
+    dx = torch.empty(n, x.shape[1], dtype=torch.bfloat16, device="cuda")
+    for grad in ({}, {"dlogits": dx, "d_dtype": 2}):
+        ctx.distill(x, ids, t, out[0], rmax=out[1], rsum=out[2], temperature=T, **grad)
+        check(out, [-logp, want[2], S], [e + (2.0 ** -20 + 2.0 ** -24) * logp.abs(), tol[2], tol[3]])
+    ctx.sync_status()
+
+
+def test_the_longest_rows_that_rise_slowly(ctx):
+    """1024 batches of one block, their maxima apart by so little that all weigh alike, so that an exponential's error a step
+    would add up.  A weight is off by 4 roundings (2^-24 each: its exponential), 7 in its batch, 3 to bring its lanes
+    together, in the mean 3.5 as other batches come and 3.5 times 2.5 as the reference moves, and the result by one: 28,
+    and the steps' own 2^-22 |y|."""
+    import torch
+    n, batches = 300, 1024
+    x = torch.empty(n, batches, 8192, device="cuda")
+    step = 2.0 ** torch.linspace(-22, -9, n, dtype=torch.float64)
+    v = (step[:, None] * torch.arange(batches, dtype=torch.float64)).float()
+    x.copy_(v[:, :, None])
+    x = x.view(n, -1)
+    y = v.double() - v.double()[:, -1:]
+    S = 8192 * y.exp().sum(1)
+    Y = -(8192 * y.exp() * y).sum(1) / S
+    e = 28 * 2.0 ** -24 + 2.0 ** -22 * Y
+    tokens = torch.zeros(n, dtype=torch.int32)
+    for k in (0, 3):
+        check(forward(ctx, x, tokens, 1.0, k)[2:4], [v[:, -1].double(), S], [torch.zeros(n, dtype=torch.float64), e * S])
+    out = [torch.zeros(n, device="cuda") for _ in range(2)]
+    ctx.distill(x, tokens[:, None].cuda(), torch.zeros(n, 1, device="cuda"), rmax=out[0], rsum=out[1])
+    check(out, [v[:, -1].double(), S], [torch.zeros(n, dtype=torch.float64), e * S])
+    ctx.sync_status()

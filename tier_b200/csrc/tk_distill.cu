@@ -223,8 +223,8 @@ __global__ void __launch_bounds__(RW_THREADS, 4) ds_kernel(const DsArgs a) {
             if (u0 == 0) held.hold(u);
         u0 += STEP;
         rw_batch<XT>(u, p, u0);
+        if (batch++ % RW_FLUSH == 0) sums.flush(c);      // (while the loads are on their way)
         add();
-        if (++batch % 16 == 0) sums.flush(c);
     }
     if (a.r.few) pdl_trigger();
     if (entry < a.k) t.x[entry] = listed;

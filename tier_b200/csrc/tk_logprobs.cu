@@ -356,6 +356,7 @@ __global__ void __launch_bounds__(RW_THREADS, 4) lp_kernel(const LpArgs a) {
     for (int u0 = 0; u0 < p.n; u0 += RW_THREADS * RW_BATCH) {
         RwUnit<XT> u[RW_BATCH];
         rw_batch<XT>(u, p, u0);
+        if (batch > 0 && batch % RW_FLUSH == 0) sums.flush(c);      // (while the loads are on their way)
         float v[RW_BATCH], top = -INFINITY;
 #pragma unroll
         for (int j = 0; j < RW_BATCH; ++j) {
@@ -370,7 +371,7 @@ __global__ void __launch_bounds__(RW_THREADS, 4) lp_kernel(const LpArgs a) {
         if (TOP) keep(v);
         if (top > sums.m) sums.raise(top, c);
         sums.batch(u, c2);
-        if (++batch % 16 == 0) sums.flush(c);      // (at most 16 batches are added in fp32)
+        ++batch;
     }
     if (a.r.few) pdl_trigger();                    // (earlier, the next call's blocks would take cache from the loads)
     sums.flush(c);
