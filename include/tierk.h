@@ -343,11 +343,13 @@ tk_status tk_draft_verify(tk_ctx *ctx, int n_seqs, const int32_t *row_start, int
  * elements, of any alignment), T = temperature (1e-4 to 1e4).  Of a row: m its
  * largest logit, S = sum_j exp((l_j - m) / T), p_j = exp((l_j - m) / T) / S.
  * Logits of -inf have p = 0, and so, in sums and gradients, have those whose
- * exponential is below 2^-126; results beyond fp32 are infinite.  A row that is needed and holds NaN, +inf or
- * only -inf has NaN in all its results (places -1) and makes tk_sync_status
- * report TK_ERR_DEVICE.  These four calls use no workspace: on several streams
- * they need no order but that of their own data.  No counterpart in the
- * reference, whose loss is the cross-entropy of one label a row. */
+ * exponential is below 2^-126; results beyond fp32 are infinite (gradients of a
+ * row infinite or NaN where its weight / T, d_logp / T or d_entropy / T is).  A
+ * row that is needed and holds NaN, +inf or only -inf has NaN in all its results
+ * (places -1) and makes tk_sync_status report TK_ERR_DEVICE.  These four calls
+ * use no workspace: on several streams they need no order but that of their own
+ * data.  No counterpart in the reference, whose loss is the cross-entropy of one
+ * label a row. */
 enum { TK_TOP_MAX = 256 };   /* top_k, k at most */
 /* Log-probabilities of given tokens, entropy and the likeliest tokens:
  * logp[i] = ln p(tokens[i]), entropy[i] = -sum_j p_j ln p_j, rmax[i] = m,

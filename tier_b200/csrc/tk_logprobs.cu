@@ -19,10 +19,12 @@
 // The gradient reads every logit and writes every gradient once.
 //
 // Measured (us; calls in a graph, L2 warm): 1 row of 262144 fp32, 20
-// alternatives 9.9 (of them the reading 3, the search 3, the meeting of 8 blocks
-// 1); 48 of 50257, 5 alternatives 9.8; 4095 x 262144 fp32, none 533 (7.2 TB/s);
-// 1024 x 262144 bf16 without 85 (6.3 TB/s), 20 97, 128 103, 256 112. Gradients
-// of 2048 x 131072 bf16, 30 % of the rows left out, 141 (6.5 TB/s).
+// alternatives 9.8 (of them the reading 3, the search 3, the meeting of 8 blocks
+// 1); 48 of 50257, 5 alternatives 9.7; 4095 x 262144 fp32, none 533 (7.2 TB/s;
+// from Python on boxes that had not run before 535 to 555); 1024 x 262144 bf16
+// without 86 (6.3 TB/s), 20 97, 128 103 (from Python 98 without, 104 to 114
+// with 128), 256 112. Gradients of 2048 x 131072 bf16, 30 % of the rows left
+// out, 141 (6.5 TB/s).
 #include "tk_rows.cuh"
 
 namespace tk {
@@ -113,8 +115,11 @@ __device__ __noinline__ unsigned long long lp_thin(LpTop& t, int k, int& turn) {
 // halves of each thread's units, a bound is found that top_k of these reach, so
 // top_k logits do (256 or 512 numbers, one counting barrier a bit); only units
 // that reach it are read again, little more than top_k of them for logits in
-// any order, a sector of memory each.  Where many logits are alike or the largest stand together,
-// candidates that do not fit are thinned on the way.
+// any order, a sector of memory each.  Where many logits are alike or the
+// largest stand together, candidates that do not fit are thinned on the way; so
+// too where fewer than top_k numbers are above -inf, which gives no bound (from
+// Python, us: 1 row of 262144 with 8 finite logits of 20 26, 48 of 50257 with 4
+// of 5 24.5, 1024 with 100 of 128 255).
 template <class XT>
 __device__ __forceinline__ void lp_search(LpTop& t, const LpArgs& a, const XT* row, const RwPart<XT>& p, bool ends,
                                           float v0, float v1) {
