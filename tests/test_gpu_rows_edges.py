@@ -325,3 +325,26 @@ def test_the_longest_rows_that_rise_slowly(ctx):
     ctx.distill(x, tokens[:, None].cuda(), torch.zeros(n, 1, device="cuda"), rmax=out[0], rsum=out[1])
     check(out, [v[:, -1].double(), S], [torch.zeros(n, dtype=torch.float64), e * S])
     ctx.sync_status()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_more_candidates_than_fit_beside_the_ends(ctx, dtype):
+    """Rows off every boundary, half of whose logits reach the bound: more than a block's candidates hold, with up to 30 ends
+    beside them.  Often enough for a slow load of an end to come behind all units' candidates."""
+    import torch
+    n, V, k = 2000, 3798, 256
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.randn(n, V, generator=g, device="cuda") * 2
+    x[:, 250:2210] += 5
+    x = put(x.to(dt(dtype)), 13, 7)
+    order = x.float().sort(dim=1, descending=True, stable=True)
+    want = order.indices[:, :k].to(torch.int32)
+    ids, lp, wrong = torch.zeros(n, k, dtype=torch.int32, device="cuda"), torch.zeros(n, k, device="cuda"), 0
+    for _ in range(200):
+        ids.fill_(-1)
+        ctx.logprobs(x, top_ids=ids, top_logp=lp, x_dtype=code(x))
+        wrong = wrong + (ids != want).any(1).sum()
+    assert wrong.item() == 0
+    exact = torch.log_softmax(x.double(), 1).gather(1, want.long())
+    assert (lp.double() - exact).abs().max() < 2.0 ** -17
+    ctx.sync_status()

@@ -157,6 +157,11 @@ __device__ __forceinline__ void lp_search(LpTop& t, const LpArgs& a, const XT* r
             if (c <= k + k / 8 + 8) break;
         }
     }
+    // the row's ends come first, whatever they hold: 30 at most, which fit (behind
+    // the units' they might not, and the units' are counted on where they do not fit)
+    const RwEnds<XT> e(row, a.r.vocab);
+    const bool end = ends && tid < e.n;
+    if (end) t.keep[atomicAdd(&t.n, 1)] = lp_key(lp_order(rw_float(row[e.place(tid)])), e.place(tid));
     const float least_x = bound ? lp_value(bound) : -INFINITY;
     if (fmaxf(v0, v1) >= least_x) {
         const float least_16 = __uint_as_float(__float_as_uint(least_x) & 0xffff0000u);   // (cut off as the slots' numbers are)
@@ -178,9 +183,6 @@ __device__ __forceinline__ void lp_search(LpTop& t, const LpArgs& a, const XT* r
             if (at < LP_LIST) t.list[at] = (uint16_t)((__ffsll(hits) - 1) * RW_THREADS + tid);
     }
     __syncthreads();
-    const RwEnds<XT> e(row, a.r.vocab);
-    const bool end = ends && tid < e.n;
-    if (end) t.keep[atomicAdd(&t.n, 1)] = lp_key(lp_order(rw_float(row[e.place(tid)])), e.place(tid));
     // the i-th unit to look through: of those listed, or (where they are too many) of all
     const bool all = t.listed > LP_LIST;
     const int total = all ? p.n : t.listed << a.shift;
