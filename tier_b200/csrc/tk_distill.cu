@@ -17,8 +17,8 @@
 // memory (no room in the L1 for loads on their way: 506 and more), 512 or 1024
 // threads a block (427, 426).
 //
-// Measured (us; calls in a graph, and from Python on boxes that had not run
-// before): 4096 x 262144 bf16 750 to 775, 751 to 828 (5.1 TB/s of floor bytes at
+// Measured (us; calls in a graph, and from Python on machines that were
+// idle before): 4096 x 262144 bf16 750 to 775, 751 to 828 (5.1 TB/s of floor bytes at
 // the most), 512 x 262144 fp32 to bf16 135 to 144, 145, 16 x 50257 fp16 7.8, 9.7;
 // the loss of 300 x 131072 fp32 29.7, 30; the gradient alone 2048 x 262144 bf16
 // 317 (6.8 TB/s), 320.

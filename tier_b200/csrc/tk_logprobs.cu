@@ -21,7 +21,7 @@
 // Measured (us; calls in a graph, L2 warm): 1 row of 262144 fp32, 20
 // alternatives 9.8 (of them the reading 3, the search 3, the meeting of 8 blocks
 // 1); 48 of 50257, 5 alternatives 9.7; 4095 x 262144 fp32, none 533 (7.2 TB/s;
-// from Python on boxes that had not run before 535 to 555); 1024 x 262144 bf16
+// from Python on machines that were idle before 535 to 555); 1024 x 262144 bf16
 // without 86 (6.3 TB/s), 20 97, 128 103 (from Python 98 without, 104 to 114
 // with 128), 256 112. Gradients of 2048 x 131072 bf16, 30 % of the rows left
 // out, 141 (6.5 TB/s).
